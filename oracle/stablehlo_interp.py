@@ -80,6 +80,7 @@ import math
 import re
 import numpy as np
 
+from . import lm_ops
 from . import lowfloat as lf
 
 # ----------------------------------------------------------------------------
@@ -1002,6 +1003,18 @@ class Parser:
                     if not c.accept(","):
                         break
             return op
+        if short == "custom_call":
+            op.attrs["target"] = c.m(c._sym)[1:]
+            c.expect("(")
+            while not c.accept(")"):
+                op.operands.append(c.ssa())
+                c.accept(",")
+            attrs = c.balanced("{", "}") if c.peek() == "{" else ""
+            mo = re.search(r"backend_config\s*=\s*\{([^}]*)\}", attrs)
+            op.attrs["config"] = lm_ops.parse_config(mo.group(1) if mo else "")
+            c.expect(":")
+            self.fn_type(op)
+            return op
         if short == "call":
             op.attrs["callee"] = c.m(c._sym)[1:]
             c.expect("(")
@@ -1831,6 +1844,13 @@ class Interpreter:
             return [tensor(gelu(xs[0].a.astype(np.float64), at.get("approximation", "NONE")), dt)]
         if n == "optimization_barrier":
             return list(xs)
+        if n == "custom_call":
+            arrays = [_rounded(x).a for x in xs]
+            if at["target"] == "rx.embedding_grad":
+                outs = [lm_ops.embedding_grad(arrays[0], arrays[1], op.types_out[0].shape[0], at["config"].get("scale", 1.0))]
+            else:
+                outs = lm_ops.evaluate(at["target"], arrays, at["config"])
+            return [Tensor(_round_to(np.asarray(a), t.dt), t.dt) for a, t in zip(outs, op.types_out)]
         if n == "call":
             return Interpreter(self.funcs, self.hifi, self.excess).run(list(xs), at["callee"])
         if n == "map":

@@ -495,14 +495,14 @@ void execute(RxExecutable* ex, int num_args, RxBuffer** args, RxDevice* dev, uin
     uint8_t* donate;
     const rx::Plan& P;
     std::vector<Mem>& bufs;
-    bool committed = false;
+    bool committed = false, started = false;
     ~Donation() {
       if (!donate) return;
       for (size_t b = 0; b < P.buffers.size(); ++b) {
         const auto& B = P.buffers[b];
         if (B.kind != rx::BufferDesc::Param || !donate[B.param_index]) continue;
         RxBuffer* a = args[B.param_index];
-        if (committed || !bufs[b]) { a->donated = true; a->mem.reset(); }
+        if (committed || !bufs[b] || (B.written && started)) { a->donated = true; a->mem.reset(); }
         else if (!a->mem) a->mem = bufs[b];
       }
     }
@@ -519,6 +519,16 @@ void execute(RxExecutable* ex, int num_args, RxBuffer** args, RxDevice* dev, uin
   if (donate)
     for (int i = 0; i < num_args; ++i)
       if (donate[i]) args[i]->mem.reset();   // the plan's buffer holds it from here on
+  // An argument that a kernel updates in place is copied where anything else still holds its memory: the caller (it is not
+  // donated), another argument, a result that was returned twice.
+  for (size_t b = 0; b < NB; ++b) {
+    const auto& B = P.buffers[b];
+    if (!B.written || bufs[b].use_count() == 1) continue;
+    Mem copy = std::make_shared<Allocation>(dev, (size_t)B.bytes);
+    HIP_CHECK(hipMemcpyAsync(copy->ptr, bufs[b]->ptr, (size_t)B.bytes, hipMemcpyDeviceToDevice, dev->stream));
+    bufs[b] = copy;
+  }
+  donation.started = true;
   // events of a timed execution; destroyed on every exit path unless handed to the executable
   struct EventList {
     std::vector<hipEvent_t> v;
@@ -587,7 +597,7 @@ void execute(RxExecutable* ex, int num_args, RxBuffer** args, RxDevice* dev, uin
       HIP_CHECK(hipMemcpyAsync(m->ptr, ex->consts[b]->ptr, (size_t)B.bytes, hipMemcpyDeviceToDevice, dev->stream));
     } else if (B.kind == rx::BufferDesc::Param && !m) {
       throw Error("internal: pass-through result lost its storage");
-    } else if (B.kind == rx::BufferDesc::Param && !(donate && donate[B.param_index])) {
+    } else if (B.kind == rx::BufferDesc::Param && !B.written && !(donate && donate[B.param_index])) {
       // an argument returned unchanged and not donated: the result is a buffer of its own, so that
       // writing into it (CopyToBuffer) or donating it later leaves the caller's argument alone
       m = std::make_shared<Allocation>(dev, std::max<size_t>((size_t)B.bytes, 1));
@@ -1132,7 +1142,8 @@ RX_EXPORT int RxExecuteNoAlloc(RxExecutable* ex, int num_args, RxBuffer** args, 
     size_t used = 0;
     for (size_t b = 0; b < NB; ++b) {
       const auto& B = P.buffers[b];
-      if (B.kind == rx::BufferDesc::Param) where[b] = args[B.param_index]->mem->ptr;
+      if (B.written) where[b] = results[first_result[b]]->mem->ptr;   // updated in place: in a copy, which is the result (below)
+      else if (B.kind == rx::BufferDesc::Param) where[b] = args[B.param_index]->mem->ptr;
       else if (B.kind == rx::BufferDesc::Const) where[b] = ex->consts[b]->ptr;
       else if (B.kind == rx::BufferDesc::Fault) where[b] = dev->fault_dev;
       else if (first_result[b] >= 0) where[b] = results[first_result[b]]->mem->ptr;
@@ -1146,6 +1157,9 @@ RX_EXPORT int RxExecuteNoAlloc(RxExecutable* ex, int num_args, RxBuffer** args, 
                   std::to_string(RX_NOALLOC_SCRATCH_BYTES) + " (use XLAExecuteSharded)");
     std::lock_guard<std::mutex> slock(dev->scratch_mu);
     HIP_CHECK(hipSetDevice(dev->ordinal));
+    for (size_t b = 0; b < NB; ++b)
+      if (P.buffers[b].written)
+        HIP_CHECK(hipMemcpyAsync(where[b], args[P.buffers[b].param_index]->mem->ptr, (size_t)P.buffers[b].bytes, hipMemcpyDeviceToDevice, dev->stream));
     std::vector<void*> ptrs, argv;
     for (size_t li = 0; li < P.launches.size(); ++li) {
       const auto& L = P.launches[li];

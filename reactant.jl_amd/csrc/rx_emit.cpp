@@ -1006,6 +1006,8 @@ std::string Emitter::emit_op(const Node& n, const Index& ix) {
     case OpK::Scan:
     case OpK::Scatter:
     case OpK::Conv:
+    case OpK::Operator:
+    case OpK::OperatorResult:
     case OpK::DotGeneral:
       throw Error("internal: reduce/dot_general reached the emitter without a buffer or binding");
   }

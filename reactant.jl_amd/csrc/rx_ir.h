@@ -54,6 +54,7 @@ enum class OpK : uint8_t {
   BroadcastInDim, Reshape, Transpose, Slice, Pad, DynamicUpdateSlice, DynamicSlice, Concatenate,
   Reverse, Window, Gather,
   Reduce, DotGeneral, Scan, Scatter, Conv,
+  Operator, OperatorResult,
 };
 
 enum class Red : uint8_t { Add, Mul, Max, Min, And, Or };
@@ -87,7 +88,10 @@ struct Node {
   //       the padded grid; the result [B, HO, WO, O] keeps p at m = (b * HP + y) * WP + x for y < HO, x < WO
   //       with a3 = {KW, SY, SX, HP, WP, HO, WO, shift} the result is [B, HP, WP, O]: row m of p, zero where it is not a
   //       result, at row m + shift, and zeros in the rows before `shift` (the next such product's zero-padded operand)
+  //   Operator (custom_call of an `rx.` target, rx_lm.h): op = the target; `attrs` its settings, a0 = {results}; the value is the first result
+  //   OperatorResult (an Operator): a0[0] = which of its further results this is
   std::vector<int64_t> a0, a1, a2, a3, a4, a5, a6;
+  std::map<std::string, std::string> attrs;
   Red red = Red::Add;
   // Constant payload: either one splat element or dense bytes in storage format
   bool splat = false;

@@ -8,6 +8,7 @@
 // suffixes (test/core/compile.jl:653-661).
 #include "rx_ir.h"
 #include "rx_gemm.h"
+#include "rx_lm.h"
 
 #include <cmath>
 #include <cstring>
@@ -272,6 +273,31 @@ struct Cur {
       }
     }
     fail("unbalanced bracket");
+  }
+  // one attribute value as text: a string without its quotes, or everything up to the next comma outside of brackets
+  std::string value() {
+    ws();
+    if (i < n && s[i] == '"') {
+      size_t j = i + 1;
+      while (j < n && s[j] != '"') j += s[j] == '\\' ? 2 : 1;
+      if (j >= n) fail("unterminated string");
+      std::string r(s + i + 1, j - i - 1);
+      i = j + 1;
+      return r;
+    }
+    int depth = 0;
+    size_t j = i;
+    for (; j < n; ++j) {
+      const char c = s[j];
+      if (c == '[' || c == '<' || c == '{' || c == '(') ++depth;
+      else if (c == ']' || c == '}' || c == ')' || (c == '>' && s[j - 1] != '-')) --depth;
+      else if (depth == 0 && (c == ',' || c == ':')) break;
+    }
+    std::string r(s + i, j - i);
+    while (!r.empty() && isspace((unsigned char)r.back())) r.pop_back();
+    if (r.empty()) fail("expected an attribute value");
+    i = j;
+    return r;
   }
   std::vector<int64_t> int_list() {
     expect("[");
@@ -588,6 +614,20 @@ struct P {
     }
   }
 
+  // the target's name and its settings: `backend_config` as a dictionary of numbers and strings
+  static void custom_call_attrs(const std::string& in, RawOp& o) {
+    Cur a(in.c_str(), in.size());
+    while (!a.eof()) {
+      const std::string key = a.ident();
+      if (!a.accept("=")) { a.accept(","); continue; }   // a unit attribute
+      std::string* to = key == "call_target_name" ? &o.sa["call_target_name"] : key == "backend_config" ? &o.sa["backend_config"] : nullptr;
+      std::string v = a.peek() == '{' ? "{" + a.balanced('{', '}') + "}" : a.value();
+      if (a.accept(":")) a.value();
+      if (to) *to = v;
+      a.accept(",");
+    }
+  }
+
   RawOp generic_op() {
     RawOp o;
     c.ws();
@@ -602,6 +642,7 @@ struct P {
       std::string in = c.balanced('{', '}');
       c.expect(">");
       generic_attrs(in, o);
+      if (o.name == "stablehlo.custom_call") custom_call_attrs(in, o);
     }
     if (c.peek() == '(') {
       c.expect("(");
@@ -612,7 +653,11 @@ struct P {
       }
       c.expect(")");
     }
-    if (c.peek() == '{') generic_attrs(c.balanced('{', '}'), o);
+    if (c.peek() == '{') {
+      const std::string in = c.balanced('{', '}');
+      generic_attrs(in, o);
+      if (o.name == "stablehlo.custom_call") custom_call_attrs(in, o);
+    }
     c.expect(":");
     fn_type(o);
     return o;
@@ -981,6 +1026,16 @@ struct P {
         c.expect(":");
         do { o.tout.push_back(c.type()); } while (c.accept(","));
       }
+      return o;
+    }
+    if (sh == "custom_call") {
+      // %0:2 = stablehlo.custom_call @target(%a, %b) {backend_config = {key = value, ..}, ..} : (types) -> (types)
+      o.sa["call_target_name"] = c.sym();
+      c.expect("(");
+      while (!c.accept(")")) { o.operands.push_back(c.ssa()); c.accept(","); }
+      if (c.peek() == '{') custom_call_attrs(c.balanced('{', '}'), o);
+      c.expect(":");
+      fn_type(o);
       return o;
     }
     if (sh == "call") {
@@ -2242,6 +2297,51 @@ struct Builder {
     return cur;
   }
 
+  // custom_call of one of the library's own operators (rx_lm.h)
+  std::vector<int> build_operator(const RawOp& o, const std::vector<int>& in) {
+    OperatorSpec spec;
+    spec.name = o.sa.count("call_target_name") ? o.sa.at("call_target_name") : "";
+    if (spec.name.size() >= 2 && spec.name.front() == '"' && spec.name.back() == '"') spec.name = spec.name.substr(1, spec.name.size() - 2);
+    if (!is_operator_name(spec.name)) fail("custom_call: unknown target '" + spec.name + "'");
+    if (o.sa.count("backend_config")) {
+      std::string body = o.sa.at("backend_config");
+      if (!body.empty() && body.front() == '{') {
+        body = body.substr(1, body.size() - 2);
+        Cur a(body.c_str(), body.size());
+        while (!a.eof()) {
+          const std::string key = a.ident();
+          a.expect("=");
+          const std::string v = a.value();
+          if (a.accept(":")) a.value();
+          if (!spec.attrs.emplace(key, v).second) fail(spec.name + ": setting '" + key + "' is given twice");
+          if (!a.accept(",") && !a.eof()) a.fail("expected ','");
+        }
+      } else if (!body.empty()) {
+        fail(spec.name + ": backend_config must be a dictionary");
+      }
+    }
+    for (int i : in) spec.in.push_back(ty(i));
+    spec.out = o.tout;
+    if (o.tin.size() != in.size()) fail(spec.name + ": one type per operand expected");
+    for (size_t k = 0; k < in.size(); ++k)
+      if (!(o.tin[k] == spec.in[k])) fail(spec.name + ": operand " + std::to_string(k) + " has type " + spec.in[k].str() + ", declared " + o.tin[k].str());
+    check_operator(spec);
+    Node n;
+    n.k = OpK::Operator;
+    n.op = spec.name;
+    n.attrs = spec.attrs;
+    n.in = in;
+    n.ty = spec.out[0];
+    n.a0 = {(int64_t)spec.out.size()};
+    std::vector<int> res{g.add(n)};
+    for (size_t r = 1; r < spec.out.size(); ++r) {
+      const int id = add_node(OpK::OperatorResult, spec.out[r], {res[0]});
+      g.nodes[id].a0 = {(int64_t)r};
+      res.push_back(id);
+    }
+    return res;
+  }
+
   std::vector<int> build(const RawOp& o, const std::vector<int>& in, int depth) {
     std::string sh = o.name;
     if (sh.rfind("stablehlo.", 0) == 0) sh = sh.substr(10);
@@ -2250,6 +2350,7 @@ struct Builder {
     Node n;
     n.in = in;
     if (sh == "optimization_barrier") return in;
+    if (sh == "custom_call") return build_operator(o, in);
     if (sh == "call") {
       auto it = p.funcs.find(o.sa.at("callee"));
       if (it == p.funcs.end()) fail("call to unknown function @" + o.sa.at("callee"));

@@ -25,6 +25,7 @@
 
 #include "rx_emit.h"
 #include "rx_gemm.h"
+#include "rx_lm.h"
 
 namespace rx {
 namespace {
@@ -51,6 +52,8 @@ bool is_arith(OpK k) {
       return false;
   }
 }
+
+bool is_operator(OpK k) { return k == OpK::Operator || k == OpK::OperatorResult; }
 
 const char* acc_ctype(DT dt) {
   if (dt == DT::F64) return "double";
@@ -133,6 +136,7 @@ struct Planner {
   std::map<int, int> row_anchor;    // reduction fused into a row kernel -> the root of that kernel
   std::ostringstream src;
   int kcount = 0;
+  bool uses_operators = false;      // the text calls device functions of rx_lm_kernels.h
 
   Planner(const Graph& gin, const PlanOptions& o) : g(gin), opt(o) {}
 
@@ -910,7 +914,7 @@ struct Planner {
     for (auto& n : g.nodes) for (int i : n.in) nuse[i]++;
     for (int r : g.results) nuse[r]++;
     auto is_leaf = [](const Node& n) {
-      return n.k == OpK::Param || (n.k == OpK::Constant && !n.splat) || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || n.k == OpK::Conv || n.k == OpK::DotGeneral;
+      return n.k == OpK::Param || (n.k == OpK::Constant && !n.splat) || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || is_operator(n.k) || n.k == OpK::Conv || n.k == OpK::DotGeneral;
     };
     for (const Node& d : g.nodes) {
       if (d.k != OpK::DotGeneral || d.ty.rank() < 2 || !d.a4.empty()) continue;
@@ -1367,7 +1371,7 @@ struct Planner {
       st.pop_back();
       if (!seen.insert(x).second) continue;
       const Node& n = g.nodes[x];
-      if (n.k == OpK::Param || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || n.k == OpK::Conv || n.k == OpK::DotGeneral) continue;
+      if (n.k == OpK::Param || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || is_operator(n.k) || n.k == OpK::Conv || n.k == OpK::DotGeneral) continue;
       if (n.k == OpK::Constant) continue;
       if (x != id && prev_mat[x]) continue;
       if (is_arith(n.k)) cost += (n.k == OpK::Unary || n.k == OpK::Gelu) ? 2 : 1;
@@ -1385,7 +1389,7 @@ struct Planner {
       if (!seen.insert(x).second || seen.size() > 64) continue;
       const Node& n = g.nodes[x];
       if (n.k == OpK::DotGeneral) return true;
-      if (n.k == OpK::Param || n.k == OpK::Constant || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || n.k == OpK::Conv) continue;
+      if (n.k == OpK::Param || n.k == OpK::Constant || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || is_operator(n.k) || n.k == OpK::Conv) continue;
       if (x != id && prev_mat[x]) continue;
       for (int i : n.in) st.push_back(i);
     }
@@ -1444,10 +1448,11 @@ struct Planner {
       const Node& n = g.nodes[x];
       // contexts in which x is evaluated
       std::set<Ctx> U;
-      bool forced = is_result[x] || n.k == OpK::Param || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || n.k == OpK::Conv || n.k == OpK::DotGeneral ||
+      bool forced = is_result[x] || n.k == OpK::Param || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || is_operator(n.k) || n.k == OpK::Conv || n.k == OpK::DotGeneral ||
                     (n.k == OpK::Constant && !n.splat);
       for (int u : users[x]) {
         const Node& un = g.nodes[u];
+        if (un.k == OpK::Operator) { forced = true; continue; }
         if (un.k == OpK::Conv) { forced = true; continue; }   // the direct-convolution kernel reads its operands from memory
         if (un.k == OpK::DotGeneral) {
           const int side = un.in[0] == x ? 0 : 1;
@@ -1491,7 +1496,7 @@ struct Planner {
             if (!(cn.k == OpK::Convert || cn.k == OpK::Unary)) break;
             int p = cn.in[0];
             const Node& pn = g.nodes[p];
-            if (pn.k == OpK::DotGeneral || pn.k == OpK::Param || pn.k == OpK::Constant || pn.k == OpK::Reduce || pn.k == OpK::Scan || pn.k == OpK::Scatter || pn.k == OpK::Conv) break;
+            if (pn.k == OpK::DotGeneral || pn.k == OpK::Param || pn.k == OpK::Constant || pn.k == OpK::Reduce || pn.k == OpK::Scan || pn.k == OpK::Scatter || is_operator(pn.k) || pn.k == OpK::Conv) break;
             if (users[p].size() != 1 || is_result[p]) break;
             cur = p;
             if (info(pn.ty.dt).size < info(g.nodes[best].ty.dt).size) best = cur;
@@ -2057,6 +2062,7 @@ struct Planner {
         case OpK::Gather: nm = "gather"; break;
         case OpK::Scan: nm = "scan"; break;
         case OpK::Scatter: nm = "scatter"; break;
+        case OpK::Operator: nm = n.op; break;
         case OpK::Conv: nm = "convolution"; break;
         case OpK::Reduce: nm = "reduce"; break;
         case OpK::DotGeneral: nm = "dot_general"; break;
@@ -2193,7 +2199,7 @@ struct Planner {
   bool probe_stencil(int root, StencilProbe* sp) {
     const Node& rn = g.nodes[root];
     const auto& dims = rn.ty.dims;
-    if (!opt.lds_stencil || rn.ty.rank() != 3 || rn.k == OpK::Reduce || rn.k == OpK::Scan || rn.k == OpK::Scatter || rn.k == OpK::Conv || rn.k == OpK::DotGeneral) return false;
+    if (!opt.lds_stencil || rn.ty.rank() != 3 || rn.k == OpK::Reduce || rn.k == OpK::Scan || rn.k == OpK::Scatter || is_operator(rn.k) || rn.k == OpK::Conv || rn.k == OpK::DotGeneral) return false;
     sp->vec = pick_vec(rn.ty);
     if (rn.ty.numel() < opt.slab_min_numel || sp->vec < 2) return false;
     Emitter probe(g, [&](int x) { return x != root && mat[x]; });
@@ -3208,7 +3214,7 @@ struct Planner {
     // rank 3: only small arrays, whose steps are bound by the launch gap (32^3 and 64^3 heat steps: 1.6x and 1.4x
     // faster in chains of four); at 128^3 the redundant halo cells cost more than the launches saved
     if (r < 1 || r > 3 || (r > opt.chain_max_rank && r != 3)) return false;
-    if (n.k == OpK::Param || n.k == OpK::Constant || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || n.k == OpK::Conv || n.k == OpK::DotGeneral) return false;
+    if (n.k == OpK::Param || n.k == OpK::Constant || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || is_operator(n.k) || n.k == OpK::Conv || n.k == OpK::DotGeneral) return false;
     const int es = info(n.ty.dt).size;
     if (es != 4 && es != 8) return false;
     if (n.ty.numel() < 2 || n.ty.numel() >= opt.slab_min_numel) return false;
@@ -4084,6 +4090,71 @@ struct Planner {
     L.algo_bytes = algo_bytes(em.inputs, {});
     L.desc = describe(rn.in[2]) + " scatter";
     plan.launches.push_back(L);
+  }
+
+  // ------------------------------------------------------------------ operators of language models (rx_lm.h)
+  // The result is an updated copy of `from`: may it be written into that value's own buffer?  A temporary that no later
+  // kernel reads, or an argument that the module lets this result take over.
+  bool updates_in_place(int result, int from, int op) const {
+    const Node& n = g.nodes[from];
+    if (n.k == OpK::Constant || !mat[from] || reshape_alias.count(from)) return false;
+    for (auto& kv : reshape_alias) if (kv.second == from) return false;
+    if (std::count(g.results.begin(), g.results.end(), from)) return false;
+    if (n.k == OpK::Param) {
+      const int r = g.aliasing_output[n.a0[0]];
+      if (r < 0 || r >= (int)g.results.size() || g.results[r] != result) return false;
+    }
+    if (std::count(g.nodes[op].in.begin(), g.nodes[op].in.end(), from) != 1) return false;
+    std::vector<int> st{from};
+    std::set<int> seen;
+    while (!st.empty()) {
+      const int y = st.back();
+      st.pop_back();
+      for (int u : users[y]) {
+        if (!live[u] || u == op || (y == from && u == result)) continue;
+        if (mat[u]) { if (launch_position(u) > op) return false; }
+        else if (seen.insert(u).second) st.push_back(u);
+      }
+    }
+    return true;
+  }
+  void emit_operator(int root) {
+    const Node& n = g.nodes[root];
+    OperatorSpec spec;
+    spec.name = n.op;
+    spec.attrs = n.attrs;
+    for (int i : n.in) spec.in.push_back(g.nodes[i].ty);
+    std::vector<int> results((size_t)n.a0[0], -1);
+    results[0] = root;
+    for (auto& r : g.nodes)
+      if (r.k == OpK::OperatorResult && r.in[0] == root) results[r.a0[0]] = r.id;
+    for (int r : results) spec.out.push_back(g.nodes[r].ty);
+    const OperatorPlan op = plan_operator(spec);
+    uses_operators = true;
+    for (size_t r = 0; r < results.size(); ++r) {
+      const int from = r < op.updates.size() ? op.updates[r] : -1;
+      if (from < 0) continue;
+      if (updates_in_place(results[r], n.in[from], root)) {
+        buf_of[results[r]] = buffer_for(n.in[from]);
+        plan.buffers[buf_of[results[r]]].written = true;
+      } else emit_map(results[r], n.in[from]);
+    }
+    std::vector<int> scratches;
+    for (int64_t b : op.scratch) scratches.push_back(scratch(b));
+    for (const OperatorKernel& k : op.kernels) {
+      Launch L;
+      L.kernel = named("@K@_" + k.suffix, finalize(k.text));
+      L.kind = k.kind;
+      for (int d = 0; d < 3; ++d) L.grid[d] = k.grid[d];
+      L.block[0] = k.block;
+      for (const OperatorArg& a : k.args)
+        L.args.push_back(a.kind == OperatorArg::Operand ? buffer_for(n.in[a.index]) : a.kind == OperatorArg::Result ? buffer_for(results[a.index]) : scratches[a.index]);
+      L.n_outputs = k.n_outputs;
+      L.algo_bytes = k.bytes;
+      L.flops = k.flops;
+      L.desc = n.op;
+      plan.launches.push_back(L);
+    }
   }
 
   // The filter of a convolution on split operands, in the order its kernel reads it: a buffer and the launch that writes it.
@@ -5990,7 +6061,7 @@ struct Planner {
       const Ctx& c = *ctx[x].begin();
       if (!c.second.empty()) continue;
       const Node& r = g.nodes[c.first];
-      if (r.k == OpK::Reduce || r.k == OpK::Scan || r.k == OpK::Scatter || r.k == OpK::Conv || r.k == OpK::DotGeneral) continue;
+      if (r.k == OpK::Reduce || r.k == OpK::Scan || r.k == OpK::Scatter || is_operator(r.k) || r.k == OpK::Conv || r.k == OpK::DotGeneral) continue;
       if (r.ty.dims != g.nodes[x].ty.dims) continue;
       // the root must not be the anchor of a row group (its reductions need the full row)
       if (!row_phases(c.first).empty()) continue;
@@ -6037,7 +6108,7 @@ struct Planner {
       const int r = ctx[x].begin()->first;
       const Node& n = g.nodes[r];
       if (n.ty.rank() != 0 || !mat[r] || absorbed_roots.count(r) || reduce_of.count(r) || reshape_alias.count(r)) continue;
-      if (n.k == OpK::Param || n.k == OpK::Constant || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || n.k == OpK::Conv || n.k == OpK::DotGeneral || n.k == OpK::Reshape) continue;
+      if (n.k == OpK::Param || n.k == OpK::Constant || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || is_operator(n.k) || n.k == OpK::Conv || n.k == OpK::DotGeneral || n.k == OpK::Reshape) continue;
       reduce_of[r] = x;
       absorbed_roots.insert(r);
     }
@@ -6075,6 +6146,11 @@ struct Planner {
         jobs.push_back({x, [this, x] { emit_scatter(x); }});
         continue;
       }
+      if (n.k == OpK::OperatorResult) continue;   // written with the operator's first result
+      if (n.k == OpK::Operator) {
+        jobs.push_back({x, [this, x] { emit_operator(x); }});
+        continue;
+      }
       if (n.k == OpK::Conv) {
         if (epilogue_of.count(x)) continue;  // emitted with its root
         jobs.push_back({x, [this, x] { emit_conv(x, x); }});
@@ -6109,7 +6185,7 @@ struct Planner {
       auto plain_map_root = [&](int x) {
         const Node& n = g.nodes[x];
         if (!live[x] || !mat[x]) return false;
-        if (n.k == OpK::Param || n.k == OpK::Constant || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || n.k == OpK::Conv || n.k == OpK::DotGeneral) return false;
+        if (n.k == OpK::Param || n.k == OpK::Constant || n.k == OpK::Reduce || n.k == OpK::Scan || n.k == OpK::Scatter || is_operator(n.k) || n.k == OpK::Conv || n.k == OpK::DotGeneral) return false;
         if (reshape_alias.count(x)) return false;
         if (absorbed_roots.count(x) || !row_phases(x).empty()) return false;
         return true;
@@ -6189,7 +6265,7 @@ struct Planner {
     // row groups claim their reductions before those would be emitted on their own
     for (auto& j : jobs) {
       const Node& n = g.nodes[j.first];
-      if (n.k != OpK::Reduce && n.k != OpK::Scan && n.k != OpK::Scatter && n.k != OpK::Conv && n.k != OpK::DotGeneral && !absorbed_roots.count(j.first))
+      if (n.k != OpK::Reduce && n.k != OpK::Scan && n.k != OpK::Scatter && !is_operator(n.k) && n.k != OpK::Conv && n.k != OpK::DotGeneral && !absorbed_roots.count(j.first))
         for (int p : row_phases(j.first)) { fused_reduces.insert(p); row_anchor[p] = j.first; }
     }
     lap("job list, chains");
@@ -6215,7 +6291,7 @@ struct Planner {
         B.last_use = (int)li;
       }
     }
-    plan.source = "#include \"rx_preamble.h\"\n#include \"rx_gemm_kernels.h\"\n\n" + src.str();
+    plan.source = std::string("#include \"rx_preamble.h\"\n#include \"rx_gemm_kernels.h\"\n") + (uses_operators ? "#include \"rx_lm_kernels.h\"\n" : "") + "\n" + src.str();
   }
 };
 
@@ -6275,6 +6351,16 @@ static void count_hlo_costs(const Graph& g, Plan* plan) {
       case OpK::Conv: {
         const TType& wt = g.nodes[n.in[1]].ty;
         flops += 2.0 * numel * (double)(wt.rank() == 2 ? wt.dims[1] : wt.dims[1] * wt.dims[2] * wt.dims[3]);
+        break;
+      }
+      case OpK::Operator: {
+        OperatorSpec spec;
+        spec.name = n.op;
+        spec.attrs = n.attrs;
+        for (int i : n.in) spec.in.push_back(g.nodes[i].ty);
+        double t = 0;
+        flops += operator_flops(spec, &t);
+        trans += t;
         break;
       }
       case OpK::Reduce: case OpK::Scan: flops += (double)g.nodes[n.in[0]].ty.numel(); break;

@@ -48,9 +48,9 @@ constexpr uint64_t kWorkerMagic = 0x5258525443454e44;
 // 0 and the code object, or non-zero and the error text.
 static int hiprtc_compile(const std::string& source, const std::string& arch, std::string* out) {
   hiprtcProgram prog;
-  const char* hdr_src[] = {kRxPreambleSrc, kRxGemmKernelsSrc};
-  const char* hdr_name[] = {"rx_preamble.h", "rx_gemm_kernels.h"};
-  hiprtcResult r = hiprtcCreateProgram(&prog, source.c_str(), "rx_module.hip", 2, hdr_src, hdr_name);
+  const char* hdr_src[] = {kRxPreambleSrc, kRxGemmKernelsSrc, kRxLmKernelsSrc};
+  const char* hdr_name[] = {"rx_preamble.h", "rx_gemm_kernels.h", "rx_lm_kernels.h"};
+  hiprtcResult r = hiprtcCreateProgram(&prog, source.c_str(), "rx_module.hip", 3, hdr_src, hdr_name);
   if (r != HIPRTC_SUCCESS) {
     *out = std::string("hiprtcCreateProgram: ") + hiprtcGetErrorString(r);
     return 1;
