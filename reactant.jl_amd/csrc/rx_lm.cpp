@@ -273,6 +273,7 @@ void check_attention(const Checker& c) {
   c.number("scale", 1.0);
   c.require(c.integer("window", 0) >= 0, "the window must not be negative");
   c.require(B <= 65535 && Hq <= 65535, "too many sequences or heads");
+  c.require(B * Hq * std::max<int64_t>(vc.dim, 1) <= kMaxRow, "too many sequences and heads");
 }
 OperatorPlan plan_attention(const OperatorSpec& s) {
   const Checker c{s};
@@ -283,19 +284,41 @@ OperatorPlan plan_attention(const OperatorSpec& s) {
   const double scale = c.number("scale", 1.0 / std::sqrt((double)kc.dim));
   const int64_t window = std::min<int64_t>(c.integer("window", 0), kMaxRow);
   const bool lse = s.out.size() == 2;
+  const int64_t G = Hq / kc.heads, NT = G > 16 ? 2 : 1, tiles = (G + 16 * NT - 1) / (16 * NT), columns = kc.heads * tiles, GT = std::min(G, 16 * NT);
+  const int64_t items = 512;   // two workgroups per compute unit
+  // positions of a sequence from the multiple of 128 below its first: chunks of 128 and more
+  const int64_t longest = window ? std::min(M * kc.slots, window + 127) : M * kc.slots;
+  const bool join = longest > 128;
+  const int64_t grid = join ? std::min(items + B * columns, B * columns * ((longest + 127) / 128)) : B * columns;
   OperatorPlan p;
   std::vector<std::pair<OperatorArg, std::string>> args;
   for (int i = 0; i < 5; ++i) args.push_back({operand(i), st(in[i])});
   args.push_back({result(0), st(s.out[0])});
   if (lse) args.push_back({result(1), "float"});
+  if (join) {
+    p.scratch = {grid * GT * vc.dim * 4, grid * GT * 8};
+    args.push_back({scratch(0), "float"});
+    args.push_back({scratch(1), "float"});
+  }
+  const std::string sizes = num(kc.slots) + ", " + num(B) + ", " + num(M) + ", " + num(window) + ", ";
+  const std::string heads = std::string(elem(in[0].dt)) + ", " + num(Hq) + ", " + num(kc.heads) + ", ";
   std::ostringstream b;
-  b << "rx_paged_attention<" << elem(in[0].dt) << ", " << Hq << ", " << kc.heads << ", " << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << kc.slots << ", " << M << ", " << window << ", "
-    << (by_slot ? "true" : "false") << ">(a0, a1, a2, a3, a4, a5, " << (lse ? "a6" : "(float*)0") << ", " << flt(scale) << ");";
-  OperatorKernel k = kernel(s, "paged_attention", 64, args, lse ? 2 : 1, b.str());
-  k.grid[0] = (unsigned)Hq;
-  k.grid[1] = (unsigned)B;
-  k.bytes = 2.0 * (double)in[0].bytes();
+  b << "rx_paged_attention<" << heads << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << sizes << (by_slot ? "true" : "false") << ", " << NT << ", " << items << ", "
+    << (join ? "true" : "false") << ">(a0, a1, a2, a3, a4, a5, " << (lse ? "a6" : "(float*)0") << ", " << (join ? (lse ? "a7, a8" : "a6, a7") : "(float*)0, (float*)0") << ", "
+    << flt(scale * 1.4426950408889634) << ");";
+  OperatorKernel k = kernel(s, "paged_attention", 256, args, (int)args.size() - 5, b.str());
+  k.grid[0] = (unsigned)grid;
+  k.bytes = 2.0 * (double)in[0].bytes();   // (and what the lengths make of the caches)
   p.kernels.push_back(k);
+  if (join) {
+    args = {{operand(4), st(in[4])}, {scratch(0), "float"}, {scratch(1), "float"}, {result(0), st(s.out[0])}};
+    if (lse) args.push_back({result(1), "float"});
+    OperatorKernel j = kernel(s, "paged_attention_join", 256, args, lse ? 2 : 1,
+                              "rx_paged_attention_join<" + heads + num(vc.dim) + ", " + sizes + num(NT) + ", " + num(items) + ">(a0, a1, a2, a3, " + (lse ? "a4" : "(float*)0") + ");");
+    j.grid[0] = (unsigned)Hq;
+    j.grid[1] = (unsigned)B;
+    p.kernels.push_back(j);
+  }
   return p;
 }
 
