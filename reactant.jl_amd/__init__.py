@@ -558,6 +558,12 @@ class ConcreteRArray:
             raise ReactantInternalError("accessing the data of a donated array")  # src/Types.jl:9-26
         return self.data.synced_buffer()
 
+    def _operand(self):
+        """The buffer as an argument of an execution, which is not waited for: a device's work is ordered on one stream."""
+        if self.donated:
+            raise ReactantInternalError("accessing the data of a donated array")  # src/Types.jl:9-26
+        return self.data.buffer
+
     def to_array(self):
         """Array(x): numbers in Julia index order (float32 for narrow floats)."""
         raw = self._buffer().to_host()
@@ -669,7 +675,7 @@ class Thunk:
         self.client = client
 
     def __call__(self, *args, donated=None, sync=False):
-        bufs = [a._buffer() for a in args]
+        bufs = [a._operand() for a in args]
         res = self.exec.execute_sharded(bufs, donated)
         if donated:
             for a, d in zip(args, donated):

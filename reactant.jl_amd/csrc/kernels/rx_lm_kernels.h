@@ -33,38 +33,226 @@ RX_DEV float rx_lm_inf() { return __builtin_inff(); }
 template <typename E, int V, int D, int T, int VEC, typename I>
 RX_DEV void rx_embedding(const typename E::S* table, const I* ids, typename E::S* out, const float scale) {
   constexpr int C = D / VEC;   // vectors of a row
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long long)T * C) return;
-  const int t = (int)(i / C), c = (int)(i % C);
-  const I id = ids[t];
-  rx_vec<typename E::S, VEC> x{};
-  if (id >= 0 && id < V) {
-    x = rx_load<rx_vec<typename E::S, VEC>>(table + (long long)id * D + c * VEC);
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)T * C; i += (long long)gridDim.x * 256) {
+    const int t = (int)(i / C), c = (int)(i % C);
+    const I id = ids[t];
+    rx_vec<typename E::S, VEC> x{};
+    if (id >= 0 && id < V) {
+      x = rx_load<rx_vec<typename E::S, VEC>>(table + (long long)id * D + c * VEC);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) x.v[k] = E::down(E::up(x.v[k]) * scale);
+      for (int k = 0; k < VEC; ++k) x.v[k] = E::down(E::up(x.v[k]) * scale);
+    }
+    rx_store(out + (long long)t * D + c * VEC, x);
   }
-  rx_store(out + (long long)t * D + c * VEC, x);
 }
 
-// gradient: a workgroup per row of the table, which goes through the tokens
-template <typename E, typename O, int D, int T, typename I>
-RX_DEV void rx_embedding_grad(const typename E::S* dy, const I* ids, typename O::S* out, const float scale) {
-  const int row = blockIdx.x;
-  __shared__ int found[256];
-  for (int c0 = 0; c0 < D; c0 += 256) {
-    const int c = c0 + (int)threadIdx.x;
-    float sum = 0.0f;
+// Gradient.  The tokens are sorted by row, in their order within a row, by one launch without exchange between workgroups: a
+// workgroup has the counters of ROWS rows in LDS and goes through all tokens twice.  The first time it counts its rows' tokens,
+// for every wavefront's stretch of the tokens apart, and the tokens of rows before its own, which is where its part of the
+// sorted list starts; the second time every wavefront puts its tokens into their places.  All counts are whole numbers, so the
+// list is the same every run.  `start` [V + 1] is where a row's tokens start in `order`; `row_of` is the row of a place.
+template <int V, int T, int ROWS, typename I>
+RX_DEV void rx_lm_sort(const I* ids, int* start, int* order, int* row_of) {
+  constexpr int WAVES = 16, STRETCH = ((T + WAVES - 1) / WAVES + 63) / 64 * 64;
+  __shared__ int counts[WAVES][ROWS], sums[WAVES];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r0 = blockIdx.x * ROWS, t0 = wave * STRETCH, t1 = t0 + STRETCH < T ? t0 + STRETCH : T;
+  for (int k = threadIdx.x; k < WAVES * ROWS; k += 1024) counts[k / ROWS][k % ROWS] = 0;
+  __syncthreads();
+  int below = 0;
+#pragma unroll 4
+  for (int t = t0 + lane; t < t1; t += 64) {
+    const I id = ids[t];
+    if (id >= 0 && id < V) {
+      if (id < r0) ++below;
+      else if (id < (long long)r0 + ROWS) atomicAdd(&counts[wave][(int)id - r0], 1);
+    }
+  }
+  below = rx_wave_reduce(below, rx_op_add());
+  if (lane == 0) sums[wave] = below;
+  __syncthreads();
+  below = 0;
+  for (int w = 0; w < WAVES; ++w) below += sums[w];
+  __syncthreads();
+  // places: rows one after the other, a row's stretches one after the other
+  int carry = below;
+  for (int k0 = 0; k0 < ROWS; k0 += 1024) {
+    const int k = k0 + (int)threadIdx.x;
+    int total = 0;
+    if (k < ROWS)
+      for (int w = 0; w < WAVES; ++w) total += counts[w][k];
+    const int upto = rx_wave_scan(total, rx_op_add());
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int at = carry + upto - total;
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) at += sums[w];
+      carry += sums[w];
+    }
+    if (k < ROWS) {
+      if (r0 + k < V) start[r0 + k] = at;
+      for (int w = 0; w < WAVES; ++w) {
+        const int n = counts[w][k];
+        counts[w][k] = at;
+        at += n;
+      }
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0 && r0 + ROWS >= V) start[V] = carry;
+#pragma unroll 4
+  for (int t = t0 + lane; t < t0 + STRETCH; t += 64) {           // (whole wavefronts: the lanes compare their rows)
+    const I id = t < t1 ? ids[t] : (I)-1;
+    const bool mine = id >= r0 && id < (long long)r0 + ROWS && id < V;
+    const int row = mine ? (int)id - r0 : -1;
+    unsigned long long left = __ballot(mine);
+    while (left) {
+      const int leader = __builtin_ctzll(left), its = __builtin_amdgcn_readlane(row, leader);
+      const unsigned long long same = __ballot(row == its);
+      int place = 0;
+      if (lane == leader) place = atomicAdd(&counts[wave][its], __popcll(same));
+      place = __builtin_amdgcn_readlane(place, leader) + __popcll(same & ((1ull << lane) - 1));
+      if (row == its) {
+        order[place] = t;
+        row_of[place] = (int)id;
+      }
+      left &= ~same;
+    }
+  }
+}
+
+template <long long N, typename S>
+RX_DEV void rx_lm_zero(S* out) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < N; i += (long long)gridDim.x * 256) out[i] = (S)0;
+}
+template <int N>
+struct rx_lm_acc { float v[N]; };
+template <typename E, int D, int VEC>
+RX_DEV void rx_lm_sum_rows(const typename E::S* dy, const int* order, int from, const int to, const int c, rx_lm_acc<VEC>& a) {
+  typedef rx_vec<typename E::S, VEC> W;
+  for (; from + 8 <= to; from += 8) {
+    W w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = rx_load<W>(dy + (long long)order[from + k] * D + c * VEC);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) a.v[e] += E::up(w[k].v[e]);
+  }
+  for (; from < to; ++from) {
+    const W w = rx_load<W>(dy + (long long)order[from] * D + c * VEC);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) a.v[e] += E::up(w.v[e]);
+  }
+}
+template <typename O, int VEC>
+RX_DEV void rx_lm_put(typename O::S* out, const rx_lm_acc<VEC>& a, const float scale) {
+  rx_vec<typename O::S, VEC> w;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) w.v[e] = O::down(a.v[e] * scale);
+  if constexpr (sizeof(w) > 16) {
+    const auto* p = (const rx_vec<typename O::S, 16 / sizeof(typename O::S)>*)&w;
+#pragma unroll
+    for (unsigned k = 0; k < sizeof(w) / 16; ++k) rx_store_nt(out + k * (16 / sizeof(typename O::S)), p[k]);
+  } else {
+    rx_store_nt(out, w);
+  }
+}
+
+// Rows of up to LONG tokens: a thread per vector of the table sums its row's tokens, in their order.  A row of more would keep
+// one thread's loads waiting for one another: those are summed in pieces, the places [LONG p, LONG p + LONG) of the list by
+// the first workgroups (a piece touches at most two such rows: it may end one and start another), and joined by the next launch.
+template <typename E, typename O, int V, int D, int T, int VEC, int LONG, bool PIECES>
+RX_DEV void rx_embedding_grad_rows(const typename E::S* dy, const int* start, const int* order, const int* row_of, typename O::S* out, float* part, const float scale) {
+  constexpr int C = D / VEC, TILES = (C + 255) / 256, NP = PIECES ? (T + LONG - 1) / LONG : 0;
+  if (PIECES && blockIdx.x < NP * TILES) {
+    const int piece = blockIdx.x / TILES, c = blockIdx.x % TILES * 256 + (int)threadIdx.x, all = start[V];
+    const int a = piece * LONG, e = a + LONG < all ? a + LONG : all;
+    if (a >= e || c >= C) return;
+    const int first = row_of[a], last = row_of[e - 1];
+    for (int k = 0; k < 2; ++k) {
+      const int row = k ? last : first;
+      if (k && last == first) break;
+      const int s0 = start[row], s1 = start[row + 1];
+      if (s1 - s0 <= LONG) continue;
+      rx_lm_acc<VEC> sum = {};
+      rx_lm_sum_rows<E, D, VEC>(dy, order, s0 > a ? s0 : a, s1 < e ? s1 : e, c, sum);
+      *(rx_lm_acc<VEC>*)(part + ((long long)(piece * 2 + k) * C + c) * VEC) = sum;
+    }
+    return;
+  }
+  const long long grid = (long long)(gridDim.x - NP * TILES) * 256;
+  for (long long i = (long long)(blockIdx.x - NP * TILES) * 256 + threadIdx.x; i < (long long)V * C; i += grid) {
+    const int row = (int)(i / C), c = (int)(i % C), s0 = start[row], s1 = start[row + 1];
+    if (PIECES && s1 - s0 > LONG) continue;
+    rx_lm_acc<VEC> sum = {};
+    rx_lm_sum_rows<E, D, VEC>(dy, order, s0, s1, c, sum);
+    rx_lm_put<O, VEC>(out + i * VEC, sum, scale);
+  }
+}
+// the rows of more than LONG tokens: by the workgroup of the piece that such a row starts in, its pieces in their order
+template <typename E, typename O, int V, int D, int T, int VEC, int LONG>
+RX_DEV void rx_embedding_grad_join(const int* start, const int* row_of, const float* part, typename O::S* out, const float scale) {
+  constexpr int C = D / VEC, TILES = (C + 255) / 256;
+  const int piece = blockIdx.x / TILES, c = blockIdx.x % TILES * 256 + (int)threadIdx.x, all = start[V];
+  const int a = piece * LONG, e = a + LONG < all ? a + LONG : all;
+  if (a >= e || c >= C) return;
+  const int row = row_of[e - 1], s0 = start[row], s1 = start[row + 1];
+  if (s1 - s0 <= LONG || s0 < a) return;
+  rx_lm_acc<VEC> sum = *(const rx_lm_acc<VEC>*)(part + ((long long)(piece * 2 + (row_of[a] != row)) * C + c) * VEC);
+#pragma unroll 4
+  for (int p = piece + 1; p * LONG < s1; ++p) {
+    const rx_lm_acc<VEC> next = *(const rx_lm_acc<VEC>*)(part + ((long long)p * 2 * C + c) * VEC);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sum.v[k] += next.v[k];
+  }
+  rx_lm_put<O, VEC>(out + ((long long)row * C + c) * VEC, sum, scale);
+}
+
+// Few tokens (FEW at most): one launch, without sorting.  A workgroup takes rows of 256 vectors together, lists the tokens of
+// these rows as it goes through all of them (a wavefront's matches in the order of its lanes, the wavefronts' one after the
+// other), and every thread sums the listed tokens of its row.
+template <typename E, typename O, int V, int D, int T, int VEC, typename I>
+RX_DEV void rx_embedding_grad_few(const typename E::S* dy, const I* ids, typename O::S* out, const float scale) {
+  constexpr int C = D / VEC;
+  __shared__ int found[T], of[T], sums[4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (long long i0 = (long long)blockIdx.x * 256; i0 < (long long)V * C; i0 += (long long)gridDim.x * 256) {
+    const long long i1 = i0 + 255 < (long long)V * C ? i0 + 255 : (long long)V * C - 1;
+    const int r0 = (int)(i0 / C), r1 = (int)(i1 / C);
+    int n = 0;
     for (int t0 = 0; t0 < T; t0 += 256) {
       const int t = t0 + (int)threadIdx.x;
-      const bool hit = t < T && ids[t] == row;
-      if (!__syncthreads_or(hit)) continue;
-      found[threadIdx.x] = hit;
+      const I id = t < T ? ids[t] : (I)-1;
+      const bool mine = id >= r0 && id <= r1;
+      const unsigned long long hits = __ballot(mine);
       __syncthreads();
-      for (int k = 0; k < 256; ++k)
-        if (found[k] && c < D) sum += E::up(dy[(long long)(t0 + k) * D + c]);
+      if (lane == 0) sums[wave] = __popcll(hits);
       __syncthreads();
+      int at = n;
+      for (int w = 0; w < 4; ++w) {
+        if (w < wave) at += sums[w];
+        n += sums[w];
+      }
+      if (mine) {
+        at += __popcll(hits & ((1ull << lane) - 1));
+        found[at] = t;
+        of[at] = (int)id;
+      }
     }
-    if (c < D) out[(long long)row * D + c] = O::down(sum * scale);
+    __syncthreads();
+    const long long i = i0 + threadIdx.x;
+    if (i <= i1) {
+      const int row = (int)(i / C), c = (int)(i % C);
+      rx_lm_acc<VEC> sum = {};
+      for (int k = 0; k < n; ++k)
+        if (of[k] == row) {
+          const auto w = rx_load<rx_vec<typename E::S, VEC>>(dy + (long long)found[k] * D + c * VEC);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) sum.v[e] += E::up(w.v[e]);
+        }
+      rx_lm_put<O, VEC>(out + i * VEC, sum, scale);
+    }
+    __syncthreads();
   }
 }
 
@@ -77,7 +265,8 @@ RX_DEV long long rx_lm_slot(long long page, int slot, int head) {
   return BY_SLOT ? ((page * S + slot) * H + head) * D : ((page * H + head) * S + slot) * D;
 }
 
-// one element of a head after rotation: x cos - y sin for the first of a pair, y cos + x sin for the second
+// One element of a head after rotation: x cos - y sin for the first of a pair, y cos + x sin for the second.  The products are
+// rounded, then their sum: `x * c - y * s` in f32.
 template <typename E, int R2, bool PAIRS>
 RX_DEV float rx_lm_rotated(const typename E::S* head, int d, const float* cos, const float* sin) {
   const float x = E::up(head[d]);
@@ -88,24 +277,107 @@ RX_DEV float rx_lm_rotated(const typename E::S* head, int d, const float* cos, c
   return second ? x * cos[a] + y * sin[a] : x * cos[a] - y * sin[a];
 }
 
-// a workgroup per token
-template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int L, int R2, bool PAIRS, bool BY_SLOT, typename I>
+// where a token goes: its position, and the slot's page and number (page -1: nowhere)
+struct rx_lm_place { long long pos; int page, slot; bool known; };
+template <int P, int S, int B, int M, int L, int R2, typename I>
+RX_DEV rx_lm_place rx_lm_place_of(const I* position, const I* sequence, const I* pages, const long long t) {
+  const I pos = position[t], seq = sequence[t];
+  rx_lm_place p = {0, -1, 0, pos >= 0 && pos < (R2 && L < (long long)M * S ? (long long)L : (long long)M * S) && seq >= 0 && seq < B};
+  if (!p.known) return p;
+  p.pos = pos;
+  const I page = pages[(long long)seq * M + (int)pos / S];
+  p.page = page >= 0 && page < P ? (int)page : -1;
+  p.slot = (int)pos % S;
+  return p;
+}
+
+// heads of any width: a workgroup per token
+template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int L, int R2, bool PAIRS, bool BY_SLOT, int T, typename I>
+RX_DEV void rx_kv_append_any(const typename E::S* q, const typename E::S* k, const typename E::S* v, const float* cos, const float* sin, const I* position, const I* sequence,
+                             const I* pages, typename E::S* qo, typename E::S* kc, typename E::S* vc) {
+  for (long long t = blockIdx.x; t < T; t += gridDim.x) {
+    const rx_lm_place p = rx_lm_place_of<P, S, B, M, L, R2>(position, sequence, pages, t);
+    const float* c = cos + p.pos * R2;
+    const float* s = sin + p.pos * R2;
+    for (int i = threadIdx.x; i < HQ * DK; i += 256)
+      qo[t * (HQ * DK) + i] = p.known ? E::down(rx_lm_rotated<E, R2, PAIRS>(q + t * (HQ * DK) + i / DK * DK, i % DK, c, s)) : E::down(0.0f);
+    if (p.page < 0) continue;
+    for (int i = threadIdx.x; i < HK * DK; i += 256)
+      kc[rx_lm_slot<S, HK, DK, BY_SLOT>(p.page, p.slot, i / DK) + i % DK] = E::down(rx_lm_rotated<E, R2, PAIRS>(k + t * (HK * DK) + i / DK * DK, i % DK, c, s));
+    for (int i = threadIdx.x; i < HK * DV; i += 256) vc[rx_lm_slot<S, HK, DV, BY_SLOT>(p.page, p.slot, i / DV) + i % DV] = v[t * (HK * DV) + i];
+  }
+}
+
+// Heads of whole vectors: a thread takes the same dimensions of HEADS heads of a token (their cosines and sines are loaded
+// once): the two vectors of a rotated stretch of pairs, or one vector that is not rotated, or whose pairs are inside of it.
+template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int L, int R2, bool PAIRS, bool BY_SLOT, int T, int HEADS, typename I>
 RX_DEV void rx_kv_append(const typename E::S* q, const typename E::S* k, const typename E::S* v, const float* cos, const float* sin, const I* position, const I* sequence,
                          const I* pages, typename E::S* qo, typename E::S* kc, typename E::S* vc) {
-  const long long t = blockIdx.x;
-  const I pos = position[t], seq = sequence[t];
-  const bool known = pos >= 0 && pos < (R2 ? (long long)L : (long long)M * S) && pos < (long long)M * S && seq >= 0 && seq < B;
-  const float* c = cos + (known ? (long long)pos * R2 : 0);
-  const float* s = sin + (known ? (long long)pos * R2 : 0);
-  for (int i = threadIdx.x; i < HQ * DK; i += 256)
-    qo[t * (HQ * DK) + i] = known ? E::down(rx_lm_rotated<E, R2, PAIRS>(q + t * (HQ * DK) + i / DK * DK, i % DK, c, s)) : E::down(0.0f);
-  if (!known) return;
-  const I page = pages[(long long)seq * M + pos / S];
-  if (page < 0 || page >= P) return;
-  const int slot = (int)(pos % S);
-  for (int i = threadIdx.x; i < HK * DK; i += 256)
-    kc[rx_lm_slot<S, HK, DK, BY_SLOT>(page, slot, i / DK) + i % DK] = E::down(rx_lm_rotated<E, R2, PAIRS>(k + t * (HK * DK) + i / DK * DK, i % DK, c, s));
-  for (int i = threadIdx.x; i < HK * DV; i += 256) vc[rx_lm_slot<S, HK, DV, BY_SLOT>(page, slot, i / DV) + i % DV] = v[t * (HK * DV) + i];
+  typedef typename E::S X;
+  constexpr int NE = 16 / sizeof(X);
+  typedef rx_vec<X, NE> W;
+  constexpr int TURNED = PAIRS ? 2 * R2 / NE : R2 / NE, UNITS = TURNED + (DK - 2 * R2) / NE;   // of a head: rotated ones first
+  constexpr int GQ = (HQ + HEADS - 1) / HEADS, GK = (HK + HEADS - 1) / HEADS, VV = (HK * DV / NE + HEADS - 1) / HEADS;
+  constexpr int ALL = (GQ + GK) * UNITS + VV;                                                     // threads of a token
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)T * ALL; i += (long long)gridDim.x * 256) {
+    const long long t = i / ALL;
+    const int u = (int)(i % ALL);
+    const rx_lm_place p = rx_lm_place_of<P, S, B, M, L, R2>(position, sequence, pages, t);
+    if (u >= (GQ + GK) * UNITS) {                                                                 // values
+#pragma unroll
+      for (int h = 0; h < HEADS; ++h) {
+        const int w = (u - (GQ + GK) * UNITS) + h * VV, head = w / (DV / NE), d = w % (DV / NE) * NE;
+        if (w >= HK * DV / NE) break;
+        const W x = rx_load<W>(v + t * (HK * DV) + head * DV + d);
+        if (p.page >= 0) rx_store(vc + rx_lm_slot<S, HK, DV, BY_SLOT>(p.page, p.slot, head) + d, x);
+      }
+      continue;
+    }
+    const int group = u / UNITS, n = u % UNITS;
+    const bool query = group < GQ;
+    const bool turned = n < TURNED;
+    const int d = turned ? n * NE : 2 * R2 + (n - TURNED) * NE;                                   // first dimension
+    float c[NE] = {}, s[NE] = {};
+    if (R2 && L && turned) {
+      const long long at = p.pos * R2 + (PAIRS ? d / 2 : d);
+#pragma unroll
+      for (int e = 0; e < (PAIRS ? NE / 2 : NE); ++e) {
+        c[e] = cos[at + e];
+        s[e] = sin[at + e];
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      const int head = (query ? group : group - GQ) * HEADS + h;
+      if (head >= (query ? HQ : HK)) break;
+      const X* x = query ? q + (t * HQ + head) * DK + d : k + (t * HK + head) * DK + d;
+      X* y = query ? qo + (t * HQ + head) * DK + d : kc + rx_lm_slot<S, HK, DK, BY_SLOT>(p.page < 0 ? 0 : p.page, p.slot, head) + d;
+      W a = rx_load<W>(x), b{};
+      if (R2 && turned) {
+        if constexpr (PAIRS) {
+#pragma unroll
+          for (int e = 0; e < NE; e += 2) {
+            const float f = E::up(a.v[e]), g = E::up(a.v[e + 1]);
+            a.v[e] = E::down(f * c[e / 2] - g * s[e / 2]);
+            a.v[e + 1] = E::down(g * c[e / 2] + f * s[e / 2]);
+          }
+        } else {
+          b = rx_load<W>(x + R2);
+#pragma unroll
+          for (int e = 0; e < NE; ++e) {
+            const float f = E::up(a.v[e]), g = E::up(b.v[e]);
+            a.v[e] = E::down(f * c[e] - g * s[e]);
+            b.v[e] = E::down(g * c[e] + f * s[e]);
+          }
+        }
+      }
+      if (query && !p.known) a = b = W{};
+      if (query || p.page >= 0) {
+        rx_store(y, a);
+        if (!PAIRS && R2 && turned) rx_store(y + R2, b);
+      }
+    }
+  }
 }
 
 // ---- attention of one token per sequence ----
@@ -459,68 +731,295 @@ RX_DEV rx_u32 rx_lm_order(float x) {
   const rx_u32 u = rx_f2u(x + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+RX_DEV float rx_lm_unorder(rx_u32 o) { return rx_u2f(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 RX_DEV rx_u64 rx_lm_key(float x, int j) { return ((rx_u64)rx_lm_order(x) << 32) | (rx_u32)~j; }
 
-// a workgroup per row
-template <typename E, int V, int K, typename I>
-RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, float* logprob, float* lse, float* entropy, float* values, int* ids) {
-  const long long t = blockIdx.x;
-  const typename E::S* x = logits + t * V;
-  __shared__ float red[4];
-  __shared__ rx_u64 red64[4];
-  float m = -rx_lm_inf();
-  for (int j = threadIdx.x; j < V; j += 256) m = rx_max(m, E::up(x[j]));
-  m = rx_block_reduce<float, rx_op_max, 4>(m, rx_op_max(), red);
-  float s = 0.0f, sx = 0.0f;
-  if (m != -rx_lm_inf())
-    for (int j = threadIdx.x; j < V; j += 256) {
-      const float v = E::up(x[j]);
-      const float e = expf(v - m);
-      s += e;
-      if (v != -rx_lm_inf()) sx += e * (v - m);
+// A row of V elements as vectors of 16 bytes that are aligned in memory: vector v holds the elements [v NE - off, v NE - off + NE),
+// off being how far the row starts inside of a vector.  The vectors at both ends may reach over the row.
+template <typename E, int V>
+struct rx_lm_row {
+  typedef typename E::S S;
+  static constexpr int NE = 16 / sizeof(S), SHIFTS = V % NE ? 1 : 0, VECTORS = (V + NE - 1) / NE + SHIFTS;
+  const S* x;
+  int off;
+  const rx_vec<S, NE>* vectors;   // counted from the tensor's start: a uniform load's address is made of aligned parts (a scalar load drops the low bits of each part)
+  RX_MEM rx_lm_row(const S* all, const long long t)
+      : x(all + t * V), off(SHIFTS ? (int)((t * (V % NE)) % NE) : 0), vectors((const rx_vec<S, NE>*)all + (t * V - off) / NE) {}
+  RX_MEM int first(const int v) const { return v * NE - off; }
+  RX_MEM bool whole(const int v) const { return V >= 2 * NE && v * NE >= off && (v + 1) * NE - off <= V; }
+  // the whole vector nearest to v, so that the loads of a loop carry no conditions; get() corrects those at the ends
+  RX_MEM rx_vec<S, NE> load(const int v) const {
+    if constexpr (V >= 2 * NE) {
+      const int lo = off > 0 ? 1 : 0, hi = (V + off) / NE - 1;
+      return vectors[v < lo ? lo : v > hi ? hi : v];
+    } else {
+      return rx_vec<S, NE>{};
     }
-  __syncthreads();
-  s = rx_block_reduce<float, rx_op_add, 4>(s, rx_op_add(), red);
-  __syncthreads();
-  sx = rx_block_reduce<float, rx_op_add, 4>(sx, rx_op_add(), red);
-  const float l = s == 0.0f ? -rx_lm_inf() : m + logf(s);
-  if (threadIdx.x == 0) {
-    const I y = targets[t];
-    lse[t] = l;
-    entropy[t] = s == 0.0f ? 0.0f : logf(s) - sx / s;
-    logprob[t] = y < 0 || y >= V ? 0.0f : s == 0.0f ? -rx_lm_inf() : E::up(x[y]) - l;
   }
-  rx_u64 below = ~0ull;   // keys from here on have been taken
-  for (int k = 0; k < K; ++k) {
-    rx_u64 best = 0;
-    for (int j = threadIdx.x; j < V; j += 256) {
-      const rx_u64 key = rx_lm_key(E::up(x[j]), j);
-      if (key < below && key > best) best = key;
+  RX_MEM void get(const rx_vec<S, NE>& r, const int v, const float fill, float (&e)[NE]) const {
+#pragma unroll
+    for (int k = 0; k < NE; ++k) e[k] = E::up(r.v[k]);
+    if (!whole(v)) {
+#pragma unroll
+      for (int k = 0; k < NE; ++k) e[k] = first(v) + k >= 0 && first(v) + k < V ? E::up(x[first(v) + k]) : fill;
     }
-    __syncthreads();
-    best = rx_block_reduce<rx_u64, rx_op_max, 4>(best, rx_op_max(), red64);
-    if (threadIdx.x == 0) {
-      const int j = (int)~(rx_u32)best;
-      ids[t * K + k] = j;
-      values[t * K + k] = s == 0.0f ? -rx_lm_inf() : E::up(x[j]) - l;
-    }
-    below = best;
+  }
+};
+
+// running (maximum, sum of e^(x - maximum), sum of e^(x - maximum) log2 e^(x - maximum)): of the sums, the second gives the entropy
+struct rx_lm_sums { float m, s, t; };
+RX_DEV rx_lm_sums rx_lm_rebase(const rx_lm_sums a, const float m) {
+  if (a.m == m || a.m == -rx_lm_inf()) return {m, a.s, a.t};   // (nothing so far: the sums are 0, or NaN)
+  const float d = (a.m - m) * RX_LM_LOG2E, f = __builtin_amdgcn_exp2f(d);
+  return {m, a.s * f, f == 0.0f ? 0.0f : (a.t + a.s * d) * f};
+}
+struct rx_op_lm_sums {
+  RX_MEM rx_lm_sums operator()(const rx_lm_sums& a, const rx_lm_sums& b) const {
+    const float m = __builtin_fmaxf(a.m, b.m);
+    const rx_lm_sums x = rx_lm_rebase(a, m), y = rx_lm_rebase(b, m);
+    return {m, x.s + y.s, x.t + y.t};
+  }
+};
+
+// the K largest of `n` keys in LDS (n up to what the caller holds), the i-th largest given to put(i, key)
+template <int K, typename F>
+RX_DEV void rx_lm_select(const rx_u64* keys, const int n, F put) {
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const rx_u64 mine = keys[i];
+    int rank = 0;
+    for (int k = 0; k < n; ++k) rank += keys[k] > mine;
+    if (rank < K) put(rank, mine);
   }
 }
 
-// d x_j = g (delta_jy - p_j) - h p_j (x_j - lse + H): a workgroup per row
+// log probability, lse and entropy of a row, and the K largest keys in `best`, from the row's sums
 template <typename E, int V, typename I>
+RX_DEV void rx_lm_row_results(const long long t, const rx_lm_sums a, const typename E::S* x, const I* targets, float* logprob, float* lse, float* entropy) {
+  const I y = targets[t];
+  const float log2s = __builtin_log2f(a.s);
+  const float l = a.s == 0.0f ? -rx_lm_inf() : a.m + log2s * 0.6931471805599453f;
+  lse[t] = l;
+  entropy[t] = a.s == 0.0f ? 0.0f : (log2s - a.t / a.s) * 0.6931471805599453f;
+  logprob[t] = y < 0 || y >= V ? 0.0f : a.s == 0.0f ? -rx_lm_inf() : E::up(x[y]) - l;
+}
+
+// A workgroup per segment of SEG vectors of a row (SPLIT segments; one: the whole row): one pass with the running sums, and the
+// alternatives without a second one.  Every thread keeps its largest vector's maximum.  With k alternatives asked for, the
+// k-th largest of the maxima of 64 groups of threads bounds the k-th largest element from below, so only threads whose own
+// maximum reaches it hold alternatives: their elements (a few per cent of the row) are read again, and the few that reach the
+// bound are ranked.  Bounds and elements compare by (value, index), so rows of equal values need no more.  Rows with a NaN, or
+// where more than CAP elements reach the bound (the largest elements all at one thread), are searched k times.
+template <typename E, int V, int K, int T, int SPLIT, typename I>
+RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, float* logprob, float* lse, float* entropy, float* values, int* ids, float* part_sums, rx_u64* part_keys) {
+  typedef typename E::S S;
+  constexpr int NE = 16 / sizeof(S), UNROLL = 4, CAP = 2048, VECTORS = rx_lm_row<E, V>::VECTORS;
+  __shared__ rx_lm_sums red[4];
+  __shared__ rx_u64 group[64], keys[K ? CAP : 1], bound, red64[4];
+  __shared__ int count, listed[256];
+  for (long long item = blockIdx.x; item < (long long)T * SPLIT; item += gridDim.x) {
+    const long long t = item / SPLIT;
+    const int seg = (int)(item % SPLIT), v0 = (int)((long long)VECTORS * seg / SPLIT), v1 = (int)((long long)VECTORS * (seg + 1) / SPLIT);
+    const rx_lm_row<E, V> row(logits, t);
+    rx_lm_sums a = {-rx_lm_inf(), 0.0f, 0.0f};
+    float best = -rx_lm_inf();
+    int best_at = 0x7fffffff;                                  // vector
+    for (int v = v0 + (int)threadIdx.x; v < v1; v += 256 * UNROLL) {
+      rx_vec<S, NE> r[UNROLL];
+      float e[UNROLL][NE], top[UNROLL];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) r[u] = row.load(v + 256 * u);
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        row.get(r[u], v + 256 * u, -rx_lm_inf(), e[u]);
+        if (SPLIT > 1 && v + 256 * u >= v1) {
+#pragma unroll
+          for (int k = 0; k < NE; ++k) e[u][k] = -rx_lm_inf();
+        }
+        top[u] = e[u][0];
+#pragma unroll
+        for (int k = 1; k < NE; ++k) top[u] = __builtin_fmaxf(top[u], e[u][k]);
+        if constexpr (K > 0) {
+          if (v + 256 * u < v1 && (top[u] > best || best_at == 0x7fffffff)) {
+            best = top[u];
+            best_at = v + 256 * u;
+          }
+        }
+      }
+      float m = a.m;
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) m = __builtin_fmaxf(m, top[u]);
+      if (m > a.m) a = rx_lm_rebase(a, m);
+      const float base = a.m == -rx_lm_inf() ? 0.0f : a.m;
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+        for (int k = 0; k < NE; ++k) {
+          const float d = (e[u][k] - base) * RX_LM_LOG2E, p = __builtin_amdgcn_exp2f(d);
+          a.s += p;
+          a.t = __builtin_fmaf(p, __builtin_fmaxf(d, -1e30f), a.t);   // (0 times -inf is no 0)
+        }
+    }
+    // the workgroup's sums
+    {
+      const float m = rx_wave_reduce(a.m, rx_op_max());
+      a = rx_lm_rebase(a, m);
+      a.s = rx_wave_reduce(a.s, rx_op_add());
+      a.t = rx_wave_reduce(a.t, rx_op_add());
+    }
+    __syncthreads();                                            // (the item before is through with the LDS)
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    rx_u64 mine = 0;
+    if constexpr (K > 0) {
+      // not above the key of the thread's largest element: the last index of its vector
+      if (best_at != 0x7fffffff) mine = rx_lm_key(best, row.first(best_at) + NE - 1);
+      rx_u64 quad = rx_max(mine, rx_dpp_t<rx_u64, 0xB1, 0xf>(mine));
+      quad = rx_max(quad, rx_dpp_t<rx_u64, 0x4E, 0xf>(quad));
+      if ((threadIdx.x & 3) == 0) group[threadIdx.x >> 2] = quad;
+      if (threadIdx.x == 0) count = 0;
+    }
+    __syncthreads();
+    a = rx_op_lm_sums()(rx_op_lm_sums()(red[0], red[1]), rx_op_lm_sums()(red[2], red[3]));
+    if (threadIdx.x == 0) {
+      if constexpr (SPLIT == 1) rx_lm_row_results<E, V>(t, a, row.x, targets, logprob, lse, entropy);
+      else {
+        part_sums[item * 3] = a.m;
+        part_sums[item * 3 + 1] = a.s;
+        part_sums[item * 3 + 2] = a.t;
+      }
+    }
+    if constexpr (K > 0) {
+      if (threadIdx.x < 64) {
+        const rx_u64 g = group[threadIdx.x];
+        int rank = 0;
+        for (int k = 0; k < 64; ++k) {
+          const rx_u64 o = group[k];
+          rank += o > g || (o == g && k < (int)threadIdx.x);    // (equal only where groups hold nothing)
+        }
+        if (rank == K - 1) bound = g;
+      }
+      __syncthreads();
+      const rx_u64 least = bound;
+      // threads with elements from there on
+      if (mine >= least && mine) listed[atomicAdd(&count, 1)] = threadIdx.x;
+      __syncthreads();
+      const int nlist = count;
+      __syncthreads();
+      if (threadIdx.x == 0) count = 0;
+      __syncthreads();
+      const bool odd = a.s != a.s;
+      const int per = (v1 - v0 + 255) / 256;                    // vectors of a thread
+      if (!odd)
+        for (int k = threadIdx.x; k < nlist * per; k += 256) {
+          const int v = v0 + listed[k / per] + 256 * (k % per), j = row.first(v);
+          if (v >= v1) continue;
+          float e[NE];
+          row.get(row.load(v), v, -rx_lm_inf(), e);
+#pragma unroll
+          for (int q = 0; q < NE; ++q) {
+            const rx_u64 key = rx_lm_key(e[q], j + q);
+            if (j + q >= 0 && j + q < V && key >= least) {
+              const int at = atomicAdd(&count, 1);
+              if (at < CAP) keys[at] = key;
+            }
+          }
+        }
+      __syncthreads();
+      int n = count;
+      if (odd || n > CAP) {
+        rx_u64 below = ~0ull;
+        for (int k = 0; k < K; ++k) {
+          rx_u64 top = 0;
+          for (int j = row.first(v0) + (int)threadIdx.x; j < row.first(v1); j += 256)
+            if (j >= 0 && j < V) {
+              const rx_u64 key = rx_lm_key(E::up(row.x[j]), j);
+              if (key < below && key > top) top = key;
+            }
+          __syncthreads();
+          top = rx_block_reduce<rx_u64, rx_op_max, 4>(top, rx_op_max(), red64);
+          if (threadIdx.x == 0) keys[k] = top;
+          below = top;
+        }
+        n = K;
+        __syncthreads();
+      }
+      const float l = a.s == 0.0f ? -rx_lm_inf() : a.m + __builtin_log2f(a.s) * 0.6931471805599453f;
+      rx_lm_select<K>(keys, n, [&](const int rank, const rx_u64 key) {
+        if constexpr (SPLIT == 1) {
+          const int j = (int)~(rx_u32)key;
+          ids[t * K + rank] = j;
+          values[t * K + rank] = a.s == 0.0f ? -rx_lm_inf() : E::up(row.x[j]) - l;
+        } else {
+          part_keys[item * K + rank] = key;
+        }
+      });
+    }
+  }
+}
+// the segments of a row, in their order: a workgroup per row
+template <typename E, int V, int K, int T, int SPLIT, typename I>
+RX_DEV void rx_token_logprobs_join(const typename E::S* logits, const I* targets, const float* part_sums, const rx_u64* part_keys, float* logprob, float* lse, float* entropy, float* values,
+                                   int* ids) {
+  __shared__ rx_u64 keys[K ? K * SPLIT : 1];
+  for (long long t = blockIdx.x; t < T; t += gridDim.x) {
+    __syncthreads();
+    for (int k = threadIdx.x; k < K * SPLIT; k += 256) keys[k] = part_keys[t * SPLIT * K + k];
+    rx_lm_sums a = {-rx_lm_inf(), 0.0f, 0.0f};
+    for (int s = 0; s < SPLIT; ++s) {
+      const float* p = part_sums + (t * SPLIT + s) * 3;
+      a = rx_op_lm_sums()(a, {p[0], p[1], p[2]});
+    }
+    const typename E::S* x = logits + t * V;
+    if (threadIdx.x == 0) rx_lm_row_results<E, V>(t, a, x, targets, logprob, lse, entropy);
+    __syncthreads();
+    if constexpr (K > 0) {
+      const float l = a.s == 0.0f ? -rx_lm_inf() : a.m + __builtin_log2f(a.s) * 0.6931471805599453f;
+      rx_lm_select<K>(keys, K * SPLIT, [&](const int rank, const rx_u64 key) {
+        const int j = (int)~(rx_u32)key;
+        ids[t * K + rank] = j;
+        values[t * K + rank] = a.s == 0.0f ? -rx_lm_inf() : E::up(x[j]) - l;
+      });
+    }
+  }
+}
+
+// d x_j = g (delta_jy - p_j) - h p_j (x_j - lse + H): a workgroup per SPAN vectors of a row
+template <typename E, int V, int T, int UNROLL, typename I>
 RX_DEV void rx_token_logprobs_grad(const typename E::S* logits, const I* targets, const float* lse, const float* entropy, const float* d_logprob, const float* d_entropy,
                                    typename E::S* out) {
-  const long long t = blockIdx.x;
-  const typename E::S* x = logits + t * V;
-  const I y = targets[t];
-  const bool counts = y >= 0 && y < V;
-  const float l = lse[t], H = entropy[t], g = counts ? d_logprob[t] : 0.0f, h = d_entropy[t];
-  for (int j = threadIdx.x; j < V; j += 256) {
-    const float z = E::up(x[j]) - l, p = l == -rx_lm_inf() ? 0.0f : expf(z);
-    float d = p == 0.0f ? 0.0f : -p * (g + h * (z + H));
-    if (counts && j == y) d += g;
-    out[t * V + j] = E::down(d);
+  typedef typename E::S S;
+  constexpr int NE = 16 / sizeof(S), VECTORS = rx_lm_row<E, V>::VECTORS, SPAN = 256 * UNROLL, PARTS = (VECTORS + SPAN - 1) / SPAN;
+  for (long long item = blockIdx.x; item < (long long)T * PARTS; item += gridDim.x) {
+    const long long t = item / PARTS;
+    const int v0 = (int)(item % PARTS) * SPAN + (int)threadIdx.x;
+    const rx_lm_row<E, V> row(logits, t);
+    S* o = out + t * V;
+    rx_vec<S, NE> r[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) r[u] = row.load(v0 + 256 * u);
+    const I y = targets[t];
+    const bool counts = y >= 0 && y < V;
+    const float l = lse[t] == -rx_lm_inf() ? rx_lm_inf() : lse[t];   // (a row of nothing: all probabilities 0)
+    const float g = counts ? d_logprob[t] : 0.0f, h = d_entropy[t], c = g + h * entropy[t];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int v = v0 + 256 * u, j = row.first(v);
+      if (v >= VECTORS) break;
+      float e[NE];
+      row.get(r[u], v, 0.0f, e);
+      rx_vec<S, NE> w;
+#pragma unroll
+      for (int k = 0; k < NE; ++k) {
+        const float z = e[k] - l, p = __builtin_amdgcn_exp2f(z * RX_LM_LOG2E);
+        float d = -p * __builtin_fmaf(h, __builtin_fmaxf(z, -200.0f), c);   // (p is 0 from there on, and 0 times -inf is no 0)
+        if (counts && (long long)y - j == k) d += g;
+        w.v[k] = E::down(d);
+      }
+      if (row.whole(v)) rx_store_nt(o + j, w);
+      else {
+#pragma unroll
+        for (int k = 0; k < NE; ++k)
+          if (j + k >= 0 && j + k < V) o[j + k] = w.v[k];
+      }
+    }
   }
 }

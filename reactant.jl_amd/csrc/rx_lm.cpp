@@ -19,6 +19,7 @@ const OpName kOperators[] = {
 
 constexpr int kMaxHeadDim = 256;
 constexpr int64_t kMaxTop = 64;
+constexpr int64_t kMaxGrid = (int64_t)1 << 22;   // workgroups; kernels with more items than that go on with the next ones
 constexpr int64_t kMaxRow = (int64_t)1 << 30;   // elements of a row or rows of a table: 32-bit indices inside a row
 
 struct Checker {
@@ -116,8 +117,6 @@ OperatorArg result(int i) { return {OperatorArg::Result, i}; }
 OperatorArg scratch(int i) { return {OperatorArg::Scratch, i}; }
 std::string st(const TType& t) { return info(t.dt).stype; }
 
-unsigned blocks(int64_t n, int64_t per) { return (unsigned)((n + per - 1) / per); }
-
 // ------------------------------------------------------------------ embedding
 void check_embedding(const Checker& c) {
   const TType &table = c.s.in[0], &ids = c.s.in[1], &out = c.s.out[0];
@@ -143,7 +142,7 @@ OperatorPlan plan_embedding(const OperatorSpec& s) {
                             std::string("rx_embedding<") + elem(s.in[0].dt) + ", " + num(V) + ", " + num(D) + ", " + num(T) + ", " + num(whole ? vec : 1) +
                                 ">(a0, a1, a2, " + flt(c.number("scale", 1.0)) + ");");
   const int64_t per = whole ? vec : 1;
-  k.grid[0] = blocks(T * ((D + per - 1) / per), 256);
+  k.grid[0] = (unsigned)std::min<int64_t>((T * (D / per) + 255) / 256, kMaxGrid);
   k.bytes = (double)(2 * s.out[0].bytes() + s.in[1].bytes());
   p.kernels.push_back(k);
   return p;
@@ -168,12 +167,38 @@ void check_embedding_grad(const Checker& c) {
 OperatorPlan plan_embedding_grad(const OperatorSpec& s) {
   const Checker c{s};
   const int64_t V = s.out[0].dims[0], D = s.out[0].dims[1], T = s.in[1].numel();
+  const std::string scale = flt(c.number("scale", 1.0)), types = std::string(elem(s.in[0].dt)) + ", " + elem(s.out[0].dt) + ", ";
+  const int64_t wide = 16 / info(s.in[0].dt).size, vec = D % wide == 0 ? wide : 1, C = D / vec;
+  const int64_t rows_grid = std::min<int64_t>((V * C + 255) / 256, kMaxGrid);
   OperatorPlan p;
-  OperatorKernel k = kernel(s, "embedding_grad", 256, {{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}, {result(0), st(s.out[0])}}, 1,
-                            std::string("rx_embedding_grad<") + elem(s.in[0].dt) + ", " + elem(s.out[0].dt) + ", " + num(D) + ", " + num(T) + ">(a0, a1, a2, " +
-                                flt(c.number("scale", 1.0)) + ");");
-  k.grid[0] = D ? (unsigned)V : 0;
+  if (rows_grid == 0) return p;
+  if (T <= 1024) {
+    const std::string sizes = num(V) + ", " + num(D) + ", " + num(std::max<int64_t>(T, 1)) + ", " + num(vec);
+    OperatorKernel k = T == 0 ? kernel(s, "embedding_grad", 256, {{result(0), st(s.out[0])}}, 1, "rx_lm_zero<" + num(V * D) + ">(a0);")
+                              : kernel(s, "embedding_grad", 256, {{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}, {result(0), st(s.out[0])}}, 1,
+                                       "rx_embedding_grad_few<" + types + sizes + ">(a0, a1, a2, " + scale + ");");
+    k.grid[0] = (unsigned)rows_grid;
+    k.bytes = (double)(s.in[0].bytes() + s.in[1].bytes() + s.out[0].bytes());
+    p.kernels.push_back(k);
+    return p;
+  }
+  // 256 workgroups sort, or as many as keep their rows' counters in LDS
+  const int64_t rows = std::min<int64_t>(512, (V + 255) / 256);
+  const int64_t piece = std::max<int64_t>(64, (T + 255) / 256), pieces = (T + piece - 1) / piece, tiles = (C + 255) / 256;
+  p.scratch = {(V + 1) * 4, T * 4, T * 4, pieces * 2 * D * 4};
+  OperatorKernel k = kernel(s, "embedding_sort", 1024, {{operand(1), st(s.in[1])}, {scratch(0), "int"}, {scratch(1), "int"}, {scratch(2), "int"}}, 3,
+                            "rx_lm_sort<" + num(V) + ", " + num(T) + ", " + num(rows) + ">(a0, a1, a2, a3);");
+  k.grid[0] = (unsigned)((V + rows - 1) / rows);
+  p.kernels.push_back(k);
+  const std::string sizes = types + num(V) + ", " + num(D) + ", " + num(T) + ", " + num(vec) + ", " + num(piece);
+  k = kernel(s, "embedding_grad", 256, {{operand(0), st(s.in[0])}, {scratch(0), "int"}, {scratch(1), "int"}, {scratch(2), "int"}, {result(0), st(s.out[0])}, {scratch(3), "float"}}, 2,
+             "rx_embedding_grad_rows<" + sizes + ", true>(a0, a1, a2, a3, a4, a5, " + scale + ");");
+  k.grid[0] = (unsigned)(rows_grid + pieces * tiles);
   k.bytes = (double)(s.in[0].bytes() + s.in[1].bytes() + s.out[0].bytes());
+  p.kernels.push_back(k);
+  k = kernel(s, "embedding_grad_join", 256, {{scratch(0), "int"}, {scratch(2), "int"}, {scratch(3), "float"}, {result(0), st(s.out[0])}}, 1,
+             "rx_embedding_grad_join<" + sizes + ">(a0, a1, a2, a3, " + scale + ");");
+  k.grid[0] = (unsigned)(pieces * tiles);
   p.kernels.push_back(k);
   return p;
 }
@@ -237,11 +262,16 @@ OperatorPlan plan_append(const OperatorSpec& s) {
   for (int i = 0; i < 8; ++i) args.push_back({operand(i), st(in[i])});
   for (int i = 0; i < 3; ++i) args.push_back({result(i), st(s.out[i])});
   std::ostringstream b;
-  b << "rx_kv_append<" << elem(in[0].dt) << ", " << in[0].dims[1] << ", " << kc.heads << ", " << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << kc.slots << ", " << in[7].dims[0]
-    << ", " << in[7].dims[1] << ", " << in[3].dims[0] << ", " << R2 << ", " << (rotation == "pairs" ? "true" : "false") << ", " << (by_slot ? "true" : "false")
-    << ">(a0, a1, a2, a3, a4, a5, a6, a7, a8, a9, a10);";
+  const int64_t ne = 16 / info(in[0].dt).size, HQ = in[0].dims[1];
+  const bool pairs = rotation == "pairs", whole = kc.dim % ne == 0 && vc.dim % ne == 0 && 2 * R2 % ne == 0 && (pairs || R2 % ne == 0);
+  const int64_t heads = T >= 256 ? 4 : 1;
+  b << (whole ? "rx_kv_append<" : "rx_kv_append_any<") << elem(in[0].dt) << ", " << HQ << ", " << kc.heads << ", " << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << kc.slots << ", "
+    << in[7].dims[0] << ", " << in[7].dims[1] << ", " << in[3].dims[0] << ", " << R2 << ", " << (pairs ? "true" : "false") << ", " << (by_slot ? "true" : "false") << ", " << T
+    << (whole ? ", " + num(heads) : std::string()) << ">(a0, a1, a2, a3, a4, a5, a6, a7, a8, a9, a10);";
   OperatorKernel k = kernel(s, "kv_append", 256, args, 3, b.str());
-  k.grid[0] = (unsigned)T;
+  const int64_t units = (pairs ? 2 * R2 : R2) / ne + (kc.dim - 2 * R2) / ne;
+  const int64_t all = ((HQ + heads - 1) / heads + (kc.heads + heads - 1) / heads) * units + (kc.heads * vc.dim / ne + heads - 1) / heads;
+  k.grid[0] = (unsigned)std::min<int64_t>(whole ? (T * all + 255) / 256 : T, kMaxGrid);
   k.bytes = 2.0 * (double)(in[0].bytes() + in[1].bytes() + in[2].bytes()) + 8.0 * (double)(T * R2) + (double)(in[5].bytes() * 3);
   p.kernels.push_back(k);
   return p;
@@ -351,15 +381,44 @@ void check_logprobs(const Checker& c) {
 OperatorPlan plan_logprobs(const OperatorSpec& s) {
   const Checker c{s};
   const int64_t V = s.in[0].dims.back(), T = s.in[1].numel(), top = c.integer("top", 0);
+  const int64_t vec = 16 / info(s.in[0].dt).size, vectors = (V + vec - 1) / vec + (V % vec ? 1 : 0);
+  // few rows: in segments, so that every compute unit has a workgroup, of at least two rounds of a workgroup's loads
+  const int64_t split = T == 0 ? 1 : std::max<int64_t>(1, std::min<int64_t>({64, (512 + T - 1) / T, vectors / 512}));
   OperatorPlan p;
-  std::vector<std::pair<OperatorArg, std::string>> args{{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}};
-  for (size_t r = 0; r < s.out.size(); ++r) args.push_back({result((int)r), st(s.out[r])});
-  OperatorKernel k = kernel(s, "token_logprobs", 256, args, (int)s.out.size(),
-                            std::string("rx_token_logprobs<") + elem(s.in[0].dt) + ", " + num(V) + ", " + num(top) + ">(a0, a1, a2, a3, a4, " + (top ? "a5, a6" : "(float*)0, (int*)0") + ");");
-  k.grid[0] = (unsigned)T;
-  k.bytes = (double)(s.in[0].bytes() + s.in[1].bytes());
-  for (auto& t : s.out) k.bytes += (double)t.bytes();
+  const std::string sizes = std::string(elem(s.in[0].dt)) + ", " + num(V) + ", " + num(top) + ", " + num(T) + ", " + num(split);
+  std::vector<std::pair<OperatorArg, std::string>> in{{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}}, out, part;
+  for (size_t r = 0; r < s.out.size(); ++r) out.push_back({result((int)r), st(s.out[r])});
+  if (split > 1) {
+    p.scratch = {T * split * 12};
+    part.push_back({scratch(0), "float"});
+    if (top) {
+      p.scratch.push_back(T * split * top * 8);
+      part.push_back({scratch(1), "rx_u64"});
+    }
+  }
+  double bytes = (double)(s.in[0].bytes() + s.in[1].bytes());
+  for (auto& t : s.out) bytes += (double)t.bytes();
+  std::vector<std::pair<OperatorArg, std::string>> args = in;
+  const std::string none = "(float*)0, (float*)0, (float*)0, (float*)0, (int*)0", tops = top ? "" : ", (float*)0, (int*)0";
+  if (split == 1) args.insert(args.end(), out.begin(), out.end());
+  args.insert(args.end(), part.begin(), part.end());
+  OperatorKernel k = kernel(s, "token_logprobs", 256, args, (int)args.size() - 2,
+                            "rx_token_logprobs<" + sizes + ">(a0, a1, " +
+                                (split == 1 ? std::string("a2, a3, a4, ") + (top ? "a5, a6" : "(float*)0, (int*)0") + ", (float*)0, (rx_u64*)0" : none + ", a2, " + (top ? "a3" : "(rx_u64*)0")) + ");");
+  k.grid[0] = (unsigned)std::min<int64_t>(T * split, kMaxGrid);
+  k.bytes = bytes;
   p.kernels.push_back(k);
+  if (split > 1) {
+    args = in;
+    args.insert(args.end(), part.begin(), part.end());
+    const size_t first = args.size();
+    args.insert(args.end(), out.begin(), out.end());
+    std::string call = "rx_token_logprobs_join<" + sizes + ">(a0, a1, a2, " + (top ? "a3" : "(const rx_u64*)0");
+    for (size_t r = 0; r < out.size(); ++r) call += ", a" + num((int64_t)(first + r));
+    OperatorKernel j = kernel(s, "token_logprobs_join", 256, args, (int)out.size(), call + tops + ");");
+    j.grid[0] = (unsigned)std::min<int64_t>(T, kMaxGrid);
+    p.kernels.push_back(j);
+  }
   return p;
 }
 
@@ -383,8 +442,10 @@ OperatorPlan plan_logprobs_grad(const OperatorSpec& s) {
   std::vector<std::pair<OperatorArg, std::string>> args;
   for (int i = 0; i < 6; ++i) args.push_back({operand(i), st(s.in[i])});
   args.push_back({result(0), st(s.out[0])});
-  OperatorKernel k = kernel(s, "token_logprobs_grad", 256, args, 1, std::string("rx_token_logprobs_grad<") + elem(s.in[0].dt) + ", " + num(V) + ">(a0, a1, a2, a3, a4, a5, a6);");
-  k.grid[0] = (unsigned)T;
+  const int64_t vec = 16 / info(s.in[0].dt).size, vectors = (V + vec - 1) / vec + (V % vec ? 1 : 0), unroll = vectors > 512 ? 4 : 1;
+  OperatorKernel k = kernel(s, "token_logprobs_grad", 256, args, 1,
+                            std::string("rx_token_logprobs_grad<") + elem(s.in[0].dt) + ", " + num(V) + ", " + num(T) + ", " + num(unroll) + ">(a0, a1, a2, a3, a4, a5, a6);");
+  k.grid[0] = (unsigned)std::min<int64_t>(T * ((vectors + 256 * unroll - 1) / (256 * unroll)), kMaxGrid);
   k.bytes = 2.0 * (double)s.in[0].bytes() + 20.0 * (double)T;
   p.kernels.push_back(k);
   return p;
