@@ -30,19 +30,28 @@ RX_DEV float rx_lm_inf() { return __builtin_inff(); }
 // ---------------------------------------------------------------------------
 // embedding: a thread per vector of VEC elements
 // ---------------------------------------------------------------------------
-template <typename E, int V, int D, int T, int VEC, typename I>
+template <typename E, int V, int D, int T, int VEC, int EACH, typename I>
 RX_DEV void rx_embedding(const typename E::S* table, const I* ids, typename E::S* out, const float scale) {
   constexpr int C = D / VEC;   // vectors of a row
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)T * C; i += (long long)gridDim.x * 256) {
-    const int t = (int)(i / C), c = (int)(i % C);
-    const I id = ids[t];
-    rx_vec<typename E::S, VEC> x{};
-    if (id >= 0 && id < V) {
-      x = rx_load<rx_vec<typename E::S, VEC>>(table + (long long)id * D + c * VEC);
+  typedef rx_vec<typename E::S, VEC> W;
+  for (long long i0 = (long long)blockIdx.x * (256 * EACH) + threadIdx.x; i0 < (long long)T * C; i0 += (long long)gridDim.x * (256 * EACH)) {
+    W x[EACH];
+    bool known[EACH];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x.v[k] = E::down(E::up(x.v[k]) * scale);
+    for (int n = 0; n < EACH; ++n) {
+      const long long i = i0 + 256 * n < (long long)T * C ? i0 + 256 * n : i0;
+      const I id = ids[i / C];
+      known[n] = id >= 0 && id < V;
+      x[n] = V ? rx_load<W>(table + (known[n] ? (long long)id * D : 0) + i % C * VEC) : W{};
     }
-    rx_store(out + (long long)t * D + c * VEC, x);
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) {
+      const long long i = i0 + 256 * n;
+      if (i >= (long long)T * C) break;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[n].v[k] = known[n] ? E::down(E::up(x[n].v[k]) * scale) : E::down(0.0f);
+      rx_store(out + i * VEC, x[n]);
+    }
   }
 }
 
@@ -126,46 +135,51 @@ RX_DEV void rx_lm_zero(S* out) {
 }
 template <int N>
 struct rx_lm_acc { float v[N]; };
-template <typename E, int D, int VEC>
-RX_DEV void rx_lm_sum_rows(const typename E::S* dy, const int* order, int from, const int to, const int c, rx_lm_acc<VEC>& a) {
+// adds the listed tokens' rows, in their order: the vectors c, c + 256, .. (EACH of them, those past the row's end are its last)
+template <typename E, int D, int VEC, int EACH, int AHEAD>
+RX_DEV int rx_lm_add_rows(const typename E::S* dy, const int* order, int from, const int to, const int c, rx_lm_acc<VEC> (&a)[EACH]) {
   typedef rx_vec<typename E::S, VEC> W;
-  for (; from + 8 <= to; from += 8) {
-    W w[8];
+  for (; AHEAD == 4 ? from < to : from + AHEAD <= to; from += AHEAD) {
+    W w[AHEAD][EACH];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] = rx_load<W>(dy + (long long)order[from + k] * D + c * VEC);
+    for (int k = 0; k < AHEAD; ++k) {
+      const typename E::S* row = dy + (long long)order[AHEAD > 4 || from + k < to ? from + k : to - 1] * D;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+      for (int n = 0; n < EACH; ++n) w[k][n] = rx_load<W>(row + (c + 256 * n < D / VEC ? c + 256 * n : D / VEC - 1) * VEC);
+    }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) a.v[e] += E::up(w[k].v[e]);
+    for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+      for (int n = 0; n < EACH; ++n)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) a[n].v[e] += AHEAD > 4 || k == 0 || from + k < to ? E::up(w[k][n].v[e]) : 0.0f;
   }
-  for (; from < to; ++from) {
-    const W w = rx_load<W>(dy + (long long)order[from] * D + c * VEC);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) a.v[e] += E::up(w.v[e]);
-  }
+  return from;
+}
+// eight tokens at a time, the last ones four at a time: loads one after the other would wait for one another
+template <typename E, int D, int VEC, int EACH>
+RX_DEV void rx_lm_sum_rows(const typename E::S* dy, const int* order, int from, const int to, const int c, rx_lm_acc<VEC> (&a)[EACH]) {
+  from = rx_lm_add_rows<E, D, VEC, EACH, 8>(dy, order, from, to, c, a);
+  rx_lm_add_rows<E, D, VEC, EACH, 4>(dy, order, from, to, c, a);
 }
 template <typename O, int VEC>
 RX_DEV void rx_lm_put(typename O::S* out, const rx_lm_acc<VEC>& a, const float scale) {
   rx_vec<typename O::S, VEC> w;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) w.v[e] = O::down(a.v[e] * scale);
-  if constexpr (sizeof(w) > 16) {
-    const auto* p = (const rx_vec<typename O::S, 16 / sizeof(typename O::S)>*)&w;
-#pragma unroll
-    for (unsigned k = 0; k < sizeof(w) / 16; ++k) rx_store_nt(out + k * (16 / sizeof(typename O::S)), p[k]);
-  } else {
-    rx_store_nt(out, w);
-  }
+  rx_store_nt(out, w);
 }
 
-// Rows of up to LONG tokens: a thread per vector of the table sums its row's tokens, in their order.  A row of more would keep
-// one thread's loads waiting for one another: those are summed in pieces, the places [LONG p, LONG p + LONG) of the list by
-// the first workgroups (a piece touches at most two such rows: it may end one and start another), and joined by the next launch.
-template <typename E, typename O, int V, int D, int T, int VEC, int LONG, bool PIECES>
+// Rows of up to LONG tokens: EACH vectors of a row to a thread (C vectors a row; several short rows to a workgroup), its tokens
+// summed in their order.  A row of more would keep one thread's loads waiting for one another: those are summed in pieces, the
+// places [LONG p, LONG p + LONG) of the list by the first workgroups (a piece touches at most two such rows: it may end one
+// and start another), and joined by the next launch.
+template <typename E, typename O, int V, int D, int T, int VEC, int LONG, int EACH>
 RX_DEV void rx_embedding_grad_rows(const typename E::S* dy, const int* start, const int* order, const int* row_of, typename O::S* out, float* part, const float scale) {
-  constexpr int C = D / VEC, TILES = (C + 255) / 256, NP = PIECES ? (T + LONG - 1) / LONG : 0;
-  if (PIECES && blockIdx.x < NP * TILES) {
-    const int piece = blockIdx.x / TILES, c = blockIdx.x % TILES * 256 + (int)threadIdx.x, all = start[V];
+  constexpr int C = D / VEC, TILES = (C + 256 * EACH - 1) / (256 * EACH), NP = (T + LONG - 1) / LONG;
+  constexpr int LANES = C < 256 ? C : 256, ROWS = 256 / LANES;   // threads along a row, rows of a workgroup
+  if (blockIdx.x < NP * TILES) {
+    const int piece = blockIdx.x / TILES, c = blockIdx.x % TILES * (256 * EACH) + (int)threadIdx.x, all = start[V];
     const int a = piece * LONG, e = a + LONG < all ? a + LONG : all;
     if (a >= e || c >= C) return;
     const int first = row_of[a], last = row_of[e - 1];
@@ -174,19 +188,27 @@ RX_DEV void rx_embedding_grad_rows(const typename E::S* dy, const int* start, co
       if (k && last == first) break;
       const int s0 = start[row], s1 = start[row + 1];
       if (s1 - s0 <= LONG) continue;
-      rx_lm_acc<VEC> sum = {};
-      rx_lm_sum_rows<E, D, VEC>(dy, order, s0 > a ? s0 : a, s1 < e ? s1 : e, c, sum);
-      *(rx_lm_acc<VEC>*)(part + ((long long)(piece * 2 + k) * C + c) * VEC) = sum;
+      rx_lm_acc<VEC> sum[EACH] = {};
+      rx_lm_sum_rows<E, D, VEC, EACH>(dy, order, s0 > a ? s0 : a, s1 < e ? s1 : e, c, sum);
+#pragma unroll
+      for (int n = 0; n < EACH; ++n)
+        if (c + 256 * n < C) *(rx_lm_acc<VEC>*)(part + ((long long)(piece * 2 + k) * C + c + 256 * n) * VEC) = sum[n];
     }
     return;
   }
-  const long long grid = (long long)(gridDim.x - NP * TILES) * 256;
-  for (long long i = (long long)(blockIdx.x - NP * TILES) * 256 + threadIdx.x; i < (long long)V * C; i += grid) {
-    const int row = (int)(i / C), c = (int)(i % C), s0 = start[row], s1 = start[row + 1];
-    if (PIECES && s1 - s0 > LONG) continue;
-    rx_lm_acc<VEC> sum = {};
-    rx_lm_sum_rows<E, D, VEC>(dy, order, s0, s1, c, sum);
-    rx_lm_put<O, VEC>(out + i * VEC, sum, scale);
+  const int l = (int)threadIdx.x % LANES, r = (int)threadIdx.x / LANES;
+  if (r >= ROWS) return;
+  const long long work = (long long)((V + ROWS - 1) / ROWS) * TILES;
+  for (long long i = blockIdx.x - NP * TILES; i < work; i += gridDim.x - NP * TILES) {
+    const int row = (int)(i / TILES) * ROWS + r, c = (int)(i % TILES) * (256 * EACH) + l;
+    if (row >= V || c >= C) continue;
+    const int s0 = start[row], s1 = start[row + 1];
+    if (s1 - s0 > LONG) continue;
+    rx_lm_acc<VEC> sum[EACH] = {};
+    rx_lm_sum_rows<E, D, VEC, EACH>(dy, order, s0, s1, c, sum);
+#pragma unroll
+    for (int n = 0; n < EACH; ++n)
+      if (c + 256 * n < C) rx_lm_put<O, VEC>(out + ((long long)row * C + c + 256 * n) * VEC, sum[n], scale);
   }
 }
 // the rows of more than LONG tokens: by the workgroup of the piece that such a row starts in, its pieces in their order

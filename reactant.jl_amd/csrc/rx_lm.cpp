@@ -138,11 +138,11 @@ OperatorPlan plan_embedding(const OperatorSpec& s) {
   OperatorPlan p;
   const int vec = (int)(16 / info(s.in[0].dt).size);
   const bool whole = D % vec == 0;
+  const int64_t per = whole ? vec : 1, each = 4;
   OperatorKernel k = kernel(s, "embedding", 256, {{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}, {result(0), st(s.out[0])}}, 1,
-                            std::string("rx_embedding<") + elem(s.in[0].dt) + ", " + num(V) + ", " + num(D) + ", " + num(T) + ", " + num(whole ? vec : 1) +
+                            std::string("rx_embedding<") + elem(s.in[0].dt) + ", " + num(V) + ", " + num(D) + ", " + num(T) + ", " + num(whole ? vec : 1) + ", " + num(each) +
                                 ">(a0, a1, a2, " + flt(c.number("scale", 1.0)) + ");");
-  const int64_t per = whole ? vec : 1;
-  k.grid[0] = (unsigned)std::min<int64_t>((T * (D / per) + 255) / 256, kMaxGrid);
+  k.grid[0] = (unsigned)std::min<int64_t>((T * (D / per) + 256 * each - 1) / (256 * each), kMaxGrid);
   k.bytes = (double)(2 * s.out[0].bytes() + s.in[1].bytes());
   p.kernels.push_back(k);
   return p;
@@ -168,7 +168,7 @@ OperatorPlan plan_embedding_grad(const OperatorSpec& s) {
   const Checker c{s};
   const int64_t V = s.out[0].dims[0], D = s.out[0].dims[1], T = s.in[1].numel();
   const std::string scale = flt(c.number("scale", 1.0)), types = std::string(elem(s.in[0].dt)) + ", " + elem(s.out[0].dt) + ", ";
-  const int64_t wide = 16 / info(s.in[0].dt).size, vec = D % wide == 0 ? wide : 1, C = D / vec;
+  const int64_t wide = 16 / info(s.out[0].dt).size, vec = D % wide == 0 ? wide : 1, C = D / vec;   // a thread writes 16 bytes
   const int64_t rows_grid = std::min<int64_t>((V * C + 255) / 256, kMaxGrid);
   OperatorPlan p;
   if (rows_grid == 0) return p;
@@ -190,10 +190,11 @@ OperatorPlan plan_embedding_grad(const OperatorSpec& s) {
                             "rx_lm_sort<" + num(V) + ", " + num(T) + ", " + num(rows) + ">(a0, a1, a2, a3);");
   k.grid[0] = (unsigned)((V + rows - 1) / rows);
   p.kernels.push_back(k);
+  const int64_t each = std::min<int64_t>(2, tiles), wide_tiles = (C + 256 * each - 1) / (256 * each), lines = C < 256 ? 256 / C : 1;
   const std::string sizes = types + num(V) + ", " + num(D) + ", " + num(T) + ", " + num(vec) + ", " + num(piece);
   k = kernel(s, "embedding_grad", 256, {{operand(0), st(s.in[0])}, {scratch(0), "int"}, {scratch(1), "int"}, {scratch(2), "int"}, {result(0), st(s.out[0])}, {scratch(3), "float"}}, 2,
-             "rx_embedding_grad_rows<" + sizes + ", true>(a0, a1, a2, a3, a4, a5, " + scale + ");");
-  k.grid[0] = (unsigned)(rows_grid + pieces * tiles);
+             "rx_embedding_grad_rows<" + sizes + ", " + num(each) + ">(a0, a1, a2, a3, a4, a5, " + scale + ");");
+  k.grid[0] = (unsigned)(std::min<int64_t>((V + lines - 1) / lines * wide_tiles, kMaxGrid) + pieces * wide_tiles);
   k.bytes = (double)(s.in[0].bytes() + s.in[1].bytes() + s.out[0].bytes());
   p.kernels.push_back(k);
   k = kernel(s, "embedding_grad_join", 256, {{scratch(0), "int"}, {scratch(2), "int"}, {scratch(3), "float"}, {result(0), st(s.out[0])}}, 1,
