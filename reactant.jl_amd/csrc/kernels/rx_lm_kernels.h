@@ -24,6 +24,26 @@ struct rx_lm_f16 {
   RX_MEM static S down(float x) { return rx_f32_to_f16(rx_apart(x)); }
 };
 
+// Values handed to the workgroup of the same launch that arrives last, on whichever die it runs: written and read past the
+// caches that belong to one die (device-scope atomic accesses), and counted in once the writes have arrived.  No workgroup
+// waits for another.  The counter is zero before the launch, and again after it.
+RX_DEV void rx_lm_put_shared(float* p, const float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename T>
+RX_DEV T rx_lm_get_shared(const T* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+RX_DEV bool rx_lm_last_to_arrive(int* counter, const int expected, int* flag) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's writes
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool l = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == expected - 1;
+    if (l) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = l;
+  }
+  __syncthreads();
+  const bool l = *flag != 0;
+  __syncthreads();
+  return l;
+}
+
 #define RX_LM_LOG2E 1.4426950408889634f
 RX_DEV float rx_lm_inf() { return __builtin_inff(); }
 
@@ -410,58 +430,56 @@ RX_DEV void rx_kv_append(const typename E::S* q, const typename E::S* k, const t
 // second one takes them (which of its k is which position is free as long as V follows suit).  V' needs the values of one
 // dimension at consecutive positions: a lane loads 16 bytes (8 dimensions) of 8 positions, and bytes are permuted in registers.
 //
-// The positions of all sequences are cut into about ITEMS chunks, equal within a sequence and as long as the sum of the lengths
-// asks for (multiples of 128: four wavefronts, 32 each), so that a batch of uneven lengths fills the chip; every workgroup works
-// the cut out from the lengths.  A sequence of one chunk is finished here; those of several leave (maximum, sum, unscaled
-// result) and rx_paged_attention_join combines them.
-struct rx_lm_cut { int n, lo, size, count; };   // length, first position, positions of a chunk (from lo rounded down to 128), chunks
+// The positions of all sequences, in units of 32, are one row that R workgroups per key head (and tile of query heads) share in
+// equal stretches, whatever the lengths: a stretch may end one sequence, hold others, and start one more.  Every workgroup
+// works its stretch out from the lengths.  Sequences inside of one stretch are finished there.  Of a longer one every workgroup
+// leaves (maximum, sum, unscaled result) of its part, and the one that arrives last combines them, in the order of the
+// positions.  A workgroup has at most two such parts: one that a workgroup before it has started, and one that it starts.
+struct rx_lm_span { int n, lo, units; };   // length, first position, units from lo rounded down to 32 (an empty sequence has one)
 template <int S, int M, int W, typename I>
-RX_DEV int rx_lm_length(const I len) { return len < 0 ? 0 : len > (I)(M * S) ? M * S : (int)len; }
-template <int W>
-RX_DEV int rx_lm_first(const int n) { return W && n > W ? n - W : 0; }
-template <int W>
-RX_DEV rx_lm_cut rx_lm_cut_of(const int n, const int chunk) {
-  rx_lm_cut c;
-  c.n = n;
-  c.lo = rx_lm_first<W>(n);
-  const int tokens = n - (c.lo & ~127);
-  const int k = tokens > chunk ? (tokens + chunk - 1) / chunk : 1;
-  c.size = tokens > 0 ? ((tokens + k - 1) / k + 127) & ~127 : 128;
-  c.count = tokens > c.size ? (tokens + c.size - 1) / c.size : 1;
-  return c;
+RX_DEV rx_lm_span rx_lm_span_of(const I len) {
+  rx_lm_span s;
+  s.n = len < 0 ? 0 : len > (I)(M * S) ? M * S : (int)len;
+  s.lo = W && s.n > W ? s.n - W : 0;
+  s.units = (s.n - (s.lo & ~31) + 31) >> 5;
+  if (s.units == 0) s.units = 1;
+  return s;
 }
-// chunk length for all sequences: every wavefront works it out for itself
-template <int S, int B, int M, int W, int COLUMNS, int ITEMS, typename I>
-RX_DEV int rx_lm_chunk(const I* lengths) {
+struct rx_lm_stretch { int b, unit, count; long long first, total; int parts; };   // sequence and its unit to start at, units; first unit in the row, units of the row, stretches
+// stretch r of up to R: at least four units each, one for every wavefront
+RX_DEV long long rx_lm_stretch_start(const long long total, const int parts, const int r) { return total * r / parts; }
+template <int S, int B, int M, int W, int R, typename I>
+RX_DEV rx_lm_stretch rx_lm_stretch_of(const I* lengths, const int r) {
   const int lane = threadIdx.x & 63;
-  long long total = 0;
-  for (int b = lane; b < B; b += 64) {
-    const int n = rx_lm_length<S, M, W>(lengths[b]);
-    total += n - (rx_lm_first<W>(n) & ~127);
-  }
-  if constexpr (B > 1) total = rx_wave_reduce(total, rx_op_add());
-  else total = rx_lane_from(total, 0);
-  const long long per = (total * COLUMNS + ITEMS - 1) / ITEMS;
-  return per < 128 ? 128 : (int)((per + 127) & ~127ll);
-}
-// the sequence that item `item` (in units of COLUMNS items) belongs to, and the number of chunks before it; B where there is none
-template <int S, int B, int M, int W, typename I>
-RX_DEV int rx_lm_find(const I* lengths, const int chunk, const int item, int* before) {
-  const int lane = threadIdx.x & 63;
-  int sum = 0;
+  rx_lm_stretch s = {B, 0, 0, 0, 0, 0};
+  for (int b0 = 0; b0 < B; b0 += 64) s.total += b0 + lane < B ? rx_lm_span_of<S, M, W>(lengths[b0 + lane]).units : 0;
+  if constexpr (B > 1) s.total = rx_wave_reduce(s.total, rx_op_add());
+  else s.total = rx_lane_from(s.total, 0);
+  s.parts = s.total < 4ll * R ? (int)((s.total + 3) / 4) : R;
+  if (r >= s.parts) return s;
+  s.first = rx_lm_stretch_start(s.total, s.parts, r);
+  s.count = (int)(rx_lm_stretch_start(s.total, s.parts, r + 1) - s.first);
+  long long sum = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
-    const int b = b0 + lane;
-    const int count = b < B ? rx_lm_cut_of<W>(rx_lm_length<S, M, W>(lengths[b]), chunk).count : 0;
-    const int upto = sum + rx_wave_scan(count, rx_op_add());
-    const unsigned long long past = __ballot(b < B && upto > item);
+    const int units = b0 + lane < B ? rx_lm_span_of<S, M, W>(lengths[b0 + lane]).units : 0;
+    const long long upto = sum + (B > 1 ? rx_wave_scan((long long)units, rx_op_add()) : (long long)units);
+    const unsigned long long past = __ballot(b0 + lane < B && upto > s.first);
     if (past) {
-      const int first = __builtin_ctzll(past);
-      *before = rx_lane_from(upto - count, first);
-      return __builtin_amdgcn_readfirstlane(b0 + first);
+      const int at = __builtin_ctzll(past);
+      s.b = b0 + at;
+      s.unit = (int)(s.first - rx_lane_from(upto - units, at));
+      return s;
     }
     sum = rx_lane_from(upto, 63);
   }
-  return B;
+  return s;
+}
+// the stretch that holds a unit of the row
+RX_DEV int rx_lm_stretch_with(const long long total, const int parts, const long long unit) {
+  int r = (int)(unit * parts / total);
+  while (r + 1 < parts && rx_lm_stretch_start(total, parts, r + 1) <= unit) ++r;
+  while (r > 0 && rx_lm_stretch_start(total, parts, r) > unit) --r;
+  return r;
 }
 
 // maximum over the four lanes that hold one head's positions (l, l ^ 16, l ^ 32, l ^ 48)
@@ -505,10 +523,10 @@ RX_DEV rx_f32x4 rx_lm_mma(const rx_u32x4 a, const rx_u32x4 b, rx_f32x4 c) {
   }
 }
 
-// HT: query heads of an item (those of one key head, up to 16 NT of them at a time); COLUMNS: items per chunk of a sequence
-template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int NT, int ITEMS, bool JOIN, typename I>
+// COLUMNS: key heads, times the tiles of up to 16 NT query heads that read one; R: stretches; JOIN: a sequence can be longer than a stretch
+template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int NT, int R, typename I>
 RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, const typename E::S* vc, const I* pages, const I* lengths, typename E::S* out, float* lse,
-                               float* part, float* stat, const float scale) {
+                               float* part, float* stat, int* arrived, const float scale) {
   typedef typename E::S T;
   constexpr int NE = 16 / sizeof(T);                   // elements of 16 bytes
   constexpr int G = HQ / HK, GT = G < 16 * NT ? G : 16 * NT, TILES = (G + GT - 1) / GT, COLUMNS = HK * TILES;
@@ -522,20 +540,21 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
     float o[4][HR][WIDTH + 4];
   } lds;
   __shared__ float join_m[4][16], join_l[4][16];
+  __shared__ int last;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
-  const int chunk = JOIN ? rx_lm_chunk<S, B, M, W, COLUMNS, ITEMS>(lengths) : 1 << 30;
-
-  const int item = blockIdx.x;
-  int before = 0;
-  const int b = B == 1 ? (item / COLUMNS < rx_lm_cut_of<W>(rx_lm_length<S, M, W>(lengths[0]), chunk).count ? 0 : B)
-                       : JOIN ? rx_lm_find<S, B, M, W>(lengths, chunk, item / COLUMNS, &before) : (before = item / COLUMNS);
-  if (b >= B) return;
-  const rx_lm_cut cut = rx_lm_cut_of<W>(rx_lm_length<S, M, W>(lengths[b]), chunk);
-  const int column = item % COLUMNS, head = column / TILES, tile = column % TILES;
-  const int p0 = (cut.lo & ~127) + (item / COLUMNS - before) * cut.size;
-  const int p1 = P == 0 ? p0 : p0 + cut.size < cut.n ? p0 + cut.size : cut.n;
+  const int column = blockIdx.x % COLUMNS, mine = blockIdx.x / COLUMNS, head = column / TILES, tile = column % TILES;
   const int h0 = head * G + tile * GT;                 // first query head
   const int heads = G - tile * GT < GT ? G - tile * GT : GT;
+  const rx_lm_stretch st = rx_lm_stretch_of<S, B, M, W, R>(lengths, mine);
+
+  int b = st.b, unit = st.unit;
+  for (int left = st.count; left > 0; ++b, unit = 0) {
+  const rx_lm_span span = rx_lm_span_of<S, M, W>(lengths[b]);
+  const int take = span.units - unit < left ? span.units - unit : left;
+  const int p0 = (span.lo & ~31) + unit * 32, p1 = P == 0 ? p0 : p0 + take * 32 < span.n ? p0 + take * 32 : span.n;
+  const bool whole = take == span.units;               // the whole sequence is in this stretch
+  const long long begin = st.first + (st.count - left) - unit;   // the sequence's first unit in the row
+  left -= take;
 
   rx_u32x4 qf[NT][NK];
 #pragma unroll
@@ -566,7 +585,7 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
     }
     __syncthreads();
     // page of a position, -1 where it is not to be looked at
-    auto where = [&](const int t) { return t >= cut.lo && t < s1 ? lds.page[t / S - page0] : -1; };
+    auto where = [&](const int t) { return t >= span.lo && t < s1 ? lds.page[t / S - page0] : -1; };
     for (int t0 = s0 + wave * 32; t0 < s1; t0 += 128) {
       const int ta = t0 + r, tb = ta + 16, pa = where(ta), pb = where(tb);
       const unsigned ok = ((unsigned)__ballot(pa >= 0) & 0xffffu) | ((unsigned)__ballot(pb >= 0) << 16);
@@ -585,7 +604,7 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
       for (int i = 0; i < 8; ++i) {
         const int tv = t0 + (i & 4) * 4 + g4 * 4 + (i & 3);
         if (S % 4 != 0 || i % 4 == 0) {
-          pv = where(S % 4 == 0 ? (tv + 3 < s1 ? tv + 3 : s1 - 1) : tv);   // (the group's first positions may lie before cut.lo)
+          pv = where(S % 4 == 0 ? (tv + 3 < s1 ? tv + 3 : s1 - 1) : tv);   // (the group's first positions may lie before span.lo)
           if (S % 4 == 0 && tv >= s1) pv = -1;
         }
         const T* v = vc + rx_lm_slot<S, HK, DV, BY_SLOT>(pv < 0 ? 0 : pv, tv % S, head);
@@ -661,7 +680,7 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
     }
   }
 
-  // the four wavefronts' parts of the chunk
+  // the four wavefronts' parts
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (t * 16 >= heads) break;
@@ -702,45 +721,55 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
           sum += hi == -rx_lm_inf() ? 0.0f : join_l[w][h] * __builtin_amdgcn_exp2f(join_m[w][h] - hi);
         }
         const int qh = h0 + t * 16 + h;
-        if (!JOIN || cut.count == 1) {
+        if (whole) {
           out[((long long)b * HQ + qh) * DV + d] = E::down(sum == 0.0f ? 0.0f : o / sum);
           if (lse && d == 0) lse[(long long)b * HQ + qh] = sum == 0.0f ? -rx_lm_inf() : (hi - SHIFT + __builtin_log2f(sum)) * 0.6931471805599453f;
         } else {
-          part[((long long)item * GT + t * 16 + h) * DV + d] = o;
+          const long long at = ((long long)blockIdx.x * 2 + (unit == 0)) * GT + t * 16 + h;
+          rx_lm_put_shared(part + at * DV + d, o);
           if (d == 0) {
-            stat[((long long)item * GT + t * 16 + h) * 2] = hi - SHIFT;
-            stat[((long long)item * GT + t * 16 + h) * 2 + 1] = sum;
+            rx_lm_put_shared(stat + at * 2, hi - SHIFT);
+            rx_lm_put_shared(stat + at * 2 + 1, sum);
           }
         }
       }
     }
   }
-}
-
-// a workgroup per query head of a sequence of several chunks: the chunks' results in their order
-template <typename E, int HQ, int HK, int DV, int S, int B, int M, int W, int NT, int ITEMS, typename I>
-RX_DEV void rx_paged_attention_join(const I* lengths, const float* part, const float* stat, typename E::S* out, float* lse) {
-  constexpr int G = HQ / HK, GT = G < 16 * NT ? G : 16 * NT, TILES = (G + GT - 1) / GT, COLUMNS = HK * TILES;
-  const int b = blockIdx.y, qh = blockIdx.x, lane = threadIdx.x & 63;
-  const int chunk = rx_lm_chunk<S, B, M, W, COLUMNS, ITEMS>(lengths);
-  const rx_lm_cut cut = rx_lm_cut_of<W>(rx_lm_length<S, M, W>(lengths[b]), chunk);
-  if (cut.count == 1) return;
-  int before = 0;
-  for (int k = lane; k < b; k += 64) before += rx_lm_cut_of<W>(rx_lm_length<S, M, W>(lengths[k]), chunk).count;
-  if constexpr (B > 1) before = rx_wave_reduce(before, rx_op_add());
-  const int tile = qh % G / GT, h = qh % G % GT, column = qh / G * TILES + tile;
-  float top = -rx_lm_inf();
-  for (int c = 0; c < cut.count; ++c) top = __builtin_fmaxf(top, stat[((long long)((before + c) * COLUMNS + column) * GT + h) * 2]);
-  for (int d = threadIdx.x; d < DV; d += 256) {
-    float o = 0.0f, sum = 0.0f;
-    for (int c = 0; c < cut.count; ++c) {
-      const long long at = (long long)((before + c) * COLUMNS + column) * GT + h;
-      const float f = top == -rx_lm_inf() ? 0.0f : __builtin_amdgcn_exp2f(stat[at * 2] - top);
-      o += f * part[at * DV + d];
-      sum += f * stat[at * 2 + 1];
+  if (whole) continue;
+  const int from = rx_lm_stretch_with(st.total, st.parts, begin), to = rx_lm_stretch_with(st.total, st.parts, begin + span.units - 1);
+  if (!rx_lm_last_to_arrive(arrived + b * COLUMNS + column, to - from + 1, &last)) continue;
+  for (int k = threadIdx.x; k < heads * DV; k += 256) {
+    const int h = k / DV, d = k % DV;
+    float o = 0.0f, sum = 0.0f, top = -rx_lm_inf();
+    for (int w = from; w <= to; w += 8) {
+      float pm[8], ps[8], po[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int v = w + i <= to ? w + i : to;
+        const long long at = ((long long)(v * COLUMNS + column) * 2 + (v == from)) * GT + h;
+        pm[i] = rx_lm_get_shared(stat + at * 2);
+        ps[i] = rx_lm_get_shared(stat + at * 2 + 1);
+        po[i] = rx_lm_get_shared(part + at * DV + d);
+      }
+      float hi = top;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) hi = __builtin_fmaxf(hi, pm[i]);
+      if (hi == -rx_lm_inf()) hi = 0.0f;
+      const float f = __builtin_amdgcn_exp2f(top - hi);
+      o *= f;
+      sum *= f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (w + i > to) break;
+        const float g = __builtin_amdgcn_exp2f(pm[i] - hi);
+        o += po[i] * g;
+        sum += ps[i] * g;
+      }
+      top = hi;
     }
-    out[((long long)b * HQ + qh) * DV + d] = E::down(sum == 0.0f ? 0.0f : o / sum);
-    if (lse && d == 0) lse[(long long)b * HQ + qh] = sum == 0.0f ? -rx_lm_inf() : (top + __builtin_log2f(sum)) * 0.6931471805599453f;
+    out[((long long)b * HQ + h0 + h) * DV + d] = E::down(sum == 0.0f ? 0.0f : o / sum);
+    if (lse && d == 0) lse[(long long)b * HQ + h0 + h] = sum == 0.0f ? -rx_lm_inf() : (top + __builtin_log2f(sum)) * 0.6931471805599453f;
+  }
   }
 }
 

@@ -91,9 +91,10 @@ std::string flt(double v) {
   return s + "f";
 }
 
-// `body` is the call of a device function on a0, a1, ..: the kernel's parameters, of which the last `outs` are written
+// `body` is the call of a device function on a0, a1, ..: the kernel's parameters, of which the last `outs` are written.
+// `waves`: wavefronts per SIMD that the registers have to allow (0: the compiler's choice)
 OperatorKernel kernel(const OperatorSpec& s, const std::string& suffix, unsigned block, const std::vector<std::pair<OperatorArg, std::string>>& args, int outs,
-                      const std::string& body) {
+                      const std::string& body, int waves = 0) {
   OperatorKernel k;
   k.suffix = suffix;
   k.kind = "lm_" + suffix;
@@ -102,7 +103,7 @@ OperatorKernel kernel(const OperatorSpec& s, const std::string& suffix, unsigned
   std::ostringstream o;
   o << "// " << s.name;
   for (auto& t : s.in) o << " " << t.str();
-  o << "\nextern \"C\" __global__ __launch_bounds__(" << block << ") void @K@_" << suffix << "(";
+  o << "\nextern \"C\" __global__ __launch_bounds__(" << block << (waves ? ", " + num(waves) : std::string()) << ") void @K@_" << suffix << "(";
   for (size_t a = 0; a < args.size(); ++a) {
     const bool in = a + (size_t)outs < args.size();
     o << (a ? ", " : "") << (in ? "const " : "") << args[a].second << "* __restrict__ a" << a;
@@ -115,6 +116,7 @@ OperatorKernel kernel(const OperatorSpec& s, const std::string& suffix, unsigned
 OperatorArg operand(int i) { return {OperatorArg::Operand, i}; }
 OperatorArg result(int i) { return {OperatorArg::Result, i}; }
 OperatorArg scratch(int i) { return {OperatorArg::Scratch, i}; }
+OperatorArg counters() { return {OperatorArg::Counters, 0}; }
 std::string st(const TType& t) { return info(t.dt).stype; }
 
 // ------------------------------------------------------------------ embedding
@@ -316,40 +318,35 @@ OperatorPlan plan_attention(const OperatorSpec& s) {
   const int64_t window = std::min<int64_t>(c.integer("window", 0), kMaxRow);
   const bool lse = s.out.size() == 2;
   const int64_t G = Hq / kc.heads, NT = G > 16 ? 2 : 1, tiles = (G + 16 * NT - 1) / (16 * NT), columns = kc.heads * tiles, GT = std::min(G, 16 * NT);
-  const int64_t items = 512;   // two workgroups per compute unit
-  // positions of a sequence from the multiple of 128 below its first: chunks of 128 and more
-  const int64_t longest = window ? std::min(M * kc.slots, window + 127) : M * kc.slots;
-  const bool join = longest > 128;
-  const int64_t grid = join ? std::min(items + B * columns, B * columns * ((longest + 127) / 128)) : B * columns;
+  // Registers of a wavefront: a step's keys and values, the queries, the result, and room for the rest.  Up to 256 of them two
+  // wavefronts share a SIMD, and two workgroups a compute unit.
+  const int64_t ne = 16 / info(in[0].dt).size, nk = (kc.dim + 4 * ne - 1) / (4 * ne), nv = (vc.dim + 16 * ne - 1) / (16 * ne);
+  const int waves = 8 * nk + 32 * nv + NT * (4 * nk + 4 * nv * ne + 24) <= 196 ? 2 : 1;
+  // every workgroup a stretch of at least four units of 32 positions, all of them on the chip at once
+  const int64_t longest = window ? std::min(M * kc.slots, window + 31) : M * kc.slots, units = std::max<int64_t>(1, (longest + 31) / 32);
+  const int64_t stretches = std::max<int64_t>(1, std::min((getenv("RXI") ? atoi(getenv("RXI")) : 256) * waves / columns, (B * units + 3) / 4)), grid = stretches * columns;
   OperatorPlan p;
   std::vector<std::pair<OperatorArg, std::string>> args;
   for (int i = 0; i < 5; ++i) args.push_back({operand(i), st(in[i])});
   args.push_back({result(0), st(s.out[0])});
   if (lse) args.push_back({result(1), "float"});
-  if (join) {
-    p.scratch = {grid * GT * vc.dim * 4, grid * GT * 8};
+  std::string shared = "(float*)0, (float*)0, (int*)0";
+  if (stretches > 1) {
+    p.scratch = {grid * 2 * GT * vc.dim * 4, grid * 2 * GT * 8};
+    p.counters = B * columns;
     args.push_back({scratch(0), "float"});
     args.push_back({scratch(1), "float"});
+    args.push_back({counters(), "int"});
+    shared = lse ? "a7, a8, a9" : "a6, a7, a8";
   }
-  const std::string sizes = num(kc.slots) + ", " + num(B) + ", " + num(M) + ", " + num(window) + ", ";
-  const std::string heads = std::string(elem(in[0].dt)) + ", " + num(Hq) + ", " + num(kc.heads) + ", ";
   std::ostringstream b;
-  b << "rx_paged_attention<" << heads << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << sizes << (by_slot ? "true" : "false") << ", " << NT << ", " << items << ", "
-    << (join ? "true" : "false") << ">(a0, a1, a2, a3, a4, a5, " << (lse ? "a6" : "(float*)0") << ", " << (join ? (lse ? "a7, a8" : "a6, a7") : "(float*)0, (float*)0") << ", "
+  b << "rx_paged_attention<" << elem(in[0].dt) << ", " << Hq << ", " << kc.heads << ", " << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << kc.slots << ", " << B << ", " << M << ", "
+    << window << ", " << (by_slot ? "true" : "false") << ", " << NT << ", " << stretches << ">(a0, a1, a2, a3, a4, a5, " << (lse ? "a6" : "(float*)0") << ", " << shared << ", "
     << flt(scale * 1.4426950408889634) << ");";
-  OperatorKernel k = kernel(s, "paged_attention", 256, args, (int)args.size() - 5, b.str());
-  k.grid[0] = (unsigned)grid;
+  OperatorKernel k = kernel(s, "paged_attention", 256, args, (int)args.size() - 5, b.str(), waves);
+  k.grid[0] = (unsigned)(B ? grid : 0);
   k.bytes = 2.0 * (double)in[0].bytes();   // (and what the lengths make of the caches)
   p.kernels.push_back(k);
-  if (join) {
-    args = {{operand(4), st(in[4])}, {scratch(0), "float"}, {scratch(1), "float"}, {result(0), st(s.out[0])}};
-    if (lse) args.push_back({result(1), "float"});
-    OperatorKernel j = kernel(s, "paged_attention_join", 256, args, lse ? 2 : 1,
-                              "rx_paged_attention_join<" + heads + num(vc.dim) + ", " + sizes + num(NT) + ", " + num(items) + ">(a0, a1, a2, a3, " + (lse ? "a4" : "(float*)0") + ");");
-    j.grid[0] = (unsigned)Hq;
-    j.grid[1] = (unsigned)B;
-    p.kernels.push_back(j);
-  }
   return p;
 }
 

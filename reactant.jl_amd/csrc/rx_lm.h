@@ -39,7 +39,7 @@ struct OperatorSpec {
 };
 
 struct OperatorArg {
-  enum Kind { Operand, Result, Scratch } kind;
+  enum Kind { Operand, Result, Scratch, Counters } kind;
   int index;
 };
 
@@ -56,6 +56,7 @@ struct OperatorKernel {
 
 struct OperatorPlan {
   std::vector<int64_t> scratch;    // bytes
+  int64_t counters = 0;            // 32-bit words that live with the executable, zero before and after every launch
   std::vector<int> updates;        // per result: the operand that it is an updated copy of, or -1 (none: empty)
   std::vector<OperatorKernel> kernels;
 };

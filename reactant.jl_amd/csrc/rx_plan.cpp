@@ -4141,6 +4141,17 @@ struct Planner {
     }
     std::vector<int> scratches;
     for (int64_t b : op.scratch) scratches.push_back(scratch(b));
+    int counters = -1;
+    if (op.counters) {
+      BufferDesc cb;
+      cb.kind = BufferDesc::Const;          // lives with the executable; zero when loaded
+      cb.ty.dt = DT::I32;
+      cb.ty.dims = {op.counters};
+      cb.bytes = op.counters * 4;
+      cb.data.assign((size_t)cb.bytes, 0);
+      plan.buffers.push_back(cb);
+      counters = (int)plan.buffers.size() - 1;
+    }
     for (const OperatorKernel& k : op.kernels) {
       Launch L;
       L.kernel = named("@K@_" + k.suffix, finalize(k.text));
@@ -4148,7 +4159,7 @@ struct Planner {
       for (int d = 0; d < 3; ++d) L.grid[d] = k.grid[d];
       L.block[0] = k.block;
       for (const OperatorArg& a : k.args)
-        L.args.push_back(a.kind == OperatorArg::Operand ? buffer_for(n.in[a.index]) : a.kind == OperatorArg::Result ? buffer_for(results[a.index]) : scratches[a.index]);
+        L.args.push_back(a.kind == OperatorArg::Operand ? buffer_for(n.in[a.index]) : a.kind == OperatorArg::Result ? buffer_for(results[a.index]) : a.kind == OperatorArg::Scratch ? scratches[a.index] : counters);
       L.n_outputs = k.n_outputs;
       L.algo_bytes = k.bytes;
       L.flops = k.flops;
