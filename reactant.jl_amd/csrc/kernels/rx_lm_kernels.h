@@ -435,14 +435,15 @@ RX_DEV void rx_kv_append(const typename E::S* q, const typename E::S* k, const t
 // works its stretch out from the lengths.  Sequences inside of one stretch are finished there.  Of a longer one every workgroup
 // leaves (maximum, sum, unscaled result) of its part, and the one that arrives last combines them, in the order of the
 // positions.  A workgroup has at most two such parts: one that a workgroup before it has started, and one that it starts.
-struct rx_lm_span { int n, lo, units; };   // length, first position, units from lo rounded down to 32 (an empty sequence has one)
-template <int S, int M, int W, typename I>
+struct rx_lm_span { int n, lo, units, cost; };   // length, first position, units from lo rounded down to 32 (an empty sequence has one); what it counts in the row
+template <int S, int B, int M, int W, typename I>
 RX_DEV rx_lm_span rx_lm_span_of(const I len) {
   rx_lm_span s;
   s.n = len < 0 ? 0 : len > (I)(M * S) ? M * S : (int)len;
   s.lo = W && s.n > W ? s.n - W : 0;
   s.units = (s.n - (s.lo & ~31) + 31) >> 5;
   if (s.units == 0) s.units = 1;
+  s.cost = s.units + (B > 1 ? 4 : 0);   // going over to another sequence takes as long as about four units (64 of 1 to 8192 positions: 0: 67 us, 2: 60, 4: 59, 8: 60, 12: 62)
   return s;
 }
 struct rx_lm_stretch { int b, unit, count; long long first, total; int parts; };   // sequence and its unit to start at, units; first unit in the row, units of the row, stretches
@@ -452,7 +453,7 @@ template <int S, int B, int M, int W, int R, typename I>
 RX_DEV rx_lm_stretch rx_lm_stretch_of(const I* lengths, const int r) {
   const int lane = threadIdx.x & 63;
   rx_lm_stretch s = {B, 0, 0, 0, 0, 0};
-  for (int b0 = 0; b0 < B; b0 += 64) s.total += b0 + lane < B ? rx_lm_span_of<S, M, W>(lengths[b0 + lane]).units : 0;
+  for (int b0 = 0; b0 < B; b0 += 64) s.total += b0 + lane < B ? rx_lm_span_of<S, B, M, W>(lengths[b0 + lane]).cost : 0;
   if constexpr (B > 1) s.total = rx_wave_reduce(s.total, rx_op_add());
   else s.total = rx_lane_from(s.total, 0);
   s.parts = s.total < 4ll * R ? (int)((s.total + 3) / 4) : R;
@@ -461,7 +462,7 @@ RX_DEV rx_lm_stretch rx_lm_stretch_of(const I* lengths, const int r) {
   s.count = (int)(rx_lm_stretch_start(s.total, s.parts, r + 1) - s.first);
   long long sum = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
-    const int units = b0 + lane < B ? rx_lm_span_of<S, M, W>(lengths[b0 + lane]).units : 0;
+    const int units = b0 + lane < B ? rx_lm_span_of<S, B, M, W>(lengths[b0 + lane]).cost : 0;
     const long long upto = sum + (B > 1 ? rx_wave_scan((long long)units, rx_op_add()) : (long long)units);
     const unsigned long long past = __ballot(b0 + lane < B && upto > s.first);
     if (past) {
@@ -549,13 +550,13 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
 
   int b = st.b, unit = st.unit;
   for (int left = st.count; left > 0; ++b, unit = 0) {
-  const rx_lm_span span = rx_lm_span_of<S, M, W>(lengths[b]);
-  const int take = span.units - unit < left ? span.units - unit : left;
+  const rx_lm_span span = rx_lm_span_of<S, B, M, W>(lengths[b]);
+  const int step = span.cost - unit < left ? span.cost - unit : left, take = span.units - unit < step ? span.units - unit : step;
+  const long long begin = st.first + (st.count - left) - unit;   // the sequence's first unit in the row
+  left -= step;
+  if (take <= 0) continue;
   const int p0 = (span.lo & ~31) + unit * 32, p1 = P == 0 ? p0 : p0 + take * 32 < span.n ? p0 + take * 32 : span.n;
   const bool whole = take == span.units;               // the whole sequence is in this stretch
-  const long long begin = st.first + (st.count - left) - unit;   // the sequence's first unit in the row
-  left -= take;
-
   rx_u32x4 qf[NT][NK];
 #pragma unroll
   for (int t = 0; t < NT; ++t)

@@ -324,7 +324,7 @@ OperatorPlan plan_attention(const OperatorSpec& s) {
   const int waves = 8 * nk + 32 * nv + NT * (4 * nk + 4 * nv * ne + 24) <= 196 ? 2 : 1;
   // every workgroup a stretch of at least four units of 32 positions, all of them on the chip at once
   const int64_t longest = window ? std::min(M * kc.slots, window + 31) : M * kc.slots, units = std::max<int64_t>(1, (longest + 31) / 32);
-  const int64_t stretches = std::max<int64_t>(1, std::min((getenv("RXI") ? atoi(getenv("RXI")) : 256) * waves / columns, (B * units + 3) / 4)), grid = stretches * columns;
+  const int64_t stretches = std::max<int64_t>(1, std::min(256 * waves / columns, (B * units + 3) / 4)), grid = stretches * columns;
   OperatorPlan p;
   std::vector<std::pair<OperatorArg, std::string>> args;
   for (int i = 0; i < 5; ++i) args.push_back({operand(i), st(in[i])});
