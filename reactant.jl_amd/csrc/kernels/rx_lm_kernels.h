@@ -27,7 +27,8 @@ struct rx_lm_f16 {
 // Values handed to the workgroup of the same launch that arrives last, on whichever die it runs: written and read past the
 // caches that belong to one die (device-scope atomic accesses), and counted in once the writes have arrived.  No workgroup
 // waits for another.  The counter is zero before the launch, and again after it.
-RX_DEV void rx_lm_put_shared(float* p, const float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename T>
+RX_DEV void rx_lm_put_shared(T* p, const T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <typename T>
 RX_DEV T rx_lm_get_shared(const T* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 RX_DEV bool rx_lm_last_to_arrive(int* counter, const int expected, int* flag) {
@@ -818,11 +819,19 @@ struct rx_lm_row {
   }
 };
 
-// running (maximum, sum of e^(x - maximum), sum of e^(x - maximum) log2 e^(x - maximum)): of the sums, the second gives the entropy
+// Running (maximum m, sum s of e^(x - m), sum t of e^(x - m) log2 e^(x - m)); the last gives the entropy.  An exponential is
+// 2^(x L - c), one fused multiply-add and the hardware's 2^y, with c the rounded product m L: that s belongs to c and not to m
+// is undone exactly where sums of another maximum come in and in lse.  (L is log2 e rounded to f32, off by 1e-8 of itself, which
+// turns e^x into e^(x (1 + 1e-8)).)  Beyond 1e30 the product would overflow: such maxima are not used as c, and their rows
+// come out as no number or nothing and are computed again with differences (`rx_lm_careful`).
+struct rx_lm_yes { static constexpr bool value = true; };
+struct rx_lm_no { static constexpr bool value = false; };
 struct rx_lm_sums { float m, s, t; };
+RX_DEV bool rx_lm_plain(const float m) { return __builtin_fabsf(m) < 1e30f; }
+RX_DEV float rx_lm_apart(const float m, const float of) { return rx_lm_plain(m) && rx_lm_plain(of) ? m * RX_LM_LOG2E - of * RX_LM_LOG2E : (m - of) * RX_LM_LOG2E; }
 RX_DEV rx_lm_sums rx_lm_rebase(const rx_lm_sums a, const float m) {
   if (a.m == m || a.m == -rx_lm_inf()) return {m, a.s, a.t};   // (nothing so far: the sums are 0, or NaN)
-  const float d = (a.m - m) * RX_LM_LOG2E, f = __builtin_amdgcn_exp2f(d);
+  const float d = rx_lm_apart(a.m, m), f = __builtin_amdgcn_exp2f(d);
   return {m, a.s * f, f == 0.0f ? 0.0f : (a.t + a.s * d) * f};
 }
 struct rx_op_lm_sums {
@@ -832,6 +841,47 @@ struct rx_op_lm_sums {
     return {m, x.s + y.s, x.t + y.t};
   }
 };
+RX_DEV float rx_lm_lse(const rx_lm_sums a) {
+  if (a.s == 0.0f) return -rx_lm_inf();
+  const float l = __builtin_log2f(a.s);
+  return rx_lm_plain(a.m) ? (a.m * RX_LM_LOG2E + l) * 0.6931471805599453f : a.m + l * 0.6931471805599453f;
+}
+// the sums of a workgroup's threads
+RX_DEV rx_lm_sums rx_lm_block_sums(rx_lm_sums a, rx_lm_sums* red /* 4 */) {
+  a = rx_lm_rebase(a, rx_wave_reduce(a.m, rx_op_max()));
+  a.s = rx_wave_reduce(a.s, rx_op_add());
+  a.t = rx_wave_reduce(a.t, rx_op_add());
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+  __syncthreads();
+  return rx_op_lm_sums()(rx_op_lm_sums()(red[0], red[1]), rx_op_lm_sums()(red[2], red[3]));
+}
+// elements [j0, j1) of a row with the differences from the maximum, in two passes
+template <typename E>
+RX_DEV rx_lm_sums rx_lm_careful(const typename E::S* x, const int j0, const int j1, rx_lm_sums* red) {
+  rx_lm_sums a = {-rx_lm_inf(), 0.0f, 0.0f};
+  for (int j = j0 + (int)threadIdx.x; j < j1; j += 256) a.m = __builtin_fmaxf(a.m, E::up(x[j]));
+  a.m = rx_lm_block_sums(a, red).m;
+  const float base = a.m == -rx_lm_inf() ? 0.0f : a.m;
+  for (int j = j0 + (int)threadIdx.x; j < j1; j += 256) {
+    const float d = (E::up(x[j]) - base) * RX_LM_LOG2E, p = __builtin_amdgcn_exp2f(d);
+    a.s += p;
+    a.t = __builtin_fmaf(p, __builtin_fmaxf(d, -1e30f), a.t);
+  }
+  return rx_lm_block_sums(a, red);
+}
+RX_DEV float rx_lm_max3(const float a, const float b, const float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));   // (without the compiler's quieting of its operands)
+  return r;
+}
+template <int N>
+RX_DEV float rx_lm_max_of(const float (&e)[N]) {
+  float m = rx_lm_max3(e[0], e[1], e[2]);
+#pragma unroll
+  for (int k = 3; k < N; k += 2) m = rx_lm_max3(m, e[k], e[k + 1 < N ? k + 1 : k]);
+  return m;
+}
 
 // the K largest of `n` keys in LDS (n up to what the caller holds), the i-th largest given to put(i, key)
 template <int K, typename F>
@@ -848,144 +898,162 @@ RX_DEV void rx_lm_select(const rx_u64* keys, const int n, F put) {
 template <typename E, int V, typename I>
 RX_DEV void rx_lm_row_results(const long long t, const rx_lm_sums a, const typename E::S* x, const I* targets, float* logprob, float* lse, float* entropy) {
   const I y = targets[t];
-  const float log2s = __builtin_log2f(a.s);
-  const float l = a.s == 0.0f ? -rx_lm_inf() : a.m + log2s * 0.6931471805599453f;
+  const float l = rx_lm_lse(a);
   lse[t] = l;
-  entropy[t] = a.s == 0.0f ? 0.0f : (log2s - a.t / a.s) * 0.6931471805599453f;
+  entropy[t] = a.s == 0.0f ? 0.0f : (__builtin_log2f(a.s) - a.t / a.s) * 0.6931471805599453f;
   logprob[t] = y < 0 || y >= V ? 0.0f : a.s == 0.0f ? -rx_lm_inf() : E::up(x[y]) - l;
 }
 
-// A workgroup per segment of SEG vectors of a row (SPLIT segments; one: the whole row): one pass with the running sums, and the
-// alternatives without a second one.  Every thread keeps its largest vector's maximum.  With k alternatives asked for, the
-// k-th largest of the maxima of 64 groups of threads bounds the k-th largest element from below, so only threads whose own
-// maximum reaches it hold alternatives: their elements (a few per cent of the row) are read again, and the few that reach the
-// bound are ranked.  Bounds and elements compare by (value, index), so rows of equal values need no more.  Rows with a NaN, or
-// where more than CAP elements reach the bound (the largest elements all at one thread), are searched k times.
+// A workgroup per segment of a row (SPLIT segments; one: the whole row), in one pass with the running sums, and the alternatives
+// almost without a second one.  With k alternatives asked for, the k-th largest of the maxima of 64 groups of four threads (of all
+// threads for many alternatives) is no larger than the k-th largest element.  Every thread leaves the maximum of each of its SECTIONS stretches in LDS (the upper
+// half of its order), so only the few stretches whose maximum reaches that bound are read again, and the elements that reach
+// it, hardly more than k, are ranked by (value, index).  Where too many do, because they are equal (a constant row, a mask that
+// leaves fewer than k tokens), the larger ones are taken, and of the equal ones the first in the row.  A row with a NaN, or
+// with more larger ones than LDS holds (far from any distribution), is searched k times.
+// Of a split row every workgroup leaves its sums and keys, and the one that arrives last combines them.
 template <typename E, int V, int K, int T, int SPLIT, typename I>
-RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, float* logprob, float* lse, float* entropy, float* values, int* ids, float* part_sums, rx_u64* part_keys) {
+RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, float* logprob, float* lse, float* entropy, float* values, int* ids, float* part_sums, rx_u64* part_keys,
+                              int* arrived) {
   typedef typename E::S S;
-  constexpr int NE = 16 / sizeof(S), UNROLL = 4, CAP = 2048, VECTORS = rx_lm_row<E, V>::VECTORS;
+  constexpr int NE = 16 / sizeof(S), UNROLL = 4, ROUND = 256 * UNROLL, VECTORS = rx_lm_row<E, V>::VECTORS;
+  constexpr int CAP = K * SPLIT > 1024 ? K * SPLIT : 1024, LIST = 1024;
+  constexpr int ROUNDS = ((VECTORS + SPLIT - 1) / SPLIT + ROUND - 1) / ROUND, EACH = (ROUNDS + 15) / 16, SECTIONS = (ROUNDS + EACH - 1) / EACH;   // rounds of a section
   __shared__ rx_lm_sums red[4];
-  __shared__ rx_u64 group[64], keys[K ? CAP : 1], bound, red64[4];
-  __shared__ int count, listed[256];
+  __shared__ rx_u64 keys[K ? CAP : 1], red64[4];
+  __shared__ rx_u16 reach[K ? SECTIONS : 1][256], listed[K ? LIST : 1];
+  constexpr int GROUPS = K <= 24 ? 64 : 256;                   // (the 64th of 64 would be a bound that hundreds reach)
+  __shared__ rx_u32 group[GROUPS], bound;
+  __shared__ int count, nlist, last;
   for (long long item = blockIdx.x; item < (long long)T * SPLIT; item += gridDim.x) {
     const long long t = item / SPLIT;
     const int seg = (int)(item % SPLIT), v0 = (int)((long long)VECTORS * seg / SPLIT), v1 = (int)((long long)VECTORS * (seg + 1) / SPLIT);
     const rx_lm_row<E, V> row(logits, t);
+    const int j0 = row.first(v0) > 0 ? row.first(v0) : 0, j1 = row.first(v1) < V ? row.first(v1) : V;   // its elements
     rx_lm_sums a = {-rx_lm_inf(), 0.0f, 0.0f};
-    float best = -rx_lm_inf();
-    int best_at = 0x7fffffff;                                  // vector
-    for (int v = v0 + (int)threadIdx.x; v < v1; v += 256 * UNROLL) {
+    float high = -rx_lm_inf();                                 // of the section
+    auto round = [&](const int v, auto ends) {                 // vectors v, v + 256, ..; ends: some may not be whole, or in the segment
       rx_vec<S, NE> r[UNROLL];
       float e[UNROLL][NE], top[UNROLL];
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) r[u] = row.load(v + 256 * u);
+      for (int u = 0; u < UNROLL; ++u) r[u] = decltype(ends)::value ? row.load(v + 256 * u) : row.vectors[v + 256 * u];
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
-        row.get(r[u], v + 256 * u, -rx_lm_inf(), e[u]);
-        if (SPLIT > 1 && v + 256 * u >= v1) {
+        if constexpr (decltype(ends)::value) {
+          row.get(r[u], v + 256 * u, -rx_lm_inf(), e[u]);
+          if (SPLIT > 1 && v + 256 * u >= v1) {
 #pragma unroll
-          for (int k = 0; k < NE; ++k) e[u][k] = -rx_lm_inf();
-        }
-        top[u] = e[u][0];
-#pragma unroll
-        for (int k = 1; k < NE; ++k) top[u] = __builtin_fmaxf(top[u], e[u][k]);
-        if constexpr (K > 0) {
-          if (v + 256 * u < v1 && (top[u] > best || best_at == 0x7fffffff)) {
-            best = top[u];
-            best_at = v + 256 * u;
+            for (int k = 0; k < NE; ++k) e[u][k] = -rx_lm_inf();
           }
-        }
-      }
-      float m = a.m;
+        } else {
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) m = __builtin_fmaxf(m, top[u]);
-      if (m > a.m) a = rx_lm_rebase(a, m);
-      const float base = a.m == -rx_lm_inf() ? 0.0f : a.m;
+          for (int k = 0; k < NE; ++k) e[u][k] = E::up(r[u].v[k]);
+        }
+        top[u] = rx_lm_max_of(e[u]);
+      }
+      high = rx_lm_max3(rx_lm_max3(high, top[0], top[1]), top[2], top[3]);
+      if (high > a.m) a = rx_lm_rebase(a, high);
+      const float c = rx_lm_plain(a.m) ? a.m * RX_LM_LOG2E : 0.0f;
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
         for (int k = 0; k < NE; ++k) {
-          const float d = (e[u][k] - base) * RX_LM_LOG2E, p = __builtin_amdgcn_exp2f(d);
+          const float d = __builtin_fmaf(e[u][k], RX_LM_LOG2E, -c), p = __builtin_amdgcn_exp2f(d);
           a.s += p;
           a.t = __builtin_fmaf(p, __builtin_fmaxf(d, -1e30f), a.t);   // (0 times -inf is no 0)
         }
-    }
-    // the workgroup's sums
-    {
-      const float m = rx_wave_reduce(a.m, rx_op_max());
-      a = rx_lm_rebase(a, m);
-      a.s = rx_wave_reduce(a.s, rx_op_add());
-      a.t = rx_wave_reduce(a.t, rx_op_add());
-    }
+    };
+    static_assert(UNROLL == 4, "maxima of four vectors");
     __syncthreads();                                            // (the item before is through with the LDS)
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
-    rx_u64 mine = 0;
-    if constexpr (K > 0) {
-      // not above the key of the thread's largest element: the last index of its vector
-      if (best_at != 0x7fffffff) mine = rx_lm_key(best, row.first(best_at) + NE - 1);
-      rx_u64 quad = rx_max(mine, rx_dpp_t<rx_u64, 0xB1, 0xf>(mine));
-      quad = rx_max(quad, rx_dpp_t<rx_u64, 0x4E, 0xf>(quad));
-      if ((threadIdx.x & 3) == 0) group[threadIdx.x >> 2] = quad;
-      if (threadIdx.x == 0) count = 0;
-    }
-    __syncthreads();
-    a = rx_op_lm_sums()(rx_op_lm_sums()(red[0], red[1]), rx_op_lm_sums()(red[2], red[3]));
-    if (threadIdx.x == 0) {
-      if constexpr (SPLIT == 1) rx_lm_row_results<E, V>(t, a, row.x, targets, logprob, lse, entropy);
-      else {
-        part_sums[item * 3] = a.m;
-        part_sums[item * 3 + 1] = a.s;
-        part_sums[item * 3 + 2] = a.t;
+    int at = v0 + (int)threadIdx.x, nth = 0;
+    for (int v = v0; v < v1; v += ROUND, at += ROUND, ++nth) {
+      if (v + ROUND <= v1 && row.whole(v) && row.whole(v + ROUND - 1)) round(at, rx_lm_no());
+      else round(at, rx_lm_yes());
+      if (K > 0 && (nth % EACH == EACH - 1 || v + ROUND >= v1)) {
+        reach[nth / EACH][threadIdx.x] = (rx_u16)(rx_lm_order(high) >> 16);
+        high = -rx_lm_inf();
       }
     }
+    const float own = a.m;
+    a = rx_lm_block_sums(a, red);
+    if (!(a.s < rx_lm_inf()) || (a.s == 0.0f && a.m != -rx_lm_inf())) a = rx_lm_careful<E>(row.x, j0, j1, red);
+    int n = 0;
     if constexpr (K > 0) {
-      if (threadIdx.x < 64) {
-        const rx_u64 g = group[threadIdx.x];
+      rx_u32 quad = rx_lm_order(own);
+      if constexpr (GROUPS == 64) {
+        quad = rx_max(quad, rx_dpp_t<rx_u32, 0xB1, 0xf>(quad));
+        quad = rx_max(quad, rx_dpp_t<rx_u32, 0x4E, 0xf>(quad));
+        if ((threadIdx.x & 3) == 0) group[threadIdx.x >> 2] = quad;
+      } else {
+        group[threadIdx.x] = quad;
+      }
+      if (threadIdx.x == 0) count = nlist = 0;
+      __syncthreads();
+      if (threadIdx.x < GROUPS) {
+        const rx_u32 g = group[threadIdx.x];
         int rank = 0;
-        for (int k = 0; k < 64; ++k) {
-          const rx_u64 o = group[k];
-          rank += o > g || (o == g && k < (int)threadIdx.x);    // (equal only where groups hold nothing)
+#pragma unroll 16
+        for (int k = 0; k < GROUPS; ++k) {
+          const rx_u32 o = group[k];
+          rank += o > g || (o == g && k < (int)threadIdx.x);
         }
         if (rank == K - 1) bound = g;
       }
       __syncthreads();
-      const rx_u64 least = bound;
-      // threads with elements from there on
-      if (mine >= least && mine) listed[atomicAdd(&count, 1)] = threadIdx.x;
-      __syncthreads();
-      const int nlist = count;
-      __syncthreads();
-      if (threadIdx.x == 0) count = 0;
-      __syncthreads();
-      const bool odd = a.s != a.s;
-      const int per = (v1 - v0 + 255) / 256;                    // vectors of a thread
-      if (!odd)
-        for (int k = threadIdx.x; k < nlist * per; k += 256) {
-          const int v = v0 + listed[k / per] + 256 * (k % per), j = row.first(v);
-          if (v >= v1) continue;
-          float e[NE];
-          row.get(row.load(v), v, -rx_lm_inf(), e);
-#pragma unroll
-          for (int q = 0; q < NE; ++q) {
-            const rx_u64 key = rx_lm_key(e[q], j + q);
-            if (j + q >= 0 && j + q < V && key >= least) {
-              const int at = atomicAdd(&count, 1);
-              if (at < CAP) keys[at] = key;
-            }
-          }
+      const rx_u32 least = bound;
+      auto take = [&](const float x, const int j, const bool also_equal) {
+        const rx_u32 o = rx_lm_order(x);
+        if (o > least || (also_equal && o == least)) {
+          const int i = atomicAdd(&count, 1);
+          if (i < CAP) keys[i] = rx_lm_key(x, j);
         }
-      __syncthreads();
-      int n = count;
-      if (odd || n > CAP) {
+      };
+      const bool nan = a.s != a.s;
+      if (!nan) {
+        for (int k = 0; k < nth; k += EACH)                     // sections that reach the bound
+          if (reach[k / EACH][threadIdx.x] >= least >> 16) {
+            const int i = atomicAdd(&nlist, 1);
+            if (i < LIST) listed[i] = (rx_u16)(k / EACH << 8 | threadIdx.x);
+          }
+        __syncthreads();
+        if (nlist <= LIST)
+          for (int k = threadIdx.x; k < nlist * EACH * UNROLL; k += 256) {
+            const int what = listed[k / (EACH * UNROLL)], v = v0 + (what >> 8) * (EACH * ROUND) + k % (EACH * UNROLL) * 256 + (what & 255), j = row.first(v);
+            if (v >= v1) continue;
+            float e[NE];
+            row.get(row.load(v), v, -rx_lm_inf(), e);
+#pragma unroll
+            for (int q = 0; q < NE; ++q)
+              if (j + q >= 0 && j + q < V) take(e[q], j + q, true);
+          }
+        __syncthreads();
+      }
+      n = count;
+      bool search = nan;
+      if (!nan && (nlist > LIST || n > CAP)) {
+        __syncthreads();
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+        for (int j = j0 + (int)threadIdx.x; j < j1; j += 256) take(E::up(row.x[j]), j, false);
+        __syncthreads();
+        n = count;
+        search = n > CAP - 256;
+        for (int j = j0; !search && n < K && j < j1; j += 256) {
+          const int mine = j + (int)threadIdx.x;
+          if (mine < j1 && rx_lm_order(E::up(row.x[mine])) == least) keys[atomicAdd(&count, 1)] = rx_lm_key(E::up(row.x[mine]), mine);
+          __syncthreads();
+          n = count;
+          __syncthreads();
+        }
+      }
+      if (search) {
         rx_u64 below = ~0ull;
         for (int k = 0; k < K; ++k) {
           rx_u64 top = 0;
-          for (int j = row.first(v0) + (int)threadIdx.x; j < row.first(v1); j += 256)
-            if (j >= 0 && j < V) {
-              const rx_u64 key = rx_lm_key(E::up(row.x[j]), j);
-              if (key < below && key > top) top = key;
-            }
+          for (int j = j0 + (int)threadIdx.x; j < j1; j += 256) {
+            const rx_u64 key = rx_lm_key(E::up(row.x[j]), j);
+            if (key < below && key > top) top = key;
+          }
           __syncthreads();
           top = rx_block_reduce<rx_u64, rx_op_max, 4>(top, rx_op_max(), red64);
           if (threadIdx.x == 0) keys[k] = top;
@@ -994,41 +1062,30 @@ RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, flo
         n = K;
         __syncthreads();
       }
-      const float l = a.s == 0.0f ? -rx_lm_inf() : a.m + __builtin_log2f(a.s) * 0.6931471805599453f;
-      rx_lm_select<K>(keys, n, [&](const int rank, const rx_u64 key) {
-        if constexpr (SPLIT == 1) {
-          const int j = (int)~(rx_u32)key;
-          ids[t * K + rank] = j;
-          values[t * K + rank] = a.s == 0.0f ? -rx_lm_inf() : E::up(row.x[j]) - l;
-        } else {
-          part_keys[item * K + rank] = key;
-        }
-      });
     }
-  }
-}
-// the segments of a row, in their order: a workgroup per row
-template <typename E, int V, int K, int T, int SPLIT, typename I>
-RX_DEV void rx_token_logprobs_join(const typename E::S* logits, const I* targets, const float* part_sums, const rx_u64* part_keys, float* logprob, float* lse, float* entropy, float* values,
-                                   int* ids) {
-  __shared__ rx_u64 keys[K ? K * SPLIT : 1];
-  for (long long t = blockIdx.x; t < T; t += gridDim.x) {
-    __syncthreads();
-    for (int k = threadIdx.x; k < K * SPLIT; k += 256) keys[k] = part_keys[t * SPLIT * K + k];
-    rx_lm_sums a = {-rx_lm_inf(), 0.0f, 0.0f};
-    for (int s = 0; s < SPLIT; ++s) {
-      const float* p = part_sums + (t * SPLIT + s) * 3;
-      a = rx_op_lm_sums()(a, {p[0], p[1], p[2]});
+    if constexpr (SPLIT > 1) {
+      if (threadIdx.x == 0) {
+        rx_lm_put_shared(part_sums + item * 3, a.m);
+        rx_lm_put_shared(part_sums + item * 3 + 1, a.s);
+        rx_lm_put_shared(part_sums + item * 3 + 2, a.t);
+      }
+      if constexpr (K > 0) rx_lm_select<K>(keys, n, [&](const int rank, const rx_u64 key) { rx_lm_put_shared(part_keys + item * K + rank, key); });
+      if (!rx_lm_last_to_arrive(arrived + t, SPLIT, &last)) continue;
+      if constexpr (K > 0)
+        for (int k = threadIdx.x; k < K * SPLIT; k += 256) keys[k] = rx_lm_get_shared(part_keys + t * (SPLIT * K) + k);
+      n = K * SPLIT;
+      a = {-rx_lm_inf(), 0.0f, 0.0f};
+      if (threadIdx.x < SPLIT) a = {rx_lm_get_shared(part_sums + (t * SPLIT + threadIdx.x) * 3), rx_lm_get_shared(part_sums + (t * SPLIT + threadIdx.x) * 3 + 1),
+                                    rx_lm_get_shared(part_sums + (t * SPLIT + threadIdx.x) * 3 + 2)};
+      a = rx_lm_block_sums(a, red);
     }
-    const typename E::S* x = logits + t * V;
-    if (threadIdx.x == 0) rx_lm_row_results<E, V>(t, a, x, targets, logprob, lse, entropy);
-    __syncthreads();
+    if (threadIdx.x == 0) rx_lm_row_results<E, V>(t, a, row.x, targets, logprob, lse, entropy);
     if constexpr (K > 0) {
-      const float l = a.s == 0.0f ? -rx_lm_inf() : a.m + __builtin_log2f(a.s) * 0.6931471805599453f;
-      rx_lm_select<K>(keys, K * SPLIT, [&](const int rank, const rx_u64 key) {
+      const float l = rx_lm_lse(a);
+      rx_lm_select<K>(keys, n, [&](const int rank, const rx_u64 key) {
         const int j = (int)~(rx_u32)key;
         ids[t * K + rank] = j;
-        values[t * K + rank] = a.s == 0.0f ? -rx_lm_inf() : E::up(x[j]) - l;
+        values[t * K + rank] = a.s == 0.0f ? -rx_lm_inf() : E::up(row.x[j]) - l;
       });
     }
   }

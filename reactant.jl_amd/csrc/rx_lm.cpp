@@ -383,40 +383,25 @@ OperatorPlan plan_logprobs(const OperatorSpec& s) {
   // few rows: in segments, so that every compute unit has a workgroup, of at least two rounds of a workgroup's loads
   const int64_t split = T == 0 ? 1 : std::max<int64_t>(1, std::min<int64_t>({64, (512 + T - 1) / T, vectors / 512}));
   OperatorPlan p;
-  const std::string sizes = std::string(elem(s.in[0].dt)) + ", " + num(V) + ", " + num(top) + ", " + num(T) + ", " + num(split);
-  std::vector<std::pair<OperatorArg, std::string>> in{{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}}, out, part;
-  for (size_t r = 0; r < s.out.size(); ++r) out.push_back({result((int)r), st(s.out[r])});
+  std::vector<std::pair<OperatorArg, std::string>> args{{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}};
+  for (size_t r = 0; r < s.out.size(); ++r) args.push_back({result((int)r), st(s.out[r])});
+  std::string call = "rx_token_logprobs<" + std::string(elem(s.in[0].dt)) + ", " + num(V) + ", " + num(top) + ", " + num(T) + ", " + num(split) + ">(a0, a1, a2, a3, a4, " +
+                     (top ? "a5, a6, " : "(float*)0, (int*)0, ");
   if (split > 1) {
-    p.scratch = {T * split * 12};
-    part.push_back({scratch(0), "float"});
-    if (top) {
-      p.scratch.push_back(T * split * top * 8);
-      part.push_back({scratch(1), "rx_u64"});
-    }
+    p.scratch = {T * split * 12, T * split * std::max<int64_t>(top, 1) * 8};
+    p.counters = T;
+    call += "a" + num((int64_t)args.size()) + ", a" + num((int64_t)args.size() + 1) + ", a" + num((int64_t)args.size() + 2) + ");";
+    args.push_back({scratch(0), "float"});
+    args.push_back({scratch(1), "rx_u64"});
+    args.push_back({counters(), "int"});
+  } else {
+    call += "(float*)0, (rx_u64*)0, (int*)0);";
   }
-  double bytes = (double)(s.in[0].bytes() + s.in[1].bytes());
-  for (auto& t : s.out) bytes += (double)t.bytes();
-  std::vector<std::pair<OperatorArg, std::string>> args = in;
-  const std::string none = "(float*)0, (float*)0, (float*)0, (float*)0, (int*)0", tops = top ? "" : ", (float*)0, (int*)0";
-  if (split == 1) args.insert(args.end(), out.begin(), out.end());
-  args.insert(args.end(), part.begin(), part.end());
-  OperatorKernel k = kernel(s, "token_logprobs", 256, args, (int)args.size() - 2,
-                            "rx_token_logprobs<" + sizes + ">(a0, a1, " +
-                                (split == 1 ? std::string("a2, a3, a4, ") + (top ? "a5, a6" : "(float*)0, (int*)0") + ", (float*)0, (rx_u64*)0" : none + ", a2, " + (top ? "a3" : "(rx_u64*)0")) + ");");
+  OperatorKernel k = kernel(s, "token_logprobs", 256, args, (int)args.size() - 2, call);
   k.grid[0] = (unsigned)std::min<int64_t>(T * split, kMaxGrid);
-  k.bytes = bytes;
+  k.bytes = (double)(s.in[0].bytes() + s.in[1].bytes());
+  for (auto& t : s.out) k.bytes += (double)t.bytes();
   p.kernels.push_back(k);
-  if (split > 1) {
-    args = in;
-    args.insert(args.end(), part.begin(), part.end());
-    const size_t first = args.size();
-    args.insert(args.end(), out.begin(), out.end());
-    std::string call = "rx_token_logprobs_join<" + sizes + ">(a0, a1, a2, " + (top ? "a3" : "(const rx_u64*)0");
-    for (size_t r = 0; r < out.size(); ++r) call += ", a" + num((int64_t)(first + r));
-    OperatorKernel j = kernel(s, "token_logprobs_join", 256, args, (int)out.size(), call + tops + ");");
-    j.grid[0] = (unsigned)std::min<int64_t>(T, kMaxGrid);
-    p.kernels.push_back(j);
-  }
   return p;
 }
 
