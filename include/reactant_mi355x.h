@@ -170,6 +170,9 @@ int RxExecuteNoAlloc(RxExecutable *exec, int num_args, RxBuffer **op_args, int n
 size_t RxNoAllocScratchBytes(void);
 /* Blocks until all work queued on the device's stream has finished. */
 void RxDeviceSynchronize(RxDevice *device);
+/* A future (FutureIsReady / FutureAwait / FreeFuture) of the device itself, for callers that ask for few of the futures of
+ * their executions: XLAExecuteSharded makes none where `futures` is NULL. */
+RxFuture *RxDeviceFuture(RxDevice *device);
 /* Plain 16-byte-per-lane copy kernel of `bytes` bytes, `iters` times; returns
  * the mean milliseconds per launch (HIP events).  Reference point for HBM
  * bandwidth and for scaling rocprofv3 FETCH_SIZE/WRITE_SIZE readings. */

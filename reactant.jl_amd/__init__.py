@@ -120,6 +120,7 @@ SIGNATURES = {
     "RxExecuteNoAlloc": (_i, [_vp, _i, _P(_vp), _i, _P(_vp)]),
     "RxNoAllocScratchBytes": (_sz, []),
     "RxDeviceSynchronize": (None, [_vp]),
+    "RxDeviceFuture": (_vp, [_vp]),
     "RxCalibrationCopy": (ctypes.c_float, [_vp, _sz, _i]),
     "RxMfmaCeiling": (_i, [_vp, _i, _i, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
     "RxGemmClockProbe": (_i, [_vp, _i, ctypes.POINTER(ctypes.c_double)]),
@@ -130,6 +131,7 @@ for _name, (_res, _args) in SIGNATURES.items():
     _fn.restype = _res
     _fn.argtypes = _args
 
+_execute_sharded, _buffer_pointer = lib.XLAExecuteSharded, lib.UnsafeBufferPointer   # (called often)
 _libc = ctypes.CDLL(None)
 _libc.free.argtypes = [_vp]
 
@@ -145,7 +147,8 @@ def _check():
 def _call(name, *args):
     lib.RxClearError()
     r = getattr(lib, name)(*args)
-    _check()
+    if lib.RxLastError():
+        _check()
     return r
 
 
@@ -280,23 +283,34 @@ class Client:
 
 
 class Future:
-    def __init__(self, handle):
-        self.handle = handle
+    """XLA.PJRT.Future (src/xla/PJRT/Future.jl) of an execution, one for all of its results.  The library's future completes
+    when the device has reached the point at which it is first asked, so it is made then: most are never asked."""
+    __slots__ = ("client", "device", "handle", "__weakref__")
+
+    def __init__(self, client, device):
+        self.client, self.device, self.handle = client, device, None
+
+    def _asked(self):
+        if self.handle is None and self.client.handle:
+            self.handle = _call("RxDeviceFuture", self.device)
+        return self.handle                          # none: its client is closed, which waits for the device
 
     def is_ready(self):
-        return bool(_call("FutureIsReady", self.handle))
+        return self._asked() is None or bool(_call("FutureIsReady", self.handle))
 
     def wait(self):
-        _call("FutureAwait", self.handle)
+        if self._asked() is not None:
+            _call("FutureAwait", self.handle)
 
     def __del__(self):
-        if getattr(self, "handle", None):
+        if self.handle:
             lib.FreeFuture(self.handle)
             self.handle = None
 
 
 class Buffer:
     """XLA.PJRT.Buffer: owns one device buffer handle (src/xla/PJRT/Buffer.jl)."""
+    __slots__ = ("handle", "client", "__weakref__")
 
     def __init__(self, handle, client):
         self.handle = handle
@@ -333,7 +347,7 @@ class Buffer:
         return bool(_call("BufferOnCPU", self.handle))
 
     def unsafe_pointer(self):
-        return _call("UnsafeBufferPointer", self.handle)
+        return _buffer_pointer(self.handle) or _call("UnsafeBufferPointer", self.handle)   # (0: an error, or an empty array)
 
     def to_host(self):
         """Storage array in device layout (blocking)."""
@@ -366,6 +380,7 @@ class Buffer:
 
 class AsyncBuffer:
     """Buffer plus the future of the execution that produces it (src/xla/PJRT/AsyncBuffer.jl:1-4)."""
+    __slots__ = ("buffer", "future", "__weakref__")
 
     def __init__(self, buffer, future=None):
         self.buffer = buffer
@@ -415,17 +430,17 @@ class LoadedExecutable:
 
     def execute_sharded(self, buffers, donated=None, device=None):
         """XLA.execute_sharded: returns AsyncBuffers (src/xla/PJRT/LoadedExecutable.jl:175-246)."""
-        n = len(buffers)
+        n, nres = len(buffers), self.num_results
         args = (_vp * n)(*[b.handle for b in buffers])
         don = (_u8 * n)(*[1 if d else 0 for d in donated]) if donated else None
-        nres = self.num_results
         res = (_vp * nres)()
-        futs = (_vp * nres)()
-        has = _u8(0)
         dev = device.handle if device is not None else None   # none: the executable's
-        _call("XLAExecuteSharded", self.handle, n, args, dev, don, nres, res, ctypes.byref(has), futs)
-        client, future = self.client, has.value
-        return [AsyncBuffer(Buffer(r, client), Future(f) if future else None) for r, f in zip(res, futs)]
+        _execute_sharded(self.handle, n, args, dev, don, nres, res, None, None)
+        if nres == 0 or not res[0]:                           # (every result of a call that succeeds has a handle)
+            _check()
+        client = self.client
+        future = Future(client, client.default_device().handle if device is None else dev)
+        return [AsyncBuffer(Buffer(r, client), future) for r in res]
 
     def execute_timed(self, buffers, donated=None, device=None):
         """Like execute_sharded, with a HIP event pair around every kernel launch: (buffers, ms list)."""

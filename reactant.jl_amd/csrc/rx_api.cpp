@@ -1228,6 +1228,16 @@ RX_EXPORT void RxDeviceSynchronize(RxDevice* d) {
   guarded_void([&] { check_device(d); HIP_CHECK(hipSetDevice(d->ordinal)); HIP_CHECK(hipStreamSynchronize(d->stream)); check_fault(d); });
 }
 
+RX_EXPORT RxFuture* RxDeviceFuture(RxDevice* d) {
+  return guarded([&]() -> RxFuture* {
+    check_device(d);
+    std::unique_ptr<RxFuture> f(new RxFuture);
+    f->device = d;
+    reg_add(f.get());
+    return f.release();
+  }, nullptr);
+}
+
 RX_EXPORT int RxMfmaCeiling(RxDevice* d, int kind, int zero_operands, double* tflops, double* clock_mhz) {
   return guarded([&]() -> int {
     check_device(d);
