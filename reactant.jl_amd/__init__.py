@@ -27,6 +27,7 @@ The HIP library is required: importing this package without
 libreactant_mi355x.so raises, there is no CPU path.
 """
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -393,6 +394,11 @@ class AsyncBuffer:
         return self.buffer
 
 
+@functools.lru_cache(maxsize=None)
+def _array_types(nargs, nres):
+    return _vp * nargs, _u8 * nargs, _vp * nres
+
+
 class LoadedExecutable:
     """XLA.PJRT.LoadedExecutable (src/xla/PJRT/LoadedExecutable.jl)."""
 
@@ -431,9 +437,10 @@ class LoadedExecutable:
     def execute_sharded(self, buffers, donated=None, device=None):
         """XLA.execute_sharded: returns AsyncBuffers (src/xla/PJRT/LoadedExecutable.jl:175-246)."""
         n, nres = len(buffers), self.num_results
-        args = (_vp * n)(*[b.handle for b in buffers])
-        don = (_u8 * n)(*[1 if d else 0 for d in donated]) if donated else None
-        res = (_vp * nres)()
+        pointers, flags, handles = _array_types(n, nres)
+        args = pointers(*[b.handle for b in buffers])
+        don = flags(*map(bool, donated)) if donated else None
+        res = handles()
         dev = device.handle if device is not None else None   # none: the executable's
         _execute_sharded(self.handle, n, args, dev, don, nres, res, None, None)
         if nres == 0 or not res[0]:                           # (every result of a call that succeeds has a handle)
@@ -564,7 +571,7 @@ class ConcreteRArray:
 
     def __init__(self, data, shape, dtype):
         self.data = data          # AsyncBuffer
-        self.shape = tuple(shape)  # Julia order
+        self.shape = shape if type(shape) is tuple else tuple(shape)  # Julia order
         self.dtype = dtype
         self.donated = False
 
@@ -572,12 +579,6 @@ class ConcreteRArray:
         if self.donated:
             raise ReactantInternalError("accessing the data of a donated array")  # src/Types.jl:9-26
         return self.data.synced_buffer()
-
-    def _operand(self):
-        """The buffer as an argument of an execution, which is not waited for: a device's work is ordered on one stream."""
-        if self.donated:
-            raise ReactantInternalError("accessing the data of a donated array")  # src/Types.jl:9-26
-        return self.data.buffer
 
     def to_array(self):
         """Array(x): numbers in Julia index order (float32 for narrow floats)."""
@@ -690,8 +691,11 @@ class Thunk:
         self.client = client
 
     def __call__(self, *args, donated=None, sync=False):
-        bufs = [a._operand() for a in args]
-        res = self.exec.execute_sharded(bufs, donated)
+        for a in args:
+            if a.donated:
+                raise ReactantInternalError("accessing the data of a donated array")  # src/Types.jl:9-26
+        # the arguments are not waited for: a device's work is ordered on one stream
+        res = self.exec.execute_sharded([a.data.buffer for a in args], donated)
         if donated:
             for a, d in zip(args, donated):
                 if d:
