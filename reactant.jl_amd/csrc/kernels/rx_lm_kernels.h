@@ -83,18 +83,33 @@ RX_DEV void rx_embedding(const typename E::S* table, const I* ids, typename E::S
 // list is the same every run.  `start` [V + 1] is where a row's tokens start in `order`; `row_of` is the row of a place.
 template <int V, int T, int ROWS, typename I>
 RX_DEV void rx_lm_sort(const I* ids, int* start, int* order, int* row_of) {
-  constexpr int WAVES = 16, STRETCH = ((T + WAVES - 1) / WAVES + 63) / 64 * 64;
+  constexpr int WAVES = 16, EACH = ((T + WAVES - 1) / WAVES + 63) / 64, STRETCH = EACH * 64;
+  constexpr int KEPT = EACH <= 32 ? EACH : 1;                   // a wavefront's tokens stay in registers where they fit
   __shared__ int counts[WAVES][ROWS], sums[WAVES];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r0 = blockIdx.x * ROWS, t0 = wave * STRETCH, t1 = t0 + STRETCH < T ? t0 + STRETCH : T;
+  int kept[KEPT];                                               // -1: no row of the table
+  if constexpr (KEPT == EACH) {
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) {
+      const I id = ids[t0 + lane + 64 * k < T ? t0 + lane + 64 * k : T - 1];
+      kept[k] = t0 + lane + 64 * k < T && id >= 0 && id < V ? (int)id : -1;
+    }
+  }
   for (int k = threadIdx.x; k < WAVES * ROWS; k += 1024) counts[k / ROWS][k % ROWS] = 0;
   __syncthreads();
   int below = 0;
+  auto tally = [&](const int id) {
+    if (id >= 0 && id < r0) ++below;
+    else if (id >= r0 && id < (long long)r0 + ROWS) atomicAdd(&counts[wave][id - r0], 1);
+  };
+  if constexpr (KEPT == EACH) {
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) tally(kept[k]);
+  } else {
 #pragma unroll 4
-  for (int t = t0 + lane; t < t1; t += 64) {
-    const I id = ids[t];
-    if (id >= 0 && id < V) {
-      if (id < r0) ++below;
-      else if (id < (long long)r0 + ROWS) atomicAdd(&counts[wave][(int)id - r0], 1);
+    for (int t = t0 + lane; t < t1; t += 64) {
+      const I id = ids[t];
+      tally(id >= 0 && id < V ? (int)id : -1);
     }
   }
   below = rx_wave_reduce(below, rx_op_add());
@@ -129,23 +144,30 @@ RX_DEV void rx_lm_sort(const I* ids, int* start, int* order, int* row_of) {
     __syncthreads();
   }
   if (threadIdx.x == 0 && r0 + ROWS >= V) start[V] = carry;
-#pragma unroll 4
-  for (int t = t0 + lane; t < t0 + STRETCH; t += 64) {           // (whole wavefronts: the lanes compare their rows)
-    const I id = t < t1 ? ids[t] : (I)-1;
-    const bool mine = id >= r0 && id < (long long)r0 + ROWS && id < V;
-    const int row = mine ? (int)id - r0 : -1;
+  auto place = [&](const int id, const int t) {                 // (whole wavefronts: the lanes compare their rows)
+    const bool mine = id >= r0 && id < (long long)r0 + ROWS;
+    const int row = mine ? id - r0 : -1;
     unsigned long long left = __ballot(mine);
     while (left) {
       const int leader = __builtin_ctzll(left), its = __builtin_amdgcn_readlane(row, leader);
       const unsigned long long same = __ballot(row == its);
-      int place = 0;
-      if (lane == leader) place = atomicAdd(&counts[wave][its], __popcll(same));
-      place = __builtin_amdgcn_readlane(place, leader) + __popcll(same & ((1ull << lane) - 1));
+      int at = 0;
+      if (lane == leader) at = atomicAdd(&counts[wave][its], __popcll(same));
+      at = __builtin_amdgcn_readlane(at, leader) + __popcll(same & ((1ull << lane) - 1));
       if (row == its) {
-        order[place] = t;
-        row_of[place] = (int)id;
+        order[at] = t;
+        row_of[at] = id;
       }
       left &= ~same;
+    }
+  };
+  if constexpr (KEPT == EACH) {
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) place(kept[k], t0 + lane + 64 * k);
+  } else {
+    for (int t = t0 + lane; t < t0 + STRETCH; t += 64) {
+      const I id = t < t1 ? ids[t] : (I)-1;
+      place(id >= 0 && id < V ? (int)id : -1, t);
     }
   }
 }
@@ -194,15 +216,16 @@ RX_DEV void rx_lm_put(typename O::S* out, const rx_lm_acc<VEC>& a, const float s
 // Rows of up to LONG tokens: EACH vectors of a row to a thread (C vectors a row; several short rows to a workgroup), its tokens
 // summed in their order.  A row of more would keep one thread's loads waiting for one another: those are summed in pieces, the
 // places [LONG p, LONG p + LONG) of the list by the first workgroups (a piece touches at most two such rows: it may end one
-// and start another), and joined by the next launch.
+// and start another), and the workgroup that arrives last adds a row's pieces in their order.
 template <typename E, typename O, int V, int D, int T, int VEC, int LONG, int EACH>
-RX_DEV void rx_embedding_grad_rows(const typename E::S* dy, const int* start, const int* order, const int* row_of, typename O::S* out, float* part, const float scale) {
+RX_DEV void rx_embedding_grad_rows(const typename E::S* dy, const int* start, const int* order, const int* row_of, typename O::S* out, float* part, int* arrived, const float scale) {
   constexpr int C = D / VEC, TILES = (C + 256 * EACH - 1) / (256 * EACH), NP = (T + LONG - 1) / LONG;
   constexpr int LANES = C < 256 ? C : 256, ROWS = 256 / LANES;   // threads along a row, rows of a workgroup
   if (blockIdx.x < NP * TILES) {
-    const int piece = blockIdx.x / TILES, c = blockIdx.x % TILES * (256 * EACH) + (int)threadIdx.x, all = start[V];
+    __shared__ int flag;
+    const int piece = blockIdx.x / TILES, tile = blockIdx.x % TILES, c = tile * (256 * EACH) + (int)threadIdx.x, all = start[V];
     const int a = piece * LONG, e = a + LONG < all ? a + LONG : all;
-    if (a >= e || c >= C) return;
+    if (a >= e) return;
     const int first = row_of[a], last = row_of[e - 1];
     for (int k = 0; k < 2; ++k) {
       const int row = k ? last : first;
@@ -210,10 +233,26 @@ RX_DEV void rx_embedding_grad_rows(const typename E::S* dy, const int* start, co
       const int s0 = start[row], s1 = start[row + 1];
       if (s1 - s0 <= LONG) continue;
       rx_lm_acc<VEC> sum[EACH] = {};
-      rx_lm_sum_rows<E, D, VEC, EACH>(dy, order, s0 > a ? s0 : a, s1 < e ? s1 : e, c, sum);
+      if (c < C) {
+        rx_lm_sum_rows<E, D, VEC, EACH>(dy, order, s0 > a ? s0 : a, s1 < e ? s1 : e, c, sum);
 #pragma unroll
-      for (int n = 0; n < EACH; ++n)
-        if (c + 256 * n < C) *(rx_lm_acc<VEC>*)(part + ((long long)(piece * 2 + k) * C + c + 256 * n) * VEC) = sum[n];
+        for (int n = 0; n < EACH; ++n)
+#pragma unroll
+          for (int q = 0; q < VEC; ++q)
+            if (c + 256 * n < C) rx_lm_put_shared(part + ((long long)(piece * 2 + k) * VEC + q) * C + c + 256 * n, sum[n].v[q]);
+      }
+      const int from = s0 / LONG, to = (s1 - 1) / LONG, starts = row_of[from * LONG] != row;   // its first piece's second row?
+      if (!rx_lm_last_to_arrive(arrived + from * TILES + tile, to - from + 1, &flag) || c >= C) continue;
+#pragma unroll
+      for (int n = 0; n < EACH; ++n) {
+        if (c + 256 * n >= C) break;
+        rx_lm_acc<VEC> total = {};
+#pragma unroll 4
+        for (int p = from; p <= to; ++p)
+#pragma unroll
+          for (int q = 0; q < VEC; ++q) total.v[q] += rx_lm_get_shared(part + ((long long)(p * 2 + (p == from && starts)) * VEC + q) * C + c + 256 * n);
+        rx_lm_put<O, VEC>(out + ((long long)row * C + c + 256 * n) * VEC, total, scale);
+      }
     }
     return;
   }
@@ -232,68 +271,64 @@ RX_DEV void rx_embedding_grad_rows(const typename E::S* dy, const int* start, co
       if (c + 256 * n < C) rx_lm_put<O, VEC>(out + ((long long)row * C + c + 256 * n) * VEC, sum[n], scale);
   }
 }
-// the rows of more than LONG tokens: by the workgroup of the piece that such a row starts in, its pieces in their order
-template <typename E, typename O, int V, int D, int T, int VEC, int LONG>
-RX_DEV void rx_embedding_grad_join(const int* start, const int* row_of, const float* part, typename O::S* out, const float scale) {
-  constexpr int C = D / VEC, TILES = (C + 255) / 256;
-  const int piece = blockIdx.x / TILES, c = blockIdx.x % TILES * 256 + (int)threadIdx.x, all = start[V];
-  const int a = piece * LONG, e = a + LONG < all ? a + LONG : all;
-  if (a >= e || c >= C) return;
-  const int row = row_of[e - 1], s0 = start[row], s1 = start[row + 1];
-  if (s1 - s0 <= LONG || s0 < a) return;
-  rx_lm_acc<VEC> sum = *(const rx_lm_acc<VEC>*)(part + ((long long)(piece * 2 + (row_of[a] != row)) * C + c) * VEC);
-#pragma unroll 4
-  for (int p = piece + 1; p * LONG < s1; ++p) {
-    const rx_lm_acc<VEC> next = *(const rx_lm_acc<VEC>*)(part + ((long long)p * 2 * C + c) * VEC);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) sum.v[k] += next.v[k];
-  }
-  rx_lm_put<O, VEC>(out + ((long long)row * C + c) * VEC, sum, scale);
-}
 
-// Few tokens (FEW at most): one launch, without sorting.  A workgroup takes rows of 256 vectors together, lists the tokens of
-// these rows as it goes through all of them (a wavefront's matches in the order of its lanes, the wavefronts' one after the
-// other), and every thread sums the listed tokens of its row.
+// Few tokens (up to 1024): one launch, without a sorted list in memory.  A workgroup takes the rows of about 1024 vectors, lists
+// the tokens of these rows as it goes through all of them (a wavefront's matches in the order of its lanes, the wavefronts' one
+// after the other), ranks the listed tokens by row, and every thread sums those of its vectors' rows.
 template <typename E, typename O, int V, int D, int T, int VEC, typename I>
 RX_DEV void rx_embedding_grad_few(const typename E::S* dy, const I* ids, typename O::S* out, const float scale) {
-  constexpr int C = D / VEC;
-  __shared__ int found[T], of[T], sums[4];
+  constexpr int C = D / VEC, ROWS = C < 1024 ? 1024 / C : 1, LOADS = (T + 255) / 256;
+  static_assert(LOADS <= 4, "tokens of a thread");
+  __shared__ int found[T], of[T], sorted[T], start[ROWS + 1], sums[LOADS][4];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (long long i0 = (long long)blockIdx.x * 256; i0 < (long long)V * C; i0 += (long long)gridDim.x * 256) {
-    const long long i1 = i0 + 255 < (long long)V * C ? i0 + 255 : (long long)V * C - 1;
-    const int r0 = (int)(i0 / C), r1 = (int)(i1 / C);
+  int id[LOADS];
+#pragma unroll
+  for (int k = 0; k < LOADS; ++k) {
+    const int t = k * 256 + (int)threadIdx.x;
+    const I i = ids[t < T ? t : T - 1];
+    id[k] = t < T && i >= 0 && i < V ? (int)i : -1;
+  }
+  for (long long r0 = (long long)blockIdx.x * ROWS; r0 < V; r0 += (long long)gridDim.x * ROWS) {
+    unsigned long long hits[LOADS];
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+      hits[k] = __ballot(id[k] >= r0 && id[k] < r0 + ROWS);
+      if (lane == 0) sums[k][wave] = __popcll(hits[k]);
+    }
+    __syncthreads();
     int n = 0;
-    for (int t0 = 0; t0 < T; t0 += 256) {
-      const int t = t0 + (int)threadIdx.x;
-      const I id = t < T ? ids[t] : (I)-1;
-      const bool mine = id >= r0 && id <= r1;
-      const unsigned long long hits = __ballot(mine);
-      __syncthreads();
-      if (lane == 0) sums[wave] = __popcll(hits);
-      __syncthreads();
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
       int at = n;
       for (int w = 0; w < 4; ++w) {
-        if (w < wave) at += sums[w];
-        n += sums[w];
+        if (w < wave) at += sums[k][w];
+        n += sums[k][w];
       }
-      if (mine) {
-        at += __popcll(hits & ((1ull << lane) - 1));
-        found[at] = t;
-        of[at] = (int)id;
+      if (id[k] >= r0 && id[k] < r0 + ROWS) {
+        at += __popcll(hits[k] & ((1ull << lane) - 1));
+        found[at] = k * 256 + (int)threadIdx.x;
+        of[at] = id[k] - (int)r0;
       }
     }
     __syncthreads();
-    const long long i = i0 + threadIdx.x;
-    if (i <= i1) {
-      const int row = (int)(i / C), c = (int)(i % C);
-      rx_lm_acc<VEC> sum = {};
-      for (int k = 0; k < n; ++k)
-        if (of[k] == row) {
-          const auto w = rx_load<rx_vec<typename E::S, VEC>>(dy + (long long)found[k] * D + c * VEC);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) sum.v[e] += E::up(w.v[e]);
-        }
-      rx_lm_put<O, VEC>(out + i * VEC, sum, scale);
+    for (int k = threadIdx.x; k < n; k += 256) {
+      const int row = of[k];
+      int rank = 0;
+      for (int i = 0; i < n; ++i) rank += of[i] < row || (of[i] == row && i < k);
+      sorted[rank] = found[k];
+    }
+    for (int k = threadIdx.x; k <= ROWS; k += 256) {
+      int before = 0;
+      for (int i = 0; i < n; ++i) before += of[i] < k;
+      start[k] = before;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < ROWS * C; i += 256) {
+      const int row = i / C, c = i % C;
+      if (r0 + row >= V) break;
+      rx_lm_acc<VEC> sum[1] = {};
+      rx_lm_sum_rows<E, D, VEC, 1>(dy, sorted, start[row], start[row + 1], c, sum);
+      rx_lm_put<O, VEC>(out + ((r0 + row) * C + c) * VEC, sum[0], scale);
     }
     __syncthreads();
   }

@@ -179,7 +179,8 @@ OperatorPlan plan_embedding_grad(const OperatorSpec& s) {
     OperatorKernel k = T == 0 ? kernel(s, "embedding_grad", 256, {{result(0), st(s.out[0])}}, 1, "rx_lm_zero<" + num(V * D) + ">(a0);")
                               : kernel(s, "embedding_grad", 256, {{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}, {result(0), st(s.out[0])}}, 1,
                                        "rx_embedding_grad_few<" + types + sizes + ">(a0, a1, a2, " + scale + ");");
-    k.grid[0] = (unsigned)rows_grid;
+    const int64_t lines = C < 1024 ? 1024 / C : 1;
+    k.grid[0] = (unsigned)(T == 0 ? rows_grid : std::min<int64_t>((V + lines - 1) / lines, kMaxGrid));
     k.bytes = (double)(s.in[0].bytes() + s.in[1].bytes() + s.out[0].bytes());
     p.kernels.push_back(k);
     return p;
@@ -194,14 +195,12 @@ OperatorPlan plan_embedding_grad(const OperatorSpec& s) {
   p.kernels.push_back(k);
   const int64_t each = std::min<int64_t>(2, tiles), wide_tiles = (C + 256 * each - 1) / (256 * each), lines = C < 256 ? 256 / C : 1;
   const std::string sizes = types + num(V) + ", " + num(D) + ", " + num(T) + ", " + num(vec) + ", " + num(piece);
-  k = kernel(s, "embedding_grad", 256, {{operand(0), st(s.in[0])}, {scratch(0), "int"}, {scratch(1), "int"}, {scratch(2), "int"}, {result(0), st(s.out[0])}, {scratch(3), "float"}}, 2,
-             "rx_embedding_grad_rows<" + sizes + ", " + num(each) + ">(a0, a1, a2, a3, a4, a5, " + scale + ");");
+  p.counters = pieces * wide_tiles;
+  k = kernel(s, "embedding_grad", 256,
+             {{operand(0), st(s.in[0])}, {scratch(0), "int"}, {scratch(1), "int"}, {scratch(2), "int"}, {result(0), st(s.out[0])}, {scratch(3), "float"}, {counters(), "int"}}, 3,
+             "rx_embedding_grad_rows<" + sizes + ", " + num(each) + ">(a0, a1, a2, a3, a4, a5, a6, " + scale + ");");
   k.grid[0] = (unsigned)(std::min<int64_t>((V + lines - 1) / lines * wide_tiles, kMaxGrid) + pieces * wide_tiles);
   k.bytes = (double)(s.in[0].bytes() + s.in[1].bytes() + s.out[0].bytes());
-  p.kernels.push_back(k);
-  k = kernel(s, "embedding_grad_join", 256, {{scratch(0), "int"}, {scratch(2), "int"}, {scratch(3), "float"}, {result(0), st(s.out[0])}}, 1,
-             "rx_embedding_grad_join<" + sizes + ">(a0, a1, a2, a3, " + scale + ");");
-  k.grid[0] = (unsigned)(pieces * tiles);
   p.kernels.push_back(k);
   return p;
 }
