@@ -71,7 +71,7 @@ RX_DEV void rx_embedding(const typename E::S* table, const I* ids, typename E::S
       if (i >= (long long)T * C) break;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) x[n].v[k] = known[n] ? E::down(E::up(x[n].v[k]) * scale) : E::down(0.0f);
-      rx_store(out + i * VEC, x[n]);
+      rx_store_nt(out + i * VEC, x[n]);
     }
   }
 }
@@ -407,7 +407,7 @@ RX_DEV void rx_kv_append(const typename E::S* q, const typename E::S* k, const t
         const int w = (u - (GQ + GK) * UNITS) + h * VV, head = w / (DV / NE), d = w % (DV / NE) * NE;
         if (w >= HK * DV / NE) break;
         const W x = rx_load<W>(v + t * (HK * DV) + head * DV + d);
-        if (p.page >= 0) rx_store(vc + rx_lm_slot<S, HK, DV, BY_SLOT>(p.page, p.slot, head) + d, x);
+        if (p.page >= 0) rx_store_nt(vc + rx_lm_slot<S, HK, DV, BY_SLOT>(p.page, p.slot, head) + d, x);
       }
       continue;
     }
@@ -451,8 +451,8 @@ RX_DEV void rx_kv_append(const typename E::S* q, const typename E::S* k, const t
       }
       if (query && !p.known) a = b = W{};
       if (query || p.page >= 0) {
-        rx_store(y, a);
-        if (!PAIRS && R2 && turned) rx_store(y + R2, b);
+        rx_store_nt(y, a);
+        if (!PAIRS && R2 && turned) rx_store_nt(y + R2, b);
       }
     }
   }
@@ -535,7 +535,7 @@ RX_DEV rx_u32x4 rx_lm_row16(const typename E::S* row, const int d) {
   constexpr int NE = 16 / sizeof(typename E::S);
   rx_u32x4 v = {0, 0, 0, 0};
   if constexpr (D % NE == 0) {
-    if (d < D) v = *(const rx_u32x4*)(row + d);
+    if (d < D) v = __builtin_nontemporal_load((const rx_u32x4*)(row + d));
   } else {
     rx_vec<typename E::S, NE> w{};
 #pragma unroll
@@ -686,12 +686,15 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
             for (int e = 0; e < NE; ++e) acc[t][j][e] *= shrink;
           m[t] = top;
         }
-        rx_vec<T, 8> w;
+        // The weights, in f32 for the sum.  For the product the matrix cores take them in the cache's type: as two numbers, the
+        // second what the first one's rounding leaves, since the first alone is off by as much as the result's own rounding.
+        rx_vec<T, 8> w, rest;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float p = __builtin_amdgcn_exp2f(x[i] - base + SHIFT);
-          l[t] += p;                                             // (in f32: lse is as exact as the scores)
-          w.v[i] = E::down(p);                                   // rounded to the cache's type, in which the matrix cores take it
+          l[t] += p;
+          w.v[i] = E::down(p);
+          rest.v[i] = E::down(p - E::up(w.v[i]));
         }
         if constexpr (NE == 8) {
           const rx_u32x4 p = __builtin_bit_cast(rx_u32x4, w);
@@ -703,6 +706,7 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
 #pragma unroll
               for (int k = 0; k < 4; ++k) a[k] = __builtin_amdgcn_perm(vf[j][2 * k + 1][e >> 1], vf[j][2 * k][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
               acc[t][j][e] = rx_lm_mma<E>(a, p, acc[t][j][e]);
+              acc[t][j][e] = rx_lm_mma<E>(a, __builtin_bit_cast(rx_u32x4, rest), acc[t][j][e]);
             }
         } else {
 #pragma unroll
@@ -839,7 +843,7 @@ struct rx_lm_row {
   RX_MEM rx_vec<S, NE> load(const int v) const {
     if constexpr (V >= 2 * NE) {
       const int lo = off > 0 ? 1 : 0, hi = (V + off) / NE - 1;
-      return vectors[v < lo ? lo : v > hi ? hi : v];
+      return rx_load_nt<rx_vec<S, NE>>(vectors + (v < lo ? lo : v > hi ? hi : v));
     } else {
       return rx_vec<S, NE>{};
     }
@@ -971,7 +975,7 @@ RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, flo
       rx_vec<S, NE> r[UNROLL];
       float e[UNROLL][NE], top[UNROLL];
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) r[u] = decltype(ends)::value ? row.load(v + 256 * u) : row.vectors[v + 256 * u];
+      for (int u = 0; u < UNROLL; ++u) r[u] = decltype(ends)::value ? row.load(v + 256 * u) : rx_load_nt<rx_vec<S, NE>>(row.vectors + v + 256 * u);
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
         if constexpr (decltype(ends)::value) {

@@ -140,7 +140,7 @@ OperatorPlan plan_embedding(const OperatorSpec& s) {
   OperatorPlan p;
   const int vec = (int)(16 / info(s.in[0].dt).size);
   const bool whole = D % vec == 0;
-  const int64_t per = whole ? vec : 1, each = 4;
+  const int64_t per = whole ? vec : 1, each = 2;
   OperatorKernel k = kernel(s, "embedding", 256, {{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}, {result(0), st(s.out[0])}}, 1,
                             std::string("rx_embedding<") + elem(s.in[0].dt) + ", " + num(V) + ", " + num(D) + ", " + num(T) + ", " + num(whole ? vec : 1) + ", " + num(each) +
                                 ">(a0, a1, a2, " + flt(c.number("scale", 1.0)) + ");");
@@ -266,7 +266,7 @@ OperatorPlan plan_append(const OperatorSpec& s) {
   std::ostringstream b;
   const int64_t ne = 16 / info(in[0].dt).size, HQ = in[0].dims[1];
   const bool pairs = rotation == "pairs", whole = kc.dim % ne == 0 && vc.dim % ne == 0 && 2 * R2 % ne == 0 && (pairs || R2 % ne == 0);
-  const int64_t heads = T >= 256 ? 4 : 1;
+  const int64_t heads = T >= 256 ? 2 : 1;
   b << (whole ? "rx_kv_append<" : "rx_kv_append_any<") << elem(in[0].dt) << ", " << HQ << ", " << kc.heads << ", " << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << kc.slots << ", "
     << in[7].dims[0] << ", " << in[7].dims[1] << ", " << in[3].dims[0] << ", " << R2 << ", " << (pairs ? "true" : "false") << ", " << (by_slot ? "true" : "false") << ", " << T
     << (whole ? ", " + num(heads) : std::string()) << ">(a0, a1, a2, a3, a4, a5, a6, a7, a8, a9, a10);";
