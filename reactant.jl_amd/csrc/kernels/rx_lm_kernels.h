@@ -530,12 +530,12 @@ RX_DEV float rx_lm_sum4(float x) {
 }
 
 // 16 bytes of a head's row from element d on; zeros past its end (D: elements of the row)
-template <typename E, int D>
+template <typename E, int D, bool ONCE = false>
 RX_DEV rx_u32x4 rx_lm_row16(const typename E::S* row, const int d) {
   constexpr int NE = 16 / sizeof(typename E::S);
   rx_u32x4 v = {0, 0, 0, 0};
   if constexpr (D % NE == 0) {
-    if (d < D) v = __builtin_nontemporal_load((const rx_u32x4*)(row + d));
+    if (d < D) v = ONCE ? __builtin_nontemporal_load((const rx_u32x4*)(row + d)) : *(const rx_u32x4*)(row + d);
   } else {
     rx_vec<typename E::S, NE> w{};
 #pragma unroll
@@ -560,13 +560,15 @@ RX_DEV rx_f32x4 rx_lm_mma(const rx_u32x4 a, const rx_u32x4 b, rx_f32x4 c) {
   }
 }
 
-// COLUMNS: key heads, times the tiles of up to 16 NT query heads that read one; R: stretches; JOIN: a sequence can be longer than a stretch
-template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int NT, int R, typename I>
+// HW: key heads of a workgroup, whose four wavefronts share the units of a head, or have a head each; COLUMNS: groups of HW key
+// heads, times the tiles of up to 16 NT query heads that read one; R: stretches; ONCE: the caches are read past the L2; DIES: a
+// stretch's columns are neighbours on one die
+template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int NT, int R, int HW, bool ONCE, bool DIES, typename I>
 RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, const typename E::S* vc, const I* pages, const I* lengths, typename E::S* out, float* lse,
                                float* part, float* stat, int* arrived, const float scale) {
   typedef typename E::S T;
   constexpr int NE = 16 / sizeof(T);                   // elements of 16 bytes
-  constexpr int G = HQ / HK, GT = G < 16 * NT ? G : 16 * NT, TILES = (G + GT - 1) / GT, COLUMNS = HK * TILES;
+  constexpr int G = HQ / HK, GT = G < 16 * NT ? G : 16 * NT, TILES = (G + GT - 1) / GT, COLUMNS = HK / HW * TILES, WPH = 4 / HW;
   constexpr int NK = (DK + 4 * NE - 1) / (4 * NE);     // 16-byte loads of a position's key by its four lanes
   constexpr int NV = (DV + 16 * NE - 1) / (16 * NE);   // of a position's value by sixteen lanes
   constexpr int BLOCK = 2048;                          // positions whose pages are held in LDS
@@ -579,8 +581,9 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
   __shared__ float join_m[4][16], join_l[4][16];
   __shared__ int last;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
-  const int column = blockIdx.x % COLUMNS, mine = blockIdx.x / COLUMNS, head = column / TILES, tile = column % TILES;
-  const int h0 = head * G + tile * GT;                 // first query head
+  const int id = DIES ? (int)rx_xcd_remap(blockIdx.x, R * COLUMNS) : (int)blockIdx.x, column = id % COLUMNS, mine = id / COLUMNS, tile = column % TILES;
+  const int head0 = column / TILES * HW, head = head0 + wave / WPH;
+  const int h0 = head * G + tile * GT;                 // first query head of this wavefront
   const int heads = G - tile * GT < GT ? G - tile * GT : GT;
   const rx_lm_stretch st = rx_lm_stretch_of<S, B, M, W, R>(lengths, mine);
 
@@ -623,7 +626,7 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
     __syncthreads();
     // page of a position, -1 where it is not to be looked at
     auto where = [&](const int t) { return t >= span.lo && t < s1 ? lds.page[t / S - page0] : -1; };
-    for (int t0 = s0 + wave * 32; t0 < s1; t0 += 128) {
+    for (int t0 = s0 + wave % WPH * 32; t0 < s1; t0 += WPH * 32) {
       const int ta = t0 + r, tb = ta + 16, pa = where(ta), pb = where(tb);
       const unsigned ok = ((unsigned)__ballot(pa >= 0) & 0xffffu) | ((unsigned)__ballot(pb >= 0) << 16);
       if (!ok) continue;
@@ -632,8 +635,8 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
       const T* kb = kc + rx_lm_slot<S, HK, DK, BY_SLOT>(pb < 0 ? 0 : pb, tb % S, head);
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
-        kf[0][k] = rx_lm_row16<E, DK>(ka, (k * 4 + g4) * NE);
-        kf[1][k] = rx_lm_row16<E, DK>(kb, (k * 4 + g4) * NE);
+        kf[0][k] = rx_lm_row16<E, DK, ONCE>(ka, (k * 4 + g4) * NE);
+        kf[1][k] = rx_lm_row16<E, DK, ONCE>(kb, (k * 4 + g4) * NE);
       }
       // values of positions t0 + 4 g4 + (0..3) and 16 further: where a page's slots are a multiple of four, on two pages
       int pv = 0;
@@ -646,7 +649,7 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
         }
         const T* v = vc + rx_lm_slot<S, HK, DV, BY_SLOT>(pv < 0 ? 0 : pv, tv % S, head);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) vf[j][i] = rx_lm_row16<E, DV>(v, (j * 16 + r) * NE);
+        for (int j = 0; j < NV; ++j) vf[j][i] = rx_lm_row16<E, DV, ONCE>(v, (j * 16 + r) * NE);
       }
       const unsigned mine = (ok >> (g4 * 4)) & 0x000f000fu;      // bit i: position 4 g4 + i, bit 16 + i: 16 further
       if (ok != ~0u) {
@@ -658,6 +661,9 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
             for (int j = 0; j < NV; ++j) vf[j][i] = rx_u32x4{0, 0, 0, 0};
           }
       }
+      // The weights, in f32 for the sum.  For the product the matrix cores take them in the cache's type: as two numbers, the
+      // second what the first one's rounding leaves, since the first alone is off by as much as the result's own rounding.
+      rx_vec<T, 8> w[NT], rest[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         rx_f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -686,38 +692,35 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
             for (int e = 0; e < NE; ++e) acc[t][j][e] *= shrink;
           m[t] = top;
         }
-        // The weights, in f32 for the sum.  For the product the matrix cores take them in the cache's type: as two numbers, the
-        // second what the first one's rounding leaves, since the first alone is off by as much as the result's own rounding.
-        rx_vec<T, 8> w, rest;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float p = __builtin_amdgcn_exp2f(x[i] - base + SHIFT);
           l[t] += p;
-          w.v[i] = E::down(p);
-          rest.v[i] = E::down(p - E::up(w.v[i]));
-        }
-        if constexpr (NE == 8) {
-          const rx_u32x4 p = __builtin_bit_cast(rx_u32x4, w);
-#pragma unroll
-          for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              rx_u32x4 a;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) a[k] = __builtin_amdgcn_perm(vf[j][2 * k + 1][e >> 1], vf[j][2 * k][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-              acc[t][j][e] = rx_lm_mma<E>(a, p, acc[t][j][e]);
-              acc[t][j][e] = rx_lm_mma<E>(a, __builtin_bit_cast(rx_u32x4, rest), acc[t][j][e]);
-            }
-        } else {
-#pragma unroll
-          for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int e = 0; e < NE; ++e)
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                acc[t][j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(rx_f32x4, vf[j][i])[e], w.v[i], acc[t][j][e], 0, 0, 0);
+          w[t].v[i] = E::down(p);
+          rest[t].v[i] = E::down(p - E::up(w[t].v[i]));
         }
       }
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          if constexpr (NE == 8) {
+            rx_u32x4 a;                                          // dimension 8 r + e of the eight positions
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a[k] = __builtin_amdgcn_perm(vf[j][2 * k + 1][e >> 1], vf[j][2 * k][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              acc[t][j][e] = rx_lm_mma<E>(a, __builtin_bit_cast(rx_u32x4, w[t]), acc[t][j][e]);
+              acc[t][j][e] = rx_lm_mma<E>(a, __builtin_bit_cast(rx_u32x4, rest[t]), acc[t][j][e]);
+            }
+          } else {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                acc[t][j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(rx_f32x4, vf[j][i])[e], w[t].v[i], acc[t][j][e], 0, 0, 0);
+          }
+        }
     }
   }
 
@@ -734,7 +737,7 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
     __syncthreads();
     float top = -rx_lm_inf();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = __builtin_fmaxf(top, join_m[w][r]);
+    for (int w = 0; w < WPH; ++w) top = __builtin_fmaxf(top, join_m[wave / WPH * WPH + w][r]);
     const float f = top == -rx_lm_inf() ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -749,24 +752,24 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
           }
       }
       __syncthreads();
-      for (int k = threadIdx.x; k < HR * WIDTH; k += 256) {
-        const int h = k / WIDTH, d = j * 16 * NE + k % WIDTH;
-        if (t * 16 + h >= heads) break;
-        if (d >= DV) continue;
+      for (int k = threadIdx.x; k < HW * HR * WIDTH; k += 256) {
+        const int hw = k / (HR * WIDTH), h = k / WIDTH % HR, d = j * 16 * NE + k % WIDTH;
+        if (t * 16 + h >= heads || d >= DV) continue;
         float o = 0.0f, sum = 0.0f, hi = -rx_lm_inf();
 #pragma unroll
-        for (int w = 0; w < 4; ++w) hi = __builtin_fmaxf(hi, join_m[w][h]);
+        for (int i = 0; i < WPH; ++i) hi = __builtin_fmaxf(hi, join_m[hw * WPH + i][h]);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int i = 0; i < WPH; ++i) {
+          const int w = hw * WPH + i;
           o += lds.o[w][h][k % WIDTH];
           sum += hi == -rx_lm_inf() ? 0.0f : join_l[w][h] * __builtin_amdgcn_exp2f(join_m[w][h] - hi);
         }
-        const int qh = h0 + t * 16 + h;
+        const int qh = (head0 + hw) * G + tile * GT + t * 16 + h;
         if (whole) {
           out[((long long)b * HQ + qh) * DV + d] = E::down(sum == 0.0f ? 0.0f : o / sum);
           if (lse && d == 0) lse[(long long)b * HQ + qh] = sum == 0.0f ? -rx_lm_inf() : (hi - SHIFT + __builtin_log2f(sum)) * 0.6931471805599453f;
         } else {
-          const long long at = ((long long)blockIdx.x * 2 + (unit == 0)) * GT + t * 16 + h;
+          const long long at = (((long long)id * 2 + (unit == 0)) * HW + hw) * GT + t * 16 + h;
           rx_lm_put_shared(part + at * DV + d, o);
           if (d == 0) {
             rx_lm_put_shared(stat + at * 2, hi - SHIFT);
@@ -779,15 +782,15 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
   if (whole) continue;
   const int from = rx_lm_stretch_with(st.total, st.parts, begin), to = rx_lm_stretch_with(st.total, st.parts, begin + span.units - 1);
   if (!rx_lm_last_to_arrive(arrived + b * COLUMNS + column, to - from + 1, &last)) continue;
-  for (int k = threadIdx.x; k < heads * DV; k += 256) {
-    const int h = k / DV, d = k % DV;
+  for (int k = threadIdx.x; k < HW * heads * DV; k += 256) {
+    const int hw = k / (heads * DV), h = k / DV % heads, d = k % DV, qh = (head0 + hw) * G + tile * GT + h;
     float o = 0.0f, sum = 0.0f, top = -rx_lm_inf();
     for (int w = from; w <= to; w += 8) {
       float pm[8], ps[8], po[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int v = w + i <= to ? w + i : to;
-        const long long at = ((long long)(v * COLUMNS + column) * 2 + (v == from)) * GT + h;
+        const long long at = (((long long)(v * COLUMNS + column) * 2 + (v == from)) * HW + hw) * GT + h;
         pm[i] = rx_lm_get_shared(stat + at * 2);
         ps[i] = rx_lm_get_shared(stat + at * 2 + 1);
         po[i] = rx_lm_get_shared(part + at * DV + d);
@@ -808,8 +811,8 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
       }
       top = hi;
     }
-    out[((long long)b * HQ + h0 + h) * DV + d] = E::down(sum == 0.0f ? 0.0f : o / sum);
-    if (lse && d == 0) lse[(long long)b * HQ + h0 + h] = sum == 0.0f ? -rx_lm_inf() : (top + __builtin_log2f(sum)) * 0.6931471805599453f;
+    out[((long long)b * HQ + qh) * DV + d] = E::down(sum == 0.0f ? 0.0f : o / sum);
+    if (lse && d == 0) lse[(long long)b * HQ + qh] = sum == 0.0f ? -rx_lm_inf() : (top + __builtin_log2f(sum)) * 0.6931471805599453f;
   }
   }
 }

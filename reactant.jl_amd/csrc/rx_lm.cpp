@@ -316,13 +316,27 @@ OperatorPlan plan_attention(const OperatorSpec& s) {
   const double scale = c.number("scale", 1.0 / std::sqrt((double)kc.dim));
   const int64_t window = std::min<int64_t>(c.integer("window", 0), kMaxRow);
   const bool lse = s.out.size() == 2;
-  const int64_t G = Hq / kc.heads, NT = G > 16 ? 2 : 1, tiles = (G + 16 * NT - 1) / (16 * NT), columns = kc.heads * tiles, GT = std::min(G, 16 * NT);
   // Registers of a wavefront: a step's keys and values, the queries, the result, and room for the rest.  Up to 256 of them two
-  // wavefronts share a SIMD, and two workgroups a compute unit.
-  const int64_t ne = 16 / info(in[0].dt).size, nk = (kc.dim + 4 * ne - 1) / (4 * ne), nv = (vc.dim + 16 * ne - 1) / (16 * ne);
-  const int waves = 8 * nk + 32 * nv + NT * (4 * nk + 4 * nv * ne + 24) <= 196 ? 2 : 1;
-  // every workgroup a stretch of at least four units of 32 positions, all of them on the chip at once
+  // wavefronts share a SIMD, and two workgroups a compute unit.  The more query heads a wavefront takes, the fewer times the
+  // cache is read (64 of one key head, 16 sequences of 61035: in tiles of 32 TILES32 us, of 64 TILES64).
+  const int64_t e = info(in[0].dt).size, ne = 16 / e, nk = (kc.dim + 4 * ne - 1) / (4 * ne), nv = (vc.dim + 16 * ne - 1) / (16 * ne);
+  const int64_t G = Hq / kc.heads;
+  auto registers = [&](int64_t n) { return 8 * nk + 32 * nv + n * (4 * nk + 4 * nv * ne + 24); };
+  int64_t NT = std::min<int64_t>(4, (G + 15) / 16);
+  while (NT > 1 && registers(NT) > 440) --NT;
+  const int64_t tiles = (G + 16 * NT - 1) / (16 * NT), GT = std::min(G, 16 * NT);
+  const int waves = registers(NT) <= 196 ? 2 : 1;
   const int64_t longest = window ? std::min(M * kc.slots, window + 31) : M * kc.slots, units = std::max<int64_t>(1, (longest + 31) / 32);
+  // A position's heads lie next to one another in a cache of slots: two heads to a workgroup read longer runs (16 sequences, 8 key
+  // heads of 128 and 64 dimensions in bf16: 5.3 -> 5.7 and 4.5 -> 5.0 TB/s; four heads 5.6 and 5.0).  Its parts of long sequences are
+  // twice as many, which costs more where a key head has many query heads, and where there may be few positions.
+  const int64_t HW = by_slot && kc.heads % 2 == 0 && kc.heads >= 4 && kc.dim * e <= 256 && G <= 8 && B * units * kc.heads >= 4096 ? 2 : 1;
+  // Rows of whole 256 bytes are read once and past the L2 (4.3 GB: 717 -> 630 us); of others it holds the lines that two reads share
+  // (rows of 160 bytes, one head to a workgroup: 4.1 TB/s against 3.4), and better so where the neighbouring heads' workgroups are on
+  // one die (4.6).
+  const bool once = kc.dim * e % 256 == 0 && vc.dim * e % 256 == 0 && tiles == 1, dies = by_slot && kc.dim * e % 128 != 0;
+  const int64_t columns = kc.heads / HW * tiles;
+  // every workgroup a stretch of at least four units of 32 positions, all of them on the chip at once
   const int64_t stretches = std::max<int64_t>(1, std::min(256 * waves / columns, (B * units + 3) / 4)), grid = stretches * columns;
   OperatorPlan p;
   std::vector<std::pair<OperatorArg, std::string>> args;
@@ -331,7 +345,7 @@ OperatorPlan plan_attention(const OperatorSpec& s) {
   if (lse) args.push_back({result(1), "float"});
   std::string shared = "(float*)0, (float*)0, (int*)0";
   if (stretches > 1) {
-    p.scratch = {grid * 2 * GT * vc.dim * 4, grid * 2 * GT * 8};
+    p.scratch = {grid * 2 * HW * GT * vc.dim * 4, grid * 2 * HW * GT * 8};
     p.counters = B * columns;
     args.push_back({scratch(0), "float"});
     args.push_back({scratch(1), "float"});
@@ -340,7 +354,8 @@ OperatorPlan plan_attention(const OperatorSpec& s) {
   }
   std::ostringstream b;
   b << "rx_paged_attention<" << elem(in[0].dt) << ", " << Hq << ", " << kc.heads << ", " << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << kc.slots << ", " << B << ", " << M << ", "
-    << window << ", " << (by_slot ? "true" : "false") << ", " << NT << ", " << stretches << ">(a0, a1, a2, a3, a4, a5, " << (lse ? "a6" : "(float*)0") << ", " << shared << ", "
+    << window << ", " << (by_slot ? "true" : "false") << ", " << NT << ", " << stretches << ", " << HW << ", "
+    << (once ? "true" : "false") << ", " << (dies ? "true" : "false") << ">(a0, a1, a2, a3, a4, a5, " << (lse ? "a6" : "(float*)0") << ", " << shared << ", "
     << flt(scale * 1.4426950408889634) << ");";
   OperatorKernel k = kernel(s, "paged_attention", 256, args, (int)args.size() - 5, b.str(), waves);
   k.grid[0] = (unsigned)(B ? grid : 0);
