@@ -316,16 +316,17 @@ OperatorPlan plan_attention(const OperatorSpec& s) {
   const double scale = c.number("scale", 1.0 / std::sqrt((double)kc.dim));
   const int64_t window = std::min<int64_t>(c.integer("window", 0), kMaxRow);
   const bool lse = s.out.size() == 2;
-  // Registers of a wavefront: a step's keys and values, the queries, the result, and room for the rest.  Up to 256 of them two
-  // wavefronts share a SIMD, and two workgroups a compute unit.  The more query heads a wavefront takes, the fewer times the
-  // cache is read (64 of one key head, 16 sequences of 61035: in tiles of 32 TILES32 us, of 64 TILES64).
+  // A wavefront takes up to 32 query heads of a key head: 64 of one key head over 16 sequences of 61035 positions in bf16 take 293 us
+  // in tiles of 16, 166 us in tiles of 32, 181 us in one of 64; of more than 128 dimensions tiles of 32 do not fit the registers.
+  // Registers of a wavefront: a step's keys and values, the queries, the result, and room for the rest, of which 32-bit values need
+  // less.  Up to 256 of them two wavefronts share a SIMD, and two workgroups a compute unit: 8 heads of 128 dimensions in f32, an
+  // estimate of 216, 94 us with two and 102 with one; 32 heads in bf16, an estimate of 208, 145 and 118.
   const int64_t e = info(in[0].dt).size, ne = 16 / e, nk = (kc.dim + 4 * ne - 1) / (4 * ne), nv = (vc.dim + 16 * ne - 1) / (16 * ne);
   const int64_t G = Hq / kc.heads;
   auto registers = [&](int64_t n) { return 8 * nk + 32 * nv + n * (4 * nk + 4 * nv * ne + 24); };
-  int64_t NT = std::min<int64_t>(4, (G + 15) / 16);
-  while (NT > 1 && registers(NT) > 440) --NT;
+  const int64_t NT = G > 16 && registers(2) < 320 ? 2 : 1;
   const int64_t tiles = (G + 16 * NT - 1) / (16 * NT), GT = std::min(G, 16 * NT);
-  const int waves = registers(NT) <= 196 ? 2 : 1;
+  const int waves = registers(NT) <= (e == 4 ? 230 : 196) ? 2 : 1;
   const int64_t longest = window ? std::min(M * kc.slots, window + 31) : M * kc.slots, units = std::max<int64_t>(1, (longest + 31) / 32);
   // A position's heads lie next to one another in a cache of slots: two heads to a workgroup read longer runs (16 sequences, 8 key
   // heads of 128 and 64 dimensions in bf16: 5.3 -> 5.7 and 4.5 -> 5.0 TB/s; four heads 5.6 and 5.0).  Its parts of long sequences are
@@ -333,8 +334,8 @@ OperatorPlan plan_attention(const OperatorSpec& s) {
   const int64_t HW = by_slot && kc.heads % 2 == 0 && kc.heads >= 4 && kc.dim * e <= 256 && G <= 8 && B * units * kc.heads >= 4096 ? 2 : 1;
   // Rows of whole 256 bytes are read once and past the L2 (4.3 GB: 717 -> 630 us); of others it holds the lines that two reads share
   // (rows of 160 bytes, one head to a workgroup: 4.1 TB/s against 3.4), and better so where the neighbouring heads' workgroups are on
-  // one die (4.6).
-  const bool once = kc.dim * e % 256 == 0 && vc.dim * e % 256 == 0 && tiles == 1, dies = by_slot && kc.dim * e % 128 != 0;
+  // one die (4.6).  So it is with the tiles of one key head (64 query heads: 194 us past the L2, 171 through it, 166 on one die).
+  const bool once = kc.dim * e % 256 == 0 && vc.dim * e % 256 == 0 && tiles == 1, dies = (by_slot && kc.dim * e % 128 != 0) || tiles > 1;
   const int64_t columns = kc.heads / HW * tiles;
   // every workgroup a stretch of at least four units of 32 positions, all of them on the chip at once
   const int64_t stretches = std::max<int64_t>(1, std::min(256 * waves / columns, (B * units + 3) / 4)), grid = stretches * columns;
