@@ -954,9 +954,9 @@ void load_plan(RxExecutable* ex, rx::PlanOptions opt) {
   }
   HIP_CHECK(hipStreamSynchronize(d->stream));   // pageable host data: wait before the plan may move
   // Steps that run as maps keep more arrays than their chain, with the same results: RxExecuteNoAlloc runs the chain where
-  // that is what its memory holds.
-  if (!opt.chains_first && ex->plan.unchained_steps && ex->plan.temporary_bytes() > (int64_t)RX_NOALLOC_SCRATCH_BYTES) {
-    opt.chains_first = true;
+  // that is what its memory holds.  So it is with operators that keep partial results (which come out in other roundings).
+  if ((ex->plan.unchained_steps || ex->plan.lean_operators) && ex->plan.temporary_bytes() > (int64_t)RX_NOALLOC_SCRATCH_BYTES) {
+    opt.chains_first = opt.lean_operators = true;
     if (plan_module(ex->text.data(), ex->text.size(), opt).temporary_bytes() > (int64_t)RX_NOALLOC_SCRATCH_BYTES) return;
     ex->small.reset(new RxExecutable);
     ex->small->client = ex->client;

@@ -20,6 +20,7 @@ const OpName kOperators[] = {
 constexpr int kMaxHeadDim = 256;
 constexpr int64_t kMaxTop = 64;
 constexpr int64_t kMaxGrid = (int64_t)1 << 22;   // workgroups; kernels with more items than that go on with the next ones
+constexpr int64_t kLeanBytes = (int64_t)1 << 20;  // of partial results in a lean plan
 constexpr int64_t kMaxRow = (int64_t)1 << 30;   // elements of a row or rows of a table: 32-bit indices inside a row
 
 struct Checker {
@@ -166,7 +167,7 @@ void check_embedding_grad(const Checker& c) {
   c.require(out.dims[0] <= kMaxRow && out.dims[1] <= kMaxRow, "the table is too large");
   c.require(ids.numel() <= kMaxRow, "too many tokens");
 }
-OperatorPlan plan_embedding_grad(const OperatorSpec& s) {
+OperatorPlan plan_embedding_grad(const OperatorSpec& s, bool lean) {
   const Checker c{s};
   const int64_t V = s.out[0].dims[0], D = s.out[0].dims[1], T = s.in[1].numel();
   const std::string scale = flt(c.number("scale", 1.0)), types = std::string(elem(s.in[0].dt)) + ", " + elem(s.out[0].dt) + ", ";
@@ -187,7 +188,8 @@ OperatorPlan plan_embedding_grad(const OperatorSpec& s) {
   }
   // 256 workgroups sort, or as many as keep their rows' counters in LDS
   const int64_t rows = std::min<int64_t>(512, (V + 255) / 256);
-  const int64_t piece = std::max<int64_t>(64, (T + 255) / 256), pieces = (T + piece - 1) / piece, tiles = (C + 255) / 256;
+  const int64_t parts = lean ? std::max<int64_t>(1, std::min<int64_t>(256, kLeanBytes / (8 * D))) : 256;
+  const int64_t piece = std::max<int64_t>(64, (T + parts - 1) / parts), pieces = (T + piece - 1) / piece, tiles = (C + 255) / 256;
   p.scratch = {(V + 1) * 4, T * 4, T * 4, pieces * 2 * D * 4};
   OperatorKernel k = kernel(s, "embedding_sort", 1024, {{operand(1), st(s.in[1])}, {scratch(0), "int"}, {scratch(1), "int"}, {scratch(2), "int"}}, 3,
                             "rx_lm_sort<" + num(V) + ", " + num(T) + ", " + num(rows) + ">(a0, a1, a2, a3);");
@@ -307,7 +309,7 @@ void check_attention(const Checker& c) {
   c.require(B <= 65535 && Hq <= 65535, "too many sequences or heads");
   c.require(B * Hq * std::max<int64_t>(vc.dim, 1) <= kMaxRow, "too many sequences and heads");
 }
-OperatorPlan plan_attention(const OperatorSpec& s) {
+OperatorPlan plan_attention(const OperatorSpec& s, bool lean) {
   const Checker c{s};
   const auto& in = s.in;
   const bool by_slot = c.word("layout", "slots", {"slots", "heads"}) == "slots";
@@ -331,14 +333,15 @@ OperatorPlan plan_attention(const OperatorSpec& s) {
   // A position's heads lie next to one another in a cache of slots: two heads to a workgroup read longer runs (16 sequences, 8 key
   // heads of 128 and 64 dimensions in bf16: 5.3 -> 5.7 and 4.5 -> 5.0 TB/s; four heads 5.6 and 5.0).  Its parts of long sequences are
   // twice as many, which costs more where a key head has many query heads, and where there may be few positions.
-  const int64_t HW = by_slot && kc.heads % 2 == 0 && kc.heads >= 4 && kc.dim * e <= 256 && G <= 8 && B * units * kc.heads >= 4096 ? 2 : 1;
+  const int64_t HW = by_slot && kc.heads % 2 == 0 && kc.heads >= 4 && kc.dim * e <= 256 && G <= 8 && B * units * kc.heads >= 4096 && !lean ? 2 : 1;
   // Rows of whole 256 bytes are read once and past the L2 (4.3 GB: 717 -> 630 us); of others it holds the lines that two reads share
   // (rows of 160 bytes, one head to a workgroup: 4.1 TB/s against 3.4), and better so where the neighbouring heads' workgroups are on
   // one die (4.6).  So it is with the tiles of one key head (64 query heads: 194 us past the L2, 171 through it, 166 on one die).
   const bool once = kc.dim * e % 256 == 0 && vc.dim * e % 256 == 0 && tiles == 1, dies = (by_slot && kc.dim * e % 128 != 0) || tiles > 1;
   const int64_t columns = kc.heads / HW * tiles;
   // every workgroup a stretch of at least four units of 32 positions, all of them on the chip at once
-  const int64_t stretches = std::max<int64_t>(1, std::min(256 * waves / columns, (B * units + 3) / 4)), grid = stretches * columns;
+  const int64_t part = 2 * HW * GT * (vc.dim * 4 + 8), most = lean ? std::min<int64_t>(256 * waves, kLeanBytes / part) : 256 * waves;
+  const int64_t stretches = std::max<int64_t>(1, std::min(most / columns, (B * units + 3) / 4)), grid = stretches * columns;
   OperatorPlan p;
   std::vector<std::pair<OperatorArg, std::string>> args;
   for (int i = 0; i < 5; ++i) args.push_back({operand(i), st(in[i])});
@@ -473,11 +476,11 @@ void check_operator(const OperatorSpec& s) {
   else c.fail("unknown operator");
 }
 
-OperatorPlan plan_operator(const OperatorSpec& s) {
+OperatorPlan plan_operator(const OperatorSpec& s, bool lean) {
   OperatorPlan p = s.name == "rx.embedding"         ? plan_embedding(s)
-                   : s.name == "rx.embedding_grad"  ? plan_embedding_grad(s)
+                   : s.name == "rx.embedding_grad"  ? plan_embedding_grad(s, lean)
                    : s.name == "rx.kv_append"       ? plan_append(s)
-                   : s.name == "rx.paged_attention" ? plan_attention(s)
+                   : s.name == "rx.paged_attention" ? plan_attention(s, lean)
                    : s.name == "rx.token_logprobs"  ? plan_logprobs(s)
                                                     : plan_logprobs_grad(s);
   // without workgroups there is nothing to compile

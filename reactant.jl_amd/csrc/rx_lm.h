@@ -64,7 +64,8 @@ struct OperatorPlan {
 bool is_operator_name(const std::string& name);
 // Throws rx::Error where the operands, results or settings are not the operator's.
 void check_operator(const OperatorSpec& spec);
-OperatorPlan plan_operator(const OperatorSpec& spec);
+// `lean`: with temporaries of up to 1 MiB for partial results (fewer workgroups share long sequences or rows).
+OperatorPlan plan_operator(const OperatorSpec& spec, bool lean = false);
 // Arithmetic of one call; *transcendentals: exponentials and logarithms, counted apart.
 double operator_flops(const OperatorSpec& spec, double* transcendentals);
 

@@ -4129,7 +4129,8 @@ struct Planner {
     for (auto& r : g.nodes)
       if (r.k == OpK::OperatorResult && r.in[0] == root) results[r.a0[0]] = r.id;
     for (int r : results) spec.out.push_back(g.nodes[r].ty);
-    const OperatorPlan op = plan_operator(spec);
+    const OperatorPlan op = plan_operator(spec, opt.lean_operators);
+    plan.lean_operators = plan.lean_operators || (!opt.lean_operators && !op.scratch.empty());
     uses_operators = true;
     for (size_t r = 0; r < results.size(); ++r) {
       const int from = r < op.updates.size() ? op.updates[r] : -1;

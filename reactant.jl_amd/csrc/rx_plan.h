@@ -49,6 +49,7 @@ struct Plan {
   std::string report() const;          // text summary for debugging
   int split_filters = 0;               // temporaries that hold a filter split in three
   bool chunked_columns = false;        // column sums that would take no temporaries in one launch take two
+  bool lean_operators = false;         // operators have plans with smaller temporaries
   bool unchained_steps = false;        // steps whose chain would keep fewer arrays run as maps
   int64_t temporary_bytes() const;     // what its temporaries take when each has memory of its own (RxExecuteNoAlloc)
 };
@@ -69,6 +70,7 @@ struct PlanOptions {
   bool fold_finals = true;      // the end of a full reduction runs in the map that reads its result
   bool column_reduce = true;    // column sums of matrices of up to 16 MB in one launch
   bool column_sums_whole = false;  // ... of up to 4096 rows, whatever their elements cost
+  bool lean_operators = false;  // language-model operators with small temporaries
   bool chains_first = false;    // rank-3 steps over rows of odd length as over others: chains where their estimate is below 4.4 us per step
   bool join_launches = true;    // small launches that do not depend on one another run as one
   bool nhwc_regions = true;     // the same for regions with several readers per value (residual additions): transposed once on the way in and out where needed

@@ -127,6 +127,35 @@ def test_append_and_attend_without_allocations(rx, client):
     T.close(want, o, T.attention_bound([q, I.Tensor(res[1].to_host(), "f32")], 32 ** -0.5, lse, mag, "f32", 120)[0])
 
 
+def test_partial_results_fit_calls_without_allocations(rx, client):
+    """Long sequences, and long rows of a table's gradient, whose partial results take more than the library's scratch array in
+    the usual plan: calls without allocations share them among fewer workgroups."""
+    rng = np.random.default_rng(8)
+    lengths, hq, hk, d, size, cols = [8100, 5000, 7777, 3], 16, 2, 128, 16, 512
+    args = T.attention_case(rng, lengths, hq, hk, d, d, 1400, size, cols, "bf16", "slots")
+    exe = rx.xla_compile(client, P.paged_attention(4, hq, hk, d, 1400, size, cols, lse=True))
+    bufs = [rx.Buffer.from_host(client, np.ascontiguousarray(rx.encode(t.a, "bf16") if t.dt == "bf16" else t.a), t.dt) for t in args]
+    ref, lse, mag = L.paged_attention(*(t.a for t in args))
+    bound, lse_bound = T.attention_bound(args, d ** -0.5, lse, mag, "bf16", cols * size)
+    res = [rx.Buffer.uninitialized(client, (4, hq, d), "bf16"), rx.Buffer.uninitialized(client, (4, hq), "f32")]
+    for _ in range(2):
+        exe.execute_no_alloc(bufs, res)
+        client.default_device().synchronize()
+        T.close(rx.decode(res[0].to_host(), "bf16"), ref, bound, "bf16")
+        T.close(res[1].to_host(), lse, lse_bound)
+    tokens, rows, width = 1100, 5, 32768
+    dy = rng.integers(-100, 100, size=(tokens, width)).astype(np.float32)          # sums that no order rounds
+    ids = rng.integers(0, rows, size=tokens).astype(np.int32)
+    exe = rx.xla_compile(client, P.embedding_grad(tokens, rows, width, dt="f32"))
+    bufs, want = [rx.Buffer.from_host(client, dy, "f32"), rx.Buffer.from_host(client, ids, "i32")], L.embedding_grad(dy, ids, rows)
+    res = [rx.Buffer.uninitialized(client, (rows, width), "f32")]
+    for _ in range(2):
+        exe.execute_no_alloc(bufs, res)
+        client.default_device().synchronize()
+        assert np.array_equal(res[0].to_host(), want)
+    assert np.array_equal(exe.execute_sharded(bufs)[0].synced_buffer().to_host(), want)
+
+
 def test_append_to_an_array_returned_twice(rx, client):
     """Two results of one buffer: appending to the donated one leaves the other alone."""
     rng = np.random.default_rng(5)
