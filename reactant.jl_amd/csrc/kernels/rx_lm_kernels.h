@@ -489,7 +489,11 @@ template <int S, int B, int M, int W, int R, typename I>
 RX_DEV rx_lm_stretch rx_lm_stretch_of(const I* lengths, const int r) {
   const int lane = threadIdx.x & 63;
   rx_lm_stretch s = {B, 0, 0, 0, 0, 0};
-  for (int b0 = 0; b0 < B; b0 += 64) s.total += b0 + lane < B ? rx_lm_span_of<S, B, M, W>(lengths[b0 + lane]).cost : 0;
+  int units = 0;
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    units = b0 + lane < B ? rx_lm_span_of<S, B, M, W>(lengths[b0 + lane]).cost : 0;
+    s.total += units;
+  }
   if constexpr (B > 1) s.total = rx_wave_reduce(s.total, rx_op_add());
   else s.total = rx_lane_from(s.total, 0);
   s.parts = s.total < 4ll * R ? (int)((s.total + 3) / 4) : R;
@@ -498,7 +502,7 @@ RX_DEV rx_lm_stretch rx_lm_stretch_of(const I* lengths, const int r) {
   s.count = (int)(rx_lm_stretch_start(s.total, s.parts, r + 1) - s.first);
   long long sum = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
-    const int units = b0 + lane < B ? rx_lm_span_of<S, B, M, W>(lengths[b0 + lane]).cost : 0;
+    if (B > 64) units = b0 + lane < B ? rx_lm_span_of<S, B, M, W>(lengths[b0 + lane]).cost : 0;
     const long long upto = sum + (B > 1 ? rx_wave_scan((long long)units, rx_op_add()) : (long long)units);
     const unsigned long long past = __ballot(b0 + lane < B && upto > s.first);
     if (past) {
@@ -562,8 +566,10 @@ RX_DEV rx_f32x4 rx_lm_mma(const rx_u32x4 a, const rx_u32x4 b, rx_f32x4 c) {
 
 // HW: key heads of a workgroup, whose four wavefronts share the units of a head, or have a head each; COLUMNS: groups of HW key
 // heads, times the tiles of up to 16 NT query heads that read one; R: stretches; ONCE: the caches are read past the L2; DIES: a
-// stretch's columns are neighbours on one die
-template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int NT, int R, int HW, bool ONCE, bool DIES, typename I>
+// stretch's columns are neighbours on one die; VECTOR: f32 caches with one query head a key head, by the vector units, since 15
+// of the matrix cores' 16 columns would be empty at a sixteenth of their 16-bit rate.  A lane multiplies its parts of two keys, and
+// the values of its eight positions, in the same registers; every column holds the one head.
+template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int NT, int R, int HW, bool ONCE, bool DIES, bool VECTOR, typename I>
 RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, const typename E::S* vc, const I* pages, const I* lengths, typename E::S* out, float* lse,
                                float* part, float* stat, int* arrived, const float scale) {
   typedef typename E::S T;
@@ -601,10 +607,10 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int k = 0; k < NK; ++k)
-      qf[t][k] = t * 16 + r < heads ? rx_lm_row16<E, DK>(q + ((long long)b * HQ + h0 + t * 16 + r) * DK, (k * 4 + g4) * NE) : rx_u32x4{0, 0, 0, 0};
+      qf[t][k] = VECTOR || t * 16 + r < heads ? rx_lm_row16<E, DK>(q + ((long long)b * HQ + h0 + (VECTOR ? 0 : t * 16 + r)) * DK, (k * 4 + g4) * NE) : rx_u32x4{0, 0, 0, 0};
 
   float m[NT], l[NT];
-  rx_f32x4 acc[NT][NV][NE];
+  rx_f32x4 acc[NT][NV][NE];                            // (VECTOR: only the first of four)
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     m[t] = -rx_lm_inf();
@@ -669,8 +675,24 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
         rx_f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
-          s[0] = rx_lm_mma<E>(kf[0][k], qf[t][k], s[0]);
-          s[1] = rx_lm_mma<E>(kf[1][k], qf[t][k], s[1]);
+          if constexpr (VECTOR) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[c][e] = __builtin_fmaf(__builtin_bit_cast(rx_f32x4, kf[c][k])[e], __builtin_bit_cast(rx_f32x4, qf[t][k])[e], s[c][e]);
+          } else {
+            s[0] = rx_lm_mma<E>(kf[0][k], qf[t][k], s[0]);
+            s[1] = rx_lm_mma<E>(kf[1][k], qf[t][k], s[1]);
+          }
+        }
+        if constexpr (VECTOR) {
+          // position r's and 16 + r's scores, and from them those of the positions whose values this lane holds
+          const float a = rx_lm_sum4((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])), b = rx_lm_sum4((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[0][i] = rx_lane_from(a, g4 * 4 + i);
+            s[1][i] = rx_lane_from(b, g4 * 4 + i);
+          }
         }
         float x[8], top = -rx_lm_inf();
 #pragma unroll
@@ -689,7 +711,10 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
 #pragma unroll
           for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int e = 0; e < NE; ++e) acc[t][j][e] *= shrink;
+            for (int e = 0; e < NE; ++e) {
+              if constexpr (VECTOR) acc[t][j][e][0] *= shrink;
+              else acc[t][j][e] *= shrink;
+            }
           m[t] = top;
         }
 #pragma unroll
@@ -718,7 +743,8 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
             for (int t = 0; t < NT; ++t)
 #pragma unroll
               for (int i = 0; i < 8; ++i)
-                acc[t][j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(rx_f32x4, vf[j][i])[e], w[t].v[i], acc[t][j][e], 0, 0, 0);
+                if constexpr (VECTOR) acc[t][j][e][0] = __builtin_fmaf(__builtin_bit_cast(rx_f32x4, vf[j][i])[e], w[t].v[i], acc[t][j][e][0]);
+                else acc[t][j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(rx_f32x4, vf[j][i])[e], w[t].v[i], acc[t][j][e], 0, 0, 0);
           }
         }
     }
@@ -742,7 +768,13 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (j) __syncthreads();
-      if (r < HR) {
+      if constexpr (VECTOR) {
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          const float sum = rx_lm_sum4(acc[t][j][e][0]) * f;
+          if (g4 == 0 && r * NE + e < WIDTH) lds.o[wave][0][r * NE + e] = sum;
+        }
+      } else if (r < HR) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
