@@ -272,13 +272,13 @@ RX_DEV void rx_embedding_grad_rows(const typename E::S* dy, const int* start, co
   }
 }
 
-// Few tokens (up to 1024): one launch, without a sorted list in memory.  A workgroup takes the rows of about 1024 vectors, lists
+// Few tokens (up to 768): one launch, without a sorted list in memory.  A workgroup takes the rows of about 1024 vectors, lists
 // the tokens of these rows as it goes through all of them (a wavefront's matches in the order of its lanes, the wavefronts' one
 // after the other), ranks the listed tokens by row, and every thread sums those of its vectors' rows.
 template <typename E, typename O, int V, int D, int T, int VEC, typename I>
 RX_DEV void rx_embedding_grad_few(const typename E::S* dy, const I* ids, typename O::S* out, const float scale) {
   constexpr int C = D / VEC, ROWS = C < 1024 ? 1024 / C : 1, LOADS = (T + 255) / 256;
-  static_assert(LOADS <= 4, "tokens of a thread");
+  static_assert(LOADS <= 3, "tokens of a thread");
   __shared__ int found[T], of[T], sorted[T], start[ROWS + 1], sums[LOADS][4];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   int id[LOADS];
@@ -388,6 +388,8 @@ RX_DEV void rx_kv_append_any(const typename E::S* q, const typename E::S* k, con
 
 // Heads of whole vectors: a thread takes the same dimensions of HEADS heads of a token (their cosines and sines are loaded
 // once): the two vectors of a rotated stretch of pairs, or one vector that is not rotated, or whose pairs are inside of it.
+// 8191 tokens of 32 and 8 heads of 128 in f16, half of the dimensions rotated, take 38 us, 5.4 TB/s of reading and writing, of which
+// a copy of this size reaches 6.2; 48 tokens take 2.8 us, what a launch and four dependent loads last.
 template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int L, int R2, bool PAIRS, bool BY_SLOT, int T, int HEADS, typename I>
 RX_DEV void rx_kv_append(const typename E::S* q, const typename E::S* k, const typename E::S* v, const float* cos, const float* sin, const I* position, const I* sequence,
                          const I* pages, typename E::S* qo, typename E::S* kc, typename E::S* vc) {
@@ -996,7 +998,7 @@ RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, flo
   __shared__ rx_lm_sums red[4];
   __shared__ rx_u64 keys[K ? CAP : 1], red64[4];
   __shared__ rx_u16 reach[K ? SECTIONS : 1][256], listed[K ? LIST : 1];
-  constexpr int GROUPS = K <= 24 ? 64 : 256;                   // (the 64th of 64 would be a bound that hundreds reach)
+  constexpr int GROUPS = K <= 48 ? 64 : 256;                   // 4096 x 65536 in bf16: 20 of 64 groups 100 us, of 256 116; 48: 120 and 122; 64: 283 (a bound that hundreds reach) and 129
   __shared__ rx_u32 group[GROUPS], bound;
   __shared__ int count, nlist, last;
   for (long long item = blockIdx.x; item < (long long)T * SPLIT; item += gridDim.x) {
@@ -1165,44 +1167,40 @@ RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, flo
   }
 }
 
-// d x_j = g (delta_jy - p_j) - h p_j (x_j - lse + H): a workgroup per SPAN vectors of a row
-template <typename E, int V, int T, int UNROLL, typename I>
+// d x_j = g (delta_jy - p_j) - h p_j (x_j - lse + H): a thread per vector of a row, a workgroup per 256 of them.  4096 rows of
+// 50021 logits in bf16 take 135 us, 6.1 TB/s of reading and writing, as a copy reaches; two vectors to a thread 138, four 142.
+template <typename E, int V, int T, typename I>
 RX_DEV void rx_token_logprobs_grad(const typename E::S* logits, const I* targets, const float* lse, const float* entropy, const float* d_logprob, const float* d_entropy,
                                    typename E::S* out) {
   typedef typename E::S S;
-  constexpr int NE = 16 / sizeof(S), VECTORS = rx_lm_row<E, V>::VECTORS, SPAN = 256 * UNROLL, PARTS = (VECTORS + SPAN - 1) / SPAN;
+  constexpr int NE = 16 / sizeof(S), VECTORS = rx_lm_row<E, V>::VECTORS, PARTS = (VECTORS + 255) / 256;
   for (long long item = blockIdx.x; item < (long long)T * PARTS; item += gridDim.x) {
     const long long t = item / PARTS;
-    const int v0 = (int)(item % PARTS) * SPAN + (int)threadIdx.x;
+    const int v = (int)(item % PARTS) * 256 + (int)threadIdx.x;
     const rx_lm_row<E, V> row(logits, t);
-    S* o = out + t * V;
-    rx_vec<S, NE> r[UNROLL];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) r[u] = row.load(v0 + 256 * u);
+    const int j = row.first(v);
+    const rx_vec<S, NE> r = row.load(v);
     const I y = targets[t];
     const bool counts = y >= 0 && y < V;
     const float l = lse[t] == -rx_lm_inf() ? rx_lm_inf() : lse[t];   // (a row of nothing: all probabilities 0)
     const float g = counts ? d_logprob[t] : 0.0f, h = d_entropy[t], c = g + h * entropy[t];
+    if (v >= VECTORS) continue;
+    float e[NE];
+    row.get(r, v, 0.0f, e);
+    rx_vec<S, NE> w;
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int v = v0 + 256 * u, j = row.first(v);
-      if (v >= VECTORS) break;
-      float e[NE];
-      row.get(r[u], v, 0.0f, e);
-      rx_vec<S, NE> w;
+    for (int k = 0; k < NE; ++k) {
+      const float z = e[k] - l, p = __builtin_amdgcn_exp2f(z * RX_LM_LOG2E);
+      float d = -p * __builtin_fmaf(h, __builtin_fmaxf(z, -200.0f), c);   // (p is 0 from there on, and 0 times -inf is no 0)
+      if (counts && (long long)y - j == k) d += g;
+      w.v[k] = E::down(d);
+    }
+    S* o = out + t * V + j;
+    if (row.whole(v)) rx_store_nt(o, w);
+    else {
 #pragma unroll
-      for (int k = 0; k < NE; ++k) {
-        const float z = e[k] - l, p = __builtin_amdgcn_exp2f(z * RX_LM_LOG2E);
-        float d = -p * __builtin_fmaf(h, __builtin_fmaxf(z, -200.0f), c);   // (p is 0 from there on, and 0 times -inf is no 0)
-        if (counts && (long long)y - j == k) d += g;
-        w.v[k] = E::down(d);
-      }
-      if (row.whole(v)) rx_store_nt(o + j, w);
-      else {
-#pragma unroll
-        for (int k = 0; k < NE; ++k)
-          if (j + k >= 0 && j + k < V) o[j + k] = w.v[k];
-      }
+      for (int k = 0; k < NE; ++k)
+        if (j + k >= 0 && j + k < V) o[k] = w.v[k];
     }
   }
 }

@@ -141,7 +141,7 @@ OperatorPlan plan_embedding(const OperatorSpec& s) {
   OperatorPlan p;
   const int vec = (int)(16 / info(s.in[0].dt).size);
   const bool whole = D % vec == 0;
-  const int64_t per = whole ? vec : 1, each = 2;
+  const int64_t per = whole ? vec : 1, each = 2;   // vectors of a thread: 16384 rows of 4096 bf16 55 us with one, 32 with two, 34 with four
   OperatorKernel k = kernel(s, "embedding", 256, {{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}, {result(0), st(s.out[0])}}, 1,
                             std::string("rx_embedding<") + elem(s.in[0].dt) + ", " + num(V) + ", " + num(D) + ", " + num(T) + ", " + num(whole ? vec : 1) + ", " + num(each) +
                                 ">(a0, a1, a2, " + flt(c.number("scale", 1.0)) + ");");
@@ -175,7 +175,10 @@ OperatorPlan plan_embedding_grad(const OperatorSpec& s, bool lean) {
   const int64_t rows_grid = std::min<int64_t>((V * C + 255) / 256, kMaxGrid);
   OperatorPlan p;
   if (rows_grid == 0) return p;
-  if (T <= 1024) {
+  // Up to 768 tokens in one launch without a sorted list (rows x dimensions of 5003 x 1024 f32, 32000 x 1024 bf16 and 512 x 768 f32:
+  // with 512 tokens 9.3, 12.7 and 9.9 us against 12.0, 17.9 and 11.6 in two; with 768 11.0, 14.9 and 12.7 against 11.7, 18.2 and 11.4;
+  // with 1024 13.1, 16.5 and 17.0 against 12.3, 19.0 and 11.4).
+  if (T <= 768) {
     const std::string sizes = num(V) + ", " + num(D) + ", " + num(std::max<int64_t>(T, 1)) + ", " + num(vec);
     OperatorKernel k = T == 0 ? kernel(s, "embedding_grad", 256, {{result(0), st(s.out[0])}}, 1, "rx_lm_zero<" + num(V * D) + ">(a0);")
                               : kernel(s, "embedding_grad", 256, {{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}, {result(0), st(s.out[0])}}, 1,
@@ -195,6 +198,7 @@ OperatorPlan plan_embedding_grad(const OperatorSpec& s, bool lean) {
                             "rx_lm_sort<" + num(V) + ", " + num(T) + ", " + num(rows) + ">(a0, a1, a2, a3);");
   k.grid[0] = (unsigned)((V + rows - 1) / rows);
   p.kernels.push_back(k);
+  // vectors of a row to a thread (16384 bf16 tokens, 65536 x 4096 f32: one 244 us, two 232, four 245)
   const int64_t each = std::min<int64_t>(2, tiles), wide_tiles = (C + 256 * each - 1) / (256 * each), lines = C < 256 ? 256 / C : 1;
   const std::string sizes = types + num(V) + ", " + num(D) + ", " + num(T) + ", " + num(vec) + ", " + num(piece);
   p.counters = pieces * wide_tiles;
@@ -268,7 +272,9 @@ OperatorPlan plan_append(const OperatorSpec& s) {
   std::ostringstream b;
   const int64_t ne = 16 / info(in[0].dt).size, HQ = in[0].dims[1];
   const bool pairs = rotation == "pairs", whole = kc.dim % ne == 0 && vc.dim % ne == 0 && 2 * R2 % ne == 0 && (pairs || R2 % ne == 0);
-  const int64_t heads = T >= 256 ? 2 : 1;
+  // two heads of the same dimensions to a thread, their cosines and sines loaded once, where there are threads enough: 8191 tokens of
+  // 40 heads of 128, half of it rotated, 42 -> 38 us, all of it 36.6 both; 512 tokens 4.1 -> 4.6, 48 tokens 2.8 -> 3.4
+  const int64_t heads = T >= 2048 ? 2 : 1;
   b << (whole ? "rx_kv_append<" : "rx_kv_append_any<") << elem(in[0].dt) << ", " << HQ << ", " << kc.heads << ", " << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << kc.slots << ", "
     << in[7].dims[0] << ", " << in[7].dims[1] << ", " << in[3].dims[0] << ", " << R2 << ", " << (pairs ? "true" : "false") << ", " << (by_slot ? "true" : "false") << ", " << T
     << (whole ? ", " + num(heads) : std::string()) << ">(a0, a1, a2, a3, a4, a5, a6, a7, a8, a9, a10);";
@@ -446,10 +452,10 @@ OperatorPlan plan_logprobs_grad(const OperatorSpec& s) {
   std::vector<std::pair<OperatorArg, std::string>> args;
   for (int i = 0; i < 6; ++i) args.push_back({operand(i), st(s.in[i])});
   args.push_back({result(0), st(s.out[0])});
-  const int64_t vec = 16 / info(s.in[0].dt).size, vectors = (V + vec - 1) / vec + (V % vec ? 1 : 0), unroll = vectors > 512 ? 4 : 1;
+  const int64_t vec = 16 / info(s.in[0].dt).size, vectors = (V + vec - 1) / vec + (V % vec ? 1 : 0);
   OperatorKernel k = kernel(s, "token_logprobs_grad", 256, args, 1,
-                            std::string("rx_token_logprobs_grad<") + elem(s.in[0].dt) + ", " + num(V) + ", " + num(T) + ", " + num(unroll) + ">(a0, a1, a2, a3, a4, a5, a6);");
-  k.grid[0] = (unsigned)std::min<int64_t>(T * ((vectors + 256 * unroll - 1) / (256 * unroll)), kMaxGrid);
+                            std::string("rx_token_logprobs_grad<") + elem(s.in[0].dt) + ", " + num(V) + ", " + num(T) + ">(a0, a1, a2, a3, a4, a5, a6);");
+  k.grid[0] = (unsigned)std::min<int64_t>(T * ((vectors + 255) / 256), kMaxGrid);
   k.bytes = 2.0 * (double)s.in[0].bytes() + 20.0 * (double)T;
   p.kernels.push_back(k);
   return p;
