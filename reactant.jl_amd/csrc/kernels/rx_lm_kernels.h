@@ -485,20 +485,28 @@ RX_DEV rx_lm_span rx_lm_span_of(const I len) {
   return s;
 }
 struct rx_lm_stretch { int b, unit, count; long long first, total; int parts; };   // sequence and its unit to start at, units; first unit in the row, units of the row, stretches
-// stretch r of up to R: at least four units each, one for every wavefront
+// Stretch r of up to R: at least four units each, one for every wavefront, and fewer for long sequences: the workgroup that joins n
+// parts takes as long over each as n workgroups gain by it, so the longest sequence of u units is to have about sqrt(Q u).  (One of
+// 65536 positions, 8 query heads of one key head of 128: 512 parts 79 us, 91 parts 31, 64 parts 32; of 4000: 31 parts 11.8.)
 RX_DEV long long rx_lm_stretch_start(const long long total, const int parts, const int r) { return total * r / parts; }
-template <int S, int B, int M, int W, int R, typename I>
+template <int S, int B, int M, int W, int R, int Q, typename I>
 RX_DEV rx_lm_stretch rx_lm_stretch_of(const I* lengths, const int r) {
   const int lane = threadIdx.x & 63;
   rx_lm_stretch s = {B, 0, 0, 0, 0, 0};
-  int units = 0;
+  int units = 0, longest = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
     units = b0 + lane < B ? rx_lm_span_of<S, B, M, W>(lengths[b0 + lane]).cost : 0;
     s.total += units;
+    longest = units > longest ? units : longest;
   }
   if constexpr (B > 1) s.total = rx_wave_reduce(s.total, rx_op_add());
   else s.total = rx_lane_from(s.total, 0);
   s.parts = s.total < 4ll * R ? (int)((s.total + 3) / 4) : R;
+  if constexpr (R > 1) {
+    longest = B > 1 ? rx_wave_reduce(longest, rx_op_max()) : rx_lane_from(longest, 0);
+    const float most = (float)s.total * __builtin_amdgcn_sqrtf((float)Q / (float)longest) + 1.0f;
+    s.parts = most < (float)s.parts ? (int)most : s.parts;
+  }
   if (r >= s.parts) return s;
   s.first = rx_lm_stretch_start(s.total, s.parts, r);
   s.count = (int)(rx_lm_stretch_start(s.total, s.parts, r + 1) - s.first);
@@ -566,12 +574,32 @@ RX_DEV rx_f32x4 rx_lm_mma(const rx_u32x4 a, const rx_u32x4 b, rx_f32x4 c) {
   }
 }
 
+// (maximum, sum, unscaled result) of parts of a sequence; the maximum goes up before parts are added
+template <int N>
+struct rx_lm_joined {
+  float m, s, o[N];
+  RX_MEM float weight(const float x, const float hi) const { return x == -rx_lm_inf() ? 0.0f : __builtin_amdgcn_exp2f(x - hi); }
+  RX_MEM void to(const float hi) {
+    const float f = weight(m, hi);
+    s *= f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] *= f;
+    m = hi;
+  }
+  RX_MEM void add(const float x, const float sum, const float (&v)[N]) {
+    const float f = weight(x, m);
+    s += sum * f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] += v[e] * f;
+  }
+};
+
 // HW: key heads of a workgroup, whose four wavefronts share the units of a head, or have a head each; COLUMNS: groups of HW key
 // heads, times the tiles of up to 16 NT query heads that read one; R: stretches; ONCE: the caches are read past the L2; DIES: a
 // stretch's columns are neighbours on one die; VECTOR: f32 caches with one query head a key head, by the vector units, since 15
 // of the matrix cores' 16 columns would be empty at a sixteenth of their 16-bit rate.  A lane multiplies its parts of two keys, and
 // the values of its eight positions, in the same registers; every column holds the one head.
-template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int NT, int R, int HW, bool ONCE, bool DIES, bool VECTOR, typename I>
+template <typename E, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int NT, int R, int HW, bool ONCE, bool DIES, bool VECTOR, int Q, typename I>
 RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, const typename E::S* vc, const I* pages, const I* lengths, typename E::S* out, float* lse,
                                float* part, float* stat, int* arrived, const float scale) {
   typedef typename E::S T;
@@ -585,6 +613,7 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
   __shared__ union {
     int page[BLOCK / S + 2];
     float o[4][HR][WIDTH + 4];
+    rx_lm_joined<DV % 4 == 0 ? 4 : 1> j[256];
   } lds;
   __shared__ float join_m[4][16], join_l[4][16];
   __shared__ int last;
@@ -593,7 +622,7 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
   const int head0 = column / TILES * HW, head = head0 + wave / WPH;
   const int h0 = head * G + tile * GT;                 // first query head of this wavefront
   const int heads = G - tile * GT < GT ? G - tile * GT : GT;
-  const rx_lm_stretch st = rx_lm_stretch_of<S, B, M, W, R>(lengths, mine);
+  const rx_lm_stretch st = rx_lm_stretch_of<S, B, M, W, R, Q>(lengths, mine);
 
   int b = st.b, unit = st.unit;
   for (int left = st.count; left > 0; ++b, unit = 0) {
@@ -816,37 +845,48 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
   if (whole) continue;
   const int from = rx_lm_stretch_with(st.total, st.parts, begin), to = rx_lm_stretch_with(st.total, st.parts, begin + span.units - 1);
   if (!rx_lm_last_to_arrive(arrived + b * COLUMNS + column, to - from + 1, &last)) continue;
-  for (int k = threadIdx.x; k < HW * heads * DV; k += 256) {
-    const int hw = k / (heads * DV), h = k / DV % heads, d = k % DV, qh = (head0 + hw) * G + tile * GT + h;
-    float o = 0.0f, sum = 0.0f, top = -rx_lm_inf();
-    for (int w = from; w <= to; w += 8) {
-      float pm[8], ps[8], po[8];
+  // VD outputs to a thread, DV / VD apart; where there are fewer than threads, the parts are shared too, and joined once more
+  constexpr int VD = DV % 4 == 0 ? 4 : 1;
+  const int outs = HW * heads * (DV / VD), ways = outs < 256 ? 256 / outs : 1, parts = to - from + 1;
+  for (int k0 = 0; k0 < outs; k0 += 256) {
+    const int k = ways > 1 ? (int)threadIdx.x % outs : k0 + (int)threadIdx.x, way = ways > 1 ? (int)threadIdx.x / outs : 0;
+    const bool on = k < outs && way < ways;
+    const int hw = k / (heads * (DV / VD)), h = k / (DV / VD) % heads, d = k % (DV / VD), qh = (head0 + hw) * G + tile * GT + h;
+    const int w1 = on ? from + parts * (way + 1) / ways : 0;
+    rx_lm_joined<VD> j = {-rx_lm_inf(), 0.0f, {}};
+    for (int w = on ? from + parts * way / ways : 0; w < w1; w += 8) {
+      float pm[8], ps[8], po[8][VD];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int v = w + i <= to ? w + i : to;
+        const int v = w + i < w1 ? w + i : w1 - 1;
         const long long at = (((long long)(v * COLUMNS + column) * 2 + (v == from)) * HW + hw) * GT + h;
         pm[i] = rx_lm_get_shared(stat + at * 2);
         ps[i] = rx_lm_get_shared(stat + at * 2 + 1);
-        po[i] = rx_lm_get_shared(part + at * DV + d);
+#pragma unroll
+        for (int e = 0; e < VD; ++e) po[i][e] = rx_lm_get_shared(part + at * DV + d + e * (DV / VD));
       }
-      float hi = top;
+      float hi = j.m;
 #pragma unroll
       for (int i = 0; i < 8; ++i) hi = __builtin_fmaxf(hi, pm[i]);
-      if (hi == -rx_lm_inf()) hi = 0.0f;
-      const float f = __builtin_amdgcn_exp2f(top - hi);
-      o *= f;
-      sum *= f;
+      j.to(hi);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (w + i > to) break;
-        const float g = __builtin_amdgcn_exp2f(pm[i] - hi);
-        o += po[i] * g;
-        sum += ps[i] * g;
-      }
-      top = hi;
+      for (int i = 0; i < 8; ++i)
+        if (w + i < w1) j.add(pm[i], ps[i], po[i]);
     }
-    out[((long long)b * HQ + qh) * DV + d] = E::down(sum == 0.0f ? 0.0f : o / sum);
-    if (lse && d == 0) lse[(long long)b * HQ + qh] = sum == 0.0f ? -rx_lm_inf() : (top + __builtin_log2f(sum)) * 0.6931471805599453f;
+    if (ways > 1) {
+      lds.j[threadIdx.x] = j;
+      __syncthreads();
+      if (way == 0)
+        for (int n = 1; n < ways; ++n) {
+          const rx_lm_joined<VD> o = lds.j[n * outs + k];
+          j.to(__builtin_fmaxf(j.m, o.m));
+          j.add(o.m, o.s, o.o);
+        }
+    }
+    if (!on || way) continue;
+#pragma unroll
+    for (int e = 0; e < VD; ++e) out[((long long)b * HQ + qh) * DV + d + e * (DV / VD)] = E::down(j.s == 0.0f ? 0.0f : j.o[e] / j.s);
+    if (lse && d == 0) lse[(long long)b * HQ + qh] = j.s == 0.0f ? -rx_lm_inf() : (j.m + __builtin_log2f(j.s)) * 0.6931471805599453f;
   }
   }
 }

@@ -178,7 +178,7 @@ OperatorPlan plan_embedding_grad(const OperatorSpec& s, bool lean) {
   // Up to 768 tokens in one launch without a sorted list (rows x dimensions of 5003 x 1024 f32, 32000 x 1024 bf16 and 512 x 768 f32:
   // with 512 tokens 9.3, 12.7 and 9.9 us against 12.0, 17.9 and 11.6 in two; with 768 11.0, 14.9 and 12.7 against 11.7, 18.2 and 11.4;
   // with 1024 13.1, 16.5 and 17.0 against 12.3, 19.0 and 11.4).
-  if (T <= 768) {
+  if (T <= (V < 4096 ? 512 : 768)) {
     const std::string sizes = num(V) + ", " + num(D) + ", " + num(std::max<int64_t>(T, 1)) + ", " + num(vec);
     OperatorKernel k = T == 0 ? kernel(s, "embedding_grad", 256, {{result(0), st(s.out[0])}}, 1, "rx_lm_zero<" + num(V * D) + ">(a0);")
                               : kernel(s, "embedding_grad", 256, {{operand(0), st(s.in[0])}, {operand(1), st(s.in[1])}, {result(0), st(s.out[0])}}, 1,
@@ -348,9 +348,9 @@ OperatorPlan plan_attention(const OperatorSpec& s, bool lean) {
   // one die (4.6).  So it is with the tiles of one key head (64 query heads: 194 us past the L2, 171 through it, 166 on one die).
   const bool once = kc.dim * e % 256 == 0 && vc.dim * e % 256 == 0 && tiles == 1, dies = (by_slot && kc.dim * e % 128 != 0) || tiles > 1;
   const int64_t columns = kc.heads / HW * tiles;
-  // every workgroup a stretch of at least four units of 32 positions, all of them on the chip at once
+  // every workgroup a stretch of at least four units of 32 positions (a sequence counts four more), all of them on the chip at once
   const int64_t part = 2 * HW * GT * (vc.dim * 4 + 8), most = lean ? std::min<int64_t>(256 * waves, kLeanBytes / part) : 256 * waves;
-  const int64_t stretches = std::max<int64_t>(1, std::min(most / columns, (B * units + 3) / 4)), grid = stretches * columns;
+  const int64_t stretches = std::max<int64_t>(1, std::min(most / columns, (B * (units + (B > 1 ? 4 : 0)) + 3) / 4)), grid = stretches * columns;
   OperatorPlan p;
   std::vector<std::pair<OperatorArg, std::string>> args;
   for (int i = 0; i < 5; ++i) args.push_back({operand(i), st(in[i])});
@@ -368,7 +368,7 @@ OperatorPlan plan_attention(const OperatorSpec& s, bool lean) {
   std::ostringstream b;
   b << "rx_paged_attention<" << elem(in[0].dt) << ", " << Hq << ", " << kc.heads << ", " << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << kc.slots << ", " << B << ", " << M << ", "
     << window << ", " << (by_slot ? "true" : "false") << ", " << NT << ", " << stretches << ", " << HW << ", "
-    << (once ? "true" : "false") << ", " << (dies ? "true" : "false") << ", " << (vector ? "true" : "false") << ">(a0, a1, a2, a3, a4, a5, " << (lse ? "a6" : "(float*)0") << ", " << shared << ", "
+    << (once ? "true" : "false") << ", " << (dies ? "true" : "false") << ", " << (vector ? "true" : "false") << ", " << std::max<int64_t>(1, std::min<int64_t>(4, 4096 / (HW * GT * vc.dim))) << ">(a0, a1, a2, a3, a4, a5, " << (lse ? "a6" : "(float*)0") << ", " << shared << ", "
     << flt(scale * 1.4426950408889634) << ");";
   OperatorKernel k = kernel(s, "paged_attention", 256, args, (int)args.size() - 5, b.str(), waves);
   k.grid[0] = (unsigned)(B ? grid : 0);
