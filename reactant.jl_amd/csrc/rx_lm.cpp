@@ -20,7 +20,7 @@ const OpName kOperators[] = {
 constexpr int kMaxHeadDim = 256;
 constexpr int64_t kMaxTop = 64;
 constexpr int64_t kMaxGrid = (int64_t)1 << 22;   // workgroups; kernels with more items than that go on with the next ones
-constexpr int64_t kLeanBytes = (int64_t)1 << 20;  // of partial results in a lean plan
+constexpr int64_t kLeanBytes = (int64_t)1 << 20;  // of partial results in a lean plan: a quarter of what calls without allocations have for all temporaries
 constexpr int64_t kMaxRow = (int64_t)1 << 30;   // elements of a row or rows of a table: 32-bit indices inside a row
 
 struct Checker {
