@@ -25,6 +25,26 @@ def uneven(rng, b, longest):
     return n.tolist()
 
 
+@pytest.mark.parametrize("lengths,hq,hk,d,dv,dt,layout", [
+    ([20000], 1, 1, 64, 64, "f32", "slots"), ([20000], 1, 1, 33, 17, "bf16", "heads"), ([30001, 3, 0], 2, 2, 8, 8, "f16", "slots"), ([9000, 9000], 3, 1, 40, 24, "bf16", "slots"),
+    ([25000], 5, 5, 16, 7, "f32", "heads"), ([1] * 40 + [12345], 8, 1, 128, 64, "bf16", "heads"),
+])
+def test_long_sequences_of_few_heads(rx, client, lengths, hq, hk, d, dv, dt, layout):
+    """Many parts of few outputs: threads share the parts among them."""
+    rng = np.random.default_rng(len(lengths) + d)
+    size, b = 16, len(lengths)
+    cols, pages = -(-max(lengths) // size) + 1, sum(-(-n // size) for n in lengths) + 2
+    args = T.attention_case(rng, lengths, hq, hk, d, dv, pages, size, cols, dt, layout)
+    text = P.paged_attention(b, hq, hk, d, pages, size, cols, dt=dt, layout=layout, lse=True, value_dim=dv)
+    got, exe = gpu_run(rx, client, text, args)
+    ref, lse, mag = L.paged_attention(*(t.a for t in args), layout=layout)
+    bound, lse_bound = T.attention_bound(args, d ** -0.5, lse, mag, dt, cols * size)
+    T.close(got[0].a, ref, bound, dt)
+    T.close(got[1].a, lse, lse_bound)
+    again, _ = gpu_run(rx, client, text, args, exe)
+    assert all(np.array_equal(x.a, y.a) for x, y in zip(got, again))
+
+
 @pytest.mark.parametrize("b,longest,hq,hk,d,size,dt,layout,window", [
     (130, 900, 4, 2, 64, 16, "bf16", "slots", 0), (70, 3000, 8, 8, 32, 7, "f16", "heads", 0), (200, 70, 2, 1, 128, 16, "f32", "slots", 0), (65, 2000, 6, 2, 48, 32, "bf16", "heads", 333),
     (9, 6000, 48, 1, 64, 64, "bf16", "slots", 0), (3, 9000, 24, 8, 256, 16, "bf16", "slots", 0),
@@ -154,6 +174,16 @@ def test_partial_results_fit_calls_without_allocations(rx, client):
         client.default_device().synchronize()
         assert np.array_equal(res[0].to_host(), want)
     assert np.array_equal(exe.execute_sharded(bufs)[0].synced_buffer().to_host(), want)
+
+
+@pytest.mark.parametrize("tokens", [512, 513, 768, 769])
+@pytest.mark.parametrize("rows", [40, 4095, 4096])
+def test_gradients_on_both_sides_of_the_sorted_list(rx, client, tokens, rows):
+    rng = np.random.default_rng(tokens + rows)
+    dy = rng.integers(-1000, 1000, size=(tokens, 72)).astype(np.float64)           # sums that no order rounds
+    ids = np.minimum((rows ** rng.random(tokens)).astype(np.int64) - 1, rows - 1)
+    got, _ = gpu_run(rx, client, P.embedding_grad(tokens, rows, 72, dt="f32"), [I.Tensor(dy, "f32"), I.Tensor(ids, "i32")])
+    assert np.array_equal(got[0].a, L.embedding_grad(dy, ids, rows))
 
 
 def test_append_to_an_array_returned_twice(rx, client):
