@@ -348,8 +348,13 @@ OperatorPlan plan_attention(const OperatorSpec& s, bool lean) {
   // one die (4.6).  So it is with the tiles of one key head (64 query heads: 194 us past the L2, 171 through it, 166 on one die).
   const bool once = kc.dim * e % 256 == 0 && vc.dim * e % 256 == 0 && tiles == 1, dies = (by_slot && kc.dim * e % 128 != 0) || tiles > 1;
   const int64_t columns = kc.heads / HW * tiles;
+  // Workgroups: all on the chip at once (half as many again: 64 sequences of 1 to 8192 positions 56 -> 60 us, one of 131072 630 -> 638),
+  // two to a compute unit where the registers allow it; but one where each reads two heads' rows of 256 bytes, whose loads are enough
+  // in flight (64 sequences of 1000 positions in bf16 55.7 -> 46.8 us, of 1 to 8192 56.1 -> 52.5; 64 dimensions of f32, 4 query heads a
+  // key head, 56.4 -> 49.0; with rows of 128 bytes 59 -> 68, with one head to a workgroup 45.0 -> 48.5).
+  const int64_t room = 256 * (HW == 2 && kc.dim * e == 256 ? 1 : waves);
   // every workgroup a stretch of at least four units of 32 positions (a sequence counts four more), all of them on the chip at once
-  const int64_t part = 2 * HW * GT * (vc.dim * 4 + 8), most = lean ? std::min<int64_t>(256 * waves, kLeanBytes / part) : 256 * waves;
+  const int64_t part = 2 * HW * GT * (vc.dim * 4 + 8), most = lean ? std::min<int64_t>(room, kLeanBytes / part) : room;
   const int64_t stretches = std::max<int64_t>(1, std::min(most / columns, (B * (units + (B > 1 ? 4 : 0)) + 3) / 4)), grid = stretches * columns;
   OperatorPlan p;
   std::vector<std::pair<OperatorArg, std::string>> args;
