@@ -484,7 +484,7 @@ RX_DEV void rx_kv_append(const typename E::S* q, const typename E::S* k, const t
 //
 // Bound by reading the caches where they are long: 8 sequences of 131072 positions, 8 key heads of 128 in bf16, 64 query heads, 4.3
 // GB, take 627 us, 6.8 TB/s, what reading alone reaches (the first form, a workgroup per query head and dot products on the vector
-// units: 192 ms); 64 sequences of 1 to 8192 positions, 257 MB, 56 us, 4.6 TB/s: what is missing is the start and the end of the launch.
+// units: 192 ms); 64 sequences of 1 to 8192 positions, 257 MB, 52 us, 4.9 TB/s: what is missing is the start and the end of the launch.
 // A chain of dependent steps where they are short: lengths, pages, keys and values, two products, the parts, the count, the parts
 // again: 8.5 us for one sequence of 1000 positions.  Loads one step ahead of the products gained nothing (two wavefronts to a SIMD
 // cover one another) and spilled registers in f32.
