@@ -523,7 +523,7 @@ void execute(RxExecutable* ex, int num_args, RxBuffer** args, RxDevice* dev, uin
   // donated), another argument, a result that was returned twice.
   for (size_t b = 0; b < NB; ++b) {
     const auto& B = P.buffers[b];
-    if (!B.written || bufs[b].use_count() == 1) continue;
+    if (B.kind != rx::BufferDesc::Param || !B.written || bufs[b].use_count() == 1) continue;
     Mem copy = std::make_shared<Allocation>(dev, (size_t)B.bytes);
     HIP_CHECK(hipMemcpyAsync(copy->ptr, bufs[b]->ptr, (size_t)B.bytes, hipMemcpyDeviceToDevice, dev->stream));
     bufs[b] = copy;
@@ -1142,8 +1142,7 @@ RX_EXPORT int RxExecuteNoAlloc(RxExecutable* ex, int num_args, RxBuffer** args, 
     size_t used = 0;
     for (size_t b = 0; b < NB; ++b) {
       const auto& B = P.buffers[b];
-      if (B.written) where[b] = results[first_result[b]]->mem->ptr;   // updated in place: in a copy, which is the result (below)
-      else if (B.kind == rx::BufferDesc::Param) where[b] = args[B.param_index]->mem->ptr;
+      if (B.kind == rx::BufferDesc::Param) where[b] = B.written ? results[first_result[b]]->mem->ptr : args[B.param_index]->mem->ptr;   // updated in place: in a copy, which is the result (below)
       else if (B.kind == rx::BufferDesc::Const) where[b] = ex->consts[b]->ptr;
       else if (B.kind == rx::BufferDesc::Fault) where[b] = dev->fault_dev;
       else if (first_result[b] >= 0) where[b] = results[first_result[b]]->mem->ptr;
@@ -1158,7 +1157,7 @@ RX_EXPORT int RxExecuteNoAlloc(RxExecutable* ex, int num_args, RxBuffer** args, 
     std::lock_guard<std::mutex> slock(dev->scratch_mu);
     HIP_CHECK(hipSetDevice(dev->ordinal));
     for (size_t b = 0; b < NB; ++b)
-      if (P.buffers[b].written)
+      if (P.buffers[b].kind == rx::BufferDesc::Param && P.buffers[b].written)
         HIP_CHECK(hipMemcpyAsync(where[b], args[P.buffers[b].param_index]->mem->ptr, (size_t)P.buffers[b].bytes, hipMemcpyDeviceToDevice, dev->stream));
     std::vector<void*> ptrs, argv;
     for (size_t li = 0; li < P.launches.size(); ++li) {

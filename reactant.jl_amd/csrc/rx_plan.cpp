@@ -4137,7 +4137,8 @@ struct Planner {
       if (from < 0) continue;
       if (updates_in_place(results[r], n.in[from], root)) {
         buf_of[results[r]] = buffer_for(n.in[from]);
-        plan.buffers[buf_of[results[r]]].written = true;
+        BufferDesc& B = plan.buffers[buf_of[results[r]]];
+        B.written = B.kind == BufferDesc::Param;   // (a temporary holds nothing of the caller's)
       } else emit_map(results[r], n.in[from]);
     }
     std::vector<int> scratches;
@@ -6324,6 +6325,8 @@ std::string Plan::report() const {
     o << "  [" << i << "] " << L.kernel << " kind=" << L.kind << " grid=" << L.grid[0] << "x" << L.grid[1] << "x" << L.grid[2] << " block=" << L.block[0]
       << " lds=" << L.lds_bytes << " algo_bytes=" << (long long)L.algo_bytes << " flops=" << (long long)L.flops << " :: " << L.desc << "\n";
   }
+  for (auto& b : buffers)
+    if (b.written) o << "updated in place: argument " << b.param_index << "\n";
   o << "module costs: flops=" << (long long)hlo_flops << " transcendentals=" << (long long)hlo_transcendentals << " bytes_accessed=" << (long long)hlo_bytes_accessed
     << " output_bytes=" << (long long)hlo_output_bytes << "\n";
   return o.str();

@@ -16,7 +16,7 @@ struct BufferDesc {
   int first_def = -1;          // index of the launch that writes it (Temp/Scratch)
   int last_use = -1;           // index of the last launch that touches it
   bool is_result = false;
-  bool written = false;        // Param: a kernel updates it in place; the caller's array is copied first unless it is donated
+  bool written = false;        // Param only: a kernel updates it in place; the caller's array is copied first unless it is donated
 };
 
 struct Launch {
