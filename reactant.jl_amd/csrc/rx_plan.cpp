@@ -134,6 +134,7 @@ struct Planner {
   std::set<std::pair<int, int>> fused_operands;   // (dot_general, side): the operand is evaluated inside the GEMM's tile loads
   std::map<int, int> epilogue_of;   // dot_general -> the elementwise root that absorbs it (the product is launched there)
   std::map<int, int> row_anchor;    // reduction fused into a row kernel -> the root of that kernel
+  std::map<int, int> reduce_of;     // elementwise root on a full reduction's scalar -> the reduction, whose kernel computes it
   std::ostringstream src;
   int kcount = 0;
   bool uses_operators = false;      // the text calls device functions of rx_lm_kernels.h
@@ -3753,13 +3754,15 @@ struct Planner {
 
   // Kernels are launched in the node order of their jobs, but some values are computed by a job
   // that comes later than their own node: a product absorbed by its epilogue runs at the
-  // epilogue's root, a reduction fused into a row kernel at the row anchor, a stencil step that
-  // lives in LDS only inside the kernel of the step that reads it.
+  // epilogue's root, a reduction fused into a row kernel at the row anchor, a full reduction whose
+  // kernel computes its scalar's reader at that reader, a stencil step that lives in LDS only inside
+  // the kernel of the step that reads it.
   int launch_position(int u) const {
     auto e = epilogue_of.find(u);
     if (e != epilogue_of.end()) return e->second;
     auto r = row_anchor.find(u);
     if (r != row_anchor.end()) return r->second;
+    for (auto& kv : reduce_of) if (kv.second == u) return kv.first;
     if (lds_only.count(u))
       for (auto& kv : fuse_prev) if (kv.second == u) return kv.first;
     return u;
@@ -6114,7 +6117,6 @@ struct Planner {
 
     // A full reduction whose only reader is elementwise on its scalar (a mean's division, a root) runs that as well: no launch
     // for one number (4 us).
-    std::map<int, int> reduce_of;   // that root -> the reduction
     for (int x = 0; x < N && opt.product_epilogues; ++x) {
       if (!live[x] || g.nodes[x].k != OpK::Reduce || ctx[x].size() != 1) continue;
       if (std::find(g.results.begin(), g.results.end(), x) != g.results.end() || red_shape(g.nodes[x]).nkeep != 0 || g.nodes[g.nodes[x].in[0]].ty.numel() == 0) continue;

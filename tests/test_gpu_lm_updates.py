@@ -54,3 +54,37 @@ def check(rx, client, text):
 @pytest.mark.parametrize("name", sorted(M.TEMPORARIES))
 def test_appends_to_temporaries(rx, client, name):
     check(rx, client, M.TEMPORARIES[name])
+
+
+@pytest.mark.parametrize("reader", ["sqrt", "negate"])
+def test_a_reduction_of_the_cache_before_an_append(rx, client, reader):
+    text = M.reduce_then_append(reader)
+    args = values(text)
+    want = [t.a for t in I.run_text(text, args, hifi=True)]
+    thunk = rx.compile(text)
+    n = args[8].a.size
+    for donated in (False, True):
+        dev = [rx.to_rarray(a.a.T, a.dt) for a in args]
+        out = thunk(*dev, donated=[False] * 8 + [True] * 2 if donated else None)
+        for got, ref in zip(out[:3], want):
+            close(got.to_array().T, ref)
+        # squares and their sum in f32: n + 1 roundings of 2^-24 at most, then the reader's
+        assert abs(float(out[3].to_array()) - float(want[3])) <= (n + 3) * 2.0 ** -24 * abs(float(want[3]))
+    bufs = [rx.Buffer.from_host(client, a.a, a.dt) for a in args]
+    res = [rx.Buffer.uninitialized(client, ref.shape, "f32") for ref in want]
+    for _ in range(2):
+        thunk.exec.execute_no_alloc(bufs, res)
+        client.default_device().synchronize()
+        close(res[1].to_host(), want[1])
+        assert abs(float(res[3].to_host()) - float(want[3])) <= (n + 3) * 2.0 ** -24 * abs(float(want[3]))
+
+
+def test_a_reduction_of_a_product_before_its_update(rx, client):
+    text = M.reduce_then_update()
+    rng = np.random.default_rng(2)
+    args = [I.Tensor(rng.integers(-3, 4, size=s).astype(np.float64), "f32") for s in ([64, 32], [32, 32])] + [I.Tensor(np.full((8, 32), 1000.0), "f32")]
+    m = args[0].a.astype(np.float64) @ args[1].a                       # whole numbers: exact, and so is the sum of their squares
+    want = m.copy()
+    want[16:24] = 1000.0
+    got = [o.to_array().T for o in rx.compile(text)(*[rx.to_rarray(a.a.T, a.dt) for a in args])]
+    assert np.array_equal(got[0], want) and abs(float(got[1]) - np.sqrt((m * m).sum())) <= 2.0 ** -22 * np.sqrt((m * m).sum())

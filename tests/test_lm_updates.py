@@ -72,6 +72,28 @@ def appends_in_a_loop(times=3):
             + "    return %%w#2, %%w#3 : %s, %s\n  }\n}\n" % (cache, cache))
 
 
+def reduce_then_append(reader="sqrt", dt="f32"):
+    """(.., k_cache, v_cache) -> (q', k_cache', v_cache', sqrt of the sum of the keys' squares as they were): the reduction ends in its reader, which stands after the append."""
+    x = P._Text()
+    (a,), kc, vc = arguments(x, (1, 2), dt)
+    total = x.op("reduce(%s init: %s) applies stablehlo.add across dimensions = [0, 1, 2, 3] : (%s, tensor<%s>)"
+                 % (x.binary("multiply", kc, kc), x.constant("0.000000e+00", [], dt), x.types[kc], dt), [], dt)
+    new = appends(x, *a, kc, vc, dt=dt)
+    return x.module("reduce_then_append", new + [x.op("%s %s : (tensor<%s>)" % (reader, total, dt), [], dt)])
+
+
+def reduce_then_update(dt="f32"):
+    """The same with a range of a product: (a, b, u) -> (a b with u in its middle, the square root of the sum of the squares of a b)."""
+    x = P._Text()
+    a, b, u = x.arg([64, 32], dt), x.arg([32, 32], dt), x.arg([8, 32], dt)
+    m = x.dot(a, b, (1, 0))
+    total = x.op("reduce(%s init: %s) applies stablehlo.add across dimensions = [0, 1] : (%s, tensor<%s>)"
+                 % (x.binary("multiply", m, m), x.constant("0.000000e+00", [], dt), x.types[m], dt), [], dt)
+    at, zero = x.constant("16", [], "i32"), x.constant("0", [], "i32")
+    new = x.op("dynamic_update_slice %s, %s, %s, %s : (%s, %s, tensor<i32>, tensor<i32>)" % (m, u, at, zero, x.types[m], x.types[u]), [64, 32], dt)
+    return x.module("reduce_then_update", [new, x.op("sqrt %s : (tensor<%s>)" % (total, dt), [], dt)])
+
+
 def report(text):
     lines = rx.compile_offline(text).splitlines()
     return [l.split("kind=")[1].split()[0] for l in lines if "kind=" in l], sorted(int(l.split("argument ")[1]) for l in lines if l.startswith("updated in place"))
@@ -92,11 +114,24 @@ def test_a_temporary_is_no_argument_to_copy(name):
     assert "lm_kv_append" in kinds and updated == []
 
 
+def test_a_reduction_that_ends_in_a_later_kernel_reads_the_cache_as_it_was():
+    """It runs where its reader does: an append before that place is to a copy."""
+    kinds, updated = report(reduce_then_append())
+    assert 9 in updated
+    assert 8 not in updated or min(i for i, k in enumerate(kinds) if k.startswith("reduce")) < kinds.index("lm_kv_append")
+
+
+def test_so_it_does_where_a_range_is_updated():
+    """In the product's own memory (kind map_in_place: the range alone is written) only after the reduction has read it."""
+    kinds, _ = report(reduce_then_update())
+    assert "map_in_place" not in kinds or min(i for i, k in enumerate(kinds) if k.startswith("reduce")) < kinds.index("map_in_place")
+
+
 def test_host_code_under_sanitizers(tmp_path):
     if not os.path.exists(HOSTCHECK):
         pytest.skip("the sanitizer program is not built")
     files = []
-    for k, text in enumerate(TEMPORARIES.values()):
+    for k, text in enumerate([*TEMPORARIES.values(), reduce_then_append(), reduce_then_update()]):
         files.append(tmp_path / ("updates%d.mlir" % k))
         files[-1].write_text(text)
     r = subprocess.run([HOSTCHECK] + [str(f) for f in files], capture_output=True, text=True)
