@@ -1173,6 +1173,7 @@ RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, flo
         __syncthreads();
         n = count;
         search = n > CAP - 256;
+        __syncthreads();                                        // (every wavefront has read the count before one adds to it)
         for (int j = j0; !search && n < K && j < j1; j += 256) {
           const int mine = j + (int)threadIdx.x;
           if (mine < j1 && rx_lm_order(E::up(row.x[mine])) == least) keys[atomicAdd(&count, 1)] = rx_lm_key(E::up(row.x[mine]), mine);
