@@ -1183,12 +1183,12 @@ RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, flo
         }
       }
       if (search) {
-        rx_u64 below = ~0ull;
+        rx_u64 below = 0;
         for (int k = 0; k < K; ++k) {
           rx_u64 top = 0;
           for (int j = j0 + (int)threadIdx.x; j < j1; j += 256) {
             const rx_u64 key = rx_lm_key(E::up(row.x[j]), j);
-            if (key < below && key > top) top = key;
+            if ((k == 0 || key < below) && key > top) top = key;   // (a NaN at index 0 has the largest key there is)
           }
           __syncthreads();
           top = rx_block_reduce<rx_u64, rx_op_max, 4>(top, rx_op_max(), red64);
