@@ -46,6 +46,7 @@ RX_DEV bool rx_lm_last_to_arrive(int* counter, const int expected, int* flag) {
 }
 
 #define RX_LM_LOG2E 1.4426950408889634f
+#define RX_LM_FLT_MAX 3.4028234663852886e38f
 RX_DEV float rx_lm_inf() { return __builtin_inff(); }
 
 // ---------------------------------------------------------------------------
@@ -749,10 +750,11 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, x[i]);
-        top = __builtin_fmaxf(m[t], rx_lm_max4(top));
-        const float base = top == -rx_lm_inf() ? 0.0f : top;     // (a head whose scores are all -inf so far)
+        // (not below the lowest number: a maximum of -inf says that there was no position, and scores that are all -inf or NaN
+        // leave a sum of nothing, or NaN, beside it: the result is NaN, not the zeros of an empty sequence)
+        top = __builtin_fmaxf(__builtin_fmaxf(m[t], rx_lm_max4(top)), -RX_LM_FLT_MAX);
         if (__any(top != m[t])) {
-          const float shrink = __builtin_amdgcn_exp2f(m[t] - base);
+          const float shrink = __builtin_amdgcn_exp2f(m[t] - top);
           l[t] *= shrink;
 #pragma unroll
           for (int j = 0; j < NV; ++j)
@@ -765,7 +767,7 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float p = __builtin_amdgcn_exp2f(x[i] - base + SHIFT);
+          const float p = __builtin_amdgcn_exp2f(x[i] - top + SHIFT);
           l[t] += p;
           w[t].v[i] = E::down(p);
           rest[t].v[i] = E::down(p - E::up(w[t].v[i]));
@@ -844,8 +846,8 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
         }
         const int qh = (head0 + hw) * G + tile * GT + t * 16 + h;
         if (whole) {
-          out[((long long)b * HQ + qh) * DV + d] = E::down(sum == 0.0f ? 0.0f : o / sum);
-          if (lse && d == 0) lse[(long long)b * HQ + qh] = sum == 0.0f ? -rx_lm_inf() : (hi - SHIFT + __builtin_log2f(sum)) * 0.6931471805599453f;
+          out[((long long)b * HQ + qh) * DV + d] = E::down(hi == -rx_lm_inf() ? 0.0f : o / sum);
+          if (lse && d == 0) lse[(long long)b * HQ + qh] = hi == -rx_lm_inf() ? -rx_lm_inf() : (hi - SHIFT + __builtin_log2f(sum)) * 0.6931471805599453f;
         } else {
           const long long at = (((long long)id * 2 + (unit == 0)) * HW + hw) * GT + t * 16 + h;
           rx_lm_put_shared(part + at * DV + d, o);
@@ -901,8 +903,8 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
     }
     if (!on || way) continue;
 #pragma unroll
-    for (int e = 0; e < VD; ++e) out[((long long)b * HQ + qh) * DV + d + e * (DV / VD)] = E::down(j.s == 0.0f ? 0.0f : j.o[e] / j.s);
-    if (lse && d == 0) lse[(long long)b * HQ + qh] = j.s == 0.0f ? -rx_lm_inf() : (j.m + __builtin_log2f(j.s)) * 0.6931471805599453f;
+    for (int e = 0; e < VD; ++e) out[((long long)b * HQ + qh) * DV + d + e * (DV / VD)] = E::down(j.m == -rx_lm_inf() ? 0.0f : j.o[e] / j.s);
+    if (lse && d == 0) lse[(long long)b * HQ + qh] = j.m == -rx_lm_inf() ? -rx_lm_inf() : (j.m + __builtin_log2f(j.s)) * 0.6931471805599453f;
   }
   }
 }

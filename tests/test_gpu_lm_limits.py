@@ -50,3 +50,69 @@ def test_alternatives_of_rows_that_are_no_numbers(rx, client, n, v, top, dt):
     for out in got[:3]:
         assert np.array_equal(np.isnan(out), no_number)
     assert np.isnan(got[3][no_number]).all() and not np.isnan(got[3][~no_number]).any()
+
+
+@pytest.mark.parametrize("lengths,hq,hk,d,size,dt,layout", [
+    ([5, 0, 70], 4, 2, 64, 16, "bf16", "slots"), ([3000, 40, 0, 1], 8, 1, 128, 16, "f16", "heads"), ([900, 33], 3, 3, 40, 7, "f32", "slots"), ([6000], 8, 2, 64, 64, "f32", "heads"),
+    ([64] * 70, 24, 1, 32, 16, "bf16", "slots"),
+])
+def test_attention_of_what_is_no_number(rx, client, lengths, hq, hk, d, size, dt, layout):
+    """A query with NaN, keys in use with NaN, and scores that are all -inf give NaN, in sequences of one part and of many; other
+    heads and sequences keep their bits, and empty ones their zeros."""
+    rng = np.random.default_rng(d)
+    b = len(lengths)
+    cols, pages = -(-max(lengths) // size) + 1, sum(-(-n // size) for n in lengths) + 2
+    args = T.attention_case(rng, lengths, hq, hk, d, d, pages, size, cols, dt, layout)
+    text = P.paged_attention(b, hq, hk, d, pages, size, cols, dt=dt, layout=layout, lse=True)
+    clean, exe = gpu_run(rx, client, text, args)
+    full = [s for s in range(b) if lengths[s]]
+
+    def others_keep(got, sequence, heads):
+        same = np.ones((b, hq), bool)
+        same[sequence, heads] = False
+        assert np.array_equal(got[0].a[same], clean[0].a[same]) and np.array_equal(got[1].a[same], clean[1].a[same])
+    for s in {full[0], full[-1]}:
+        q = args[0].a.copy()
+        q[s, 1, 3] = np.nan                                             # every score of one head
+        got, _ = gpu_run(rx, client, text, [I.Tensor(q, dt)] + args[1:], exe)
+        assert np.isnan(got[0].a[s, 1]).all() and np.isnan(got[1].a[s, 1])
+        others_keep(got, s, [1])
+        at = rng.integers(0, lengths[s])                                # one key of one head
+        k = args[1].a.copy()
+        page, slot = args[3].a[s, at // size], at % size
+        k[(page, slot, 0) if layout == "slots" else (page, 0, slot)] = np.nan
+        got, _ = gpu_run(rx, client, text, [args[0], I.Tensor(k, dt)] + args[2:], exe)
+        assert np.isnan(got[0].a[s, :hq // hk]).all() and np.isnan(got[1].a[s, :hq // hk]).all()
+        others_keep(got, s, range(hq // hk))
+        q = args[0].a.copy()
+        q[s, 0] = 0.0
+        q[s, 0, 0] = -np.inf                                            # all scores -inf: a sum of nothing
+        k = args[1].a.copy()
+        k[..., 0] = np.where(np.isnan(k[..., 0]), np.nan, 1.0)
+        got, _ = gpu_run(rx, client, text, [I.Tensor(q, dt), I.Tensor(k, dt)] + args[2:], exe)
+        assert np.isnan(got[0].a[s, 0]).all() and got[1].a[s, 0] == -np.inf
+    for s in range(b):
+        if not lengths[s]:
+            assert np.all(clean[0].a[s] == 0) and np.all(clean[1].a[s] == -np.inf)
+
+
+def test_attention_of_a_few_scores_of_minus_infinity(rx, client):
+    """Positions whose scores are -inf among others count nothing, wherever the first finite one stands."""
+    n, pages = 300, 20
+    rng = np.random.default_rng(4)
+    args = T.attention_case(rng, [n, 31], 4, 2, 64, 64, pages + 2, 16, 20, "f32", "heads")
+    k = args[1].a
+    k[..., 0] = np.where(np.isnan(k[..., 0]), np.nan, 1.0)
+    finite = [5, 40, 299], [30]
+    for s, js in enumerate(finite):
+        for j in js:
+            k[args[3].a[s, j // 16], :, j % 16] = 0.0
+    args[0].a[:, :, 0] = -3.0e38                                        # times 1.0 and the scale's 8 beyond f32
+    text = P.paged_attention(2, 4, 2, 64, pages + 2, 16, 20, dt="f32", layout="heads", lse=True, scale=8.0)
+    got, _ = gpu_run(rx, client, text, args)
+    v = args[2].a
+    for s, js in enumerate(finite):                                     # scores of 0: their mean
+        rows = np.stack([v[args[3].a[s, j // 16], :, j % 16] for j in js]).astype(np.float64)
+        for h in range(4):
+            assert np.all(np.abs(got[0].a[s, h] - rows[:, h // 2].mean(0)) <= 8 * T.UF * np.abs(rows[:, h // 2]).max(0))
+            assert abs(got[1].a[s, h] - np.log(len(js))) <= 4 * T.UF
