@@ -955,7 +955,7 @@ struct rx_lm_row {
 
 // Running (maximum m, sum s of e^(x - m), sum t of e^(x - m) log2 e^(x - m)); the last gives the entropy.  An exponential is
 // 2^(x L - c), one fused multiply-add and the hardware's 2^y, with c the rounded product m L: that s belongs to c and not to m
-// is undone exactly where sums of another maximum come in and in lse.  (L is log2 e rounded to f32, off by 1e-8 of itself, which
+// is undone exactly where sums of another maximum come in and in the log of s.  (L is log2 e rounded to f32, off by 1e-8 of itself, which
 // turns e^x into e^(x (1 + 1e-8)).)  Beyond 1e30 the product would overflow: such maxima are not used as c, and their rows
 // come out as no number or nothing and are computed again with differences (`rx_lm_careful`).
 struct rx_lm_yes { static constexpr bool value = true; };
@@ -975,11 +975,14 @@ struct rx_op_lm_sums {
     return {m, x.s + y.s, x.t + y.t};
   }
 };
-RX_DEV float rx_lm_lse(const rx_lm_sums a) {
-  if (a.s == 0.0f) return -rx_lm_inf();
-  const float l = __builtin_log2f(a.s);
-  return rx_lm_plain(a.m) ? (a.m * RX_LM_LOG2E + l) * 0.6931471805599453f : a.m + l * 0.6931471805599453f;
+// log of the sum of e^(x - m): what the rounding of c took from m L, known exactly, is in s as a factor
+RX_DEV float rx_lm_log_sum(const rx_lm_sums a) {
+  const float c = a.m * RX_LM_LOG2E, left = rx_lm_plain(a.m) ? __builtin_fmaf(a.m, RX_LM_LOG2E, -c) : 0.0f;
+  return (__builtin_log2f(a.s) - left) * 0.6931471805599453f;
 }
+RX_DEV float rx_lm_lse(const rx_lm_sums a) { return a.s == 0.0f ? -rx_lm_inf() : a.m + rx_lm_log_sum(a); }
+// x - lse, the difference from the maximum first: lse's own rounding would be far larger than the result where logits are
+RX_DEV float rx_lm_log_probability(const float x, const rx_lm_sums a) { return a.s == 0.0f ? -rx_lm_inf() : (x - a.m) - rx_lm_log_sum(a); }
 // the sums of a workgroup's threads
 RX_DEV rx_lm_sums rx_lm_block_sums(rx_lm_sums a, rx_lm_sums* red /* 4 */) {
   a = rx_lm_rebase(a, rx_wave_reduce(a.m, rx_op_max()));
@@ -1032,10 +1035,9 @@ RX_DEV void rx_lm_select(const rx_u64* keys, const int n, F put) {
 template <typename E, int V, typename I>
 RX_DEV void rx_lm_row_results(const long long t, const rx_lm_sums a, const typename E::S* x, const I* targets, float* logprob, float* lse, float* entropy) {
   const I y = targets[t];
-  const float l = rx_lm_lse(a);
-  lse[t] = l;
+  lse[t] = rx_lm_lse(a);
   entropy[t] = a.s == 0.0f ? 0.0f : (__builtin_log2f(a.s) - a.t / a.s) * 0.6931471805599453f;
-  logprob[t] = y < 0 || y >= V ? 0.0f : a.s == 0.0f ? -rx_lm_inf() : E::up(x[y]) - l;
+  logprob[t] = y < 0 || y >= V ? 0.0f : rx_lm_log_probability(E::up(x[y]), a);
 }
 
 // A workgroup per segment of a row (SPLIT segments; one: the whole row), in one pass with the running sums, and the alternatives
@@ -1219,11 +1221,10 @@ RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, flo
     }
     if (threadIdx.x == 0) rx_lm_row_results<E, V>(t, a, row.x, targets, logprob, lse, entropy);
     if constexpr (K > 0) {
-      const float l = rx_lm_lse(a);
       rx_lm_select<K>(keys, n, [&](const int rank, const rx_u64 key) {
         const int j = (int)~(rx_u32)key;
         ids[t * K + rank] = j;
-        values[t * K + rank] = a.s == 0.0f ? -rx_lm_inf() : E::up(row.x[j]) - l;
+        values[t * K + rank] = rx_lm_log_probability(E::up(row.x[j]), a);
       });
     }
   }

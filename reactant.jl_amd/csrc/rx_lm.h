@@ -23,7 +23,8 @@
 //   rx.token_logprobs(logits [.., V], targets [..]) {top} -> (logprob, lse, entropy [, values [.., top], ids [.., top]])
 //       log softmax at the target (0 where it is outside [0, V)), log of the sum of exponentials, entropy, and the `top`
 //       largest log probabilities with their indices, largest first, equal ones by index.  -inf logits have probability 0; a row of
-//       nothing else has lse = logprob = -inf and entropy 0, and its values are -inf.
+//       nothing else has lse = logprob = -inf and entropy 0, and its values are -inf.  A row with +inf or NaN has no probabilities:
+//       its numbers are NaN, and its alternatives those of its logits, NaN before +inf.
 //   rx.token_logprobs_grad(logits, targets, lse, entropy, d_logprob, d_entropy) -> d_logits
 //
 // Caches are [pages, S, Hk, D] (layout "slots") or [pages, Hk, S, D] ("heads").  Floats are f32, bf16 or f16, one type per operator

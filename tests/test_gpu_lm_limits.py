@@ -116,3 +116,34 @@ def test_attention_of_a_few_scores_of_minus_infinity(rx, client):
         for h in range(4):
             assert np.all(np.abs(got[0].a[s, h] - rows[:, h // 2].mean(0)) <= 8 * T.UF * np.abs(rows[:, h // 2]).max(0))
             assert abs(got[1].a[s, h] - np.log(len(js))) <= 4 * T.UF
+
+
+@pytest.mark.parametrize("n,v,top,dt,around", [(5, 1000, 5, "f32", 3.0e4), (5, 1000, 5, "f32", -3.0e4), (4, 33000, 20, "f16", 4.0e4), (3, 70001, 3, "bf16", 1.0e4), (600, 777, 1, "f32", 1.0e6), (4, 5000, 0, "f32", 5.0e3)])
+def test_log_probabilities_of_large_logits(rx, client, n, v, top, dt, around):
+    """A log probability is a difference of logits less the log of a sum of moderate size, whatever the logits' own magnitude: off by
+    the sum's error (as for small logits) and roundings of the difference and of that log; the log of the sum of exponentials
+    itself by those and its own rounding."""
+    rng = np.random.default_rng(v)
+    x = T.rounded(around + rng.normal(size=(n, v)) * 3, dt)
+    y = np.argmax(x.a, 1)
+    got = [t.a.astype(np.float64) for t in gpu_run(rx, client, P.token_logprobs(n, v, top=top, dt=dt), [x, I.Tensor(y, "i32")])[0]]
+    want = L.token_logprobs(x.a, y, top)
+    e = (v / 64 + 64 + 44) * T.UF
+    below = want[1] - x.a.max(1)                                        # log of the sum of e^(x - max)
+    error = e + 4 * T.UF * (np.abs(below) + 1)
+    assert np.all(np.abs(got[1] - want[1]) <= error + T.UF * np.abs(want[1]))
+    assert np.all(np.abs(got[0] - want[0]) <= error)
+    assert np.all(np.abs(got[2] - want[2]) <= 2 * e * (1 + np.abs(want[2])) + 4 * T.UF * (np.abs(want[2]) + 1))
+    if top:
+        assert np.array_equal(got[4], want[4])
+        far = x.a.max(1, keepdims=True) - np.take_along_axis(x.a, want[4], 1)
+        assert np.all(np.abs(got[3] - want[3]) <= error[:, None] + 4 * T.UF * far)
+
+
+def test_rows_with_plus_infinity_have_no_probabilities(rx, client):
+    x = np.zeros((3, 5000))
+    x[0, 7] = x[1, 0] = np.inf
+    got = [t.a for t in gpu_run(rx, client, P.token_logprobs(3, 5000, top=3, dt="f32"), [I.Tensor(x, "f32"), I.Tensor([7, 3, 3], "i32")])[0]]
+    for out in got[:4]:
+        assert np.isnan(out[:2]).all() and not np.isnan(out[2]).any()
+    assert np.array_equal(got[4], [[7, 0, 1], [0, 1, 2], [0, 1, 2]])
