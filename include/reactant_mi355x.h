@@ -139,6 +139,9 @@ int RxCompileOffline(const char *mlir_text, size_t mlir_len, int with_source, ch
 const char *RxExecutableReport(RxExecutable *exec);
 int RxExecutableNumLaunches(RxExecutable *exec);
 int RxExecutableNumResults(RxExecutable *exec);
+/* Whether kernels of the executable wait, for a bounded time, for other workgroups of their launch (the one-launch scan): the
+ * only work whose failure shows after the call, when the device is next waited for (FutureAwait, BufferToHost, RxDeviceSynchronize). */
+int RxExecutableWaits(RxExecutable *exec);
 void RxExecutableLaunchInfo(RxExecutable *exec, int index, const char **kernel, const char **kind,
                             double *algorithmic_bytes, double *flops);
 /* XLAExecuteSharded with a HIP event pair attached to every kernel launch (start and stop

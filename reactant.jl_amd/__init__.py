@@ -114,6 +114,7 @@ SIGNATURES = {
     "RxExecutableReport": (_cp, [_vp]),
     "RxExecutableNumLaunches": (_i, [_vp]),
     "RxExecutableNumResults": (_i, [_vp]),
+    "RxExecutableWaits": (_i, [_vp]),
     "RxExecutableLaunchInfo": (None, [_vp, _i, _P(_cp), _P(_cp), _P(ctypes.c_double), _P(ctypes.c_double)]),
     "RxExecuteTimed": (None, [_vp, _i, _P(_vp), _vp, _P(_u8), _i, _P(_vp), _P(ctypes.c_float)]),
     "RxExecuteProfiled": (None, [_vp, _i, _P(_vp), _vp, _P(_u8), _i, _P(_vp)]),
@@ -286,10 +287,10 @@ class Client:
 class Future:
     """XLA.PJRT.Future (src/xla/PJRT/Future.jl) of an execution, one for all of its results.  The library's future completes
     when the device has reached the point at which it is first asked, so it is made then: most are never asked."""
-    __slots__ = ("client", "device", "handle", "__weakref__")
+    __slots__ = ("client", "device", "handle", "may_fail", "__weakref__")
 
-    def __init__(self, client, device):
-        self.client, self.device, self.handle = client, device, None
+    def __init__(self, client, device, may_fail=False):
+        self.client, self.device, self.handle, self.may_fail = client, device, None, may_fail
 
     def _asked(self):
         if self.handle is None and self.client.handle:
@@ -406,6 +407,7 @@ class LoadedExecutable:
         self.handle = handle
         self.client = client
         self.num_results = _call("RxExecutableNumResults", handle)
+        self.waits = bool(_call("RxExecutableWaits", handle))   # an execution can fail after the call
         self.result_types = None   # (shape in Julia order, element type) of every result: the module's, read off the first execution's
 
     def report(self):
@@ -446,7 +448,7 @@ class LoadedExecutable:
         if nres == 0 or not res[0]:                           # (every result of a call that succeeds has a handle)
             _check()
         client = self.client
-        future = Future(client, client.default_device().handle if device is None else dev)
+        future = Future(client, client.default_device().handle if device is None else dev, self.waits)
         return [AsyncBuffer(Buffer(r, client), future) for r in res]
 
     def execute_timed(self, buffers, donated=None, device=None):
@@ -691,11 +693,15 @@ class Thunk:
         self.client = client
 
     def __call__(self, *args, donated=None, sync=False):
+        bufs = []
         for a in args:
             if a.donated:
                 raise ReactantInternalError("accessing the data of a donated array")  # src/Types.jl:9-26
-        # the arguments are not waited for: a device's work is ordered on one stream
-        res = self.exec.execute_sharded([a.data.buffer for a in args], donated)
+            # An argument is waited for only where the execution that makes it can fail after its call, so that the error
+            # comes here and not after the argument has been used: a device's work is ordered on one stream.
+            data = a.data
+            bufs.append(data.buffer if data.future is None or not data.future.may_fail else data.synced_buffer())
+        res = self.exec.execute_sharded(bufs, donated)
         if donated:
             for a, d in zip(args, donated):
                 if d:

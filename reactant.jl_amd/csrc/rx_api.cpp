@@ -1046,6 +1046,7 @@ RX_EXPORT void RxExecutableCostAnalysis(RxExecutable* ex, float* props11) {
 RX_EXPORT const char* RxExecutableReport(RxExecutable* ex) { return guarded([&]() -> const char* { check_exec(ex); return ex->report.c_str(); }, ""); }
 RX_EXPORT int RxExecutableNumLaunches(RxExecutable* ex) { return guarded([&] { check_exec(ex); return (int)ex->plan.launches.size(); }, 0); }
 RX_EXPORT int RxExecutableNumResults(RxExecutable* ex) { return guarded([&] { check_exec(ex); return (int)ex->plan.result_types.size(); }, 0); }
+RX_EXPORT int RxExecutableWaits(RxExecutable* ex) { return guarded([&] { check_exec(ex); std::lock_guard<std::mutex> lock(ex->mu); return ex->waits ? 1 : 0; }, 0); }
 RX_EXPORT void RxExecutableLaunchInfo(RxExecutable* ex, int i, const char** kernel, const char** kind, double* bytes, double* flops) {
   guarded_void([&] {
     check_exec(ex);
