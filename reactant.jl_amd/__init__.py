@@ -444,6 +444,8 @@ class LoadedExecutable:
         don = flags(*map(bool, donated)) if donated else None
         res = handles()
         dev = device.handle if device is not None else None   # none: the executable's
+        if nres == 0:
+            lib.RxClearError()                                # (an older call's)
         _execute_sharded(self.handle, n, args, dev, don, nres, res, None, None)
         if nres == 0 or not res[0]:                           # (every result of a call that succeeds has a handle)
             _check()

@@ -10,6 +10,13 @@ class Handle:
     handle = 1
 
 
+class Client:
+    handle = 1
+
+    def default_device(self):
+        return Handle()
+
+
 class Execution:
     """Stands for an executable of one result."""
     result_types = [((2,), "f32")]
@@ -43,3 +50,15 @@ def test_a_call_raises_the_error_of_the_execution_that_made_its_argument():
     with pytest.raises(rx.ReactantInternalError, match="expired"):
         call(good, bad, donated=[True, True])
     assert len(exe.calls) == 1 and not good.donated and not bad.donated
+
+
+def test_a_call_without_results_raises_no_older_error(monkeypatch):
+    exe = object.__new__(rx.LoadedExecutable)
+    exe.handle, exe.client, exe.num_results, exe.waits = None, Client(), 0, False
+    monkeypatch.setattr(rx, "_execute_sharded", lambda *args: None)
+    rx.lib.RxExecutableNumResults(None)                         # an error that nobody asked for
+    assert rx.lib.RxLastError()
+    assert exe.execute_sharded([]) == []
+    monkeypatch.undo()
+    with pytest.raises(rx.ReactantInternalError):               # its own
+        exe.execute_sharded([])
