@@ -147,3 +147,32 @@ def test_rows_with_plus_infinity_have_no_probabilities(rx, client):
     for out in got[:4]:
         assert np.isnan(out[:2]).all() and not np.isnan(out[2]).any()
     assert np.array_equal(got[4], [[7, 0, 1], [0, 1, 2], [0, 1, 2]])
+
+
+@pytest.mark.parametrize("lengths,hq,hk,d,dt", [([64, 7, 2], 8, 2, 64, "bf16"), ([64, 7, 2], 8, 2, 64, "f16"), ([40], 16, 1, 128, "bf16"), ([7, 2], 24, 1, 128, "f16")])
+def test_attention_weights_are_not_rounded_to_the_caches_type(rx, client, lengths, hq, hk, d, dt):
+    """Values of 1 and -1 under nearly equal weights: results near zero, of which an error of the weights is a large part.  The weights
+    enter the product as two 16-bit numbers, off by u of u of themselves; scores and sums are off as in test_gpu_lm_operators.py.  Weights
+    rounded once, in the formula, do not meet the bound."""
+    rng = np.random.default_rng(d + hq)
+    b, size, scale = len(lengths), 16, 0.005
+    cols, pages = -(-max(lengths) // size) + 1, sum(-(-n // size) for n in lengths) + 2
+    args = T.attention_case(rng, lengths, hq, hk, d, d, pages, size, cols, dt, "slots")
+    args[2].a[...] = np.where(np.isnan(args[2].a), np.nan, np.sign(args[2].a))
+    got, _ = gpu_run(rx, client, P.paged_attention(b, hq, hk, d, pages, size, cols, dt=dt, scale=scale), args)
+    a = [t.a for t in args]
+    ref, lse, mag = L.paged_attention(*a, scale=scale)
+    q, k = a[0].astype(np.float64), np.abs(np.nan_to_num(a[1].astype(np.float64))).max()
+    s = (d + 2) * T.UF * scale * np.abs(q).sum(-1).max() * k
+    bound = mag * (T.U[dt] ** 2 + 2 * s + (max(lengths) + 16) * T.UF) + T.U[dt] * np.abs(ref)
+    assert np.all(np.abs(got[0].a.astype(np.float64) - ref) <= bound)
+    worst = 0.0
+    for j, n in enumerate(lengths):                                     # the mistake, in the formula
+        rows = [(a[3][j, t // size], t % size) for t in range(n)]
+        keys, vals = (np.stack([c[r] for r in rows]).astype(np.float64) for c in a[1:3])
+        for h in range(hq):
+            x = scale * keys[:, h // (hq // hk)] @ q[j, h]
+            p = np.exp(x - x.max())
+            wrong = (T.rounded(p, dt).a.astype(np.float64) @ vals[:, h // (hq // hk)]) / p.sum()
+            worst = max(worst, (np.abs(wrong - ref[j, h]) / bound[j, h]).max())
+    assert worst > 1
