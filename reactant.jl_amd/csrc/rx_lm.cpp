@@ -54,6 +54,11 @@ struct Checker {
     require(end && *end == 0 && end != it->second.c_str() && std::isfinite(v), std::string("setting '") + key + "' must be a finite number, got '" + it->second + "'");
     return v;
   }
+  // a factor that the kernels hold in f32 (attention's times log2 e)
+  void scale() const {
+    const double v = number("scale", 1.0);
+    require(std::fabs(v) <= 2e38, "setting 'scale' must be a number that f32 holds, up to 2e38, got '" + (s.attrs.count("scale") ? s.attrs.at("scale") : std::string()) + "'");
+  }
   int64_t integer(const char* key, int64_t otherwise) const {
     const double v = number(key, (double)otherwise);
     require(v == std::floor(v) && std::fabs(v) < 1e15, std::string("setting '") + key + "' must be a whole number");
@@ -124,7 +129,7 @@ std::string st(const TType& t) { return info(t.dt).stype; }
 void check_embedding(const Checker& c) {
   const TType &table = c.s.in[0], &ids = c.s.in[1], &out = c.s.out[0];
   c.settings({"scale"});
-  c.number("scale", 1.0);
+  c.scale();
   c.rank(table, 2, "the table");
   c.floats(table, "the table");
   c.ints(ids, "ids");
@@ -154,7 +159,7 @@ OperatorPlan plan_embedding(const OperatorSpec& s) {
 void check_embedding_grad(const Checker& c) {
   const TType &dy = c.s.in[0], &ids = c.s.in[1], &out = c.s.out[0];
   c.settings({"scale"});
-  c.number("scale", 1.0);
+  c.scale();
   c.floats(dy, "dy");
   c.ints(ids, "ids");
   c.require(dy.rank() >= 1, "dy must have a dimension");
@@ -310,7 +315,7 @@ void check_attention(const Checker& c) {
     c.f32(c.s.out[1], "lse");
     c.dims(c.s.out[1], {B, Hq}, "lse");
   }
-  c.number("scale", 1.0);
+  c.scale();
   c.require(c.integer("window", 0) >= 0, "the window must not be negative");
   c.require(B <= 65535 && Hq <= 65535, "too many sequences or heads");
   c.require(B * Hq * std::max<int64_t>(vc.dim, 1) <= kMaxRow, "too many sequences and heads");
