@@ -54,10 +54,11 @@ struct Checker {
     require(end && *end == 0 && end != it->second.c_str() && std::isfinite(v), std::string("setting '") + key + "' must be a finite number, got '" + it->second + "'");
     return v;
   }
-  // a factor that the kernels hold in f32 (attention's times log2 e)
-  void scale() const {
+  // a factor that the kernels hold in f32, `times` another
+  void scale(double times = 1.0) const {
     const double v = number("scale", 1.0);
-    require(std::fabs(v) <= 2e38, "setting 'scale' must be a number that f32 holds, up to 2e38, got '" + (s.attrs.count("scale") ? s.attrs.at("scale") : std::string()) + "'");
+    require(std::fabs(v * times) <= 3.4028234e38, "setting 'scale' must be a number that f32 holds" + std::string(times > 1 ? " times log2 e" : "") + ", got '" +
+                                                     (s.attrs.count("scale") ? s.attrs.at("scale") : std::string()) + "'");
   }
   int64_t integer(const char* key, int64_t otherwise) const {
     const double v = number(key, (double)otherwise);
@@ -315,7 +316,7 @@ void check_attention(const Checker& c) {
     c.f32(c.s.out[1], "lse");
     c.dims(c.s.out[1], {B, Hq}, "lse");
   }
-  c.scale();
+  c.scale(1.4426950408889634);
   c.require(c.integer("window", 0) >= 0, "the window must not be negative");
   c.require(B <= 65535 && Hq <= 65535, "too many sequences or heads");
   c.require(B * Hq * std::max<int64_t>(vc.dim, 1) <= kMaxRow, "too many sequences and heads");
