@@ -956,13 +956,18 @@ struct rx_lm_row {
 // Running (maximum m, sum s of e^(x - m), sum t of e^(x - m) log2 e^(x - m)); the last gives the entropy.  An exponential is
 // 2^(x L - c), one fused multiply-add and the hardware's 2^y, with c the rounded product m L: that s belongs to c and not to m
 // is undone exactly where sums of another maximum come in and in the log of s.  (L is log2 e rounded to f32, off by 1e-8 of itself, which
-// turns e^x into e^(x (1 + 1e-8)).)  Beyond 1e30 the product would overflow: such maxima are not used as c, and their rows
-// come out as no number or nothing and are computed again with differences (`rx_lm_careful`).
+// turns e^x into e^(x (1 + 1e-8)).)  From 1e8 on c is off by up to 8 and more, and a sum soon has no room for the factor: the sums
+// of such a maximum belong to m, with differences from it (`rx_lm_careful`).  A row goes there from half of that on, so that what a
+// thread lost whose own maximum was lower is e^-5e7 and less of the row's.
 struct rx_lm_yes { static constexpr bool value = true; };
 struct rx_lm_no { static constexpr bool value = false; };
 struct rx_lm_sums { float m, s, t; };
-RX_DEV bool rx_lm_plain(const float m) { return __builtin_fabsf(m) < 1e30f; }
-RX_DEV float rx_lm_apart(const float m, const float of) { return rx_lm_plain(m) && rx_lm_plain(of) ? m * RX_LM_LOG2E - of * RX_LM_LOG2E : (m - of) * RX_LM_LOG2E; }
+RX_DEV bool rx_lm_plain(const float m) { return __builtin_fabsf(m) < 1e8f; }   // its sums belong to c
+// what the rounding of c took from m L, exactly
+RX_DEV float rx_lm_left(const float m) { return rx_lm_plain(m) ? __builtin_fmaf(m, RX_LM_LOG2E, -(m * RX_LM_LOG2E)) : 0.0f; }
+RX_DEV float rx_lm_apart(const float m, const float of) {
+  return rx_lm_plain(m) && rx_lm_plain(of) ? m * RX_LM_LOG2E - of * RX_LM_LOG2E : (m - of) * RX_LM_LOG2E - rx_lm_left(m) + rx_lm_left(of);
+}
 RX_DEV rx_lm_sums rx_lm_rebase(const rx_lm_sums a, const float m) {
   if (a.m == m || a.m == -rx_lm_inf()) return {m, a.s, a.t};   // (nothing so far: the sums are 0, or NaN)
   const float d = rx_lm_apart(a.m, m), f = __builtin_amdgcn_exp2f(d);
@@ -975,11 +980,8 @@ struct rx_op_lm_sums {
     return {m, x.s + y.s, x.t + y.t};
   }
 };
-// log of the sum of e^(x - m): what the rounding of c took from m L, known exactly, is in s as a factor
-RX_DEV float rx_lm_log_sum(const rx_lm_sums a) {
-  const float c = a.m * RX_LM_LOG2E, left = rx_lm_plain(a.m) ? __builtin_fmaf(a.m, RX_LM_LOG2E, -c) : 0.0f;
-  return (__builtin_log2f(a.s) - left) * 0.6931471805599453f;
-}
+// log of the sum of e^(x - m)
+RX_DEV float rx_lm_log_sum(const rx_lm_sums a) { return (__builtin_log2f(a.s) - rx_lm_left(a.m)) * 0.6931471805599453f; }
 RX_DEV float rx_lm_lse(const rx_lm_sums a) { return a.s == 0.0f ? -rx_lm_inf() : a.m + rx_lm_log_sum(a); }
 // x - lse, the difference from the maximum first: lse's own rounding would be far larger than the result where logits are
 RX_DEV float rx_lm_log_probability(const float x, const rx_lm_sums a) { return a.s == 0.0f ? -rx_lm_inf() : (x - a.m) - rx_lm_log_sum(a); }
@@ -993,15 +995,16 @@ RX_DEV rx_lm_sums rx_lm_block_sums(rx_lm_sums a, rx_lm_sums* red /* 4 */) {
   __syncthreads();
   return rx_op_lm_sums()(rx_op_lm_sums()(red[0], red[1]), rx_op_lm_sums()(red[2], red[3]));
 }
-// elements [j0, j1) of a row with the differences from the maximum, in two passes
+// elements [j0, j1) of a row in two passes, the second with the maximum of all
 template <typename E>
 RX_DEV rx_lm_sums rx_lm_careful(const typename E::S* x, const int j0, const int j1, rx_lm_sums* red) {
   rx_lm_sums a = {-rx_lm_inf(), 0.0f, 0.0f};
   for (int j = j0 + (int)threadIdx.x; j < j1; j += 256) a.m = __builtin_fmaxf(a.m, E::up(x[j]));
   a.m = rx_lm_block_sums(a, red).m;
-  const float base = a.m == -rx_lm_inf() ? 0.0f : a.m;
+  const float base = a.m == -rx_lm_inf() ? 0.0f : a.m, c = base * RX_LM_LOG2E;
+  const bool plain = rx_lm_plain(a.m);
   for (int j = j0 + (int)threadIdx.x; j < j1; j += 256) {
-    const float d = (E::up(x[j]) - base) * RX_LM_LOG2E, p = __builtin_amdgcn_exp2f(d);
+    const float e = E::up(x[j]), d = plain ? __builtin_fmaf(e, RX_LM_LOG2E, -c) : (e - base) * RX_LM_LOG2E, p = __builtin_amdgcn_exp2f(d);
     a.s += p;
     a.t = __builtin_fmaf(p, __builtin_fmaxf(d, -1e30f), a.t);
   }
@@ -1115,7 +1118,7 @@ RX_DEV void rx_token_logprobs(const typename E::S* logits, const I* targets, flo
     }
     const float own = a.m;
     a = rx_lm_block_sums(a, red);
-    if (!(a.s < rx_lm_inf()) || (a.s == 0.0f && a.m != -rx_lm_inf())) a = rx_lm_careful<E>(row.x, j0, j1, red);
+    if (!(a.s < rx_lm_inf()) || (__builtin_fabsf(a.m) >= 5e7f && a.m != -rx_lm_inf())) a = rx_lm_careful<E>(row.x, j0, j1, red);
     int n = 0;
     if constexpr (K > 0) {
       rx_u32 quad = rx_lm_order(own);

@@ -176,3 +176,37 @@ def test_attention_weights_are_not_rounded_to_the_caches_type(rx, client, length
             wrong = (T.rounded(p, dt).a.astype(np.float64) @ vals[:, h // (hq // hk)]) / p.sum()
             worst = max(worst, (np.abs(wrong - ref[j, h]) / bound[j, h]).max())
     assert worst > 1
+
+
+@pytest.mark.parametrize("n,v,top", [(40, 500, 3), (6, 30001, 20), (600, 4099, 0)])
+def test_logits_of_every_size(rx, client, n, v, top):
+    """Rows whose maximum lies anywhere from -3e38 to 3e38, others far below it or equal to it, whole and split among workgroups."""
+    rng = np.random.default_rng(n)
+    sizes = np.array([-np.inf, -3e38, -1e31, -1e29, -4e10, -1e9 - 64, -1e9, -1e8 - 8, -1e8, -1e8 + 8, -5e7 - 4, -5e7, -5e7 + 4, -50.0, 0.0, 5.0, 1e5, 5e7 - 4, 5e7, 5e7 + 4, 1e8 - 8, 1e8, 1e8 + 8,
+                      1e9, 1e9 + 64, 4e10, 1e29, 2e30, 3e38])
+    x = np.empty((n, v))
+    for t in range(n):
+        high = 1 + t % (len(sizes) - 1)
+        x[t] = sizes[rng.integers(0, high + 1, size=v)] if t % 3 else sizes[rng.integers(max(0, high - 2), high)]
+        x[t, rng.integers(0, v, size=1 + t % 4)] = sizes[high]
+    x = I.Tensor(x.astype(np.float32).astype(np.float64), "f32")
+    y = rng.integers(0, v, n)
+    got = [t.a.astype(np.float64) for t in gpu_run(rx, client, P.token_logprobs(n, v, top=top, dt="f32"), [x, I.Tensor(y, "i32")])[0]]
+    want = L.token_logprobs(x.a, y, top)
+    # (64 bits are not enough for x - lse here: differences from the maximum, less the log of their sum)
+    big = x.a.astype(np.float64)
+    far = big - big.max(1, keepdims=True)
+    below = np.log(np.exp(far).sum(1))
+    logprob = (far - below[:, None])[np.arange(n), y]
+    e = (v / 64 + 64 + 44) * T.UF
+    assert np.all(np.abs(got[1] - (big.max(1) + below)) <= e + 4 * T.UF * (np.abs(below) + 1) + T.UF * np.abs(want[1]))
+
+    def near(a, b):
+        with np.errstate(invalid="ignore", over="ignore"):
+            return (a == b) | (np.abs(a - b) <= e + 8 * T.UF * (np.abs(b) + 20)) | (np.isneginf(a) & (b < -3.4e38))
+    assert near(got[0], logprob).all()
+    p = np.exp(far) / np.exp(far).sum(1, keepdims=True)
+    entropy = below - np.where(p > 0, p * np.maximum(far, -1e300), 0.0).sum(1)
+    assert np.all(np.abs(got[2] - entropy) <= 2 * e * (1 + np.abs(entropy)) + 8 * T.UF * (np.abs(entropy) + 1))
+    if top:
+        assert np.array_equal(got[4], want[4]) and near(got[3], np.take_along_axis(far, want[4], 1) - below[:, None]).all()
