@@ -357,7 +357,9 @@ OperatorPlan plan_attention(const OperatorSpec& s, bool lean) {
   // Workgroups: all on the chip at once (half as many again: 64 sequences of 1 to 8192 positions 56 -> 60 us, one of 131072 630 -> 638),
   // two to a compute unit where the registers allow it; but one where each reads two heads' rows of 256 bytes, whose loads are enough
   // in flight (64 sequences of 1000 positions in bf16 55.7 -> 46.8 us, of 1 to 8192 56.1 -> 52.5; 64 dimensions of f32, 4 query heads a
-  // key head, 56.4 -> 49.0; with rows of 128 bytes 59 -> 68, with one head to a workgroup 45.0 -> 48.5).
+  // key head, 56.4 -> 49.0; with rows of 128 bytes 59 -> 68, with one head to a workgroup 45.0 -> 48.5).  Shorter rows keep two: 64 uneven
+  // sequences and 16 of 16384, 8 key heads in bf16, two and one: 128 bytes 29 and 36, 108 and 133 us; 160: 44 and 51, 137 and 159; 192: 48 and
+  // 53, 155 and 167; 224: 57 and 60, 180 and 185; 256: 56 and 52, 180 and 175; f32 of 160 and 192 bytes 47 and 57, 141 and 186; 49 and 60, 155 and 192.
   const int64_t room = 256 * (HW == 2 && kc.dim * e == 256 ? 1 : waves);
   // every workgroup a stretch of at least four units of 32 positions (a sequence counts four more), all of them on the chip at once
   const int64_t part = 2 * HW * GT * (vc.dim * 4 + 8), most = lean ? std::min<int64_t>(room, kLeanBytes / part) : room;
