@@ -210,3 +210,34 @@ def test_logits_of_every_size(rx, client, n, v, top):
     assert np.all(np.abs(got[2] - entropy) <= 2 * e * (1 + np.abs(entropy)) + 8 * T.UF * (np.abs(entropy) + 1))
     if top:
         assert np.array_equal(got[4], want[4]) and near(got[3], np.take_along_axis(far, want[4], 1) - below[:, None]).all()
+
+
+@pytest.mark.parametrize("pages,cols,seqs,positions,hq", [(0, 4, 2, 64, 8), (10, 0, 2, 64, 8), (10, 4, 0, 64, 8), (10, 4, 2, 0, 8), (10, 4, 2, 64, 0)])
+def test_append_where_there_is_nothing(rx, client, pages, cols, seqs, positions, hq):
+    """No pages, no page table, no sequences, no angles, no query heads: everything is padding but in the last one."""
+    rng = np.random.default_rng(1)
+    q, k, v = (T.rounded(rng.normal(size=(3, h, 64)), "f32") for h in (hq, 2, 2))
+    angle = rng.uniform(-3, 3, size=(positions, 32))
+    table = I.Tensor(rng.permutation(10)[:seqs * cols].reshape(seqs, cols), "i32")
+    caches = [T.rounded(rng.normal(size=(pages, 16, 2, 64)), "f32") for _ in range(2)]
+    args = [q, k, v, I.Tensor(np.cos(angle), "f32"), I.Tensor(np.sin(angle), "f32"), I.Tensor([0, 5, 17], "i32"), I.Tensor([0, 1, 0], "i32"), table] + caches
+    thunk = rx.compile(P.kv_append(3, seqs, hq, 2, 64, pages, 16, cols, positions, dt="f32"))
+    want = L.kv_append(*[t.a for t in args])
+    for donated in (None, [False] * 8 + [True] * 2):
+        out = thunk(*[rx.to_rarray(t.a.T, t.dt) for t in args], donated=donated)
+        for got, ref in zip(out, want):
+            got = got.to_array().T
+            assert got.shape == ref.shape and np.all(np.abs(got - ref) <= 3 * T.UF * 8)
+    res = [rx.Buffer.uninitialized(client, t.shape, "f32") for t in (q, *caches)]
+    thunk.exec.execute_no_alloc([rx.Buffer.from_host(client, t.a, t.dt) for t in args], res)
+    client.default_device().synchronize()
+    for got, ref in zip(res, want):
+        assert np.all(np.abs(got.to_host() - ref) <= 3 * T.UF * 8)
+
+
+@pytest.mark.parametrize("pages,cols", [(0, 4), (10, 0), (0, 0)])
+def test_attention_where_there_is_nothing(rx, client, pages, cols):
+    q = T.rounded(np.random.default_rng(2).normal(size=(3, 8, 64)), "bf16")
+    cache = I.Tensor(np.ones((pages, 16, 2, 64)), "bf16")
+    got, _ = gpu_run(rx, client, P.paged_attention(3, 8, 2, 64, pages, 16, cols, lse=True), [q, cache, cache, I.Tensor(np.zeros((3, cols)), "i32"), I.Tensor([0, 5, 64], "i32")])
+    assert np.all(got[0].a == 0) and np.all(got[1].a == -np.inf)
