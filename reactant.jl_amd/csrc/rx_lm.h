@@ -19,7 +19,7 @@
 //       softmax(scale q k') v of one token per sequence over the positions [max(0, n - window), n) of its sequence (window = 0:
 //       all), n = lengths[b] clamped to [0, M S].  Query head h reads head h div (Hq / Hk).  Positions on pages outside the cache
 //       are left out.  Nothing left: out = 0, lse = -inf.  What lies in slots beyond a sequence is not looked at.  Scores of
-//       positions in use that hold NaN or +inf, or are all -inf, give NaN.
+//       positions in use that hold NaN or +inf give NaN; so do scores that are all -inf, with an lse of -inf.
 //   rx.token_logprobs(logits [.., V], targets [..]) {top} -> (logprob, lse, entropy [, values [.., top], ids [.., top]])
 //       log softmax at the target (0 where it is outside [0, V)), log of the sum of exponentials, entropy, and the `top`
 //       largest log probabilities with their indices, largest first, equal ones by index.  -inf logits have probability 0; a row of
