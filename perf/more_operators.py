@@ -166,11 +166,12 @@ def _inputs(case, seed):
         out = {}
         for name in ("k", "v"):
             codes = torch.empty(shape, device="cuda", dtype=_TORCH[dt])
-            scales = torch.empty(shape[:-1], device="cuda")
+            scales = torch.empty((pages, case["kv_heads"], case["page"]), device="cuda")     # a head's scales of a page lie together
             step = max(1, (1 << 28) // max(1, int(np.prod(shape[1:]))))
             for lo in range(0, pages, step):                 # not all in 32 bits at once
                 x = torch.randn((min(step, pages - lo),) + shape[1:], generator=dev, device="cuda")
-                codes[lo:lo + step], scales[lo:lo + step] = _quantized(x, dt)
+                codes[lo:lo + step], s = _quantized(x, dt)
+                scales[lo:lo + step] = s.transpose(1, 2) if case["layout"] == "slots" else s
             out[name + "_cache"], out[name + "_scale"] = codes, scales
         return {k: out[k] for k in ("k_cache", "v_cache", "k_scale", "v_scale")}
 
@@ -380,7 +381,7 @@ def _plain(case, x):
         for name, new in (("k", _plain_rotate(x["k"], cos, sin, case["rotation"])), ("v", x["v"].float())):
             if case["cache"] in _LARGEST:
                 new, scale = _quantized(new, case["cache"])
-                _put(x[name + "_scale"], page, slot, scale[keep], case["layout"])
+                _put(x[name + "_scale"], page, slot, scale[keep], "heads")
             else:
                 new = new.to(_TORCH[case["cache"]])
             _put(_raw(x[name + "_cache"]), page, slot, _raw(new)[keep], case["layout"])
@@ -392,8 +393,8 @@ def _plain(case, x):
         to, source = (base + torch.arange(case["steps"], device=path.device))[b, i], (base + path)[b, i]
         pages = x["pages"].long()
         to, source = ((pages[b, t // case["page"]], t % case["page"]) for t in (to, source))
-        for cache in map(_raw, caches):
-            _put(cache, *to, cache[source] if case["layout"] == "slots" else cache[source[0], :, source[1]], case["layout"])
+        for cache, layout in zip(map(_raw, caches), [case["layout"]] * 2 + ["heads"] * 2):
+            _put(cache, *to, cache[source] if layout == "slots" else cache[source[0], :, source[1]], layout)
         return caches
     b, n, hq, d = x["q"].shape
     hk, lengths = case["kv_heads"], x["lengths"].long()
@@ -401,10 +402,10 @@ def _plain(case, x):
 
     def gathered(name):
         t = _raw(x[name + "_cache"])[pages].view(x[name + "_cache"].dtype).float()     # [sequence, page, ..]
-        if name + "_scale" in x:
-            t = t * x[name + "_scale"][pages][..., None]
         if case["layout"] == "heads":
             t = t.transpose(2, 3)
+        if name + "_scale" in x:
+            t = t * x[name + "_scale"][pages].transpose(2, 3)[..., None]
         return t.reshape(b, -1, hk, d).permute(0, 2, 1, 3).contiguous()       # [sequence, head, position, dim]
     q = x["q"].float().reshape(b, n, hk, hq // hk, d).transpose(1, 2).reshape(b, hk, -1, d)
     s = torch.matmul(q, gathered("k").transpose(2, 3).contiguous()) / math.sqrt(d)
@@ -510,7 +511,7 @@ def exact(case, seed):
             if case["cache"] in _LARGEST:
                 new, scale = _codes(new, case["cache"])
                 held_scale = x[name + "_scale"].double()
-                (held_scale if case["layout"] == "slots" else held_scale.transpose(1, 2)).index_put_((pages, slots), scale[there])
+                held_scale.transpose(1, 2).index_put_((pages, slots), scale[there])
                 scales.append(held_scale)
             (held if case["layout"] == "slots" else held.transpose(1, 2)).index_put_((pages, slots), new[there])
             caches.append(held)
@@ -521,7 +522,7 @@ def exact(case, seed):
             if key not in x:
                 continue
             cache = x[key].double()
-            rows = cache if case["layout"] == "slots" else cache.transpose(1, 2)
+            rows = cache if case["layout"] == "slots" and key.endswith("cache") else cache.transpose(1, 2)
             held = rows.clone()
             b, i = (x["path"] >= 0).nonzero(as_tuple=True)
             n, pages = x["lengths"].long()[b], x["pages"].long()
@@ -543,7 +544,7 @@ def exact(case, seed):
         for h in range(hk):
             k, v = (((_raw(c)[pages, :, h] if case["layout"] == "slots" else _raw(c)[pages, h]).view(c.dtype)).reshape(-1, d)[:length + n].double() for c in (x["k_cache"], x["v_cache"]))
             if "k_scale" in x:
-                k, v = (t * (s[pages, :, h] if case["layout"] == "slots" else s[pages, h]).reshape(-1, 1)[:length + n].double() for t, s in ((k, x["k_scale"]), (v, x["v_scale"])))
+                k, v = (t * s[pages, h].reshape(-1, 1)[:length + n].double() for t, s in ((k, x["k_scale"]), (v, x["v_scale"])))
             q = x["q"][b, some, h * g:(h + 1) * g].double()                    # [token, head, dim]
             s = (q.reshape(-1, d) @ k.t() / math.sqrt(d)).reshape(q.shape[0], g, -1)
             w = torch.softmax(s.masked_fill(~sees[some][:, None], -math.inf), -1)
