@@ -151,8 +151,140 @@ def token_logprobs_grad(logits, targets, lse, entropy, d_logprob, d_entropy):
     return out.reshape(x.shape)
 
 
-def evaluate(target, arrays, config):
-    """Results of one custom_call on numpy arrays (numbers)."""
+LARGEST = {"f8E4M3FN": 448.0, "i8": 127.0}
+
+
+def quantize(x, dt):
+    """(numbers, scales) of the last dimension's rows: numbers not yet rounded to f8E4M3FN, which writing them down does."""
+    x = np.asarray(x, dtype=np.float64)
+    with np.errstate(invalid="ignore"):
+        top = np.abs(x).max(-1, initial=0.0)
+        scale = np.where(np.isfinite(x).all(-1), np.maximum(top, 2.0 ** -100) / LARGEST[dt], np.nan)
+        y = np.where(np.isnan(scale)[..., None], 0.0, x / scale[..., None])
+    return (np.rint(y) if dt == "i8" else y), scale
+
+
+def rms_norm(x, residual, weight, eps=1e-6, out=None):
+    """[h,] y [, scale]; `out`: the type of 8 bits."""
+    h = np.asarray(x, dtype=np.float64) + (0.0 if residual is None else np.asarray(residual, dtype=np.float64))
+    y = h / np.sqrt((h * h).mean(-1, keepdims=True) + eps) * np.asarray(weight, dtype=np.float64)
+    return ([] if residual is None else [h]) + (list(quantize(y, out)) if out in LARGEST else [y])
+
+
+def rms_norm_grad(h, weight, dy, dh=None, eps=1e-6):
+    h, w, dy = (np.asarray(a, dtype=np.float64) for a in (h, weight, dy))
+    width = h.shape[-1]
+    dx, dw = np.zeros(h.shape), np.zeros(width)
+    for t in np.ndindex(h.shape[:-1]):
+        rms = np.sqrt((h[t] ** 2).sum() / width + eps)
+        u, g = h[t] / rms, dy[t] * w
+        dx[t] = (g - u * (g @ u) / width) / rms
+        dw += dy[t] * u
+    return dx + (0.0 if dh is None else np.asarray(dh, dtype=np.float64)), dw
+
+
+def kv_write(q, k, v, cos, sin, angle, position, sequence, pages, k_cache, v_cache, k_scale=None, v_scale=None, rotation="halves", layout="slots", sections=None, cache=None):
+    """q', caches [, scales]; `cache`: their type where it is of 8 bits."""
+    caches = [np.array(c, dtype=np.float64) for c in (k_cache, v_cache)]
+    scales = [np.array(s, dtype=np.float64) for s in (k_scale, v_scale)] if k_scale is not None else []
+    out, size, half = np.zeros(q.shape), _page_size(caches[0], layout), cos.shape[1]
+    axis = np.repeat(np.arange(len(angle)), [int(n) for n in str(sections).split(",")] if sections is not None else [half])
+    for t in range(q.shape[0]):
+        p, s = int(position[t]), int(sequence[t])
+        rows = np.array([int(angle[a][t]) for a in range(len(angle))])
+        if not (0 <= p < pages.shape[1] * size and 0 <= s < pages.shape[0]):
+            continue
+        c = d = np.zeros(0)
+        if rotation != "none" and half:
+            if rows.min() < 0 or rows.max() >= cos.shape[0]:
+                continue
+            c, d = (m[rows[axis], np.arange(half)] for m in (cos, sin))
+        out[t] = rotate(q[t], c, d, rotation)
+        page = int(pages[s, p // size])
+        if not 0 <= page < caches[0].shape[0]:
+            continue
+        for i, new in enumerate((rotate(k[t], c, d, rotation), np.asarray(v[t], dtype=np.float64))):
+            if scales:
+                new, scales[i][page, :, p % size] = quantize(new, cache)
+            _slot(caches[i], page, p % size, layout)[...] = new
+    return [out] + caches + scales
+
+
+def kv_move(lengths, path, pages, k_cache, v_cache, k_scale=None, v_scale=None, layout="slots"):
+    olds = [np.asarray(c) for c in (k_cache, v_cache, k_scale, v_scale) if c is not None]
+    news = [c.copy() for c in olds]
+    size = _page_size(olds[0], layout)
+    for b in range(len(lengths)):
+        for i in range(path.shape[1]):
+            to, source = int(lengths[b]) + i, int(lengths[b]) + int(path[b, i])
+            if lengths[b] < 0 or path[b, i] < 0 or max(to, source) >= pages.shape[1] * size:
+                continue
+            there, here = int(pages[b, to // size]), int(pages[b, source // size])
+            if 0 <= there < olds[0].shape[0] and 0 <= here < olds[0].shape[0]:
+                for n, (new, old) in enumerate(zip(news, olds)):
+                    how = layout if n < 2 else "heads"
+                    _slot(new, there, to % size, how)[...] = _slot(old, here, source % size, how)
+    return news
+
+
+def tree_attention(q, k_cache, v_cache, pages, lengths, mask=None, k_scale=None, v_scale=None, scale=None, window=0, layout="slots"):
+    """(out, lse, sum of weights times |v|)"""
+    b, n, hq, d = q.shape
+    size = _page_size(k_cache, layout)
+    hk = k_cache.shape[2] if layout == "slots" else k_cache.shape[1]
+    scale = d ** -0.5 if scale is None else scale
+    if mask is None:
+        mask = np.tril(np.ones((n, n), dtype=bool))
+    mask = np.broadcast_to(np.asarray(mask) != 0, (b, n, n))
+    out, lse, mag = np.zeros((b, n, hq, v_cache.shape[3])), np.full((b, n, hq), -np.inf), np.zeros((b, n, hq, v_cache.shape[3]))
+    for s in range(b):
+        if lengths[s] < 0:
+            continue
+        before = min(int(lengths[s]), pages.shape[1] * size)
+        total = min(before + n, pages.shape[1] * size)
+        exists = np.array([0 <= pages[s, j // size] < k_cache.shape[0] for j in range(total)], dtype=bool)
+        where = [(int(pages[s, j // size]), j % size) if exists[j] else None for j in range(total)]
+
+        def gathered(cache, scales):
+            rows = np.zeros((total, hk, cache.shape[3]))
+            for j, w in enumerate(where):
+                if w is not None:
+                    rows[j] = _slot(cache, *w, layout)
+                    if scales is not None:
+                        rows[j] *= scales[w[0], :, w[1]][:, None].astype(np.float64)
+            return rows
+        k, v = gathered(k_cache, k_scale), gathered(v_cache, v_scale)
+        for i in range(n):
+            sees = exists.copy()
+            sees[before:] &= mask[s, i, :total - before]
+            if window:
+                sees[:max(0, before - (window - int(mask[s, i].sum())))] = False
+            if not sees.any():
+                continue
+            for h in range(hq):
+                x = scale * (k[sees, h // (hq // hk)] @ q[s, i, h].astype(np.float64))
+                e = np.exp(x - x.max())
+                w = e / e.sum()
+                out[s, i, h] = w @ v[sees, h // (hq // hk)]
+                mag[s, i, h] = w @ np.abs(v[sees, h // (hq // hk)])
+                lse[s, i, h] = x.max() + np.log(e.sum())
+    return out, lse, mag
+
+
+def evaluate(target, arrays, config, types=None):
+    """Results of one custom_call on numpy arrays (numbers); `types`: element types of the results."""
+    if target == "rx.rms_norm":
+        eight = [t for t in types if t in LARGEST]
+        return rms_norm(arrays[0], arrays[1] if len(arrays) == 3 else None, arrays[-1], out=eight[0] if eight else None, **config)
+    if target == "rx.rms_norm_grad":
+        return list(rms_norm_grad(*arrays, **config))
+    if target == "rx.kv_write":
+        return kv_write(*arrays, cache=types[1], **config)
+    if target == "rx.kv_move":
+        return kv_move(*arrays, **config)
+    if target == "rx.tree_attention":
+        mask = [arrays[5]] if len(arrays) % 2 == 0 else [None]
+        return list(tree_attention(*arrays[:5], *mask, *(arrays[-2:] if len(arrays) >= 7 else []), **config)[:2])
     if target == "rx.embedding":
         return [embedding(*arrays, scale=config.get("scale", 1.0))]
     if target == "rx.kv_append":

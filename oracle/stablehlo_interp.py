@@ -1849,7 +1849,7 @@ class Interpreter:
             if at["target"] == "rx.embedding_grad":
                 outs = [lm_ops.embedding_grad(arrays[0], arrays[1], op.types_out[0].shape[0], at["config"].get("scale", 1.0))]
             else:
-                outs = lm_ops.evaluate(at["target"], arrays, at["config"])
+                outs = lm_ops.evaluate(at["target"], arrays, at["config"], [t.dt for t in op.types_out])
             return [Tensor(_round_to(np.asarray(a), t.dt), t.dt) for a, t in zip(outs, op.types_out)]
         if n == "call":
             return Interpreter(self.funcs, self.hifi, self.excess).run(list(xs), at["callee"])

@@ -37,7 +37,8 @@ def _embed():
     out = os.path.join(CSRC, "rx_embedded.inc")
     parts = ["// generated by build.py from csrc/kernels/*.h -- do not edit\n"]
     for var, fname in (("kRxPreambleSrc", "rx_preamble.h"), ("kRxGemmKernelsSrc", "rx_gemm_kernels.h"),
-                       ("kRxLmKernelsSrc", "rx_lm_kernels.h")):
+                       ("kRxLmKernelsSrc", "rx_lm_kernels.h"), ("kRxLmNormKernelsSrc", "rx_lm_norm_kernels.h"),
+                       ("kRxLmCacheKernelsSrc", "rx_lm_cache_kernels.h")):
         with open(os.path.join(CSRC, "kernels", fname)) as f:
             text = f.read()
         assert ')RXSRC"' not in text
@@ -107,7 +108,7 @@ def build_hostcheck():
     of the program builders).  No device code, no HIP runtime: ROCm's clang++ as a plain host compiler (the sources use
     _Float16, which the image's g++ 11 does not have in C++), sanitizer runtimes linked statically."""
     os.makedirs(OBJ, exist_ok=True)
-    srcs = [os.path.join(CSRC, f) for f in ("rx_hostcheck.cpp", "rx_parse.cpp", "rx_plan.cpp", "rx_emit.cpp", "rx_gemm.cpp", "rx_lm.cpp")]
+    srcs = [os.path.join(CSRC, f) for f in ("rx_hostcheck.cpp", "rx_parse.cpp", "rx_plan.cpp", "rx_emit.cpp", "rx_gemm.cpp", "rx_lm.cpp", "rx_lm_serve.cpp")]
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     if _stale(HOSTCHECK, srcs + headers):
         _run([os.environ.get("CXX", "/opt/rocm/lib/llvm/bin/clang++"), "-std=c++17", "-O1", "-g", "-fno-omit-frame-pointer",

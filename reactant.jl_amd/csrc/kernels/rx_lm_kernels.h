@@ -505,13 +505,14 @@ struct rx_lm_stretch { int b, unit, count; long long first, total; int parts; };
 // parts takes as long over each as n workgroups gain by it, so the longest sequence of u units is to have about sqrt(Q u).  (One of
 // 65536 positions, 8 query heads of one key head of 128: 512 parts 79 us, 91 parts 31, 64 parts 32; of 4000: 31 parts 11.8.)
 RX_DEV long long rx_lm_stretch_start(const long long total, const int parts, const int r) { return total * r / parts; }
-template <int S, int B, int M, int W, int R, int Q, typename I>
-RX_DEV rx_lm_stretch rx_lm_stretch_of(const I* lengths, const int r) {
+// `cost(b)`: what sequence b counts in the row
+template <int B, int R, int Q, typename F>
+RX_DEV rx_lm_stretch rx_lm_stretch_of(F cost, const int r) {
   const int lane = threadIdx.x & 63;
   rx_lm_stretch s = {B, 0, 0, 0, 0, 0};
   int units = 0, longest = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
-    units = b0 + lane < B ? rx_lm_span_of<S, B, M, W>(lengths[b0 + lane]).cost : 0;
+    units = b0 + lane < B ? cost(b0 + lane) : 0;
     s.total += units;
     longest = units > longest ? units : longest;
   }
@@ -528,7 +529,7 @@ RX_DEV rx_lm_stretch rx_lm_stretch_of(const I* lengths, const int r) {
   s.count = (int)(rx_lm_stretch_start(s.total, s.parts, r + 1) - s.first);
   long long sum = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
-    if (B > 64) units = b0 + lane < B ? rx_lm_span_of<S, B, M, W>(lengths[b0 + lane]).cost : 0;
+    if (B > 64) units = b0 + lane < B ? cost(b0 + lane) : 0;
     const long long upto = sum + (B > 1 ? rx_wave_scan((long long)units, rx_op_add()) : (long long)units);
     const unsigned long long past = __ballot(b0 + lane < B && upto > s.first);
     if (past) {
@@ -638,7 +639,7 @@ RX_DEV void rx_paged_attention(const typename E::S* q, const typename E::S* kc, 
   const int head0 = column / TILES * HW, head = head0 + wave / WPH;
   const int h0 = head * G + tile * GT;                 // first query head of this wavefront
   const int heads = G - tile * GT < GT ? G - tile * GT : GT;
-  const rx_lm_stretch st = rx_lm_stretch_of<S, B, M, W, R, Q>(lengths, mine);
+  const rx_lm_stretch st = rx_lm_stretch_of<B, R, Q>([&](const int at) { return rx_lm_span_of<S, B, M, W>(lengths[at]).cost; }, mine);
 
   int b = st.b, unit = st.unit;
   for (int left = st.count; left > 0; ++b, unit = 0) {

@@ -1,130 +1,17 @@
 // Checks and launches of the language-model operators (rx_lm.h).
-#include "rx_lm.h"
-
-#include <algorithm>
-#include <cmath>
-#include <cstdio>
-#include <cstdlib>
-#include <set>
-#include <sstream>
+#include "rx_lm_plan.h"
 
 namespace rx {
+using namespace lm;
 namespace {
 
-struct OpName { const char* name; int in, out_min, out_max; };
+struct OpName { const char* name; int in_min, in_max, out_min, out_max; };
 const OpName kOperators[] = {
-    {"rx.embedding", 2, 1, 1},       {"rx.embedding_grad", 2, 1, 1},  {"rx.kv_append", 10, 3, 3},
-    {"rx.paged_attention", 5, 1, 2}, {"rx.token_logprobs", 2, 3, 5}, {"rx.token_logprobs_grad", 6, 1, 1},
+    {"rx.embedding", 2, 2, 1, 1},       {"rx.embedding_grad", 2, 2, 1, 1},  {"rx.kv_append", 10, 10, 3, 3},
+    {"rx.paged_attention", 5, 5, 1, 2}, {"rx.token_logprobs", 2, 2, 3, 5}, {"rx.token_logprobs_grad", 6, 6, 1, 1},
+    {"rx.rms_norm", 2, 3, 1, 3},        {"rx.rms_norm_grad", 3, 4, 2, 2},   {"rx.kv_write", 11, 13, 3, 5},
+    {"rx.kv_move", 5, 7, 2, 4},         {"rx.tree_attention", 5, 8, 1, 2},
 };
-
-constexpr int kMaxHeadDim = 256;
-constexpr int64_t kMaxTop = 64;
-constexpr int64_t kMaxGrid = (int64_t)1 << 22;   // workgroups; kernels with more items than that go on with the next ones
-constexpr int64_t kLeanBytes = (int64_t)1 << 20;  // of partial results in a lean plan: a quarter of what calls without allocations have for all temporaries
-constexpr int64_t kMaxRow = (int64_t)1 << 30;   // elements of a row or rows of a table: 32-bit indices inside a row
-
-struct Checker {
-  const OperatorSpec& s;
-  [[noreturn]] void fail(const std::string& m) const { throw Error(s.name + ": " + m); }
-  void require(bool ok, const std::string& m) const { if (!ok) fail(m); }
-  void rank(const TType& t, int r, const char* what) const {
-    require(t.rank() == r, std::string(what) + " must have " + std::to_string(r) + " dimensions, got " + t.str());
-  }
-  void floats(const TType& t, const char* what) const {
-    require(t.dt == DT::F32 || t.dt == DT::BF16 || t.dt == DT::F16, std::string(what) + " must be f32, bf16 or f16, got " + t.str());
-  }
-  void f32(const TType& t, const char* what) const { require(t.dt == DT::F32, std::string(what) + " must be f32, got " + t.str()); }
-  void ints(const TType& t, const char* what) const {
-    require(t.dt == DT::I32 || t.dt == DT::I64, std::string(what) + " must be i32 or i64, got " + t.str());
-  }
-  void same(const TType& a, const TType& b, const char* what) const { require(a == b, std::string(what) + ": " + a.str() + " and " + b.str() + " differ"); }
-  void dims(const TType& t, const std::vector<int64_t>& d, const char* what) const {
-    TType w = t;
-    w.dims = d;
-    require(t.dims == d, std::string(what) + " must be " + w.str() + ", got " + t.str());
-  }
-  void settings(const std::set<std::string>& known) const {
-    for (auto& kv : s.attrs) require(known.count(kv.first) != 0, "unknown setting '" + kv.first + "'");
-  }
-  double number(const char* key, double otherwise) const {
-    auto it = s.attrs.find(key);
-    if (it == s.attrs.end()) return otherwise;
-    char* end = nullptr;
-    const double v = std::strtod(it->second.c_str(), &end);
-    require(end && *end == 0 && end != it->second.c_str() && std::isfinite(v), std::string("setting '") + key + "' must be a finite number, got '" + it->second + "'");
-    return v;
-  }
-  // a factor that the kernels hold in f32, `times` another
-  void scale(double times = 1.0) const {
-    const double v = number("scale", 1.0);
-    require(std::fabs(v * times) <= 3.4028234e38, "setting 'scale' must be a number that f32 holds" + std::string(times > 1 ? " times log2 e" : "") + ", got '" +
-                                                     (s.attrs.count("scale") ? s.attrs.at("scale") : std::string()) + "'");
-  }
-  int64_t integer(const char* key, int64_t otherwise) const {
-    const double v = number(key, (double)otherwise);
-    require(v == std::floor(v) && std::fabs(v) < 1e15, std::string("setting '") + key + "' must be a whole number");
-    return (int64_t)v;
-  }
-  std::string word(const char* key, const std::string& otherwise, const std::set<std::string>& known) const {
-    auto it = s.attrs.find(key);
-    const std::string v = it == s.attrs.end() ? otherwise : it->second;
-    std::string all;
-    for (auto& k : known) all += (all.empty() ? "'" : ", '") + k + "'";
-    require(known.count(v) != 0, std::string("setting '") + key + "' must be one of " + all + ", got '" + v + "'");
-    return v;
-  }
-};
-
-struct Cache {   // [pages, slots of a page, heads, dim] or [pages, heads, slots, dim]
-  int64_t pages, slots, heads, dim;
-  bool by_slot;
-  Cache(const TType& t, bool slots_first) : pages(t.dims[0]), slots(t.dims[slots_first ? 1 : 2]), heads(t.dims[slots_first ? 2 : 1]), dim(t.dims[3]), by_slot(slots_first) {}
-};
-
-std::vector<int64_t> without_last(const TType& t) { return std::vector<int64_t>(t.dims.begin(), t.dims.end() - 1); }
-int64_t product(const std::vector<int64_t>& d) {
-  int64_t n = 1;
-  for (int64_t x : d) n *= x;
-  return n;
-}
-
-const char* elem(DT t) { return t == DT::F32 ? "rx_lm_f32" : t == DT::BF16 ? "rx_lm_bf16" : "rx_lm_f16"; }
-std::string num(int64_t v) { return std::to_string(v); }
-std::string flt(double v) {
-  char b[40];
-  snprintf(b, sizeof b, "%.9g", v);
-  std::string s = b;
-  if (s.find_first_of(".en") == std::string::npos) s += ".0";
-  return s + "f";
-}
-
-// `body` is the call of a device function on a0, a1, ..: the kernel's parameters, of which the last `outs` are written.
-// `waves`: wavefronts per SIMD that the registers have to allow (0: the compiler's choice)
-OperatorKernel kernel(const OperatorSpec& s, const std::string& suffix, unsigned block, const std::vector<std::pair<OperatorArg, std::string>>& args, int outs,
-                      const std::string& body, int waves = 0) {
-  OperatorKernel k;
-  k.suffix = suffix;
-  k.kind = "lm_" + suffix;
-  k.block = block;
-  k.n_outputs = outs;
-  std::ostringstream o;
-  o << "// " << s.name;
-  for (auto& t : s.in) o << " " << t.str();
-  o << "\nextern \"C\" __global__ __launch_bounds__(" << block << (waves ? ", " + num(waves) : std::string()) << ") void @K@_" << suffix << "(";
-  for (size_t a = 0; a < args.size(); ++a) {
-    const bool in = a + (size_t)outs < args.size();
-    o << (a ? ", " : "") << (in ? "const " : "") << args[a].second << "* __restrict__ a" << a;
-    k.args.push_back(args[a].first);
-  }
-  o << ") {\n  " << body << "\n}\n\n";
-  k.text = o.str();
-  return k;
-}
-OperatorArg operand(int i) { return {OperatorArg::Operand, i}; }
-OperatorArg result(int i) { return {OperatorArg::Result, i}; }
-OperatorArg scratch(int i) { return {OperatorArg::Scratch, i}; }
-OperatorArg counters() { return {OperatorArg::Counters, 0}; }
-std::string st(const TType& t) { return info(t.dt).stype; }
 
 // ------------------------------------------------------------------ embedding
 void check_embedding(const Checker& c) {
@@ -485,7 +372,8 @@ void check_operator(const OperatorSpec& s) {
   const Checker c{s};
   for (auto& o : kOperators) {
     if (s.name != o.name) continue;
-    c.require((int)s.in.size() == o.in, "expected " + num(o.in) + " operands, got " + num((int64_t)s.in.size()));
+    c.require((int)s.in.size() >= o.in_min && (int)s.in.size() <= o.in_max,
+              "expected " + num(o.in_min) + (o.in_max > o.in_min ? " to " + num(o.in_max) : std::string()) + " operands, got " + num((int64_t)s.in.size()));
     c.require((int)s.out.size() >= o.out_min && (int)s.out.size() <= o.out_max, "wrong number of results: " + num((int64_t)s.out.size()));
   }
   for (auto& t : s.in) for (int64_t d : t.dims) c.require(d >= 0, "negative dimension");
@@ -495,6 +383,11 @@ void check_operator(const OperatorSpec& s) {
   else if (s.name == "rx.paged_attention") check_attention(c);
   else if (s.name == "rx.token_logprobs") check_logprobs(c);
   else if (s.name == "rx.token_logprobs_grad") check_logprobs_grad(c);
+  else if (s.name == "rx.rms_norm") check_norm(c);
+  else if (s.name == "rx.rms_norm_grad") check_norm_grad(c);
+  else if (s.name == "rx.kv_write") check_write(c);
+  else if (s.name == "rx.kv_move") check_move(c);
+  else if (s.name == "rx.tree_attention") check_tree(c);
   else c.fail("unknown operator");
 }
 
@@ -504,6 +397,11 @@ OperatorPlan plan_operator(const OperatorSpec& s, bool lean) {
                    : s.name == "rx.kv_append"       ? plan_append(s)
                    : s.name == "rx.paged_attention" ? plan_attention(s, lean)
                    : s.name == "rx.token_logprobs"  ? plan_logprobs(s)
+                   : s.name == "rx.rms_norm"        ? plan_norm(s)
+                   : s.name == "rx.rms_norm_grad"   ? plan_norm_grad(s, lean)
+                   : s.name == "rx.kv_write"        ? plan_write(s)
+                   : s.name == "rx.kv_move"         ? plan_move(s)
+                   : s.name == "rx.tree_attention"  ? plan_tree(s, lean)
                                                     : plan_logprobs_grad(s);
   // without workgroups there is nothing to compile
   p.kernels.erase(std::remove_if(p.kernels.begin(), p.kernels.end(), [](const OperatorKernel& k) { return !k.grid[0] || !k.grid[1] || !k.grid[2]; }), p.kernels.end());
@@ -524,6 +422,7 @@ double operator_flops(const OperatorSpec& s, double* transcendentals) {
     *transcendentals = n;
     return 2.0 * n * (double)(kc.dim + s.in[2].dims[3]);
   }
+  if (s.name != "rx.token_logprobs" && s.name != "rx.token_logprobs_grad") return serve_flops(s, transcendentals);
   const double n = (double)s.in[0].numel();
   *transcendentals = n;
   return (s.name == "rx.token_logprobs" ? 5.0 : 6.0) * n;

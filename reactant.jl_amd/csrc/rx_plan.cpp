@@ -137,7 +137,7 @@ struct Planner {
   std::map<int, int> reduce_of;     // elementwise root on a full reduction's scalar -> the reduction, whose kernel computes it
   std::ostringstream src;
   int kcount = 0;
-  bool uses_operators = false;      // the text calls device functions of rx_lm_kernels.h
+  std::set<std::string> operator_headers;   // whose device functions the text calls
 
   Planner(const Graph& gin, const PlanOptions& o) : g(gin), opt(o) {}
 
@@ -4134,7 +4134,7 @@ struct Planner {
     for (int r : results) spec.out.push_back(g.nodes[r].ty);
     const OperatorPlan op = plan_operator(spec, opt.lean_operators);
     plan.lean_operators = plan.lean_operators || (!opt.lean_operators && !op.scratch.empty());
-    uses_operators = true;
+    if (!op.kernels.empty()) operator_headers.insert(op.header);
     for (size_t r = 0; r < results.size(); ++r) {
       const int from = r < op.updates.size() ? op.updates[r] : -1;
       if (from < 0) continue;
@@ -6306,7 +6306,9 @@ struct Planner {
         B.last_use = (int)li;
       }
     }
-    plan.source = std::string("#include \"rx_preamble.h\"\n#include \"rx_gemm_kernels.h\"\n") + (uses_operators ? "#include \"rx_lm_kernels.h\"\n" : "") + "\n" + src.str();
+    plan.source = "#include \"rx_preamble.h\"\n#include \"rx_gemm_kernels.h\"\n";
+    for (auto& h : operator_headers) plan.source += "#include \"" + h + "\"\n";
+    plan.source += "\n" + src.str();
   }
 };
 

@@ -8,6 +8,9 @@ stated in csrc/rx_lm.h.  Arguments come in the order of the operands.  Cache arg
 take them over: a call with them donated updates the caches in place, one without copies them first."""
 
 
+EIGHT_BITS = ("f8E4M3FN", "i8")     # types of numbers that stand for their product with a scale
+
+
 def tt(shape, dt):
     return "tensor<" + "".join("%dx" % d for d in shape) + dt + ">"
 
@@ -101,6 +104,63 @@ def token_logprobs_grad(tokens, vocab, dt="bf16", ids="i32"):
     return _module("token_logprobs_grad", "rx.token_logprobs_grad", [logits, tt([tokens], ids), one, one, one, one], [logits])
 
 
+def rms_norm(rows, width, dt="bf16", out=None, eps=1e-6, residual=True):
+    """(x [rows, width] [, residual], weight [width]) -> ([h = x + residual,] norm of h times weight in type `out`).  `out` of 8 bits
+    (f8E4M3FN or i8) gives the rows' scales [rows] as one more result."""
+    x, out = tt([rows, width], dt), out or dt
+    res = ([x] if residual else []) + [tt([rows, width], out)] + ([tt([rows], "f32")] if out in EIGHT_BITS else [])
+    return _module("rms_norm", "rx.rms_norm", [x, x, tt([width], dt)] if residual else [x, tt([width], dt)], res, {"eps": float(eps)})
+
+
+def rms_norm_grad(rows, width, dt="bf16", out="f32", eps=1e-6, residual=True):
+    """(h [rows, width], weight [width], dy [, dh]) -> (gradient by h, gradient by weight in type `out`, f32 or dt)."""
+    x, w = tt([rows, width], dt), tt([width], dt)
+    return _module("rms_norm_grad", "rx.rms_norm_grad", [x, w, x, x] if residual else [x, w, x], [x, tt([width], out)], {"eps": float(eps)})
+
+
+def _caches(num_pages, page_size, kv_heads, head_dim, value_dim, layout, cache):
+    """Types of the caches, and of their scales where they hold 8 bits."""
+    scale = tt([num_pages, kv_heads, page_size], "f32")
+    return [tt(cache_shape(num_pages, page_size, kv_heads, d, layout), cache) for d in (head_dim, value_dim)] + ([scale, scale] if cache in EIGHT_BITS else [])
+
+
+def kv_write(tokens, sequences, q_heads, kv_heads, head_dim, num_pages, page_size, table_pages, positions, dt="bf16", cache=None, sections=None, rotary_dim=None,
+             rotation="halves", layout="slots", ids="i32", value_dim=None):
+    """(q, k, v, cos, sin, angle [axes, tokens], position, sequence, page table, k_cache, v_cache [, k_scale, v_scale]) -> (rotated q, the
+    caches and their scales).  `sections`: rotated pairs that follow each axis' angles (one axis if not given); `cache`: the caches' type,
+    dt or of 8 bits, which have scales.  Donate the caches to update them in place."""
+    rotary_dim = (2 * sum(sections) if sections else head_dim) if rotary_dim is None else rotary_dim
+    value_dim, axes = value_dim or head_dim, len(sections) if sections else 1
+    stored = _caches(num_pages, page_size, kv_heads, head_dim, value_dim, layout, cache or dt)
+    q, angles, index = tt([tokens, q_heads, head_dim], dt), tt([positions, rotary_dim // 2], "f32"), tt([tokens], ids)
+    args = [q, tt([tokens, kv_heads, head_dim], dt), tt([tokens, kv_heads, value_dim], dt), angles, angles, tt([axes, tokens], ids), index, index,
+            tt([sequences, table_pages], ids)] + stored
+    return _module("kv_write", "rx.kv_write", args, [q] + stored,
+                   {"rotation": rotation, "layout": layout, "sections": ",".join(map(str, sections)) if sections else None}, {9 + i: 1 + i for i in range(len(stored))})
+
+
+def kv_move(sequences, steps, kv_heads, head_dim, num_pages, page_size, table_pages, cache="bf16", layout="slots", ids="i32", value_dim=None):
+    """(lengths [sequences], path [sequences, steps], page table, k_cache, v_cache [, k_scale, v_scale]) -> the caches, where position
+    lengths + i holds what position lengths + path[i] held.  Donate the caches to update them in place."""
+    stored = _caches(num_pages, page_size, kv_heads, head_dim, value_dim or head_dim, layout, cache)
+    return _module("kv_move", "rx.kv_move", [tt([sequences], ids), tt([sequences, steps], ids), tt([sequences, table_pages], ids)] + stored, stored, {"layout": layout},
+                   {3 + i: i for i in range(len(stored))})
+
+
+def tree_attention(sequences, drafted, q_heads, kv_heads, head_dim, num_pages, page_size, table_pages, dt="bf16", cache=None, mask=True, scale=None, window=0, layout="slots",
+                   ids="i32", value_dim=None, lse=False):
+    """(q [sequences, drafted, q_heads, head_dim], k_cache, v_cache, page table, lengths [, mask] [, k_scale, v_scale]) -> attention of the
+    drafted tokens, which lie behind the first `lengths` positions of the cache.  `mask`: True for one [drafted, drafted] per sequence,
+    "shared" for one of all, False for none: a token then sees itself and those before it."""
+    value_dim = value_dim or head_dim
+    stored = _caches(num_pages, page_size, kv_heads, head_dim, value_dim, layout, cache or dt)
+    q = [sequences, drafted, q_heads]
+    args = [tt(q + [head_dim], dt), stored[0], stored[1], tt([sequences, table_pages], ids), tt([sequences], ids)]
+    args += [tt(([] if mask == "shared" else [sequences]) + [drafted, drafted], "i1")] if mask else []
+    return _module("tree_attention", "rx.tree_attention", args + stored[2:], [tt(q + [value_dim], dt)] + ([tt(q, "f32")] if lse else []),
+                   {"scale": None if scale is None else float(scale), "window": window, "layout": layout})
+
+
 # ----------------------------------------------------------------------------
 # the operators together
 # ----------------------------------------------------------------------------
@@ -126,6 +186,13 @@ class _Text:
     def binary(self, op, a, b):
         return self.op("%s %s, %s : (%s, %s)" % (op, a, b, self.types[a], self.types[b]), *self.shapes[a])
 
+    def select(self, where, a, b):
+        self.n += 1
+        name = "%%v%d" % self.n
+        self.types[name], self.shapes[name] = self.types[a], self.shapes[a]
+        self.lines.append("    %s = stablehlo.select %s, %s, %s : %s, %s\n" % (name, where, a, b, self.types[where], self.types[a]))
+        return name
+
     def constant(self, literal, shape, dt):
         self.n += 1
         name = "%%c%d" % self.n
@@ -133,11 +200,13 @@ class _Text:
         self.lines.append("    %s = stablehlo.constant dense<%s> : %s\n" % (name, literal, tt(shape, dt)))
         return name
 
-    def iota(self, n):
+    def iota(self, n, dim=0):
+        """0, 1, .. along a dimension of `n` (a size, or several)."""
+        shape = list(n) if isinstance(n, (list, tuple)) else [n]
         self.n += 1
         name = "%%v%d" % self.n
-        self.types[name], self.shapes[name] = tt([n], "i32"), ([n], "i32")
-        self.lines.append("    %s = stablehlo.iota dim = 0 : %s\n" % (name, tt([n], "i32")))
+        self.types[name], self.shapes[name] = tt(shape, "i32"), (shape, "i32")
+        self.lines.append("    %s = stablehlo.iota dim = %d : %s\n" % (name, dim, tt(shape, "i32")))
         return name
 
     def convert(self, x, dt):
@@ -229,6 +298,80 @@ def decode_step(sequences, vocab, width, q_heads, kv_heads, head_dim, hidden, nu
     one = ([b], "f32")
     out = x.operator("rx.token_logprobs", [logits, targets], [one, one, one, ([b, top], "f32"), ([b, top], "i32")], {"top": top})
     return x.module("decode_step", out + caches), [x.shapes["%%arg%d" % k] for k in range(len(x.args))], list(range(first_cache, first_cache + 2 * layers))
+
+
+def verify_step(sequences, drafted, vocab, width, q_heads, kv_heads, head_dim, hidden, num_pages, page_size, table_pages, positions, layers=1, axes=1, top=5, dt="bf16",
+                cache="f8E4M3FN", products="f8E4M3FN", layout="slots", rotation="halves"):
+    """A tree of drafted tokens of every sequence through a transformer with paged caches: embedding, then per layer norm, keys and
+    values written behind the sequence's positions (`cache`: their type), attention that the tree masks, sum with the residual and norm,
+    a gated MLP, and the log probabilities of every token's successor.  The norms give 8 bits for the products that follow them
+    (`products`: their type, that of the weights [outputs, inputs] there, whose factors are numbers; or dt).  With one drafted token
+    this is a decoding step.  Returns (text, [(shape, element type)] of the arguments, results that are caches).  Arguments are tokens
+    [sequences, drafted], targets (the successor that is asked about), angle [axes, sequences, drafted] (rows of the tables of angles),
+    lengths (-1: takes no part), mask, page table, cos, sin, embedding table, per layer (norm, wq, wk, wv, wo, norm, gate, up, down,
+    then the factors of wq, wk, wv, gate and up where the products have 8 bits, k_cache, v_cache and their scales), norm and head;
+    results are (logprob, lse, entropy, top log probabilities, top indices) and the caches, which the cache arguments may be donated
+    to.  `rx.kv_move` brings together what the accepted branch has written."""
+    b, n, x = sequences, drafted, _Text()
+    t, eight, stored = b * n, products in EIGHT_BITS, cache in EIGHT_BITS
+    tokens, targets = (x.arg([b, n], "i32") for _ in range(2))
+    angle, lengths, mask, pages = x.arg([axes, b, n], "i32"), x.arg([b], "i32"), x.arg([b, n, n], "i1"), x.arg([b, table_pages], "i32")
+    cos, sin = (x.arg([positions, head_dim // 2], "f32") for _ in range(2))
+    table = x.arg([vocab, width], dt)
+    first_cache, held = 5, 4 if stored else 2
+    weights = []
+    for l in range(layers):
+        w = {"norm1": x.arg([width], dt)}
+        for key, heads in (("q", q_heads), ("k", kv_heads), ("v", kv_heads)):
+            w[key] = x.arg([heads * head_dim, width], products)
+        w["o"], w["norm2"] = x.arg([width, q_heads * head_dim], dt), x.arg([width], dt)
+        w["gate"], w["up"], w["down"] = x.arg([hidden, width], products), x.arg([hidden, width], products), x.arg([width, hidden], dt)
+        if eight:
+            w["factor"] = {key: x.arg([], "f32") for key in ("q", "k", "v", "gate", "up")}
+        shapes = [(cache_shape(num_pages, page_size, kv_heads, head_dim, layout), cache)] * 2 + [([num_pages, kv_heads, page_size], "f32")] * (held - 2)
+        w["caches"] = [x.arg(*s, first_cache + held * l + k) for k, s in enumerate(shapes)]
+        weights.append(w)
+    norm, head = x.arg([width], dt), x.arg([vocab, width], dt)
+    sequence = x.reshape(x.iota([b, n]), [t])
+    base = x.spread(lengths, [0], [b, n])
+    there = x.op("compare GE, %s, %s, SIGNED : (%s, %s)" % (base, x.constant("0", [b, n], "i32"), x.types[base], x.types[base]), [b, n], "i1")
+    position = x.binary("add", base, x.iota([b, n], 1))
+    position = x.select(there, position, x.constant("-1", [b, n], "i32"))
+    position, angle = x.reshape(position, [t]), x.reshape(angle, [axes, t])
+    half = head_dim // 2
+    sections = [half - (axes - 1) * (half // axes)] + [half // axes] * (axes - 1)
+
+    def normed(v, residual, weight, out):
+        """([h,] norm, scale) of v [+ residual]."""
+        rows = [([t, width], dt)] if residual else []
+        res = rows + [([t, width], out)] + ([([t], "f32")] if out in EIGHT_BITS else [])
+        got = x.operator("rx.rms_norm", [v] + ([residual] if residual else []) + [weight], res, {"eps": 1e-6})
+        return (got[0] if residual else v,) + tuple(got[1 if residual else 0:]) + (() if out in EIGHT_BITS else (None,))
+
+    def product(y, scale, w, factor, outputs):
+        if not eight:
+            return x.dot(y, w, (1, 1))
+        f = x.binary("multiply", x.dot(y, w, (1, 1), "f32"), x.spread(scale, [0], [t, outputs]))
+        return x.convert(x.binary("multiply", f, x.spread(factor, [], [t, outputs])), dt)
+
+    h, late, caches = x.reshape(x.operator("rx.embedding", [table, tokens], [([b, n, width], dt)], {"scale": 1.0})[0], [t, width]), None, []
+    for w in weights:
+        factor = w.get("factor", {})
+        h, y, scale = normed(late or h, h if late else None, w["norm1"], products)
+        q, k, v = (x.reshape(product(y, scale, w[key], factor.get(key), heads * head_dim), [t, heads, head_dim]) for key, heads in (("q", q_heads), ("k", kv_heads), ("v", kv_heads)))
+        q, *now = x.operator("rx.kv_write", [q, k, v, cos, sin, angle, position, sequence, pages] + w["caches"],
+                             [([t, q_heads, head_dim], dt)] + [x.shapes[c] for c in w["caches"]], {"rotation": rotation, "layout": layout, "sections": ",".join(map(str, sections))})
+        caches += now
+        a = x.operator("rx.tree_attention", [x.reshape(q, [b, n, q_heads, head_dim]), now[0], now[1], pages, lengths, mask] + now[2:], [([b, n, q_heads, head_dim], dt)], {"layout": layout})[0]
+        h, y, scale = normed(x.dot(x.reshape(a, [t, q_heads * head_dim]), w["o"], (1, 1)), h, w["norm2"], products)
+        gate, up = (product(y, scale, w[key], factor.get(key), hidden) for key in ("gate", "up"))
+        act = x.binary("multiply", gate, x.op("logistic %s : (%s)" % (gate, x.types[gate]), [t, hidden], dt))
+        late = x.dot(x.binary("multiply", act, up), w["down"], (1, 1))
+    y = normed(late, h, norm, dt)[1]
+    logits = x.dot(y, head, (1, 1))
+    one = ([t], "f32")
+    out = x.operator("rx.token_logprobs", [logits, x.reshape(targets, [t])], [one, one, one, ([t, top], "f32"), ([t, top], "i32")], {"top": top})
+    return x.module("verify_step", out + caches), [x.shapes["%%arg%d" % k] for k in range(len(x.args))], list(range(first_cache, first_cache + held * layers))
 
 
 def tied_head_step(tokens, vocab, width, dt="f32", entropy_weight=0.0):
