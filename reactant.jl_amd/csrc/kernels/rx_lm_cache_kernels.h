@@ -7,9 +7,19 @@ template <bool B, typename X, typename Y> struct rx_lm_if { typedef X type; };
 template <typename X, typename Y> struct rx_lm_if<false, X, Y> { typedef Y type; };
 constexpr int rx_lm_pow2(const int n) { return n <= 1 ? 1 : 2 * rx_lm_pow2((n + 1) / 2); }
 
+// the row of the angles that pair a is turned by: of the axis whose section holds it
+template <int A, int S0, int S1, int S2, typename I>
+RX_DEV I rx_lm_axis_row(const int a, const I r0, const I r1, const I r2, const I r3) {
+  I r = r0;
+  if constexpr (A > 1) r = a < S0 ? r : r1;
+  if constexpr (A > 2) r = a < S1 ? r : r2;
+  if constexpr (A > 3) r = a < S2 ? r : r3;
+  return r;
+}
 // A token's heads, EACH of them after one another, to a group of LANES lanes, NE elements of 16 bytes to a lane: what a head's
 // largest magnitude is found over, and what the cosines and sines of its dimensions are loaded for once.  Every lane loads the
-// pairs' other elements itself.
+// pairs' other elements itself.  8191 tokens of 32 and 8 heads of 128 in bf16 into 8 bits, 189 MB, take 38.6 us, 4.9 TB/s: the index
+// arithmetic and the divisions take about half of the vector units' time.  48 tokens take 3.4 us, a launch and four dependent loads.
 template <typename E, typename C, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int L, int R2, int A, int S0, int S1, int S2, bool PAIRS, bool BY_SLOT, int T,
           bool WHOLE, int EACH, typename I>
 RX_DEV void rx_kv_write(const typename E::S* q, const typename E::S* k, const typename E::S* v, const float* cos, const float* sin, const I* angle, const I* position,
@@ -20,39 +30,78 @@ RX_DEV void rx_kv_write(const typename E::S* q, const typename E::S* k, const ty
   constexpr bool BITS8 = rx_lm_is8<C>::value;
   typedef rx_vec<X, NE> W;
   const int lane = threadIdx.x % LANES, d = lane * NE;
-  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES; i < (long long)T * ALL; i += (long long)gridDim.x * (256 / LANES)) {
-    const long long t = i / ALL;
+  // (32 bits where they count all groups: a division of 64 is a dozen operations more)
+  typedef typename rx_lm_if<((long long)T * ALL < (1ll << 30)), rx_u32, rx_u64>::type Z;
+  for (Z i = (Z)(((rx_u64)blockIdx.x * 256 + threadIdx.x) / LANES); i < (Z)T * ALL; i += (Z)gridDim.x * (256 / LANES)) {
+    const long long t = (long long)(i / ALL);
     const int u = (int)(i % ALL), kind = u < GQ ? 0 : u < GQ + GK ? 1 : 2, first = (u - (kind == 0 ? 0 : kind == 1 ? GQ : GQ + GK)) * EACH;
     const I pos = position[t], seq = sequence[t];
     bool known = pos >= 0 && pos < (I)(M * S) && seq >= 0 && seq < B;
-    I row[A] = {};
+    I row0 = 0, row1 = 0, row2 = 0, row3 = 0;
     if constexpr (R2 > 0) {
-#pragma unroll
-      for (int a = 0; a < A; ++a) {
-        row[a] = angle[(long long)a * T + t];
-        known = known && row[a] >= 0 && row[a] < L;
-      }
+      row0 = angle[t];
+      if constexpr (A > 1) row1 = angle[(long long)T + t];
+      if constexpr (A > 2) row2 = angle[2ll * T + t];
+      if constexpr (A > 3) row3 = angle[3ll * T + t];
+      auto inside = [&](const I r) { return r >= 0 && r < L; };
+      known = known && inside(row0) && (A < 2 || inside(row1)) && (A < 3 || inside(row2)) && (A < 4 || inside(row3));
     }
     int page = -1, slot = 0;
     if (known) {
-      const I p = pages[(long long)seq * M + (int)pos / S];
+      const I p = pages[(long long)seq * M + (rx_u32)pos / S];
       page = p >= 0 && p < P ? (int)p : -1;
-      slot = (int)pos % S;
+      slot = (int)((rx_u32)pos % S);
     }
     const int D = kind == 2 ? DV : DK, heads = kind == 0 ? HQ : HK;
     const X* in = (kind == 0 ? q : kind == 1 ? k : v) + t * heads * D;
     float c[NE], s[NE];
     const bool turns = R2 > 0 && L > 0 && known && kind < 2;
+    auto axis_row = [row0, row1, row2, row3](const int a) { return rx_lm_axis_row<A, S0, S1, S2>(a, row0, row1, row2, row3); };
+    // Sections of at least a lane's pairs: they lie in at most two of them, and come from the rows of the first and the last (8191 tokens of three axes
+    // 43.8 -> 38.6 us, together with 32-bit indices).
+    constexpr int NP = PAIRS ? NE / 2 : NE;
+    constexpr bool TWO = WHOLE && R2 % 4 == 0 && NP % 4 == 0 && (A < 2 || (S0 >= NP && (A < 3 ? R2 - S0 : S1 - S0) >= NP)) && (A < 3 || (A < 4 ? R2 - S1 : S2 - S1) >= NP) && (A < 4 || R2 - S2 >= NP);
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
       c[e] = 1.0f;
       s[e] = 0.0f;
-      if (turns && d + e < 2 * R2) {
-        const int a = PAIRS ? (d + e) >> 1 : d + e < R2 ? d + e : d + e - R2;
-        const I r = A == 1 || a < S0 ? row[0] : A == 2 || a < S1 ? row[A > 1 ? 1 : 0] : A == 3 || a < S2 ? row[A > 2 ? 2 : 0] : row[A > 3 ? 3 : 0];
-        c[e] = cos[(long long)r * R2 + a];
-        s[e] = sin[(long long)r * R2 + a];
+    }
+    if constexpr (TWO) {
+      if (turns && d < 2 * R2) {
+        typedef rx_vec<float, 4> Q;
+        const int a0 = PAIRS ? d >> 1 : d < R2 ? d : d - R2;
+        const I r0 = axis_row(a0), r1 = axis_row(a0 + NP - 1);
+        Q v[2][2][NP / 4];
+#pragma unroll
+        for (int k = 0; k < NP / 4; ++k) {
+          v[0][0][k] = rx_load<Q>(cos + (long long)r0 * R2 + a0 + 4 * k);
+          v[0][1][k] = rx_load<Q>(sin + (long long)r0 * R2 + a0 + 4 * k);
+          if constexpr (A > 1) {
+            v[1][0][k] = rx_load<Q>(cos + (long long)r1 * R2 + a0 + 4 * k);
+            v[1][1][k] = rx_load<Q>(sin + (long long)r1 * R2 + a0 + 4 * k);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          const int p = PAIRS ? e / 2 : e;
+          c[e] = v[0][0][p / 4].v[p % 4];
+          s[e] = v[0][1][p / 4].v[p % 4];
+          if constexpr (A > 1) {
+            const bool last = axis_row(a0 + p) != r0;
+            c[e] = last ? v[1][0][p / 4].v[p % 4] : c[e];
+            s[e] = last ? v[1][1][p / 4].v[p % 4] : s[e];
+          }
+        }
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < NE; ++e)
+        if (turns && d + e < 2 * R2) {
+          const int a = PAIRS ? (d + e) >> 1 : d + e < R2 ? d + e : d + e - R2;
+          const I r = axis_row(a);
+          c[e] = cos[(long long)r * R2 + a];
+          s[e] = sin[(long long)r * R2 + a];
+        }
     }
 #pragma unroll
     for (int n = 0; n < EACH; ++n) {
@@ -122,17 +171,18 @@ RX_DEV void rx_kv_write(const typename E::S* q, const typename E::S* k, const ty
 
 // ---------------------------------------------------------------------------
 // slots moved together: a thread takes the same bytes (a unit) of all of a sequence's steps, and loads them all before it stores the
-// first, so that a slot may be moved from and moved to.
+// first, so that a slot may be moved from and moved to.  A chain of four dependent loads and a store: 48 sequences of 5 steps in 8 bits
+// (0.4 MB) 5.0 us, 256 of 16 steps in bf16 (16 MB) 6.9; with the page table read once more for the addresses 7.4 and 11.7.
 // ---------------------------------------------------------------------------
-template <int S, typename U, int A, typename F, typename G>
-RX_DEV void rx_lm_move(U* base, const int (&from)[A], const int (&to)[A], F page_of, G place) {
+template <int S, typename U, int A, typename G>
+RX_DEV void rx_lm_move(U* base, const int (&from)[A], const int (&there)[A], const int (&here)[A], const int n, G place) {
   U held[A];
 #pragma unroll
   for (int a = 0; a < A; ++a)
-    if (to[a] >= 0) held[a] = base[place(page_of(from[a]), from[a] % S)];
+    if (from[a] >= 0) held[a] = base[place(there[a], (rx_u32)from[a] % S)];
 #pragma unroll
   for (int a = 0; a < A; ++a)
-    if (to[a] >= 0) base[place(page_of(to[a]), to[a] % S)] = held[a];
+    if (from[a] >= 0) base[place(here[a], (rx_u32)(n + a) % S)] = held[a];
 }
 template <typename U, int KU, int VU, int HK, int P, int S, int B, int M, int A, bool BY_SLOT, bool SCALES, typename I>
 RX_DEV void rx_kv_move(const I* lengths, const I* path, const I* pages, U* kc, U* vc, float* ks, float* vs) {
@@ -140,27 +190,32 @@ RX_DEV void rx_kv_move(const I* lengths, const I* path, const I* pages, U* kc, U
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)B * UNITS; i += (long long)gridDim.x * 256) {
     const long long b = i / UNITS;
     const int u = (int)(i % UNITS);
-    const I n = lengths[b];
-    if (n < 0 || n >= (I)(M * S)) continue;
-    int from[A], to[A];                                 // positions; -1: not moved
+    // all loads of one kind before the first of the next: lengths and path, pages, units
+    const I len = lengths[b];
+    I p[A];
+#pragma unroll
+    for (int a = 0; a < A; ++a) p[a] = path[b * A + a];
+    if (len < 0 || len >= (I)(M * S)) continue;
+    const int n = (int)len;
+    int from[A], there[A], here[A];                     // position that is moved (-1: none), its page and the page it is moved to
 #pragma unroll
     for (int a = 0; a < A; ++a) {
-      const I p = path[b * A + a];
-      from[a] = to[a] = -1;
-      if (p < 0 || p == a || p >= (I)(M * S) - n || a >= (I)(M * S) - n) continue;
-      const int f = (int)(n + p), t = (int)n + a;
-      const I fp = pages[b * M + f / S], tp = pages[b * M + t / S];
-      if (fp < 0 || fp >= P || tp < 0 || tp >= P) continue;
-      from[a] = f;
-      to[a] = t;
+      const bool moves = p[a] >= 0 && p[a] != a && p[a] < (I)(M * S - n) && a < M * S - n;
+      from[a] = moves ? n + (int)p[a] : -1;
+      const I fp = pages[b * M + (rx_u32)(moves ? from[a] : 0) / S], tp = pages[b * M + (rx_u32)(moves ? n + a : 0) / S];
+      there[a] = fp >= 0 && fp < P ? (int)fp : -1;
+      here[a] = tp >= 0 && tp < P ? (int)tp : -1;
     }
-    auto page_of = [&](const int at) { return (long long)pages[b * M + at / S]; };
-    if (u < HK * KU) rx_lm_move<S>(kc, from, to, page_of, [&](const long long page, const int slot) { return rx_lm_slot<S, HK, KU, BY_SLOT>(page, slot, u / KU) + u % KU; });
+#pragma unroll
+    for (int a = 0; a < A; ++a)
+      if (there[a] < 0 || here[a] < 0) from[a] = -1;
+    if (u < HK * KU)
+      rx_lm_move<S>(kc, from, there, here, n, [u](const int page, const int slot) { return rx_lm_slot<S, HK, KU, BY_SLOT>(page, slot, u / KU) + u % KU; });
     else if (u < HK * (KU + VU))
-      rx_lm_move<S>(vc, from, to, page_of, [&](const long long page, const int slot) { return rx_lm_slot<S, HK, VU, BY_SLOT>(page, slot, (u - HK * KU) / VU) + (u - HK * KU) % VU; });
+      rx_lm_move<S>(vc, from, there, here, n, [u](const int page, const int slot) { return rx_lm_slot<S, HK, VU, BY_SLOT>(page, slot, (u - HK * KU) / VU) + (u - HK * KU) % VU; });
     else if constexpr (SCALES) {
       const int h = u - HK * (KU + VU);
-      rx_lm_move<S>(h < HK ? ks : vs, from, to, page_of, [&](const long long page, const int slot) { return rx_lm_slot<S, HK, 1, false>(page, slot, h % HK); });
+      rx_lm_move<S>(h < HK ? ks : vs, from, there, here, n, [h](const int page, const int slot) { return rx_lm_slot<S, HK, 1, false>(page, slot, h % HK); });
     }
   }
 }
@@ -220,6 +275,34 @@ RX_DEV rx_u32x4 rx_lm_eight_up(const rx_u32 a, const rx_u32 b) {
   return rx_u32x4{rx_lm_pair_up<C>(a, false), rx_lm_pair_up<C>(a, true), rx_lm_pair_up<C>(b, false), rx_lm_pair_up<C>(b, true)};
 }
 
+// two numbers (no products) rounded to a 16-bit type, by one operation: what is unpacked again is not rounded again
+template <typename F>
+RX_DEV rx_u32 rx_lm_pair_down(const float x, const float y) {
+  rx_u32 p;
+  if constexpr (F::BF16) {
+    typedef __bf16 P __attribute__((ext_vector_type(2)));
+    p = __builtin_bit_cast(rx_u32, P{(__bf16)x, (__bf16)y});
+  } else {
+    typedef _Float16 P __attribute__((ext_vector_type(2)));
+    p = __builtin_bit_cast(rx_u32, P{(_Float16)x, (_Float16)y});
+  }
+  rx_pin(p);
+  return p;
+}
+// the largest of the four lanes l, l ^ 16, l ^ 32, l ^ 48, by exchanges of rows of lanes
+RX_DEV float rx_lm_rows_max(const float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(rx_f2u(x), rx_f2u(x), false, false);
+  const float y = __builtin_fmaxf(rx_u2f(a[0]), rx_u2f(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(rx_f2u(y), rx_f2u(y), false, false);
+  return __builtin_fmaxf(rx_u2f(b[0]), rx_u2f(b[1]));
+}
+// offset of a slot's head in a cache, of pages whose elements 32 bits count where they do
+template <int S, int H, int D, bool BY_SLOT>
+RX_DEV rx_u64 rx_lm_at(const rx_u32 page, const rx_u32 slot, const rx_u32 head) {
+  if constexpr ((long long)S * H * D < (1ll << 31)) return (rx_u64)page * (rx_u32)(S * H * D) + (BY_SLOT ? slot * (H * D) + head * D : head * (S * D) + slot * D);
+  else return rx_lm_slot<S, H, D, BY_SLOT>(page, slot, head);
+}
+
 // What the rows of a wavefront have seen: maxima, sums, unscaled results, for NT tiles of 16 rows.
 // E: of the queries and the result, C: of the caches, F: of the products.  Caches of 8 bits are multiplied as bf16, which holds their numbers
 // exactly; queries of more digits than bf16's go in as a sum of up to three bf16 (f16: two hold it exactly, f32: three leave 2^-24).
@@ -276,10 +359,10 @@ struct rx_lm_tree {
     }
   }
   // One step.  kf: keys of positions r and 16 + r; value(j, e): dimension VE r + e (of 16 VE) of the eight positions 4 g4 + (0..3) and
-  // 16 further as an operand; seen[t]: which of those eight the lane's row sees, where `some` do not; factor: of the scores;
-  // ks, vs: the scales of the eight positions, ks times factor already.
-  template <typename V>
-  RX_MEM void step(const rx_u32x4 (&kf)[2][KF], V value, const bool some, const unsigned (&seen)[NT], const float factor, const float (&ks)[8], const float (&vs)[8]) {
+  // 16 further as an operand; SOME: some rows do not see some positions, and seen[t] says which of those eight the lane's row
+  // sees; factor: of the scores; ks, vs: the scales of the eight positions, ks times factor already.  load_values(): before the first value.
+  template <bool SOME, typename V, typename L>
+  RX_MEM void step(const rx_u32x4 (&kf)[2][KF], L load_values, V value, const unsigned (&seen)[NT], const float factor, const float (&ks)[8], const float (&vs)[8]) {
     rx_u32x4 w[NT][NP];                                   // 16-bit weights of the eight positions
     float wide[NT][8];
 #pragma unroll
@@ -292,20 +375,23 @@ struct rx_lm_tree {
           s[0] = rx_lm_mma<F>(kf[0][k], q[t][n][k], s[0]);
           s[1] = rx_lm_mma<F>(kf[1][k], q[t][n][k], s[1]);
         }
+      // Where all positions have one factor the largest score is that of the products, times it, and weights take one operation more.
+      // (Not below the lowest number: a maximum of -inf says that there was no position.)
       float x[8], top = -rx_lm_inf();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3] * (BITS8 ? ks[i] : factor);
-      // (not below the lowest number: a maximum of -inf says that there was no position)
-      if (some) {
+      for (int i = 0; i < 8; ++i) x[i] = BITS8 || SOME ? s[i >> 2][i & 3] * (BITS8 ? ks[i] : factor) : s[i >> 2][i & 3];
+      if constexpr (SOME) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, (seen[t] >> i) & 1u ? __builtin_fmaxf(x[i], -RX_LM_FLT_MAX) : -rx_lm_inf());
       } else {
+        const bool down = !BITS8 && factor < 0.0f;
+        float far = x[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, x[i]);
-        top = __builtin_fmaxf(top, -RX_LM_FLT_MAX);
+        for (int i = 1; i < 8; ++i) far = down ? __builtin_fminf(far, x[i]) : __builtin_fmaxf(far, x[i]);
+        top = __builtin_fmaxf(BITS8 ? far : far * factor, -RX_LM_FLT_MAX);
       }
-      top = __builtin_fmaxf(m[t], rx_lm_max4(top));
-      if (__any(top != m[t])) {
+      top = __builtin_fmaxf(m[t], rx_lm_rows_max(top));
+      if (__builtin_expect(__any(top != m[t]), 0)) {
         const float shrink = top == m[t] ? 1.0f : __builtin_amdgcn_exp2f(m[t] - top);
         l[t] *= shrink;
 #pragma unroll
@@ -314,35 +400,36 @@ struct rx_lm_tree {
           for (int e = 0; e < VE; ++e) acc[t][j][e] *= shrink;
         m[t] = top;
       }
+      const float base = SHIFT - top;
       float p[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(x[i] - top + SHIFT);
-      if (some) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = (seen[t] >> i) & 1u ? p[i] : 0.0f;
+      for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(BITS8 || SOME ? x[i] + base : __builtin_fmaf(x[i], factor, base));
+        if (SOME) p[i] = (seen[t] >> i) & 1u ? p[i] : 0.0f;
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) l[t] += p[i];
+      l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
       if constexpr (BITS8) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = some && !((seen[t] >> i) & 1u) ? 0.0f : p[i] * vs[i];
+        for (int i = 0; i < 8; ++i) p[i] = SOME && !((seen[t] >> i) & 1u) ? 0.0f : p[i] * vs[i];
       }
       if constexpr (WIDE) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) wide[t][i] = p[i];
       } else {
 #pragma unroll
-        for (int n = 0; n < NP; ++n) {
-          rx_vec<rx_u16, 8> o;
+        for (int n = 0; n < NP; ++n)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            o.v[i] = F::down(p[i]);
-            if (n + 1 < NP) p[i] -= F::up(o.v[i]);
+          for (int i = 0; i < 4; ++i) {
+            const rx_u32 pair = rx_lm_pair_down<F>(p[2 * i], p[2 * i + 1]);
+            w[t][n][i] = pair;
+            if (n + 1 < NP) {
+              p[2 * i] -= F::up((rx_u16)pair);
+              p[2 * i + 1] -= F::up((rx_u16)(pair >> 16));
+            }
           }
-          w[t][n] = __builtin_bit_cast(rx_u32x4, o);
-        }
       }
     }
+    load_values();
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -360,29 +447,6 @@ struct rx_lm_tree {
           }
         }
       }
-  }
-  // Infinities and NaN among the values of a step that some rows do not see (a weight of zero would make them NaN there): they are
-  // taken out of the values before the step, and added here to the rows that see them.  at(p, d): value of position p (of 32).
-  template <typename A>
-  RX_MEM void add_special(const unsigned (&seen)[NT], A at) {
-    const int r = threadIdx.x & 15, g4 = (threadIdx.x & 63) >> 4;
-    for (int p = 0; p < 32; ++p) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const unsigned bits = rx_lane_from(seen[t], (((p >> 2) & 3) << 4) + r);
-        const bool sees = (bits >> ((p >> 4) * 4 + (p & 3))) & 1u;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int e = 0; e < VE; ++e)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int d = (j * 16 + g4 * 4 + i) * VE + e;
-              const float v = sees && d < DV ? at(p, d) : 0.0f;
-              if (!(__builtin_fabsf(v) <= RX_LM_FLT_MAX)) acc[t][j][e][i] += v;
-            }
-      }
-    }
   }
 };
 
@@ -402,6 +466,23 @@ RX_DEV rx_u32 rx_lm_special(const rx_u32 w) {
     constexpr rx_u32 e = X::BF16 ? 0x7f80u : 0x7c00u;
     return ((w & e) == e ? 0xffffu : 0u) | (((w >> 16) & e) == e ? 0xffff0000u : 0u);
   }
+}
+
+// Parts of a result in memory as rx_lm_put_shared writes single numbers, four at a time: 16 bytes that one thread writes, device-wide
+// (sc1, as the compiler has device-scope atomic accesses), and reads after they have been counted in.
+RX_DEV void rx_lm_put_shared4(const __amdgpu_buffer_rsrc_t to, const unsigned byte, const rx_f32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(rx_u32x4, v), to, byte, 0, 16);
+}
+RX_DEV rx_f32x4 rx_lm_get_shared4(const __amdgpu_buffer_rsrc_t from, const unsigned byte) {
+  return __builtin_bit_cast(rx_f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, byte, 0, 16));
+}
+RX_DEV __amdgpu_buffer_rsrc_t rx_lm_shared(float* base, const unsigned bytes) { return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000); }
+
+// Operands that the compiler takes for others from here on: what follows in one branch is not the other branch's, and is not moved before both.
+template <int N>
+RX_DEV void rx_lm_hold(rx_u32x4 (&f)[2][N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) asm volatile("" : "+v"(f[0][k]), "+v"(f[1][k]));
 }
 
 // MASK: 0 every drafted token sees itself and those before it, 2 [N, N] for all sequences, 3 [B, N, N].  NT: tiles of 16 rows to a
@@ -433,23 +514,30 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
   __shared__ __attribute__((aligned(16))) typename F::S vt[SHARED ? 2 : 1][SHARED ? 32 : 1][SHARED ? VP : FE];
   __shared__ float st_k[2][32], st_v[2][32];
   __shared__ unsigned st_ok[2];
-  __shared__ int last;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
+  __shared__ int last, any;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
   const int id = DIES ? (int)rx_xcd_remap(blockIdx.x, R * COLUMNS) : (int)blockIdx.x, column = id % COLUMNS, mine = id / COLUMNS, tile = column % TILES;
   const int head0 = column / TILES * HW, head = head0 + (SHARED ? 0 : wave / WPH);
   const int row0 = tile * TR + (SHARED ? wave * 16 * NT : 0);                 // first row of this wavefront
   const int rows = ROWS - tile * TR < TR ? ROWS - tile * TR : TR;             // of the workgroup
   const rx_lm_stretch st = rx_lm_stretch_of<B, R, Q>([&](const int at) { return rx_lm_tree_span_of<S, B, M, N, W>(lengths[at]).cost; }, mine);
   auto result_of = [&](const int b, const int row, const int h) { return ((long long)b * N + row / G) * HQ + h * G + row % G; };   // row of the results
+  const __amdgpu_buffer_rsrc_t parts_at = rx_lm_shared(part, (unsigned)R * COLUMNS * 2 * HW * RT * DV * 4);
   int buf = 0;
   if constexpr (SHARED && (DK + FE - 1) / FE * FE < KF * 4 * A::NE) {          // what no chunk of a key covers
     for (int i = threadIdx.x; i < 64 * KP; i += 256) (&kt[0][0][0])[i] = F::down(0.0f);
     __syncthreads();
   }
 
-  int b = st.b, unit = st.unit;
-  for (int left = st.count; left > 0; ++b, unit = 0) {
-  const rx_lm_tree_span span = rx_lm_tree_span_of<S, B, M, N, W>(lengths[b]);
+  // (what all lanes have alike is kept in scalar registers)
+  int b = __builtin_amdgcn_readfirstlane(st.b), unit = __builtin_amdgcn_readfirstlane(st.unit);
+  for (int left = __builtin_amdgcn_readfirstlane(st.count); left > 0; ++b, unit = 0) {
+  rx_lm_tree_span span = rx_lm_tree_span_of<S, B, M, N, W>(lengths[b]);
+  span.n = __builtin_amdgcn_readfirstlane(span.n);
+  span.lo = __builtin_amdgcn_readfirstlane(span.lo);
+  span.units = __builtin_amdgcn_readfirstlane(span.units);
+  span.cost = __builtin_amdgcn_readfirstlane(span.cost);
+  span.prefix = __builtin_amdgcn_readfirstlane(span.prefix);
   const int step = span.cost - unit < left ? span.cost - unit : left, take = span.units - unit < step ? span.units - unit : step;
   const long long begin = st.first + (st.count - left) - unit;                // the sequence's first unit in the row
   left -= step;
@@ -458,43 +546,48 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
   const bool whole = take == span.units;                                      // the whole sequence is in this stretch
   A a;
   a.clear();
-  int token[NT], first[NT];                                                   // of the lane's rows: the drafted token, and the first position of the prefix that it sees
-  bool inside[NT];
+  // With a window the last of its places are taken by the drafted tokens that a token sees; where it begins among the positions before them.
+  auto first_of = [&](const int token) {
+    if constexpr (W == 0) return 0;
+    int sees = 0;
+    if constexpr (MASK == 0) sees = token + 1;
+    else
+      for (int j = 0; j < N; ++j) sees += mask[((long long)(MASK == 3 ? b : 0) * N + token) * N + j] != 0;
+    return span.prefix - (W - sees) > 0 ? span.prefix - (W - sees) : 0;
+  };
+  auto sees = [&](const int token, const int first, const int p) {
+    if (p < span.prefix) return p >= first;
+    if constexpr (MASK == 0) return p - span.prefix <= token;
+    else return mask[((long long)(MASK == 3 ? b : 0) * N + token) * N + (p - span.prefix)] != 0;
+  };
+  int token[NT], first[NT];                                                   // of the lane's rows
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int row = row0 + t * 16 + r;
-    inside[t] = row < ROWS;
-    token[t] = inside[t] ? row / G : 0;
-    first[t] = 0;
-    a.load(t, q + result_of(b, inside[t] ? row : 0, head) * DK, inside[t]);
-    if constexpr (W > 0) {                                                    // the window's last places are taken by the drafted tokens that it sees
-      int sees = 0;
-      if constexpr (MASK == 0) sees = token[t] + 1;
-      else
-        for (int j = 0; j < N; ++j) sees += mask[((long long)(MASK == 3 ? b : 0) * N + token[t]) * N + j] != 0;
-      first[t] = span.prefix - (W - sees) > 0 ? span.prefix - (W - sees) : 0;
-    }
+    int row = row0 + t * 16 + r;
+    rx_pin(row);
+    const bool inside = row < ROWS;
+    token[t] = inside ? row / G : 0;
+    first[t] = first_of(token[t]);
+    a.load(t, q + result_of(b, inside ? row : 0, head) * DK, inside);
   }
-  const int edge = W > 0 && span.prefix - W + N > 0 ? span.prefix - W + N : 0;   // every row sees the prefix from here on
+  // Rows differ in what they see of the steps before `edge` and of those from `mixed` on.
+  const int edge = W > 0 && span.prefix - W + N > 0 ? (span.prefix - W + N + 31) & ~31 : 0, mixed = span.prefix & ~31;
   // bits of the lane's eight positions of a step that its rows see
   auto seen_by = [&](const int t0, const unsigned ok, unsigned (&seen)[NT]) {
+    int g = g4;
+    rx_pin(g);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       seen[t] = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int at = (i & 4) * 4 + g4 * 4 + (i & 3), p = t0 + at, j = p - span.prefix;
-        bool see = (ok >> at) & 1u;
-        if (see) {
-          if (j < 0) see = p >= first[t];
-          else if constexpr (MASK == 0) see = j <= token[t];
-          else see = mask[((long long)(MASK == 3 ? b : 0) * N + token[t]) * N + j] != 0;
-        }
-        seen[t] |= see ? 1u << i : 0u;
+        const int at = (i & 4) * 4 + g * 4 + (i & 3);
+        seen[t] |= ((ok >> at) & 1u) && sees(token[t], first[t], t0 + at) ? 1u << i : 0u;
       }
     }
   };
-  auto some_of = [&](const int t0, const unsigned ok) { return ok != ~0u || t0 + 32 > span.prefix || (W > 0 && t0 < edge); };
+  rx_u32 special = 0;                                                         // infinities or NaN have been taken out of values
+  auto differ = [&](const int t0) { return t0 >= mixed || (W > 0 && t0 < edge); };
 
   if constexpr (!SHARED) {
     constexpr int KR = BITS8 ? (DK + 63) / 64 : KF;    // 16-byte loads of a key by its four lanes
@@ -509,14 +602,14 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
       }
       __syncthreads();
       // page of a position, -1 where it is not to be looked at
-      auto where = [&](const int t) { return t >= span.lo && t < s1 ? lds.page[t / S - page0] : -1; };
+      auto where = [&](const int t) { return t >= span.lo && t < s1 ? lds.page[(rx_u32)t / S - page0] : -1; };
       for (int t0 = s0 + wave % WPH * 32; t0 < s1; t0 += WPH * 32) {
         const int ta = t0 + r, tb = ta + 16, pa = where(ta), pb = where(tb);
         const unsigned ok = ((unsigned)__ballot(pa >= 0) & 0xffffu) | ((unsigned)__ballot(pb >= 0) << 16);
         if (!ok) continue;
         rx_vec<rx_u32, 4> raw[2][KR];
-        const T* ka = kc + rx_lm_slot<S, HK, DK, BY_SLOT>(pa < 0 ? 0 : pa, ta % S, head);
-        const T* kb = kc + rx_lm_slot<S, HK, DK, BY_SLOT>(pb < 0 ? 0 : pb, tb % S, head);
+        const T* ka = kc + rx_lm_at<S, HK, DK, BY_SLOT>(pa < 0 ? 0 : pa, (rx_u32)ta % S, head);
+        const T* kb = kc + rx_lm_at<S, HK, DK, BY_SLOT>(pb < 0 ? 0 : pb, (rx_u32)tb % S, head);
 #pragma unroll
         for (int k = 0; k < KR; ++k) {
           raw[0][k] = rx_lm_part<T, DK, 16 / sizeof(T), ONCE>(ka, (k * 4 + g4) * (16 / sizeof(T)));
@@ -533,7 +626,7 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
             pv = where(S % 4 == 0 ? (tv + 3 < s1 ? tv + 3 : s1 - 1) : tv);   // (the group's first positions may lie before span.lo)
             if (S % 4 == 0 && tv >= s1) pv = -1;
           }
-          const T* v = vc + rx_lm_slot<S, HK, DV, BY_SLOT>(pv < 0 ? 0 : pv, tv % S, head);
+          const T* v = vc + rx_lm_at<S, HK, DV, BY_SLOT>(pv < 0 ? 0 : pv, (rx_u32)tv % S, head);
 #pragma unroll
           for (int j = 0; j < NV; ++j) vf[j][i] = rx_lm_part<T, DV, VE, ONCE>(v, (j * 16 + r) * VE);
           if constexpr (BITS8) {
@@ -563,22 +656,6 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
               for (int j = 0; j < NV; ++j) vf[j][i] = CV{};
             }
         }
-        unsigned seen[NT] = {};
-        rx_u32 special = 0;
-        const bool some = some_of(t0, ok);
-        if (some) {
-          seen_by(t0, ok, seen);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-#pragma unroll
-              for (int n = 0; n < (int)(sizeof(CV) / 4); ++n) {
-                const rx_u32 x = rx_lm_special<C>(vf[j][i].v[n]);
-                vf[j][i].v[n] &= ~x;
-                special |= x;
-              }
-        }
         rx_u32x4 kf[2][KF];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -587,7 +664,7 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
             if constexpr (BITS8) kf[h][k] = rx_lm_eight_up<C>(raw[h][k / 2].v[k % 2 * 2], raw[h][k / 2].v[k % 2 * 2 + 1]);
             else kf[h][k] = __builtin_bit_cast(rx_u32x4, raw[h][k]);
           }
-        a.step(kf, [&](const int j, const int e, const int half) {
+        auto value = [&](const int j, const int e, const int half) {
           rx_u32x4 o;
           if constexpr (A::WIDE) {
 #pragma unroll
@@ -601,50 +678,63 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
             for (int k = 0; k < 4; ++k) o[k] = __builtin_amdgcn_perm(vf[j][2 * k + 1].v[e >> 1], vf[j][2 * k].v[e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
           }
           return o;
-        }, some, seen, scale, kscale, vscale);
-        if (some && __any(special != 0)) {
-          a.add_special(seen, [&](const int p, const int d) {
-            const int page = where(t0 + p);
-            return page < 0 ? 0.0f : C::up(vc[rx_lm_slot<S, HK, DV, BY_SLOT>(page, (t0 + p) % S, head) + d]);
-          });
+        };
+        unsigned seen[NT] = {};
+        if (__builtin_expect(ok == ~0u && !differ(t0), 1)) {
+          a.template step<false>(kf, [] {}, value, seen, scale, kscale, vscale);
+        } else {
+          rx_lm_hold(kf);
+          seen_by(t0, ok, seen);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+              for (int n = 0; n < (int)(sizeof(CV) / 4); ++n) {
+                const rx_u32 x = differ(t0) ? rx_lm_special<C>(vf[j][i].v[n]) : 0u;
+                vf[j][i].v[n] &= ~x;
+                special |= x;
+              }
+          a.template step<true>(kf, [] {}, value, seen, scale, kscale, vscale);
         }
       }
     }
   } else {
     constexpr int CE = 16 / sizeof(T), CK = (DK + CE - 1) / CE, CV = (DV + CE - 1) / CE, LK = (32 * CK + 255) / 256, LV = (32 * CV + 255) / 256;
     rx_vec<rx_u32, 4> rk[LK], rv[LV];
-    int pk[LK], pv[LV], ps = -1;                        // pages of the next step's loads; of position threadIdx.x
+    I pk[LK], pv[LV], ps = 0;                           // page table's entries of the next step's loads; of position threadIdx.x
     float sk = 0.0f, sv = 0.0f;
     bool there = false;
-    auto page_of = [&](const int t) {
-      if (t < span.lo || t >= p1) return -1;
-      const I page = pages[(long long)b * M + t / S];
-      return page >= 0 && page < P ? (int)page : -1;
-    };
+    const I* table = pages + (long long)b * M;
+    // (No condition between a load and the next: each would wait for the data of the one before.  Positions past the end are the last.)
+    auto entry = [&](const int t) { return table[(rx_u32)(t < p1 ? t : p1 - 1) / S]; };
+    auto known = [&](const int t, const I page) { return t >= span.lo && t < p1 && page >= 0 && page < P; };
     auto find = [&](const int t0) {
 #pragma unroll
-      for (int n = 0; n < LK; ++n) pk[n] = n * 256 + (int)threadIdx.x < 32 * CK ? page_of(t0 + (n * 256 + (int)threadIdx.x) / CK) : -1;
+      for (int n = 0; n < LK; ++n) pk[n] = entry(t0 + (n * 256 + (int)threadIdx.x) / CK);
 #pragma unroll
-      for (int n = 0; n < LV; ++n) pv[n] = n * 256 + (int)threadIdx.x < 32 * CV ? page_of(t0 + (n * 256 + (int)threadIdx.x) / CV) : -1;
-      ps = threadIdx.x < 32 ? page_of(t0 + (int)threadIdx.x) : -1;
+      for (int n = 0; n < LV; ++n) pv[n] = CV == CK ? pk[n < LK ? n : 0] : entry(t0 + (n * 256 + (int)threadIdx.x) / CV);
+      ps = entry(t0 + (int)threadIdx.x);
     };
     auto fetch = [&](const int t0) {
+      bool on[LK];
 #pragma unroll
       for (int n = 0; n < LK; ++n) {
         const int i = n * 256 + (int)threadIdx.x, t = t0 + i / CK;
-        rk[n] = rx_vec<rx_u32, 4>{};
-        if (pk[n] >= 0) rk[n] = rx_lm_part<T, DK, CE, ONCE>(kc + rx_lm_slot<S, HK, DK, BY_SLOT>(pk[n], t % S, head), i % CK * CE);
+        on[n] = known(t, pk[n]);
+        rk[n] = rx_lm_part<T, DK, CE, ONCE>(kc + rx_lm_at<S, HK, DK, BY_SLOT>(on[n] ? (rx_u32)pk[n] : 0u, (rx_u32)t % S, head), i % CK * CE);
       }
 #pragma unroll
       for (int n = 0; n < LV; ++n) {
         const int i = n * 256 + (int)threadIdx.x, t = t0 + i / CV;
-        rv[n] = rx_vec<rx_u32, 4>{};
-        if (pv[n] >= 0) rv[n] = rx_lm_part<T, DV, CE, ONCE>(vc + rx_lm_slot<S, HK, DV, BY_SLOT>(pv[n], t % S, head), i % CV * CE);
+        const bool in = CV == CK ? on[n < LK ? n : 0] : known(t, pv[n]);
+        rv[n] = rx_lm_part<T, DV, CE, ONCE>(vc + rx_lm_at<S, HK, DV, BY_SLOT>(in ? (rx_u32)pv[n] : 0u, (rx_u32)t % S, head), i % CV * CE);
       }
-      there = ps >= 0;
+      there = threadIdx.x < 32 && known(t0 + (int)threadIdx.x, ps);
       if constexpr (BITS8) {
-        sk = there ? ks[rx_lm_slot<S, HK, 1, false>(ps, (t0 + (int)threadIdx.x) % S, head)] * scale : 0.0f;
-        sv = there ? vs[rx_lm_slot<S, HK, 1, false>(ps, (t0 + (int)threadIdx.x) % S, head)] : 0.0f;
+        const long long at = rx_lm_slot<S, HK, 1, false>(there ? (long long)ps : 0, (t0 + (int)threadIdx.x) % S, head);
+        sk = ks[at];
+        sv = vs[at];
       }
     };
     auto store = [&](typename F::S* to, const rx_vec<rx_u32, 4>& x) {
@@ -675,17 +765,17 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
         const unsigned long long all = __ballot(there);
         if (lane == 0) st_ok[buf] = (unsigned)all;
         if (BITS8 && lane < 32) {
-          st_k[buf][lane] = sk;
-          st_v[buf][lane] = sv;
+          st_k[buf][lane] = there ? sk * scale : 0.0f;
+          st_v[buf][lane] = there ? sv : 0.0f;
         }
       }
       __syncthreads();      // (the other buffer's readers have arrived here before it is written again)
-      if (t0 + 32 < p1) {
+      if (__builtin_expect(t0 + 32 < p1, 1)) {
         fetch(t0 + 32);
         find(t0 + 64);
       }
-      const unsigned ok = st_ok[buf];
-      if (!ok || row0 >= ROWS) continue;
+      const unsigned ok = __builtin_amdgcn_readfirstlane(st_ok[buf]);
+      if (__builtin_expect(!ok || row0 >= ROWS, 0)) continue;
       rx_u32x4 kf[2][KF];
       FV vf[NV][8];
       float kscale[8] = {}, vscale[8] = {};
@@ -694,10 +784,14 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
         kf[0][k] = *(const rx_u32x4*)&kt[buf][r][(k * 4 + g4) * A::NE];
         kf[1][k] = *(const rx_u32x4*)&kt[buf][16 + r][(k * 4 + g4) * A::NE];
       }
+      // (not before the weights are done: keys and values in registers at once leave none for a second wavefront)
+      auto load_values = [&] {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < NV; ++j) vf[j][i] = *(const FV*)&vt[buf][(i & 4) * 4 + g4 * 4 + (i & 3)][(j * 16 + r) * VE];
+          for (int j = 0; j < NV; ++j) vf[j][i] = *(const FV*)&vt[buf][(i & 4) * 4 + g4 * 4 + (i & 3)][(j * 16 + r) * VE];
+      };
       if constexpr (BITS8) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -705,23 +799,7 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
           vscale[i] = st_v[buf][(i & 4) * 4 + g4 * 4 + (i & 3)];
         }
       }
-      unsigned seen[NT] = {};
-      rx_u32 special = 0;
-      const bool some = some_of(t0, ok);
-      if (some) {
-        seen_by(t0, ok, seen);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int n = 0; n < (int)(sizeof(FV) / 4); ++n) {
-              const rx_u32 x = (j * 16 + r) * VE < DV ? rx_lm_special<F>(vf[j][i].v[n]) : ~0u;
-              vf[j][i].v[n] &= ~x;
-              special |= (j * 16 + r) * VE < DV ? x : 0u;
-            }
-      }
-      a.step(kf, [&](const int j, const int e, const int half) {
+      auto value = [&](const int j, const int e, const int half) {
         rx_u32x4 o;
         if constexpr (A::WIDE) {
 #pragma unroll
@@ -731,11 +809,39 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
           for (int k = 0; k < 4; ++k) o[k] = __builtin_amdgcn_perm(vf[j][2 * k + 1].v[e >> 1], vf[j][2 * k].v[e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
         }
         return o;
-      }, some, seen, scale, kscale, vscale);
-      if (some && __any(special != 0)) a.add_special(seen, [&](const int p, const int d) { return F::up(vt[buf][p][d]); });
+      };
+      unsigned seen[NT] = {};
+      if (__builtin_expect(ok == ~0u && !differ(t0), 1)) {
+        a.template step<false>(kf, load_values, value, seen, scale, kscale, vscale);
+      } else {
+        rx_lm_hold(kf);
+        seen_by(t0, ok, seen);
+        a.template step<true>(kf, [&] {
+          load_values();
+          int g = g4;
+          rx_pin(g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const bool exists = (ok >> ((i & 4) * 4 + g * 4 + (i & 3))) & 1u;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+              for (int n = 0; n < (int)(sizeof(FV) / 4); ++n) {
+                // (what lies in other slots, and past a value's end, may be anything, and NaN times a weight of zero is not zero)
+                const bool in = exists && (j * 16 + r) * VE < DV;
+                const rx_u32 x = in && differ(t0) ? rx_lm_special<F>(vf[j][i].v[n]) : 0u;
+                vf[j][i].v[n] &= in ? ~x : 0u;
+                special |= x;
+              }
+          }
+        }, value, seen, scale, kscale, vscale);
+      }
     }
   }
-
+  // (indices from here on are worked out here: what does not depend on the sequence would wait in registers through all of its steps)
+  int tid = threadIdx.x;
+  rx_pin(tid);
+  const int er = tid & 15, eg = (tid & 63) >> 4;
   if constexpr (!SHARED) {
     // the four wavefronts' parts
 #pragma unroll
@@ -743,51 +849,51 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
       if (t * 16 >= rows) break;
       const float total = rx_lm_sum4(a.l[t]);
       __syncthreads();
-      if (g4 == 0) {
-        join_m[wave][r] = a.m[t];
-        join_l[wave][r] = total;
+      if (eg == 0) {
+        join_m[wave][er] = a.m[t];
+        join_l[wave][er] = total;
       }
       __syncthreads();
       float top = -rx_lm_inf();
 #pragma unroll
-      for (int w = 0; w < WPH; ++w) top = __builtin_fmaxf(top, join_m[wave / WPH * WPH + w][r]);
+      for (int w = 0; w < WPH; ++w) top = __builtin_fmaxf(top, join_m[wave / WPH * WPH + w][er]);
       const float f = top == -rx_lm_inf() ? 0.0f : __builtin_amdgcn_exp2f(a.m[t] - top);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (j) __syncthreads();
-        if (r < HR) {
+        if (er < HR) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
-              const int d = (g4 * 4 + i) * VE + e;
-              if (d < WIDTH) lds.o[wave][r][d] = a.acc[t][j][e][i] * f;
+              const int d = (eg * 4 + i) * VE + e;
+              if (d < WIDTH) lds.o[wave][er][d] = a.acc[t][j][e][i] * f;
             }
         }
         __syncthreads();
-        for (int k = threadIdx.x; k < HW * HR * WIDTH; k += 256) {
-          const int hw = k / (HR * WIDTH), h = k / WIDTH % HR, d = j * 16 * VE + k % WIDTH, row = t * 16 + h;
+        for (int k = tid; k < HW * HR * (WIDTH / VD); k += 256) {
+          const int hw = k / (HR * (WIDTH / VD)), h = k / (WIDTH / VD) % HR, c = k % (WIDTH / VD) * VD, d = j * 16 * VE + c, row = t * 16 + h;
           if (row >= rows || d >= DV) continue;
-          float o = 0.0f, sum = 0.0f, hi = -rx_lm_inf();
+          float o[VD] = {}, sum = 0.0f, hi = -rx_lm_inf();
 #pragma unroll
           for (int i = 0; i < WPH; ++i) hi = __builtin_fmaxf(hi, join_m[hw * WPH + i][h]);
 #pragma unroll
           for (int i = 0; i < WPH; ++i) {
             const int w = hw * WPH + i;
-            o += lds.o[w][h][k % WIDTH];
+#pragma unroll
+            for (int e = 0; e < VD; ++e) o[e] += lds.o[w][h][c + e];
             sum += hi == -rx_lm_inf() ? 0.0f : join_l[w][h] * __builtin_amdgcn_exp2f(join_m[w][h] - hi);
           }
           if (whole) {
             const long long at = result_of(b, tile * TR + row, head0 + hw);
-            out[at * DV + d] = E::down(hi == -rx_lm_inf() ? 0.0f : o / sum);
+#pragma unroll
+            for (int e = 0; e < VD; ++e) out[at * DV + d + e] = E::down(hi == -rx_lm_inf() ? 0.0f : o[e] / sum);
             if (lse && d == 0) lse[at] = hi == -rx_lm_inf() ? -rx_lm_inf() : (hi - A::SHIFT + __builtin_log2f(sum)) * 0.6931471805599453f;
           } else {
             const long long at = (((long long)id * 2 + (unit == 0)) * HW + hw) * RT + row;
-            rx_lm_put_shared(part + at * DV + d, o);
-            if (d == 0) {
-              rx_lm_put_shared(stat + at * 2, hi - A::SHIFT);
-              rx_lm_put_shared(stat + at * 2 + 1, sum);
-            }
+            if constexpr (VD == 4) rx_lm_put_shared4(parts_at, (unsigned)(at * DV + d) * 4, rx_f32x4{o[0], o[1], o[2], o[3]});
+            else rx_lm_put_shared(part + at * DV + d, o[0]);
+            if (d == 0) rx_lm_put_shared((rx_u64*)stat + at, (rx_u64)rx_f2u(hi - A::SHIFT) | (rx_u64)rx_f2u(sum) << 32);
           }
         }
       }
@@ -796,76 +902,126 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const float sum = rx_lm_sum4(a.l[t]), hi = a.m[t];
-      if (!inside[t]) continue;
-      const int row = row0 + t * 16 + r - tile * TR;
+      if (row0 + t * 16 + er >= ROWS) continue;
+      const int row = row0 + t * 16 + er - tile * TR;
       const long long at = whole ? result_of(b, tile * TR + row, head) : ((long long)id * 2 + (unit == 0)) * RT + row;
-      if (g4 == 0) {
-        if (!whole) {
-          rx_lm_put_shared(stat + at * 2, hi - A::SHIFT);
-          rx_lm_put_shared(stat + at * 2 + 1, sum);
-        } else if (lse) {
-          lse[at] = hi == -rx_lm_inf() ? -rx_lm_inf() : (hi - A::SHIFT + __builtin_log2f(sum)) * 0.6931471805599453f;
-        }
+      if (eg == 0) {
+        if (!whole) rx_lm_put_shared((rx_u64*)stat + at, (rx_u64)rx_f2u(hi - A::SHIFT) | (rx_u64)rx_f2u(sum) << 32);
+        else if (lse) lse[at] = hi == -rx_lm_inf() ? -rx_lm_inf() : (hi - A::SHIFT + __builtin_log2f(sum)) * 0.6931471805599453f;
       }
+      const float f = hi == -rx_lm_inf() ? 0.0f : 1.0f / sum;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const int d = (j * 16 + g4 * 4 + i) * VE + e;
+          for (int e = 0; e < VE; e += VD) {
+            const int d = (j * 16 + eg * 4 + i) * VE + e;
             if (d >= DV) continue;
-            if (whole) out[at * DV + d] = E::down(hi == -rx_lm_inf() ? 0.0f : a.acc[t][j][e][i] / sum);
-            else rx_lm_put_shared(part + at * DV + d, a.acc[t][j][e][i]);
+            if (whole) {
+#pragma unroll
+              for (int c = 0; c < VD; ++c) out[at * DV + d + c] = E::down(hi == -rx_lm_inf() ? 0.0f : a.acc[t][j][e + c][i] * f);
+            } else if constexpr (VD == 4) {
+              rx_lm_put_shared4(parts_at, (unsigned)(at * DV + d) * 4, rx_f32x4{a.acc[t][j][e][i], a.acc[t][j][e + 1][i], a.acc[t][j][e + 2][i], a.acc[t][j][e + 3][i]});
+            } else {
+              rx_lm_put_shared(part + at * DV + d, a.acc[t][j][e][i]);
+            }
           }
+    }
+  }
+  // Infinities and NaN among the values of steps whose rows differ have been taken out (a weight of zero would make them NaN in rows that
+  // do not see them): they are added to the results of the rows that do.
+  if ((p1 > mixed || (W > 0 && p0 < edge)) && p0 < p1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's results
+  if ((p1 > mixed || (W > 0 && p0 < edge)) && p0 < p1 && __builtin_expect(rx_block_any(special != 0, &any), 0)) {
+    for (int k = tid; k < HW * rows * DV; k += 256) {
+      const int hw = k / (rows * DV), row = k / DV % rows, d = k % DV, token = (tile * TR + row) / G, first = first_of(token);
+      float more = 0.0f;
+      for (int p = p0; p < p1; ++p) {
+        if (!differ(p & ~31)) {
+          p = mixed > p ? mixed - 1 : p;
+          continue;
+        }
+        if (p < span.lo || !sees(token, first, p)) continue;
+        const I page = pages[(long long)b * M + p / S];
+        const float v = page >= 0 && page < P ? C::up(vc[rx_lm_slot<S, HK, DV, BY_SLOT>(page, p % S, head0 + hw) + d]) : 0.0f;
+        if (!(__builtin_fabsf(v) <= RX_LM_FLT_MAX)) more += v;
+      }
+      if (more == 0.0f) continue;
+      if (whole) {
+        const long long at = result_of(b, tile * TR + row, head0 + hw) * DV + d;
+        out[at] = E::down(E::up(out[at]) + more);
+      } else {
+        const long long at = ((((long long)id * 2 + (unit == 0)) * HW + hw) * RT + row) * DV + d;
+        rx_lm_put_shared(part + at, rx_lm_get_shared(part + at) + more);
+      }
     }
   }
   if (whole) continue;
   const int from = rx_lm_stretch_with(st.total, st.parts, begin), to = rx_lm_stretch_with(st.total, st.parts, begin + span.units - 1);
   if (!rx_lm_last_to_arrive(arrived + b * COLUMNS + column, to - from + 1, &last)) continue;
-  // VD outputs to a thread, DV / VD apart, so that lanes read consecutive words; where there are fewer than threads, the parts are
-  // shared too, and joined once more
+  // VD outputs to a thread; where there are fewer than threads, the parts are shared too, and joined once more; where there are more,
+  // a thread has up to four times VD, so that sixteen loads are on their way.
+  constexpr int MORE = HW * RT * (DV / VD) >= 1024 ? 4 : HW * RT * (DV / VD) >= 512 ? 2 : 1, AT = 16 / MORE;
   const int outs = HW * rows * (DV / VD), ways = outs < 256 ? 256 / outs : 1, parts = to - from + 1;
-  for (int k0 = 0; k0 < outs; k0 += 256) {
-    const int k = ways > 1 ? (int)threadIdx.x % outs : k0 + (int)threadIdx.x, way = ways > 1 ? (int)threadIdx.x / outs : 0;
-    const bool on = k < outs && way < ways;
-    const int hw = k / (rows * (DV / VD)), h = k / (DV / VD) % rows, d = k % (DV / VD);
+  for (int k0 = 0; k0 < outs; k0 += 256 * MORE) {
+    const int way = ways > 1 ? tid / outs : 0, k1 = ways > 1 ? tid % outs : k0 + tid;
+    const bool on = k1 < outs && way < ways;
     const int w1 = on ? from + parts * (way + 1) / ways : 0;
-    rx_lm_joined<VD> j = {-rx_lm_inf(), 0.0f, {}};
-    for (int w = on ? from + parts * way / ways : 0; w < w1; w += 8) {
-      float pm[8], psum[8], po[8][VD];
+    rx_lm_joined<VD> j[MORE];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int v = w + i < w1 ? w + i : w1 - 1;
-        const long long at = (((long long)(v * COLUMNS + column) * 2 + (v == from)) * HW + hw) * RT + h;
-        pm[i] = rx_lm_get_shared(stat + at * 2);
-        psum[i] = rx_lm_get_shared(stat + at * 2 + 1);
+    for (int u = 0; u < MORE; ++u) j[u] = {-rx_lm_inf(), 0.0f, {}};
+    for (int w = on ? from + parts * way / ways : 0; w < w1; w += AT) {
+      float pm[MORE][AT], psum[MORE][AT], po[MORE][AT][VD];
 #pragma unroll
-        for (int e = 0; e < VD; ++e) po[i][e] = rx_lm_get_shared(part + at * DV + d + e * (DV / VD));
+      for (int u = 0; u < MORE; ++u) {
+        const int k = k1 + 256 * u < outs ? k1 + 256 * u : k1, hw = k / (rows * (DV / VD)), h = k / (DV / VD) % rows, d = k % (DV / VD) * VD;
+#pragma unroll
+        for (int i = 0; i < AT; ++i) {
+          const int v = w + i < w1 ? w + i : w1 - 1;
+          const long long at = (((long long)(v * COLUMNS + column) * 2 + (v == from)) * HW + hw) * RT + h;
+          const rx_u64 both = rx_lm_get_shared((const rx_u64*)stat + at);
+          pm[u][i] = rx_u2f((rx_u32)both);
+          psum[u][i] = rx_u2f((rx_u32)(both >> 32));
+          if constexpr (VD == 4) {
+            const rx_f32x4 x = rx_lm_get_shared4(parts_at, (unsigned)(at * DV + d) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) po[u][i][e] = x[e];
+          } else {
+            po[u][i][0] = rx_lm_get_shared(part + at * DV + d);
+          }
+        }
       }
-      float hi = j.m;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) hi = __builtin_fmaxf(hi, pm[i]);
-      j.to(hi);
+      for (int u = 0; u < MORE; ++u) {
+        float hi = j[u].m;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (w + i < w1) j.add(pm[i], psum[i], po[i]);
+        for (int i = 0; i < AT; ++i) hi = __builtin_fmaxf(hi, pm[u][i]);
+        j[u].to(hi);
+#pragma unroll
+        for (int i = 0; i < AT; ++i)
+          if (w + i < w1) j[u].add(pm[u][i], psum[u][i], po[u][i]);
+      }
     }
     if (ways > 1) {
-      lds.j[threadIdx.x] = j;
+      lds.j[tid] = j[0];
       __syncthreads();
       if (way == 0)
         for (int n = 1; n < ways; ++n) {
-          const rx_lm_joined<VD> o = lds.j[n * outs + k];
-          j.to(__builtin_fmaxf(j.m, o.m));
-          j.add(o.m, o.s, o.o);
+          const rx_lm_joined<VD> o = lds.j[n * outs + k1];
+          j[0].to(__builtin_fmaxf(j[0].m, o.m));
+          j[0].add(o.m, o.s, o.o);
         }
     }
     if (!on || way) continue;
-    const long long at = result_of(b, tile * TR + h, head0 + hw);
 #pragma unroll
-    for (int e = 0; e < VD; ++e) out[at * DV + d + e * (DV / VD)] = E::down(j.m == -rx_lm_inf() ? 0.0f : j.o[e] / j.s);
-    if (lse && d == 0) lse[at] = j.m == -rx_lm_inf() ? -rx_lm_inf() : (j.m + __builtin_log2f(j.s)) * 0.6931471805599453f;
+    for (int u = 0; u < MORE; ++u) {
+      const int k = k1 + 256 * u, hw = k / (rows * (DV / VD)), h = k / (DV / VD) % rows, d = k % (DV / VD) * VD;
+      if (k >= outs) break;
+      const long long at = result_of(b, tile * TR + h, head0 + hw);
+#pragma unroll
+      for (int e = 0; e < VD; ++e) out[at * DV + d + e] = E::down(j[u].m == -rx_lm_inf() ? 0.0f : j[u].o[e] / j[u].s);
+      if (lse && d == 0) lse[at] = j[u].m == -rx_lm_inf() ? -rx_lm_inf() : (j[u].m + __builtin_log2f(j[u].s)) * 0.6931471805599453f;
+    }
   }
   }
 }

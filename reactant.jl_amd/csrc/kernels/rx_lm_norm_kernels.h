@@ -147,15 +147,17 @@ RX_DEV void rx_rms_norm_grad(const typename E::S* h, const typename E::S* weight
   const int lane = threadIdx.x % LANES, line = threadIdx.x / LANES;
   float acc[EACH][VEC] = {};
   int turn = 0;
+  W w[EACH];
+#pragma unroll
+  for (int n = 0; n < EACH; ++n) w[n] = rx_load<W>(weight + (lane + n * LANES < C ? lane + n * LANES : C - 1) * VEC);
   for (long long row = (long long)blockIdx.x * LINES + line; row < ROWS; row += (long long)GROUPS * LINES, ++turn) {
-    W a[EACH], b[EACH], d[EACH], w[EACH];
+    W a[EACH], b[EACH], d[EACH];
 #pragma unroll
     for (int n = 0; n < EACH; ++n) {
-      const int c = lane + n * LANES < C ? lane + n * LANES : C - 1;
-      a[n] = rx_load_nt<W>(h + row * D + c * VEC);
-      b[n] = rx_load_nt<W>(dy + row * D + c * VEC);
-      if constexpr (RES) d[n] = rx_load_nt<W>(dh + row * D + c * VEC);
-      w[n] = rx_load<W>(weight + c * VEC);
+      const long long at = row * D + (lane + n * LANES < C ? lane + n * LANES : C - 1) * VEC;
+      a[n] = rx_load_nt<W>(h + at);
+      b[n] = rx_load_nt<W>(dy + at);
+      if constexpr (RES) d[n] = rx_load_nt<W>(dh + at);
     }
     rx_vec<float, 2> s = {{0.0f, 0.0f}};                          // squares of h, products g h
 #pragma unroll
@@ -216,20 +218,33 @@ RX_DEV void rx_rms_norm_grad(const typename E::S* h, const typename E::S* weight
         for (int e = 0; e < VEC; ++e) part[(long long)blockIdx.x * D + (lane + n * LANES) * VEC + e] = acc[n][e];
   }
 }
-// The weight's gradient from the workgroups' parts: 32 columns to a workgroup, whose eight lines of threads take every eighth part.
+// The weight's gradient from the workgroups' parts: 64 columns to a workgroup, a vector of four to each of 16 lanes, whose 64 lines of
+// lanes take every 64th part, eight of them at a time.
 template <typename O, int D, int GROUPS>
 RX_DEV void rx_rms_norm_weight(const float* part, typename O::S* dweight) {
-  __shared__ float lines[8][33];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), line = threadIdx.x >> 5;
-  float t = 0.0f;
+  constexpr int VEC = D % 4 == 0 ? 4 : 1, LANES = 16, LINES = 1024 / LANES;
+  typedef rx_vec<float, VEC> W;
+  __shared__ W lines[LINES][LANES];
+  const int lane = threadIdx.x % LANES, line = threadIdx.x / LANES, c = (blockIdx.x * LANES + lane) * VEC;
+  W t{};
   if (c < D) {
-#pragma unroll 8
-    for (int g = line; g < GROUPS; g += 8) t += part[(long long)g * D + c];
-  }
-  lines[line][threadIdx.x & 31] = t;
-  __syncthreads();
-  if (line || c >= D) return;
+    for (int g0 = line; g0 < GROUPS; g0 += 8 * LINES) {
+      W x[8];
 #pragma unroll
-  for (int k = 1; k < 8; ++k) t += lines[k][threadIdx.x];
-  dweight[c] = O::down(t);
+      for (int k = 0; k < 8; ++k) x[k] = rx_load<W>(part + (long long)(g0 + k * LINES < GROUPS ? g0 + k * LINES : g0) * D + c);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (g0 + k * LINES < GROUPS)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) t.v[e] += x[k].v[e];
+    }
+  }
+  lines[line][lane] = t;
+  __syncthreads();
+  const int o = threadIdx.x;
+  if (o >= LANES * VEC || blockIdx.x * LANES * VEC + o >= D) return;
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int k = 0; k < LINES; ++k) sum += lines[k][o / VEC].v[o % VEC];
+  dweight[blockIdx.x * LANES * VEC + o] = O::down(sum);
 }
