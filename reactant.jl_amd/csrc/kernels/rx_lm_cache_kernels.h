@@ -359,10 +359,11 @@ struct rx_lm_tree {
     }
   }
   // One step.  kf: keys of positions r and 16 + r; value(j, e): dimension VE r + e (of 16 VE) of the eight positions 4 g4 + (0..3) and
-  // 16 further as an operand; SOME: some rows do not see some positions, and seen[t] says which of those eight the lane's row
-  // sees; factor: of the scores; ks, vs: the scales of the eight positions, ks times factor already.  load_values(): before the first value.
-  template <bool SOME, typename V, typename L>
-  RX_MEM void step(const rx_u32x4 (&kf)[2][KF], L load_values, V value, const unsigned (&seen)[NT], const float factor, const float (&ks)[8], const float (&vs)[8]) {
+  // 16 further as an operand, after load_values(); factor: of the scores; ks, vs: the scales of the eight positions, ks times factor already.
+  // Where `some` rows do not see some of the positions, seen[t] says which of those eight the lane's row sees: their scores become -inf, and
+  // the rest is the same code, since code that runs once or twice is paid for by loading it.
+  template <typename V, typename L>
+  RX_MEM void step(const rx_u32x4 (&kf)[2][KF], L load_values, V value, const bool some, const unsigned (&seen)[NT], const float factor, const float (&ks)[8], const float (&vs)[8]) {
     rx_u32x4 w[NT][NP];                                   // 16-bit weights of the eight positions
     float wide[NT][8];
 #pragma unroll
@@ -376,23 +377,22 @@ struct rx_lm_tree {
           s[1] = rx_lm_mma<F>(kf[1][k], q[t][n][k], s[1]);
         }
       // Where all positions have one factor the largest score is that of the products, times it, and weights take one operation more.
-      // (Not below the lowest number: a maximum of -inf says that there was no position.)
-      float x[8], top = -rx_lm_inf();
+      // (A factor of zero is multiplied first: masked scores are infinite.)
+      const bool first = BITS8 || factor == 0.0f, down = !first && factor < 0.0f;
+      float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = BITS8 || SOME ? s[i >> 2][i & 3] * (BITS8 ? ks[i] : factor) : s[i >> 2][i & 3];
-      if constexpr (SOME) {
+      for (int i = 0; i < 8; ++i) x[i] = first ? s[i >> 2][i & 3] * (BITS8 ? ks[i] : factor) : s[i >> 2][i & 3];
+      if (__builtin_expect(some, 0)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, (seen[t] >> i) & 1u ? __builtin_fmaxf(x[i], -RX_LM_FLT_MAX) : -rx_lm_inf());
-      } else {
-        const bool down = !BITS8 && factor < 0.0f;
-        float far = x[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) far = down ? __builtin_fminf(far, x[i]) : __builtin_fmaxf(far, x[i]);
-        top = __builtin_fmaxf(BITS8 ? far : far * factor, -RX_LM_FLT_MAX);
+        for (int i = 0; i < 8; ++i) x[i] = (seen[t] >> i) & 1u ? x[i] : down ? rx_lm_inf() : -rx_lm_inf();
       }
-      top = __builtin_fmaxf(m[t], rx_lm_rows_max(top));
+      float far = x[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) far = down ? __builtin_fminf(far, x[i]) : __builtin_fmaxf(far, x[i]);
+      // (not below the lowest number, so that differences from it are numbers)
+      const float top = __builtin_fmaxf(m[t], rx_lm_rows_max(__builtin_fmaxf(first ? far : far * factor, -RX_LM_FLT_MAX)));
       if (__builtin_expect(__any(top != m[t]), 0)) {
-        const float shrink = top == m[t] ? 1.0f : __builtin_amdgcn_exp2f(m[t] - top);
+        const float shrink = __builtin_amdgcn_exp2f(m[t] - top);
         l[t] *= shrink;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -403,14 +403,11 @@ struct rx_lm_tree {
       const float base = SHIFT - top;
       float p[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(BITS8 || SOME ? x[i] + base : __builtin_fmaf(x[i], factor, base));
-        if (SOME) p[i] = (seen[t] >> i) & 1u ? p[i] : 0.0f;
-      }
+      for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(first ? x[i] + base : __builtin_fmaf(x[i], factor, base));
       l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
       if constexpr (BITS8) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = SOME && !((seen[t] >> i) & 1u) ? 0.0f : p[i] * vs[i];
+        for (int i = 0; i < 8; ++i) p[i] *= vs[i];
       }
       if constexpr (WIDE) {
 #pragma unroll
@@ -478,40 +475,88 @@ RX_DEV rx_f32x4 rx_lm_get_shared4(const __amdgpu_buffer_rsrc_t from, const unsig
 }
 RX_DEV __amdgpu_buffer_rsrc_t rx_lm_shared(float* base, const unsigned bytes) { return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000); }
 
-// Operands that the compiler takes for others from here on: what follows in one branch is not the other branch's, and is not moved before both.
-template <int N>
-RX_DEV void rx_lm_hold(rx_u32x4 (&f)[2][N]) {
-#pragma unroll
-  for (int k = 0; k < N; ++k) asm volatile("" : "+v"(f[0][k]), "+v"(f[1][k]));
+// Reads of LDS that other loads are on their way to.  The compiler has every read of its own wait for all loads into LDS, whichever place they
+// go to; these are of places that have arrived, and wait for nothing but themselves.
+RX_DEV rx_u32 rx_lm_lds(const void* p) { return (rx_u32)(unsigned long long)(RX_LDS const void*)p; }
+// four places, and the four OFF bytes further
+template <int OFF, int AT>
+RX_DEV void rx_lm_lds_eight(rx_u32x4 (&x)[4], rx_u32x4 (&y)[4], const rx_u32 (&a)[4]) {
+  asm volatile(
+      "ds_read_b128 %0, %8 offset:%12\n\tds_read_b128 %1, %9 offset:%12\n\tds_read_b128 %2, %10 offset:%12\n\tds_read_b128 %3, %11 offset:%12\n\t"
+      "ds_read_b128 %4, %8 offset:%13\n\tds_read_b128 %5, %9 offset:%13\n\tds_read_b128 %6, %10 offset:%13\n\tds_read_b128 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(AT), "n"(AT + OFF)
+      : "memory");
+}
+template <int OFF, int AT>
+RX_DEV void rx_lm_lds_eight(rx_u32x2 (&x)[4], rx_u32x2 (&y)[4], const rx_u32 (&a)[4]) {
+  asm volatile(
+      "ds_read_b64 %0, %8 offset:%12\n\tds_read_b64 %1, %9 offset:%12\n\tds_read_b64 %2, %10 offset:%12\n\tds_read_b64 %3, %11 offset:%12\n\t"
+      "ds_read_b64 %4, %8 offset:%13\n\tds_read_b64 %5, %9 offset:%13\n\tds_read_b64 %6, %10 offset:%13\n\tds_read_b64 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(AT), "n"(AT + OFF)
+      : "memory");
+}
+template <int OFF, int AT>
+RX_DEV void rx_lm_lds_eight(rx_u32 (&x)[4], rx_u32 (&y)[4], const rx_u32 (&a)[4]) {
+  asm volatile(
+      "ds_read_b32 %0, %8 offset:%12\n\tds_read_b32 %1, %9 offset:%12\n\tds_read_b32 %2, %10 offset:%12\n\tds_read_b32 %3, %11 offset:%12\n\t"
+      "ds_read_b32 %4, %8 offset:%13\n\tds_read_b32 %5, %9 offset:%13\n\tds_read_b32 %6, %10 offset:%13\n\tds_read_b32 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(AT), "n"(AT + OFF)
+      : "memory");
+}
+// two places, and the two OFF bytes further
+template <int OFF>
+RX_DEV void rx_lm_lds_four(rx_u32x4& x0, rx_u32x4& x1, rx_u32x4& y0, rx_u32x4& y1, const rx_u32 a0, const rx_u32 a1) {
+  asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %4 offset:%6\n\tds_read_b128 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(x0), "=&v"(x1), "=&v"(y0), "=&v"(y1)
+               : "v"(a0), "v"(a1), "n"(OFF)
+               : "memory");
+}
+RX_DEV void rx_lm_lds_words(int (&x)[4], const rx_u32 (&a)[4]) {
+  asm volatile("ds_read_b32 %0, %4\n\tds_read_b32 %1, %5\n\tds_read_b32 %2, %6\n\tds_read_b32 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+               : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3])
+               : "memory");
 }
 
 // MASK: 0 every drafted token sees itself and those before it, 2 [N, N] for all sequences, 3 [B, N, N].  NT: tiles of 16 rows to a
 // wavefront.  WR: wavefronts that have rows of their own: 1 (few rows) the four share the positions, and read the caches into their
-// registers; 4 (many rows) they share keys and values, which pass through LDS, 8-bit numbers as bf16, the next step's being loaded
-// while this one's are multiplied.  R, HW, ONCE, DIES, Q: as for rx_paged_attention.
-template <typename E, typename C, int N, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int MASK, int NT, int WR, int R, int HW, bool ONCE, bool DIES,
-          int Q, typename I>
+// registers; 4 (many rows) they share keys and values, which pass through LDS: with a RING of that many stages of 32 positions, loaded without
+// registers; without one (rows that are no whole 16 bytes) through registers, 8-bit numbers as bf16, the next step's being loaded while this
+// one's are multiplied.  R, HW, ONCE, DIES, Q: as for rx_paged_attention.
+template <typename E, typename C, int N, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int MASK, int NT, int WR, int RING, int R, int HW, bool ONCE,
+          bool DIES, int Q, typename I>
 RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, const typename C::S* vc, const I* pages, const I* lengths, const rx_u8* mask, const float* ks,
                               const float* vs, typename E::S* out, float* lse, float* part, float* stat, int* arrived, const float scale) {
   constexpr bool SHARED = WR > 1, BITS8 = rx_lm_is8<C>::value;
-  typedef rx_lm_tree<E, C, DK, DV, NT, BITS8 && !SHARED> A;
+  typedef rx_lm_tree<E, C, DK, DV, NT, BITS8 && (!SHARED || RING)> A;
   typedef typename A::F F;
   typedef typename C::S T;
   constexpr int G = HQ / HK, ROWS = N * G, TR = 16 * NT * WR, RT = ROWS < TR ? ROWS : TR, TILES = (ROWS + TR - 1) / TR, COLUMNS = HK / HW * TILES, WPH = 4 / HW;
   constexpr int KF = A::KF, VE = A::VE, NV = A::NV;
-  constexpr int BLOCK = 2048;                          // positions whose pages are held in LDS
+  constexpr int BLOCK = RING ? 1024 * (S < 256 ? S : 256) : 2048;   // positions whose pages are held in LDS
   constexpr int HR = RT < 16 ? RT : 16, WIDTH = 16 * VE < DV ? 16 * VE : DV;   // rows and dimensions that are joined at a time
   constexpr int VD = DV % 4 == 0 ? 4 : 1;
   constexpr int FE = 16 / sizeof(typename F::S), KP = KF * 4 * A::NE + FE, VP = NV * 16 * VE + FE;   // rows of keys and values in LDS: 16 bytes longer, for its banks
   typedef rx_vec<rx_u32, VE * sizeof(typename F::S) / 4> FV;   // a lane's part of a value
+  // A stage of the ring: 32 keys and 32 values in chunks of 16 bytes, as many to a row as the next power of two holds, chunk c of row i at
+  // place c ^ turn(i), so that sixteen rows' chunks lie on different banks.
+  constexpr int CE = 16 / sizeof(T), CK = (DK + CE - 1) / CE, CV = (DV + CE - 1) / CE, PK = rx_lm_pow2(CK) < 4 ? 4 : rx_lm_pow2(CK), PV = rx_lm_pow2(CV) < 4 ? 4 : rx_lm_pow2(CV);
+  constexpr int STAGE = 32 * 16 * (PK + PV);
+  constexpr int ROOM = SHARED ? 4 * 16 * (16 * VE + 4) * 4 : 16;   // for the results of four wavefronts' 16 rows
+  __shared__ __attribute__((aligned(1024))) rx_u8 ring[RING * STAGE > ROOM ? RING * STAGE : ROOM];
+  __shared__ int table[RING ? BLOCK / S + 2 : 1];
+  __shared__ float ring_s[RING ? RING : 1][64];
   __shared__ union {
     int page[SHARED ? 1 : BLOCK / S + 2];
     float o[SHARED ? 1 : 4][HR][WIDTH + 4];
     rx_lm_joined<VD> j[256];
   } lds;
   __shared__ float join_m[4][16], join_l[4][16];
-  __shared__ __attribute__((aligned(16))) typename F::S kt[SHARED ? 2 : 1][SHARED ? 32 : 1][SHARED ? KP : FE];
-  __shared__ __attribute__((aligned(16))) typename F::S vt[SHARED ? 2 : 1][SHARED ? 32 : 1][SHARED ? VP : FE];
+  __shared__ __attribute__((aligned(16))) typename F::S kt[SHARED && !RING ? 2 : 1][SHARED && !RING ? 32 : 1][SHARED && !RING ? KP : FE];
+  __shared__ __attribute__((aligned(16))) typename F::S vt[SHARED && !RING ? 2 : 1][SHARED && !RING ? 32 : 1][SHARED && !RING ? VP : FE];
   __shared__ float st_k[2][32], st_v[2][32];
   __shared__ unsigned st_ok[2];
   __shared__ int last, any;
@@ -524,7 +569,7 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
   auto result_of = [&](const int b, const int row, const int h) { return ((long long)b * N + row / G) * HQ + h * G + row % G; };   // row of the results
   const __amdgpu_buffer_rsrc_t parts_at = rx_lm_shared(part, (unsigned)R * COLUMNS * 2 * HW * RT * DV * 4);
   int buf = 0;
-  if constexpr (SHARED && (DK + FE - 1) / FE * FE < KF * 4 * A::NE) {          // what no chunk of a key covers
+  if constexpr (SHARED && !RING && (DK + FE - 1) / FE * FE < KF * 4 * A::NE) {          // what no chunk of a key covers
     for (int i = threadIdx.x; i < 64 * KP; i += 256) (&kt[0][0][0])[i] = F::down(0.0f);
     __syncthreads();
   }
@@ -576,18 +621,39 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
   auto seen_by = [&](const int t0, const unsigned ok, unsigned (&seen)[NT]) {
     int g = g4;
     rx_pin(g);
+    // (all of the mask's loads before the first of them is looked at: one under a condition waits for the one before)
+    rx_u8 drafted[NT][8];
+    if constexpr (MASK != 0) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = t0 + (i & 4) * 4 + g * 4 + (i & 3) - span.prefix;
+          drafted[t][i] = mask[((long long)(MASK == 3 ? b : 0) * N + token[t]) * N + (j < 0 ? 0 : j < N ? j : N - 1)];
+        }
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       seen[t] = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int at = (i & 4) * 4 + g * 4 + (i & 3);
-        seen[t] |= ((ok >> at) & 1u) && sees(token[t], first[t], t0 + at) ? 1u << i : 0u;
+        const int at = (i & 4) * 4 + g * 4 + (i & 3), p = t0 + at;
+        bool see = p >= first[t];
+        if constexpr (MASK == 0) see = p < span.prefix ? see : p - span.prefix <= token[t];
+        else see = p < span.prefix ? see : drafted[t][i] != 0;
+        seen[t] |= ((ok >> at) & 1u) && see ? 1u << i : 0u;
       }
     }
   };
-  rx_u32 special = 0;                                                         // infinities or NaN have been taken out of values
   auto differ = [&](const int t0) { return t0 >= mixed || (W > 0 && t0 < edge); };
+  rx_u32 special = 0;                                                         // infinities or NaN have been taken out of values
+  unsigned saw[NT] = {};                                                      // positions that the lane's rows have seen
+  bool all = false;                                                           // in a step that all rows see alike
+  auto look = [&](const int t0, const unsigned ok, unsigned (&seen)[NT]) {
+    seen_by(t0, ok, seen);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) saw[t] |= seen[t];
+  };
 
   if constexpr (!SHARED) {
     constexpr int KR = BITS8 ? (DK + 63) / 64 : KF;    // 16-byte loads of a key by its four lanes
@@ -680,27 +746,214 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
           return o;
         };
         unsigned seen[NT] = {};
-        if (__builtin_expect(ok == ~0u && !differ(t0), 1)) {
-          a.template step<false>(kf, [] {}, value, seen, scale, kscale, vscale);
-        } else {
-          rx_lm_hold(kf);
-          seen_by(t0, ok, seen);
+        const bool some = ok != ~0u || differ(t0);
+        if (__builtin_expect(some, 0)) {
+          look(t0, ok, seen);
+          if (differ(t0)) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-#pragma unroll
-              for (int n = 0; n < (int)(sizeof(CV) / 4); ++n) {
-                const rx_u32 x = differ(t0) ? rx_lm_special<C>(vf[j][i].v[n]) : 0u;
-                vf[j][i].v[n] &= ~x;
-                special |= x;
+            for (int i = 0; i < 8; ++i) {
+              if (BITS8 && !(__builtin_fabsf(vscale[i]) <= RX_LM_FLT_MAX)) {
+                special |= (there >> ((i & 4) * 4 + (i & 3))) & 1u;
+                vscale[i] = 0.0f;
               }
-          a.template step<true>(kf, [] {}, value, seen, scale, kscale, vscale);
+#pragma unroll
+              for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int n = 0; n < (int)(sizeof(CV) / 4); ++n) {
+                  const rx_u32 x = rx_lm_special<C>(vf[j][i].v[n]);
+                  vf[j][i].v[n] &= ~x;
+                  special |= x;
+                }
+            }
+          }
+          if constexpr (BITS8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) vscale[i] = (there >> ((i & 4) * 4 + (i & 3))) & 1u ? vscale[i] : 0.0f;
+          }
+        } else {
+          all = true;
         }
+        a.step(kf, [] {}, value, some, seen, scale, kscale, vscale);
       }
     }
+  } else if constexpr (RING > 0) {
+    // Keys and values pass through LDS without registers, RING - 1 steps ahead: the loads of a step are started when the step before
+    // last has been used, and waited for by count.
+    constexpr int PER = (PK + PV) / 8, COUNT = PER + (BITS8 ? 1 : 0), AHEAD = RING - 1;   // loads of a wavefront in a step
+    static_assert((PK + PV) % 8 == 0, "a step's loads are shared equally");
+    typedef rx_vec<rx_u32, VE * sizeof(T) / 4> CVEC;
+    constexpr int KR = BITS8 ? KF / 2 : KF;
+    auto turn = [](const int row, const int places) { return places >= 16 ? row & 15 : (row / (16 / places)) & (places - 1); };
+    const int key_turn = turn(r, PK);
+    for (int s0 = p0; s0 < p1; s0 += BLOCK) {
+      const int s1 = s0 + BLOCK < p1 ? s0 + BLOCK : p1, page0 = (rx_u32)s0 / S, npages = (rx_u32)(s1 - 1) / S - page0 + 1;
+      __syncthreads();
+      for (int i = threadIdx.x; i < npages; i += 256) {
+        const I page = pages[(long long)b * M + page0 + i];
+        table[i] = page >= 0 && page < P ? (int)page : -1;
+      }
+      __syncthreads();
+      // Pages of a step's rows: of the rows that the lane loads, and of position lane mod 32.  Positions that are not to be looked at have the table's
+      // first or last entry, and are told by `here`.
+      auto entry = [&](const int t) { return rx_lm_lds(table) + 4 * ((rx_u32)(t < s1 ? t : s1 - 1) / S - page0); };
+      auto here = [&](const int t, const int page) { return t >= span.lo && t < s1 && page >= 0; };
+      auto start = [&](const int t0, const int stage) {
+        constexpr int LOOK = PER + (BITS8 ? 1 : 0);
+        int page[(LOOK + 3) / 4 * 4];
+#pragma unroll
+        for (int n = 0; n < LOOK; n += 4) {
+          rx_u32 a[4];
+          int w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int at = (n + k) * 4 + wave, i = (at < PK / 2 ? at : at - PK / 2) * 64 + lane;
+            a[k] = n + k < PER ? entry(t0 + i / (at < PK / 2 ? PK : PV)) : entry(t0 + (lane & 31));
+          }
+          rx_lm_lds_words(w, a);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) page[n + k] = w[k];
+        }
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+          const int at = n * 4 + wave;                    // kilobyte of the stage: keys, then values
+          const bool key = at < PK / 2;
+          const int i = (key ? at : at - PK / 2) * 64 + lane, places = key ? PK : PV, row = i / places, c = (i % places) ^ turn(row, places);
+          const int chunk = c < (key ? CK : CV) ? c : (key ? CK : CV) - 1;
+          const rx_u32 slot = (rx_u32)(t0 + row) % S, p = page[n] < 0 ? 0 : page[n];
+          const T* from = key ? kc + rx_lm_at<S, HK, DK, BY_SLOT>(p, slot, head) + chunk * CE : vc + rx_lm_at<S, HK, DV, BY_SLOT>(p, slot, head) + chunk * CE;
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (RX_LDS void*)(ring + stage * STAGE + at * 1024), 16, 0, 0);
+        }
+        if constexpr (BITS8) {                            // (every wavefront the same, so that all count the same loads)
+          const float* from = (lane < 32 ? ks : vs) + rx_lm_slot<S, HK, 1, false>(page[PER] < 0 ? 0 : page[PER], (rx_u32)(t0 + (lane & 31)) % S, head);
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (RX_LDS void*)&ring_s[stage][0], 4, 0, 0);
+        }
+      };
+      int next = 0, now = 0;
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {
+        start(s0 + n * 32, next);
+        next = next + 1 == RING ? 0 : next + 1;
+      }
+      for (int t0 = s0; t0 < s1; t0 += 32) {
+        rx_wait_vmcnt<(AHEAD - 1) * COUNT>();
+        rx_lds_barrier();                                 // (and the stage that is loaded next has been read)
+        start(t0 + AHEAD * 32, next);                     // (past the end: slots that nothing reads)
+        const int stage = now;
+        next = next + 1 == RING ? 0 : next + 1;
+        now = now + 1 == RING ? 0 : now + 1;
+        const rx_u32 keys = rx_lm_lds(ring) + stage * STAGE + r * (PK * 16), values = rx_lm_lds(ring) + stage * STAGE + 512 * PK, scales = rx_lm_lds(ring_s) + stage * 256 + g4 * 16;
+        unsigned ok;
+        {
+          const rx_u32 a[4] = {entry(t0 + (lane & 31)), entry(t0), entry(t0), entry(t0)};
+          int w[4];
+          rx_lm_lds_words(w, a);
+          ok = (unsigned)__ballot(lane < 32 && here(t0 + lane, w[0]));
+        }
+        if (__builtin_expect(!ok, 0)) continue;
+        const bool some = ok != ~0u || differ(t0);
+        if (__builtin_expect(some, 0)) {
+          // What lies in other slots may be anything, and NaN times a weight of zero is not zero; the same of infinities and NaN in slots that some
+          // rows see, which are taken out here.
+          rx_u8* const tile_v = ring + stage * STAGE + 512 * PK;
+          for (int i = threadIdx.x; i < 32 * PV; i += 256) {
+            const int row = i / PV;
+            const bool exists = (ok >> row) & 1u, whole_row = ((i % PV) ^ turn(row, PV)) < CV;
+            rx_vec<rx_u32, 4> x = rx_load<rx_vec<rx_u32, 4>>(tile_v + i * 16);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const rx_u32 out_of = exists && differ(t0) ? rx_lm_special<C>(x.v[n]) : 0u;
+              x.v[n] &= exists ? ~out_of : 0u;
+              special |= whole_row ? out_of : 0u;
+            }
+            rx_store(tile_v + i * 16, x);
+          }
+          if (BITS8 && threadIdx.x < 32) {
+            const bool exists = (ok >> threadIdx.x) & 1u, finite = __builtin_fabsf(ring_s[stage][32 + threadIdx.x]) <= RX_LM_FLT_MAX;
+            if (!exists || (!finite && differ(t0))) ring_s[stage][32 + threadIdx.x] = 0.0f;
+            special |= exists && !finite && differ(t0) ? 1u : 0u;
+          }
+          rx_lds_barrier();
+        }
+        if (__builtin_expect(row0 >= ROWS, 0)) continue;
+        rx_u32x4 kf[2][KF];
+#pragma unroll
+        for (int k0 = 0; k0 < KR; k0 += 4) {
+          rx_u32x4 x[4], y[4];
+          rx_u32 a[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) a[k] = keys + (((k0 + k < KR ? k0 + k : KR - 1) * 4 + g4) ^ key_turn) * 16;
+          if constexpr (KR <= 2) rx_lm_lds_four<256 * PK>(x[0], x[1], y[0], y[1], a[0], a[1]);
+          else rx_lm_lds_eight<256 * PK, 0>(x, y, a);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (k0 + k >= KR) break;
+            if constexpr (BITS8) {
+              kf[0][2 * (k0 + k)] = rx_lm_eight_up<C>(x[k][0], x[k][1]);
+              kf[0][2 * (k0 + k) + 1] = rx_lm_eight_up<C>(x[k][2], x[k][3]);
+              kf[1][2 * (k0 + k)] = rx_lm_eight_up<C>(y[k][0], y[k][1]);
+              kf[1][2 * (k0 + k) + 1] = rx_lm_eight_up<C>(y[k][2], y[k][3]);
+            } else {
+              kf[0][k0 + k] = x[k];
+              kf[1][k0 + k] = y[k];
+            }
+          }
+        }
+        CVEC vf[NV][8];
+        float kscale[8] = {}, vscale[8] = {};
+        if constexpr (BITS8) {
+          rx_u32x4 x0, x1, y0, y1;
+          rx_lm_lds_four<128>(x0, x1, y0, y1, scales, scales + 64);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            kscale[i] = rx_u2f(x0[i]) * scale;
+            kscale[4 + i] = rx_u2f(x1[i]) * scale;
+            vscale[i] = rx_u2f(y0[i]);
+            vscale[4 + i] = rx_u2f(y1[i]);
+          }
+        }
+        // (not before the weights are done: keys and values in registers at once leave none for a second wavefront)
+        auto load_values = [&] {
+          typedef typename rx_lm_if<sizeof(CVEC) == 16, rx_u32x4, typename rx_lm_if<sizeof(CVEC) == 8, rx_u32x2, rx_u32>::type>::type X;
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            rx_u32 a[4];
+            X x[4], y[4];
+            const int byte = (j * 16 + r) * VE * (int)sizeof(T);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = values + (g4 * 4 + i) * (PV * 16) + (((byte / 16) & (PV - 1)) ^ turn(g4 * 4 + i, PV)) * 16 + byte % 16;
+            rx_lm_lds_eight<256 * PV, 0>(x, y, a);        // (rows 16 further have the same turn)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              vf[j][i] = __builtin_bit_cast(CVEC, x[i]);
+              vf[j][4 + i] = __builtin_bit_cast(CVEC, y[i]);
+            }
+          }
+        };
+        auto value = [&](const int j, const int e, const int half) {
+          rx_u32x4 o;
+          if constexpr (A::WIDE) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = vf[j][half * 4 + i].v[e];
+          } else if constexpr (BITS8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              o[k] = rx_lm_pair_up<C>(__builtin_amdgcn_perm(vf[j][2 * k + 1].v[e >> 2], vf[j][2 * k].v[e >> 2], e & 2 ? 0x07030602u : 0x05010400u), e & 1);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = __builtin_amdgcn_perm(vf[j][2 * k + 1].v[e >> 1], vf[j][2 * k].v[e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+          }
+          return o;
+        };
+        unsigned seen[NT] = {};
+        if (__builtin_expect(some, 0)) look(t0, ok, seen);
+        else all = true;
+        a.step(kf, load_values, value, some, seen, scale, kscale, vscale);
+      }
+      rx_wait_vmcnt<0>();
+    }
   } else {
-    constexpr int CE = 16 / sizeof(T), CK = (DK + CE - 1) / CE, CV = (DV + CE - 1) / CE, LK = (32 * CK + 255) / 256, LV = (32 * CV + 255) / 256;
+    constexpr int LK = (32 * CK + 255) / 256, LV = (32 * CV + 255) / 256;
     rx_vec<rx_u32, 4> rk[LK], rv[LV];
     I pk[LK], pv[LV], ps = 0;                           // page table's entries of the next step's loads; of position threadIdx.x
     float sk = 0.0f, sv = 0.0f;
@@ -811,18 +1064,25 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
         return o;
       };
       unsigned seen[NT] = {};
-      if (__builtin_expect(ok == ~0u && !differ(t0), 1)) {
-        a.template step<false>(kf, load_values, value, seen, scale, kscale, vscale);
-      } else {
-        rx_lm_hold(kf);
-        seen_by(t0, ok, seen);
-        a.template step<true>(kf, [&] {
-          load_values();
-          int g = g4;
-          rx_pin(g);
+      const bool some = ok != ~0u || differ(t0);
+      if (__builtin_expect(some, 0)) look(t0, ok, seen);
+      else all = true;
+      if constexpr (BITS8) {
+        if (__builtin_expect(some, 0)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (!(__builtin_fabsf(vscale[i]) <= RX_LM_FLT_MAX) && differ(t0)) {
+              special |= 1u;              // (those of slots that do not exist are zero already)
+              vscale[i] = 0.0f;
+            }
+        }
+      }
+      a.step(kf, [&] {
+        load_values();
+        if (__builtin_expect(some, 0)) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const bool exists = (ok >> ((i & 4) * 4 + g * 4 + (i & 3))) & 1u;
+            const bool exists = (ok >> ((i & 4) * 4 + g4 * 4 + (i & 3))) & 1u;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -834,10 +1094,18 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
                 special |= x;
               }
           }
-        }, value, seen, scale, kscale, vscale);
-      }
+        }
+      }, value, some, seen, scale, kscale, vscale);
     }
   }
+
+  // Rows that have seen nothing: no maximum, no sum.
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    if (!all && rx_lm_rows_max(saw[t] ? 1.0f : 0.0f) == 0.0f) {
+      a.m[t] = -rx_lm_inf();
+      a.l[t] = 0.0f;
+    }
   // (indices from here on are worked out here: what does not depend on the sequence would wait in registers through all of its steps)
   int tid = threadIdx.x;
   rx_pin(tid);
@@ -886,8 +1154,10 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
           }
           if (whole) {
             const long long at = result_of(b, tile * TR + row, head0 + hw);
+            rx_vec<typename E::S, VD> x;
 #pragma unroll
-            for (int e = 0; e < VD; ++e) out[at * DV + d + e] = E::down(hi == -rx_lm_inf() ? 0.0f : o[e] / sum);
+            for (int e = 0; e < VD; ++e) x.v[e] = E::down(hi == -rx_lm_inf() ? 0.0f : o[e] / sum);
+            rx_store(out + at * DV + d, x);
             if (lse && d == 0) lse[at] = hi == -rx_lm_inf() ? -rx_lm_inf() : (hi - A::SHIFT + __builtin_log2f(sum)) * 0.6931471805599453f;
           } else {
             const long long at = (((long long)id * 2 + (unit == 0)) * HW + hw) * RT + row;
@@ -899,34 +1169,43 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
       }
     }
   } else {
+    // Every wavefront's rows through its own part of LDS, so that a loop of a few instructions writes rows of consecutive words.
+    __syncthreads();
+    float* const o = (float*)ring + wave * (16 * (16 * VE + 4));
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const float sum = rx_lm_sum4(a.l[t]), hi = a.m[t];
-      if (row0 + t * 16 + er >= ROWS) continue;
-      const int row = row0 + t * 16 + er - tile * TR;
-      const long long at = whole ? result_of(b, tile * TR + row, head) : ((long long)id * 2 + (unit == 0)) * RT + row;
+      const float total = rx_lm_sum4(a.l[t]);
       if (eg == 0) {
-        if (!whole) rx_lm_put_shared((rx_u64*)stat + at, (rx_u64)rx_f2u(hi - A::SHIFT) | (rx_u64)rx_f2u(sum) << 32);
-        else if (lse) lse[at] = hi == -rx_lm_inf() ? -rx_lm_inf() : (hi - A::SHIFT + __builtin_log2f(sum)) * 0.6931471805599453f;
+        join_m[wave][er] = a.m[t];
+        join_l[wave][er] = total;
       }
-      const float f = hi == -rx_lm_inf() ? 0.0f : 1.0f / sum;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int e = 0; e < VE; e += VD) {
-            const int d = (j * 16 + eg * 4 + i) * VE + e;
-            if (d >= DV) continue;
-            if (whole) {
+          for (int e = 0; e < VE; e += 4)
+            rx_store(o + er * (16 * VE + 4) + (eg * 4 + i) * VE + e, rx_vec<float, 4>{{a.acc[t][j][e][i], a.acc[t][j][e + 1][i], a.acc[t][j][e + 2][i], a.acc[t][j][e + 3][i]}});
+        for (int k = tid & 63; k < 16 * (16 * VE / VD); k += 64) {
+          const int h = k / (16 * VE / VD), c = k % (16 * VE / VD) * VD, d = j * 16 * VE + c, row = row0 + t * 16 + h;
+          if (row >= ROWS || d >= DV) continue;
+          const rx_vec<float, VD> x = rx_load<rx_vec<float, VD>>(o + h * (16 * VE + 4) + c);
+          const float hi = join_m[wave][h], sum = join_l[wave][h];
+          if (whole) {
+            const long long at = result_of(b, row, head);
+            rx_vec<typename E::S, VD> y;
 #pragma unroll
-              for (int c = 0; c < VD; ++c) out[at * DV + d + c] = E::down(hi == -rx_lm_inf() ? 0.0f : a.acc[t][j][e + c][i] * f);
-            } else if constexpr (VD == 4) {
-              rx_lm_put_shared4(parts_at, (unsigned)(at * DV + d) * 4, rx_f32x4{a.acc[t][j][e][i], a.acc[t][j][e + 1][i], a.acc[t][j][e + 2][i], a.acc[t][j][e + 3][i]});
-            } else {
-              rx_lm_put_shared(part + at * DV + d, a.acc[t][j][e][i]);
-            }
+            for (int e = 0; e < VD; ++e) y.v[e] = E::down(hi == -rx_lm_inf() ? 0.0f : x.v[e] / sum);
+            rx_store(out + at * DV + d, y);
+            if (lse && d == 0) lse[at] = hi == -rx_lm_inf() ? -rx_lm_inf() : (hi - A::SHIFT + __builtin_log2f(sum)) * 0.6931471805599453f;
+          } else {
+            const long long at = ((long long)id * 2 + (unit == 0)) * RT + row - tile * TR;
+            if constexpr (VD == 4) rx_lm_put_shared4(parts_at, (unsigned)(at * DV + d) * 4, rx_f32x4{x.v[0], x.v[1], x.v[2], x.v[3]});
+            else rx_lm_put_shared(part + at * DV + d, x.v[0]);
+            if (d == 0) rx_lm_put_shared((rx_u64*)stat + at, (rx_u64)rx_f2u(hi - A::SHIFT) | (rx_u64)rx_f2u(sum) << 32);
           }
+        }
+      }
     }
   }
   // Infinities and NaN among the values of steps whose rows differ have been taken out (a weight of zero would make them NaN in rows that
@@ -943,7 +1222,9 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
         }
         if (p < span.lo || !sees(token, first, p)) continue;
         const I page = pages[(long long)b * M + p / S];
-        const float v = page >= 0 && page < P ? C::up(vc[rx_lm_slot<S, HK, DV, BY_SLOT>(page, p % S, head0 + hw) + d]) : 0.0f;
+        if (page < 0 || page >= P) continue;
+        float v = C::up(vc[rx_lm_slot<S, HK, DV, BY_SLOT>(page, p % S, head0 + hw) + d]);
+        if constexpr (BITS8) v *= vs[rx_lm_slot<S, HK, 1, false>(page, p % S, head0 + hw)];
         if (!(__builtin_fabsf(v) <= RX_LM_FLT_MAX)) more += v;
       }
       if (more == 0.0f) continue;
@@ -1018,8 +1299,10 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
       const int k = k1 + 256 * u, hw = k / (rows * (DV / VD)), h = k / (DV / VD) % rows, d = k % (DV / VD) * VD;
       if (k >= outs) break;
       const long long at = result_of(b, tile * TR + h, head0 + hw);
+      rx_vec<typename E::S, VD> x;
 #pragma unroll
-      for (int e = 0; e < VD; ++e) out[at * DV + d + e] = E::down(j[u].m == -rx_lm_inf() ? 0.0f : j[u].o[e] / j[u].s);
+      for (int e = 0; e < VD; ++e) x.v[e] = E::down(j[u].m == -rx_lm_inf() ? 0.0f : j[u].o[e] / j[u].s);
+      rx_store(out + at * DV + d, x);
       if (lse && d == 0) lse[at] = j[u].m == -rx_lm_inf() ? -rx_lm_inf() : (j[u].m + __builtin_log2f(j[u].s)) * 0.6931471805599453f;
     }
   }

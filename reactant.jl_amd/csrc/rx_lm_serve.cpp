@@ -292,6 +292,11 @@ OperatorPlan plan_move(const OperatorSpec& s) {
 
 // ------------------------------------------------------------------ attention of drafted tokens
 namespace {
+int64_t pow2(int64_t n) {
+  int64_t p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
 // which operand is the mask (0: none), and the first of the scales (0: none)
 int mask_of(const OperatorSpec& s) { return s.in.size() % 2 == 0 ? 5 : 0; }
 int scales_of(const OperatorSpec& s) { return s.in.size() >= 7 ? (int)s.in.size() - 2 : 0; }
@@ -351,17 +356,21 @@ OperatorPlan plan_tree(const OperatorSpec& s, bool lean) {
   const int64_t ve = wide || vc.dim <= 64 ? 4 : 8, nv = (vc.dim + 16 * ve - 1) / (16 * ve);
   // Up to 32 rows the wavefronts share the positions; more rows share keys and values through LDS, 64 or 128 to a workgroup.
   const bool shared = rows > 32;
-  const int64_t kf = !shared && q8 ? 2 * ((kc.dim + 63) / 64) : (kc.dim + 4 * fe - 1) / (4 * fe);
+  // rows of whole 16 bytes: keys and values pass through a ring of stages, as many as leave room for a second workgroup
+  const int64_t ce = 16 / e, places_k = std::max<int64_t>(4, pow2((kc.dim + ce - 1) / ce)), places_v = std::max<int64_t>(4, pow2((vc.dim + ce - 1) / ce)), stage = 512 * (places_k + places_v);
+  const bool rings = shared && kc.dim % ce == 0 && vc.dim % ce == 0 && (places_k + places_v) % 8 == 0 && !getenv("NORING");
+  const int64_t ring = !rings ? 0 : getenv("RINGN") ? atoi(getenv("RINGN")) : stage <= 16384 ? 4 : 2;
+  const int64_t kf = q8 && (!shared || rings) ? 2 * ((kc.dim + 63) / 64) : (kc.dim + 4 * fe - 1) / (4 * fe);
   // registers of a wavefront: a step's keys and values (and in many rows' case the next one's), the queries, the result, and room for the rest
   auto registers = [&](int64_t n) {
-    const int64_t staged = shared ? ((32 * kc.dim * e + 4095) / 4096 + (32 * vc.dim * e + 4095) / 4096) * 4 : 0;
+    const int64_t staged = shared && !rings ? ((32 * kc.dim * e + 4095) / 4096 + (32 * vc.dim * e + 4095) / 4096) * 4 : 0;
     return 8 * kf + 8 * nv * ve * size / 4 + staged + n * (4 * nq * kf + 4 * nv * ve + 24);
   };
   int64_t NT = 1;
   if (shared) NT = rows > 64 && registers(2) < 330 ? 2 : 1;
   else NT = rows > 16 && registers(2) < 320 ? 2 : 1;
   const int64_t WR = shared ? 4 : 1, TR = 16 * NT * WR, tiles = (rows + TR - 1) / TR, RT = std::min(rows, TR);
-  const int64_t lds = shared ? 2 * 32 * ((kf * 4 * fe + 16 / size) + (nv * 16 * ve + 16 / size)) * size : 0;
+  const int64_t lds = rings ? ring * stage + 4096 : shared ? 2 * 32 * ((kf * 4 * fe + 16 / size) + (nv * 16 * ve + 16 / size)) * size : 0;
   const int waves = registers(NT) <= (wide || shared ? 230 : 196) && lds <= 80000 ? 2 : 1;
   const int64_t longest = window ? std::min(M * kc.slots, window + N + 31) : M * kc.slots, units = std::max<int64_t>(1, (longest + 31) / 32);
   const int64_t HW = 1;
@@ -387,7 +396,7 @@ OperatorPlan plan_tree(const OperatorSpec& s, bool lean) {
   }
   std::ostringstream b;
   b << "rx_tree_attention<" << elem(in[0].dt) << ", " << stored(in[1].dt) << ", " << N << ", " << Hq << ", " << kc.heads << ", " << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << kc.slots << ", "
-    << B << ", " << M << ", " << window << ", " << (by_slot ? "true" : "false") << ", " << (mask ? in[mask].rank() : 0) << ", " << NT << ", " << WR << ", " << stretches << ", " << HW << ", "
+    << B << ", " << M << ", " << window << ", " << (by_slot ? "true" : "false") << ", " << (mask ? in[mask].rank() : 0) << ", " << NT << ", " << WR << ", " << ring << ", " << stretches << ", " << HW << ", "
     << (once ? "true" : "false") << ", " << (dies ? "true" : "false") << ", " << std::max<int64_t>(1, std::min<int64_t>(4, 4096 / (HW * RT * vc.dim))) << ">(a0, a1, a2, a3, a4, "
     << (mask ? a(mask) : "(rx_u8*)0") << ", " << (scales ? a(scales) + ", " + a(scales + 1) : "(float*)0, (float*)0") << ", " << a(o) << ", " << (lse ? a(o + 1) : "(float*)0") << ", " << shared_args
     << ", " << flt(scale * 1.4426950408889634) << ");";
