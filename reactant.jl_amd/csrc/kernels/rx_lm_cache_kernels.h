@@ -525,8 +525,8 @@ RX_DEV void rx_lm_lds_words(int (&x)[4], const rx_u32 (&a)[4]) {
 // wavefront.  WR: wavefronts that have rows of their own: 1 (few rows) the four share the positions, and read the caches into their
 // registers; 4 (many rows) they share keys and values, which pass through LDS: with a RING of that many stages of 32 positions, loaded without
 // registers; without one (rows that are no whole 16 bytes) through registers, 8-bit numbers as bf16, the next step's being loaded while this
-// one's are multiplied.  R, HW, ONCE, DIES, Q: as for rx_paged_attention.
-template <typename E, typename C, int N, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int MASK, int NT, int WR, int RING, int R, int HW, bool ONCE,
+// one's are multiplied.  R, ONCE, DIES, Q: as for rx_paged_attention.
+template <typename E, typename C, int N, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int W, bool BY_SLOT, int MASK, int NT, int WR, int RING, int R, bool ONCE,
           bool DIES, int Q, typename I>
 RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, const typename C::S* vc, const I* pages, const I* lengths, const rx_u8* mask, const float* ks,
                               const float* vs, typename E::S* out, float* lse, float* part, float* stat, int* arrived, const float scale) {
@@ -534,7 +534,7 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
   typedef rx_lm_tree<E, C, DK, DV, NT, BITS8 && (!SHARED || RING)> A;
   typedef typename A::F F;
   typedef typename C::S T;
-  constexpr int G = HQ / HK, ROWS = N * G, TR = 16 * NT * WR, RT = ROWS < TR ? ROWS : TR, TILES = (ROWS + TR - 1) / TR, COLUMNS = HK / HW * TILES, WPH = 4 / HW;
+  constexpr int G = HQ / HK, ROWS = N * G, TR = 16 * NT * WR, RT = ROWS < TR ? ROWS : TR, TILES = (ROWS + TR - 1) / TR, COLUMNS = HK * TILES;
   constexpr int KF = A::KF, VE = A::VE, NV = A::NV;
   constexpr int BLOCK = RING ? 1024 * (S < 256 ? S : 256) : 2048;   // positions whose pages are held in LDS
   constexpr int HR = RT < 16 ? RT : 16, WIDTH = 16 * VE < DV ? 16 * VE : DV;   // rows and dimensions that are joined at a time
@@ -562,12 +562,12 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
   __shared__ int last, any;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
   const int id = DIES ? (int)rx_xcd_remap(blockIdx.x, R * COLUMNS) : (int)blockIdx.x, column = id % COLUMNS, mine = id / COLUMNS, tile = column % TILES;
-  const int head0 = column / TILES * HW, head = head0 + (SHARED ? 0 : wave / WPH);
+  const int head = column / TILES;
   const int row0 = tile * TR + (SHARED ? wave * 16 * NT : 0);                 // first row of this wavefront
   const int rows = ROWS - tile * TR < TR ? ROWS - tile * TR : TR;             // of the workgroup
   const rx_lm_stretch st = rx_lm_stretch_of<B, R, Q>([&](const int at) { return rx_lm_tree_span_of<S, B, M, N, W>(lengths[at]).cost; }, mine);
   auto result_of = [&](const int b, const int row, const int h) { return ((long long)b * N + row / G) * HQ + h * G + row % G; };   // row of the results
-  const __amdgpu_buffer_rsrc_t parts_at = rx_lm_shared(part, (unsigned)R * COLUMNS * 2 * HW * RT * DV * 4);
+  const __amdgpu_buffer_rsrc_t parts_at = rx_lm_shared(part, (unsigned)R * COLUMNS * 2 * RT * DV * 4);
   int buf = 0;
   if constexpr (SHARED && !RING && (DK + FE - 1) / FE * FE < KF * 4 * A::NE) {          // what no chunk of a key covers
     for (int i = threadIdx.x; i < 64 * KP; i += 256) (&kt[0][0][0])[i] = F::down(0.0f);
@@ -669,7 +669,7 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
       __syncthreads();
       // page of a position, -1 where it is not to be looked at
       auto where = [&](const int t) { return t >= span.lo && t < s1 ? lds.page[(rx_u32)t / S - page0] : -1; };
-      for (int t0 = s0 + wave % WPH * 32; t0 < s1; t0 += WPH * 32) {
+      for (int t0 = s0 + wave * 32; t0 < s1; t0 += 128) {
         const int ta = t0 + r, tb = ta + 16, pa = where(ta), pb = where(tb);
         const unsigned ok = ((unsigned)__ballot(pa >= 0) & 0xffffu) | ((unsigned)__ballot(pb >= 0) << 16);
         if (!ok) continue;
@@ -1124,7 +1124,7 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
       __syncthreads();
       float top = -rx_lm_inf();
 #pragma unroll
-      for (int w = 0; w < WPH; ++w) top = __builtin_fmaxf(top, join_m[wave / WPH * WPH + w][er]);
+      for (int w = 0; w < 4; ++w) top = __builtin_fmaxf(top, join_m[w][er]);
       const float f = top == -rx_lm_inf() ? 0.0f : __builtin_amdgcn_exp2f(a.m[t] - top);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -1139,28 +1139,27 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
             }
         }
         __syncthreads();
-        for (int k = tid; k < HW * HR * (WIDTH / VD); k += 256) {
-          const int hw = k / (HR * (WIDTH / VD)), h = k / (WIDTH / VD) % HR, c = k % (WIDTH / VD) * VD, d = j * 16 * VE + c, row = t * 16 + h;
+        for (int k = tid; k < HR * (WIDTH / VD); k += 256) {
+          const int h = k / (WIDTH / VD), c = k % (WIDTH / VD) * VD, d = j * 16 * VE + c, row = t * 16 + h;
           if (row >= rows || d >= DV) continue;
           float o[VD] = {}, sum = 0.0f, hi = -rx_lm_inf();
 #pragma unroll
-          for (int i = 0; i < WPH; ++i) hi = __builtin_fmaxf(hi, join_m[hw * WPH + i][h]);
+          for (int w = 0; w < 4; ++w) hi = __builtin_fmaxf(hi, join_m[w][h]);
 #pragma unroll
-          for (int i = 0; i < WPH; ++i) {
-            const int w = hw * WPH + i;
+          for (int w = 0; w < 4; ++w) {
 #pragma unroll
             for (int e = 0; e < VD; ++e) o[e] += lds.o[w][h][c + e];
             sum += hi == -rx_lm_inf() ? 0.0f : join_l[w][h] * __builtin_amdgcn_exp2f(join_m[w][h] - hi);
           }
           if (whole) {
-            const long long at = result_of(b, tile * TR + row, head0 + hw);
+            const long long at = result_of(b, tile * TR + row, head);
             rx_vec<typename E::S, VD> x;
 #pragma unroll
             for (int e = 0; e < VD; ++e) x.v[e] = E::down(hi == -rx_lm_inf() ? 0.0f : o[e] / sum);
             rx_store(out + at * DV + d, x);
             if (lse && d == 0) lse[at] = hi == -rx_lm_inf() ? -rx_lm_inf() : (hi - A::SHIFT + __builtin_log2f(sum)) * 0.6931471805599453f;
           } else {
-            const long long at = (((long long)id * 2 + (unit == 0)) * HW + hw) * RT + row;
+            const long long at = ((long long)id * 2 + (unit == 0)) * RT + row;
             if constexpr (VD == 4) rx_lm_put_shared4(parts_at, (unsigned)(at * DV + d) * 4, rx_f32x4{o[0], o[1], o[2], o[3]});
             else rx_lm_put_shared(part + at * DV + d, o[0]);
             if (d == 0) rx_lm_put_shared((rx_u64*)stat + at, (rx_u64)rx_f2u(hi - A::SHIFT) | (rx_u64)rx_f2u(sum) << 32);
@@ -1212,8 +1211,8 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
   // do not see them): they are added to the results of the rows that do.
   if ((p1 > mixed || (W > 0 && p0 < edge)) && p0 < p1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's results
   if ((p1 > mixed || (W > 0 && p0 < edge)) && p0 < p1 && __builtin_expect(rx_block_any(special != 0, &any), 0)) {
-    for (int k = tid; k < HW * rows * DV; k += 256) {
-      const int hw = k / (rows * DV), row = k / DV % rows, d = k % DV, token = (tile * TR + row) / G, first = first_of(token);
+    for (int k = tid; k < rows * DV; k += 256) {
+      const int row = k / DV, d = k % DV, token = (tile * TR + row) / G, first = first_of(token);
       float more = 0.0f;
       for (int p = p0; p < p1; ++p) {
         if (!differ(p & ~31)) {
@@ -1223,16 +1222,16 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
         if (p < span.lo || !sees(token, first, p)) continue;
         const I page = pages[(long long)b * M + p / S];
         if (page < 0 || page >= P) continue;
-        float v = C::up(vc[rx_lm_slot<S, HK, DV, BY_SLOT>(page, p % S, head0 + hw) + d]);
-        if constexpr (BITS8) v *= vs[rx_lm_slot<S, HK, 1, false>(page, p % S, head0 + hw)];
+        float v = C::up(vc[rx_lm_slot<S, HK, DV, BY_SLOT>(page, p % S, head) + d]);
+        if constexpr (BITS8) v *= vs[rx_lm_slot<S, HK, 1, false>(page, p % S, head)];
         if (!(__builtin_fabsf(v) <= RX_LM_FLT_MAX)) more += v;
       }
       if (more == 0.0f) continue;
       if (whole) {
-        const long long at = result_of(b, tile * TR + row, head0 + hw) * DV + d;
+        const long long at = result_of(b, tile * TR + row, head) * DV + d;
         out[at] = E::down(E::up(out[at]) + more);
       } else {
-        const long long at = ((((long long)id * 2 + (unit == 0)) * HW + hw) * RT + row) * DV + d;
+        const long long at = (((long long)id * 2 + (unit == 0)) * RT + row) * DV + d;
         rx_lm_put_shared(part + at, rx_lm_get_shared(part + at) + more);
       }
     }
@@ -1242,8 +1241,8 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
   if (!rx_lm_last_to_arrive(arrived + b * COLUMNS + column, to - from + 1, &last)) continue;
   // VD outputs to a thread; where there are fewer than threads, the parts are shared too, and joined once more; where there are more,
   // a thread has up to four times VD, so that sixteen loads are on their way.
-  constexpr int MORE = HW * RT * (DV / VD) >= 1024 ? 4 : HW * RT * (DV / VD) >= 512 ? 2 : 1, AT = 16 / MORE;
-  const int outs = HW * rows * (DV / VD), ways = outs < 256 ? 256 / outs : 1, parts = to - from + 1;
+  constexpr int MORE = RT * (DV / VD) >= 1024 ? 4 : RT * (DV / VD) >= 512 ? 2 : 1, AT = 16 / MORE;
+  const int outs = rows * (DV / VD), ways = outs < 256 ? 256 / outs : 1, parts = to - from + 1;
   for (int k0 = 0; k0 < outs; k0 += 256 * MORE) {
     const int way = ways > 1 ? tid / outs : 0, k1 = ways > 1 ? tid % outs : k0 + tid;
     const bool on = k1 < outs && way < ways;
@@ -1255,11 +1254,11 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
       float pm[MORE][AT], psum[MORE][AT], po[MORE][AT][VD];
 #pragma unroll
       for (int u = 0; u < MORE; ++u) {
-        const int k = k1 + 256 * u < outs ? k1 + 256 * u : k1, hw = k / (rows * (DV / VD)), h = k / (DV / VD) % rows, d = k % (DV / VD) * VD;
+        const int k = k1 + 256 * u < outs ? k1 + 256 * u : k1, h = k / (DV / VD), d = k % (DV / VD) * VD;
 #pragma unroll
         for (int i = 0; i < AT; ++i) {
           const int v = w + i < w1 ? w + i : w1 - 1;
-          const long long at = (((long long)(v * COLUMNS + column) * 2 + (v == from)) * HW + hw) * RT + h;
+          const long long at = ((long long)(v * COLUMNS + column) * 2 + (v == from)) * RT + h;
           const rx_u64 both = rx_lm_get_shared((const rx_u64*)stat + at);
           pm[u][i] = rx_u2f((rx_u32)both);
           psum[u][i] = rx_u2f((rx_u32)(both >> 32));
@@ -1296,9 +1295,9 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
     if (!on || way) continue;
 #pragma unroll
     for (int u = 0; u < MORE; ++u) {
-      const int k = k1 + 256 * u, hw = k / (rows * (DV / VD)), h = k / (DV / VD) % rows, d = k % (DV / VD) * VD;
+      const int k = k1 + 256 * u, h = k / (DV / VD), d = k % (DV / VD) * VD;
       if (k >= outs) break;
-      const long long at = result_of(b, tile * TR + h, head0 + hw);
+      const long long at = result_of(b, tile * TR + h, head);
       rx_vec<typename E::S, VD> x;
 #pragma unroll
       for (int e = 0; e < VD; ++e) x.v[e] = E::down(j[u].m == -rx_lm_inf() ? 0.0f : j[u].o[e] / j[u].s);

@@ -354,12 +354,13 @@ OperatorPlan plan_tree(const OperatorSpec& s, bool lean) {
   const bool wide = !q8 && qe == 4;
   const int64_t fe = wide ? 4 : 8, size = wide ? 4 : 2, nq = !q8 ? 1 : qe == 4 ? 3 : in[0].dt == DT::F16 ? 2 : 1;
   const int64_t ve = wide || vc.dim <= 64 ? 4 : 8, nv = (vc.dim + 16 * ve - 1) / (16 * ve);
-  // Up to 32 rows the wavefronts share the positions; more rows share keys and values through LDS, 64 or 128 to a workgroup.
+  // Up to 32 rows the wavefronts share the positions; more rows share keys and values through LDS, 64 or 128 to a workgroup (64 rows as two tiles of 32
+  // that share positions: 218 us and more against 125, 512 as sixteen 555 against 380; 64 rows as half of 128: 178 against 125).
   const bool shared = rows > 32;
   // rows of whole 16 bytes: keys and values pass through a ring of stages, as many as leave room for a second workgroup
   const int64_t ce = 16 / e, places_k = std::max<int64_t>(4, pow2((kc.dim + ce - 1) / ce)), places_v = std::max<int64_t>(4, pow2((vc.dim + ce - 1) / ce)), stage = 512 * (places_k + places_v);
-  const bool rings = shared && kc.dim % ce == 0 && vc.dim % ce == 0 && (places_k + places_v) % 8 == 0 && !getenv("NORING");
-  const int64_t ring = !rings ? 0 : getenv("RINGN") ? atoi(getenv("RINGN")) : stage <= 16384 ? 4 : 2;
+  const bool rings = shared && kc.dim % ce == 0 && vc.dim % ce == 0 && (places_k + places_v) % 8 == 0;
+  const int64_t ring = !rings ? 0 : stage <= 16384 ? 4 : 2;   // (of 8 KB 3, 4 and 6: 120, 119 and 121 us for 64 sequences of 16 drafted tokens; of 16 KB 3 and 4: 383, 387)
   const int64_t kf = q8 && (!shared || rings) ? 2 * ((kc.dim + 63) / 64) : (kc.dim + 4 * fe - 1) / (4 * fe);
   // registers of a wavefront: a step's keys and values (and in many rows' case the next one's), the queries, the result, and room for the rest
   auto registers = [&](int64_t n) {
@@ -371,13 +372,14 @@ OperatorPlan plan_tree(const OperatorSpec& s, bool lean) {
   else NT = rows > 16 && registers(2) < 320 ? 2 : 1;
   const int64_t WR = shared ? 4 : 1, TR = 16 * NT * WR, tiles = (rows + TR - 1) / TR, RT = std::min(rows, TR);
   const int64_t lds = rings ? ring * stage + 4096 : shared ? 2 * 32 * ((kf * 4 * fe + 16 / size) + (nv * 16 * ve + 16 / size)) * size : 0;
-  const int waves = registers(NT) <= (wide || shared ? 230 : 196) && lds <= 80000 ? 2 : 1;
+  // Two wavefronts to a SIMD where the estimate allows it: 64 rows of 128 dimensions to a wavefront pair 610 us with one, 380 with two (16 sequences
+  // of 4001 positions, 64 heads); 32 rows of one sequence of 1000 positions, an estimate of 208, 18.6 and 17.8; four tiles of 16 rows to a wavefront, one to a SIMD, 614.
+  const int waves = registers(NT) <= (wide || shared ? 230 : 210) && lds <= 80000 ? 2 : 1;
   const int64_t longest = window ? std::min(M * kc.slots, window + N + 31) : M * kc.slots, units = std::max<int64_t>(1, (longest + 31) / 32);
-  const int64_t HW = 1;
   const bool once = kc.dim * e % 256 == 0 && vc.dim * e % 256 == 0 && tiles == 1, dies = (by_slot && kc.dim * e % 128 != 0) || tiles > 1;
-  const int64_t columns = kc.heads / HW * tiles, room = 256 * waves;
+  const int64_t columns = kc.heads * tiles, room = 256 * waves;
   // every workgroup a stretch of at least four units of 32 positions (a sequence counts four more), all of them on the chip at once
-  const int64_t part = 2 * HW * RT * (vc.dim * 4 + 8), most = lean ? std::min<int64_t>(room, kLeanBytes / part) : room;
+  const int64_t part = 2 * RT * (vc.dim * 4 + 8), most = lean ? std::min<int64_t>(room, kLeanBytes / part) : room;
   const int64_t stretches = std::max<int64_t>(1, std::min(most / columns, (B * (units + (B > 1 ? 4 : 0)) + 3) / 4)), grid = stretches * columns;
   std::vector<std::pair<OperatorArg, std::string>> args;
   for (int i = 0; i < (int)in.size(); ++i) args.push_back({operand(i), i == 1 || i == 2 ? cell(in[i]) : st(in[i])});
@@ -386,7 +388,7 @@ OperatorPlan plan_tree(const OperatorSpec& s, bool lean) {
   const int o = (int)in.size();
   std::string shared_args = "(float*)0, (float*)0, (int*)0";
   if (stretches > 1) {
-    p.scratch = {grid * 2 * HW * RT * vc.dim * 4, grid * 2 * HW * RT * 8};
+    p.scratch = {grid * 2 * RT * vc.dim * 4, grid * 2 * RT * 8};
     p.counters = B * columns;
     const int at = (int)args.size();
     args.push_back({scratch(0), "float"});
@@ -396,8 +398,8 @@ OperatorPlan plan_tree(const OperatorSpec& s, bool lean) {
   }
   std::ostringstream b;
   b << "rx_tree_attention<" << elem(in[0].dt) << ", " << stored(in[1].dt) << ", " << N << ", " << Hq << ", " << kc.heads << ", " << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << kc.slots << ", "
-    << B << ", " << M << ", " << window << ", " << (by_slot ? "true" : "false") << ", " << (mask ? in[mask].rank() : 0) << ", " << NT << ", " << WR << ", " << ring << ", " << stretches << ", " << HW << ", "
-    << (once ? "true" : "false") << ", " << (dies ? "true" : "false") << ", " << std::max<int64_t>(1, std::min<int64_t>(4, 4096 / (HW * RT * vc.dim))) << ">(a0, a1, a2, a3, a4, "
+    << B << ", " << M << ", " << window << ", " << (by_slot ? "true" : "false") << ", " << (mask ? in[mask].rank() : 0) << ", " << NT << ", " << WR << ", " << ring << ", " << stretches << ", "
+    << (once ? "true" : "false") << ", " << (dies ? "true" : "false") << ", " << std::max<int64_t>(1, std::min<int64_t>(4, 4096 / (RT * vc.dim))) << ">(a0, a1, a2, a3, a4, "
     << (mask ? a(mask) : "(rx_u8*)0") << ", " << (scales ? a(scales) + ", " + a(scales + 1) : "(float*)0, (float*)0") << ", " << a(o) << ", " << (lse ? a(o + 1) : "(float*)0") << ", " << shared_args
     << ", " << flt(scale * 1.4426950408889634) << ");";
   OperatorKernel k = kernel(s, "tree_attention", 256, args, (int)args.size() - o, b.str(), waves);
