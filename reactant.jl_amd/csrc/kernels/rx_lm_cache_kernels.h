@@ -717,6 +717,11 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
             }
           }
         }
+        // (the mask's loads start behind those of keys and values, before any of them is waited for)
+        unsigned seen[NT] = {};
+        const bool some = ok != ~0u || differ(t0);
+        if (__builtin_expect(some, 0)) look(t0, ok, seen);
+        else all = true;
         const unsigned there = (ok >> (g4 * 4)) & 0x000f000fu;   // bit i: position 4 g4 + i, bit 16 + i: 16 further
         if (ok != ~0u) {
           // what lies in other slots may be anything, and NaN times a weight of zero is not zero
@@ -750,10 +755,7 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
           }
           return o;
         };
-        unsigned seen[NT] = {};
-        const bool some = ok != ~0u || differ(t0);
         if (__builtin_expect(some, 0)) {
-          look(t0, ok, seen);
           if (differ(t0)) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -775,8 +777,6 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
 #pragma unroll
             for (int i = 0; i < 8; ++i) vscale[i] = (there >> ((i & 4) * 4 + (i & 3))) & 1u ? vscale[i] : 0.0f;
           }
-        } else {
-          all = true;
         }
         a.step(kf, [] {}, value, some, seen, scale, kscale, vscale);
       }

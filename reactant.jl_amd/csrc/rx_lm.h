@@ -37,7 +37,7 @@
 //       dimensions is turned by row angle[a, t] of the tables, a the section that i lies in.  `sections` names the pairs of each of the A <= 4
 //       axes ("16,24,24": time, height, width), in order; all R / 2 follow the one axis without it.  Caches of the type of k, or of 8 bits
 //       with scales.  A token whose position is outside [0, M S), whose sequence is outside [0, B) or of whose rows one is outside [0, L)
-//       (where it is turned) is padding: as for rx.kv_append.
+//       (where it is turned) is padding: as for rx.kv_append.  No two tokens may name one slot.
 //   rx.kv_move(lengths [B], path [B, A], pages [B, M], k_cache, v_cache [, k_scale, v_scale]) {layout} -> (k_cache', v_cache' [, k_scale', v_scale'])
 //       Position lengths[b] + i of sequence b takes what position lengths[b] + path[b, i] held before the call: an accepted branch
 //       moves together.  Not moved: where path[b, i] is negative, or either position is outside [0, M S) or on a page outside the cache.  A <= 64;

@@ -542,6 +542,53 @@ def test_cache_of_more_than_2_to_the_31_numbers(rx, client):
     T.close(got[0].to_array().T, ref, bound + attention_bound([last, I.Tensor(kc, "f32")], [I.Tensor(ks, "f32")], d ** -0.5, mag, "bf16", "f8E4M3FN", n)[0], "bf16")
 
 
+def test_scores_of_a_factor_of_zero(rx, client):
+    """All weights alike: the mean of the values that a token sees, masked ones left out."""
+    rng = np.random.default_rng(14)
+    for n, cache in ((3, "bf16"), (40, "bf16"), (3, "i8"), (40, "f8E4M3FN")):
+        args, scales = attention_case(rng, [70, 0], n, 4, 2, 64, 64, 16, 8, "bf16", cache, "slots")
+        check_tree(rx, client, args, scales, tree(rng, 2, n), n, 4, 2, 64, 64, 16, 8, "bf16", cache, "slots", 0, scale=0.0)
+
+
+def test_norms_of_other_ranks(rx, client):
+    """Rows in several dimensions, and one row alone."""
+    rng = np.random.default_rng(15)
+    text = P.rms_norm(6, 40, dt="f32", out="i8")
+    x, res, w = (T.rounded(rng.normal(size=s), "f32") for s in ((6, 40), (6, 40), 40))
+    flat = [g.a for g in gpu_run(rx, client, text, [x, res, w])[0]]
+    deep = text.replace("tensor<6x40x", "tensor<2x3x40x").replace("tensor<6xf32>", "tensor<2x3xf32>")
+    got = [g.a for g in gpu_run(rx, client, deep, [I.Tensor(x.a.reshape(2, 3, 40), "f32"), I.Tensor(res.a.reshape(2, 3, 40), "f32"), w])[0]]
+    assert [g.shape for g in got] == [(2, 3, 40), (2, 3, 40), (2, 3)] and all(np.array_equal(g.reshape(f.shape), f) for g, f in zip(got, flat))
+    one = text.replace("tensor<6x40x", "tensor<40x").replace("tensor<6xf32>", "tensor<f32>")
+    got = [g.a for g in gpu_run(rx, client, one, [I.Tensor(x.a[2], "f32"), I.Tensor(res.a[2], "f32"), w])[0]]
+    assert got[2].shape == () and np.array_equal(got[1], flat[1][2]) and got[2] == flat[2][2]
+    grad = P.rms_norm_grad(6, 40, dt="f32")
+    args = [x, w, res, res]
+    dx, dw = (g.a for g in gpu_run(rx, client, grad, args)[0])
+    deep = [I.Tensor(a.a.reshape(3, 2, 40), "f32") if a.a.ndim == 2 else a for a in args]
+    got = [g.a for g in gpu_run(rx, client, grad.replace("tensor<6x40x", "tensor<3x2x40x"), deep)[0]]
+    assert np.array_equal(got[0].reshape(6, 40), dx) and np.array_equal(got[1], dw)
+
+
+def test_one_array_given_twice(rx, client):
+    """The same array as both caches, and as both scales: every result is its own."""
+    rng = np.random.default_rng(16)
+    args = write_case(rng, 9, 2, 4, 2, 24, 24, 8, 4, 3, 12, 24, 1, "f32", "i8", "slots", "i32")
+    args[10], args[12] = args[9], args[11]
+    thunk = rx.compile(P.kv_write(9, 2, 4, 2, 24, 8, 4, 3, 12, dt="f32", cache="i8"))
+    dev = [rx.to_rarray(t.a.T, t.dt) for t in args[:9]]
+    cache, scale = rx.to_rarray(args[9].a.T, "i8"), rx.to_rarray(args[11].a.T, "f32")
+    out = thunk(*dev, cache, cache, scale, scale, donated=[False] * 9 + [True] * 4)
+    check_write([o.to_array().T for o in out], args, np.zeros(12, int), "f32", "i8", "halves", "slots")
+
+
+def test_moves_without_pages(rx, client):
+    for pages, cols in ((0, 3), (2, 0)):
+        c = I.Tensor(np.arange(pages * 8.0).reshape(pages, 4, 1, 2), "f32")
+        got, _ = gpu_run(rx, client, P.kv_move(2, 3, 1, 2, pages, 4, cols, cache="f32"), [I.Tensor([1, 0], "i32"), I.Tensor([[2, 1, 0]] * 2, "i32"), I.Tensor(np.zeros((2, cols)), "i32"), c, c])
+        assert all(np.array_equal(g.a, c.a) for g in got)
+
+
 # ----------------------------------------------------------------------------
 # together
 # ----------------------------------------------------------------------------
