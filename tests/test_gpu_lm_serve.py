@@ -373,6 +373,9 @@ TREES = [
     ([3000], 34, 8, 4, 64, 64, 16, 200, "bf16", "i8", "heads", 64, "i32", "tree"), ([100, 41, 900], 16, 12, 4, 128, 40, 48, 30, "f32", "f8E4M3FN", "heads", 0, "i32", "tree"),
     ([20] * 40, 37, 1, 1, 20, 20, 8, 8, "f32", "i8", "slots", 0, "i32", "none"), ([500, 100], 200, 2, 1, 64, 64, 32, 24, "bf16", "bf16", "slots", 0, "i32", "none"), ([64], 300, 1, 1, 100, 100, 12, 40, "f16", "f8E4M3FN", "heads", 301, "i32", "shared"),
     ([12000, 4], 40, 2, 2, 64, 64, 16, 760, "bf16", "f8E4M3FN", "heads", 0, "i32", "tree"),
+    # the largest stages in LDS, and rows of no whole 16 bytes
+    ([90, 3], 40, 2, 1, 256, 256, 16, 10, "f32", "f32", "heads", 0, "i32", "tree"), ([77], 70, 2, 1, 255, 250, 16, 10, "f32", "f32", "slots", 0, "i32", "none"),
+    ([60, 200], 36, 2, 2, 256, 256, 8, 30, "f16", "f16", "slots", 0, "i32", "tree"), ([50], 33, 3, 1, 250, 255, 16, 6, "f32", "i8", "heads", 40, "i32", "none"),
 ]
 
 
