@@ -892,6 +892,8 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             if (k0 + k >= KR) break;
+            // (places past a key's end hold its last chunk again, and an infinity there times a query's zero is NaN; 8 bits have no infinity)
+            if (!BITS8 && CK % 4 != 0 && k0 + k == KR - 1 && g4 >= CK % 4) x[k] = y[k] = rx_u32x4{0, 0, 0, 0};
             if constexpr (BITS8) {
               kf[0][2 * (k0 + k)] = rx_lm_eight_up<C>(x[k][0], x[k][1]);
               kf[0][2 * (k0 + k) + 1] = rx_lm_eight_up<C>(x[k][2], x[k][3]);

@@ -420,6 +420,33 @@ def test_special_values_that_a_token_does_not_see(rx, client, n, hq, dt, cache):
     assert not scales or not np.isfinite(out[:, 5]).any()
 
 
+@pytest.mark.parametrize("n", [3, 20])
+@pytest.mark.parametrize("d,dt,scale", [(80, "bf16", None), (72, "f16", 0.2), (40, "bf16", -0.1), (100, "f32", None), (20, "f32", -0.3), (33, "f16", None)])
+def test_infinite_keys_have_no_weight(rx, client, n, d, dt, scale):
+    """Infinities in a key's last dimensions that make its scores -inf, among the positions before the drafted tokens and among those:
+    weights of zero.  Heads whose keys are no whole fragments."""
+    rng = np.random.default_rng(d + n)
+    hq, hk, size, cols, lengths = 4, 2, 16, 8, [70, 0, 33]
+    args, scales = attention_case(rng, lengths, n, hq, hk, d, d, size, cols, dt, dt, "slots")
+    last = 4 if dt == "f32" else 8                                          # dimensions of 16 bytes
+    args[0].a[..., -last:] = np.abs(args[0].a[..., -last:]) + 0.5           # one sign for every query
+    args[0] = T.rounded(args[0].a, dt)
+    mask = tree(rng, 3, n)
+    finite = [I.Tensor(np.array(a.a), a.dt) for a in args]
+    table = args[3].a
+    for s, j, dim in ((0, 5, d - 1), (0, 50, d - last), (0, 71, d - 2), (1, 1, d - 1), (2, 20, d - 3), (2, 34, d - 1)):
+        args[1].a[table[s, j // size], j % size, :, dim] = np.inf if scale is not None and scale < 0 else -np.inf
+    text = P.tree_attention(3, n, hq, hk, d, args[1].shape[0], size, cols, dt=dt, mask=True, lse=True, scale=scale)
+    got, _ = gpu_run(rx, client, text, args + [I.Tensor(mask, "i1")])
+    with np.errstate(invalid="ignore"):
+        out, lse, mag = L.tree_attention(*(t.a for t in args), mask, scale=scale)
+    assert np.isfinite(out[0]).all() and np.isfinite(out[2]).all()
+    lse[np.isnan(lse)] = -np.inf                                            # a token of the second sequence may see that key alone
+    bound, lse_bound = attention_bound(finite, scales, d ** -0.5 if scale is None else abs(scale), mag, dt, dt, cols * size)
+    T.close(got[0].a, out, bound, dt)
+    T.close(got[1].a, lse, lse_bound)
+
+
 def test_scores_far_apart_and_pages_that_do_not_exist(rx, client):
     rng = np.random.default_rng(8)
     for n in (5, 20):
