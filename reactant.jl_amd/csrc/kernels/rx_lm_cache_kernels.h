@@ -325,6 +325,7 @@ struct rx_lm_tree {
   static constexpr float SHIFT = !WIDE && !F::BF16 ? 15.0f : 0.0f;   // f16 weights are taken times 2^15: the smallest would be lost below 2^-24
   rx_u32x4 q[NT][NQ][KF];
   float m[NT], l[NT];
+  bool careful[NT];                                                                                 // a row's maximum is beyond 2^20, or the factor zero
   rx_f32x4 acc[NT][NV][VE];
 
   RX_MEM void clear() {
@@ -332,6 +333,7 @@ struct rx_lm_tree {
     for (int t = 0; t < NT; ++t) {
       m[t] = -rx_lm_inf();
       l[t] = 0.0f;
+      careful[t] = false;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -382,11 +384,10 @@ struct rx_lm_tree {
           s[1] = rx_lm_mma<F>(kf[1][k], q[t][n][k], s[1]);
         }
       // Where all positions have one factor the largest score is that of the products, times it, and weights take one operation more.
-      // (A factor of zero is multiplied first: masked scores are infinite.)
-      const bool first = BITS8 || factor == 0.0f, down = !first && factor < 0.0f;
+      const bool down = !BITS8 && factor < 0.0f;
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = first ? s[i >> 2][i & 3] * (BITS8 ? ks[i] : factor) : s[i >> 2][i & 3];
+      for (int i = 0; i < 8; ++i) x[i] = BITS8 ? s[i >> 2][i & 3] * ks[i] : s[i >> 2][i & 3];
       if (__builtin_expect(some, 0)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = (seen[t] >> i) & 1u ? x[i] : down ? rx_lm_inf() : -rx_lm_inf();
@@ -395,7 +396,7 @@ struct rx_lm_tree {
 #pragma unroll
       for (int i = 1; i < 8; ++i) far = down ? __builtin_fminf(far, x[i]) : __builtin_fmaxf(far, x[i]);
       // (not below the lowest number, so that differences from it are numbers)
-      const float top = __builtin_fmaxf(m[t], rx_lm_rows_max(__builtin_fmaxf(first ? far : far * factor, -RX_LM_FLT_MAX)));
+      const float top = __builtin_fmaxf(m[t], rx_lm_rows_max(__builtin_fmaxf(BITS8 ? far : far * factor, -RX_LM_FLT_MAX)));
       if (__builtin_expect(__any(top != m[t]), 0)) {
         const float shrink = __builtin_amdgcn_exp2f(m[t] - top);
         l[t] *= shrink;
@@ -404,11 +405,21 @@ struct rx_lm_tree {
 #pragma unroll
           for (int e = 0; e < VE; ++e) acc[t][j][e] *= shrink;
         m[t] = top;
+        careful[t] = !BITS8 && (factor == 0.0f || __any(__builtin_fabsf(top) >= 0x1p20f));
       }
-      const float base = SHIFT - top;
+      // One operation to a weight's exponent, whose error, the roundings of `top` and `base`, is below 2^-3 up to a maximum of 2^20.  Beyond, where
+      // weights would grow without bound, differences are taken from the rounded products, of which the maximum is one; with a factor of zero
+      // too, whose product with a masked score would be no number.  (The branch is 1 % of the time of 64 tokens of 64 heads.)
+      float base = SHIFT - top, times = factor;
+      if (!BITS8 && __builtin_expect(careful[t], 0)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = !some || ((seen[t] >> i) & 1u) ? x[i] * factor - top + SHIFT : -rx_lm_inf();
+        base = 0.0f;
+        times = 1.0f;
+      }
       float p[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(first ? x[i] + base : __builtin_fmaf(x[i], factor, base));
+      for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(BITS8 ? x[i] + base : __builtin_fmaf(x[i], times, base));
       l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
       if constexpr (BITS8) {
 #pragma unroll

@@ -447,6 +447,36 @@ def test_infinite_keys_have_no_weight(rx, client, n, d, dt, scale):
     T.close(got[1].a, lse, lse_bound)
 
 
+@pytest.mark.parametrize("n", [2, 20])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dt,cache,power", [("f16", "f16", 18), ("f16", "f16", 20), ("f16", "f16", 21), ("f16", "f16", 24), ("f16", "f16", 25), ("f16", "f16", 26), ("f16", "f16", 27), ("f16", "f16", 100),
+                                            ("bf16", "bf16", 21), ("bf16", "bf16", 33), ("bf16", "bf16", 40), ("f32", "f32", 33), ("f32", "f32", 100), ("bf16", "i8", 25), ("f16", "f8E4M3FN", 40)])
+def test_large_finite_scores(rx, client, n, sign, dt, cache, power):
+    """Scores of about 2^power (their logarithms to base 2): the largest of them has all of the weight, or shares it with its equals.
+    One dimension, of whole numbers, so that products are exact; others are further from the largest than f32 rounds it.  The sum of
+    exponentials is then their number, and lse is off by five roundings before its own: the factor's, its product's, those of the shift
+    of f16 weights and of the sum's logarithm, which are added to it, and that of ln 2."""
+    rng = np.random.default_rng(power + n)
+    hq, hk, d, size, cols, lengths = 4, 2, 64, 16, 160, [2500, 40, 3]
+    args, scales = attention_case(rng, lengths, n, hq, hk, d, d, size, cols, dt, cache, "slots")
+    bits = {"f16": 11, "f32": 11, "bf16": 8, "i8": 7, "f8E4M3FN": 4}
+    for t, b in ((args[0], bits[dt]), (args[1], bits[cache])):
+        t.a[...] = 0
+        t.a[..., 9] = rng.integers(2 ** (b - 1), 2 ** b, size=t.a.shape[:-1])
+    args[0].a[..., 9] *= rng.choice([-1, 1], size=args[0].shape[:-1])
+    for t in scales[:1]:
+        t.a[...] = 1
+    scale = sign * 1.3 * 2.0 ** (power + 1 - bits[dt] - bits[cache])       # (products with it are rounded)
+    mask = tree(rng, 3, n)
+    text = P.tree_attention(3, n, hq, hk, d, args[1].shape[0], size, cols, dt=dt, cache=cache, mask=True, lse=True, scale=scale)
+    got, exe = gpu_run(rx, client, text, args + [I.Tensor(mask, "i1")] + scales)
+    out, lse, mag = L.tree_attention(*(t.a for t in args), mask, *(scales and [t.a for t in scales] or [None, None]), scale=scale)
+    split = 0 if dt == "f32" and not scales else 2.0 ** -22 if dt == "f16" and not scales else 2.0 ** -16
+    T.close(got[0].a, out, mag * (2 * split + (cols * size + 17) * UF), dt)
+    with np.errstate(invalid="ignore"):
+        T.close(got[1].a, lse, 5 * UF * np.abs(lse) + (cols * size + 16) * 2 * UF)
+
+
 def test_scores_far_apart_and_pages_that_do_not_exist(rx, client):
     rng = np.random.default_rng(8)
     for n in (5, 20):
