@@ -310,7 +310,7 @@ RX_DEV rx_u64 rx_lm_at(const rx_u32 page, const rx_u32 slot, const rx_u32 head) 
 
 // What the rows of a wavefront have seen: maxima, sums, unscaled results, for NT tiles of 16 rows.
 // E: of the queries and the result, C: of the caches, F: of the products.  Caches of 8 bits are multiplied as bf16, which holds their numbers
-// exactly; queries of more digits than bf16's go in as a sum of up to three bf16 (f16: two hold it exactly, f32: three leave 2^-24).
+// exactly; queries of more digits than bf16's go in as a sum of bf16, which holds them exactly too (f16: two, f32: three).
 // KF: fragments of a key (16 bytes of its dimensions to each of four lanes), PERMUTED: in the order that 16 bytes of 8-bit numbers give.
 template <typename E, typename C, int DK, int DV, int NT, bool PERMUTED>
 struct rx_lm_tree {
@@ -346,7 +346,7 @@ struct rx_lm_tree {
     const int g4 = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int k = 0; k < KF; ++k) {
-      if constexpr (!BITS8) {
+      if constexpr (NQ == 1) {
         q[t][0][k] = there ? rx_lm_row16<E, DK>(row, dim(k, g4)) : rx_u32x4{0, 0, 0, 0};
       } else {
         rx_vec<rx_u16, 8> part[NQ];
@@ -356,7 +356,8 @@ struct rx_lm_tree {
           const bool finite = __builtin_fabsf(x) <= RX_LM_FLT_MAX;
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {
-            part[n].v[e] = rx_f32_to_bf16(x);
+            // (digits cut off, not rounded: 8 and 8 and 8 are all that f32 has, and neither a part nor a sum of them exceeds the number)
+            part[n].v[e] = finite ? (rx_u16)(rx_f2u(x) >> 16) : rx_f32_to_bf16(x);
             x = finite ? x - rx_bf16_to_f32(part[n].v[e]) : 0.0f;
           }
         }

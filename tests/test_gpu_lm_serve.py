@@ -477,6 +477,21 @@ def test_large_finite_scores(rx, client, n, sign, dt, cache, power):
         T.close(got[1].a, lse, 5 * UF * np.abs(lse) + (cols * size + 16) * 2 * UF)
 
 
+@pytest.mark.parametrize("n", [2, 20])
+def test_queries_beyond_the_largest_of_bf16(rx, client, n):
+    """Queries in f32 up to its largest number over caches of 8 bits: their parts in bf16 are finite, and scores with small scales of keys ordinary."""
+    rng = np.random.default_rng(n)
+    hq, hk, d, size, cols = 4, 2, 64, 16, 8
+    args, scales = attention_case(rng, [70, 3, 0], n, hq, hk, d, d, size, cols, "f32", "f8E4M3FN", "slots")
+    args[0].a[...] = 0
+    args[0].a[..., 40] = rng.choice([-1, 1], size=args[0].shape[:-1]) * np.where(rng.random(args[0].shape[:-1]) < 0.5, np.float64(np.finfo(np.float32).max), 3.395e38)
+    args[0] = T.rounded(args[0].a, "f32")
+    args[1].a[...] = LF.round_e4m3fn(rng.uniform(-1, 1, size=args[1].shape).astype(np.float32))    # (no product beyond f32)
+    scales[0].a[...] = 2.0 ** -123
+    mask = tree(rng, 3, n)
+    check_tree(rx, client, args, scales, mask, n, hq, hk, d, d, size, cols, "f32", "f8E4M3FN", "slots", 0, scale=0.5)
+
+
 def test_scores_far_apart_and_pages_that_do_not_exist(rx, client):
     rng = np.random.default_rng(8)
     for n in (5, 20):
