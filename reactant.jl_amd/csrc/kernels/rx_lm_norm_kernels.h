@@ -51,16 +51,25 @@ struct rx_lm_umax {
 };
 
 // Sum or maximum over the lanes of a row: a wavefront, or a workgroup, whose exchange alternates between two places so that
-// one barrier is enough.
+// one barrier is enough.  The wavefronts' values are joined two by two: at most 6 + 4 roundings of a sum behind a lane's own.
+template <int WAVES, typename T, typename OP>
+RX_DEV T rx_lm_join_waves(const T (&v)[WAVES], OP op) {
+  T x[WAVES];
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) x[w] = v[w];
+#pragma unroll
+  for (int n = WAVES / 2; n > 0; n /= 2)
+#pragma unroll
+    for (int w = 0; w < n; ++w) x[w] = op(x[w], x[w + n]);
+  return x[0];
+}
 template <int LANES, typename T, typename OP>
 RX_DEV T rx_lm_row_reduce(T v, OP op, T (*red)[LANES / 64], const int turn) {
   v = rx_wave_reduce(v, op);
   if constexpr (LANES > 64) {
     if ((threadIdx.x & 63) == 0) red[turn & 1][threadIdx.x >> 6] = v;
     __syncthreads();
-    v = red[turn & 1][0];
-#pragma unroll
-    for (int w = 1; w < LANES / 64; ++w) v = op(v, red[turn & 1][w]);
+    v = rx_lm_join_waves(red[turn & 1], op);
   }
   return v;
 }
@@ -176,12 +185,7 @@ RX_DEV void rx_rms_norm_grad(const typename E::S* h, const typename E::S* weight
     if constexpr (LANES > 64) {
       if ((threadIdx.x & 63) == 0) sums[turn & 1][threadIdx.x >> 6] = s;
       __syncthreads();
-      s = sums[turn & 1][0];
-#pragma unroll
-      for (int k = 1; k < LANES / 64; ++k) {
-        s.v[0] += sums[turn & 1][k].v[0];
-        s.v[1] += sums[turn & 1][k].v[1];
-      }
+      s = rx_lm_join_waves(sums[turn & 1], [](const rx_vec<float, 2>& a, const rx_vec<float, 2>& b) { return rx_vec<float, 2>{{a.v[0] + b.v[0], a.v[1] + b.v[1]}}; });
     }
     const float r = rx_rsqrt(s.v[0] / (float)D + eps), m = s.v[1] * r / (float)D;
 #pragma unroll

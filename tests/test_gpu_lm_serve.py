@@ -100,6 +100,19 @@ def test_norm_of_special_values(rx, client):
     assert np.all(y == 0) and np.all(scale[3:] == np.float32(2.0 ** -100) / np.float32(127))
 
 
+@pytest.mark.parametrize("width", [8193, 20000, 32768])
+def test_norm_of_wide_rows_in_f32(rx, client, width):
+    """A lane's 32 squares, 6 steps of a wavefront and 4 that join sixteen of them: (32 + 10 + 2) U of the mean, half of it in the root, and 5 U
+    of the division, the root, its reciprocal and two products.  Magnitudes over many powers of two, and equal ones, whose roundings agree."""
+    rng = np.random.default_rng(width)
+    x = np.exp(rng.uniform(-8, 8, size=(4, width)))
+    x[1], x[2] = 1 / 3, np.sort(x[2])
+    x, w = T.rounded(x, "f32"), T.rounded(1 + 0.2 * rng.normal(size=width), "f32")
+    got, _ = gpu_run(rx, client, P.rms_norm(4, width, dt="f32", residual=False), [x, w])
+    y = L.rms_norm(x.a, None, w.a)[0]
+    assert np.all(np.abs(got[0].a - y) <= 27 * UF * np.abs(y))
+
+
 GRADS = [(1, 1, "f32", "f32", True), (513, 1001, "f32", "f32", False), (40, 64, "bf16", "bf16", True), (7, 8192, "f16", "f32", True), (3, 8193, "f32", "f32", True), (2, 32768, "bf16", "f32", False),
          (0, 100, "f32", "f32", True), (5000, 96, "bf16", "f32", True), (1300, 1040, "f16", "f16", True), (5, 20011, "f32", "f32", True)]
 
