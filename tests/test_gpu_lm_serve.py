@@ -813,3 +813,163 @@ def test_a_whole_step_in_8_bits_runs(rx, client):
             new, old = new.transpose(0, 2, 1), old.transpose(0, 2, 1)
         assert same_bits(new[~written], old[~written]) and np.isfinite(new[written]).all()
         assert np.any(new[written] != old[written])
+
+
+class Near:
+    """Numbers v in 64 bits, and e, what the device's may be off by."""
+
+    def __init__(self, v, e=0.0):
+        self.v = np.asarray(v, dtype=np.float64)
+        self.e = np.broadcast_to(np.asarray(e, dtype=np.float64), self.v.shape)
+
+    def rounds(self, n):
+        """After n roundings to f32."""
+        return Near(self.v, self.e + n * UF * (np.abs(self.v) + self.e))
+
+    def __add__(self, o):
+        return Near(self.v + o.v, self.e + o.e).rounds(1)
+
+    def __mul__(self, o):
+        return Near(self.v * o.v, self.e * np.abs(o.v) + np.abs(self.v) * o.e + self.e * o.e).rounds(1)
+
+    def __getitem__(self, i):
+        return Near(self.v[i], self.e[i])
+
+    def reshape(self, *s):
+        return Near(self.v.reshape(*s), self.e.reshape(*s))
+
+    def product(self, w):
+        """With rows of w that hold few numbers beside zeros: their products and sums."""
+        a, b = np.abs(self.v) + self.e, np.abs(w)
+        return Near(self.v @ w.T, self.e @ b.T + ((w != 0).sum(1) + 4) * UF * (a @ b.T))
+
+    def normed(self, w):
+        """The root is off by half of what the mean of the squares is, relative to it; of a row no longer than a wavefront, whose sum takes 6 steps,
+        (1 + 6 + 2) / 2 + 5 U more."""
+        a, mean = np.abs(self.v), (self.v ** 2).mean(-1, keepdims=True) + 1e-6
+        off = (2 * a * self.e + self.e ** 2).mean(-1, keepdims=True) / mean
+        assert np.all(off < 0.5)
+        r, y = mean ** -0.5, self.v * mean ** -0.5 * w
+        return Near(y, self.e * r * np.abs(w) * (1 + off) + np.abs(y) * (off + 10 * UF))
+
+    def quantized(self, dt):
+        """(numbers, scales): numbers go either way where their values lie next to a border."""
+        top = np.abs(self.v).max(-1)
+        scale = Near(np.maximum(top, 2.0 ** -100) / L.LARGEST[dt], self.e.max(-1) / L.LARGEST[dt]).rounds(1)
+        z = self.v / scale.v[..., None]
+        off = (self.e / scale.v[..., None] + np.abs(z) * (scale.e / (scale.v - scale.e))[..., None]) * 1.001 + UF * np.abs(z)
+
+        def near(x):
+            x = np.clip(x, -L.LARGEST[dt], L.LARGEST[dt])
+            return np.rint(x) if dt == "i8" else LF.round_e4m3fn(x.astype(np.float32)).astype(np.float64)
+        codes = near(z)
+        return Near(codes, np.maximum(np.abs(near(z - off) - codes), np.abs(near(z + off) - codes))), scale
+
+
+def assert_near(got, ref):
+    got = np.asarray(got, dtype=np.float64)
+    ok = np.abs(got - ref.v) <= ref.e
+    assert got.shape == ref.v.shape and ok.all(), "%d of %d, first at %s: %r for %r, bound %r" % ((~ok).sum(), ok.size, np.argwhere(~ok)[0], got[~ok][0], ref.v[~ok][0], ref.e[~ok][0])
+
+
+@pytest.mark.parametrize("seed,cache,products,layout,rotation,axes", [(17, "f8E4M3FN", "f8E4M3FN", "slots", "halves", 1), (3, "i8", "f8E4M3FN", "heads", "pairs", 3), (3, "f8E4M3FN", "i8", "heads", "halves", 2)])
+def test_values_of_a_whole_step_in_8_bits(rx, client, seed, cache, products, layout, rotation, axes):
+    """One module of two layers, f32 between its 8 bits, against the operators' definitions in 64 bits, with what every operation may be off
+    by carried along: numbers that the device may round the other way count with their whole step.  Inputs that have next to none of those, so
+    that the results' bounds are small."""
+    b, n, vocab, width, hq, hk, d, hidden, pages, size, cols, positions = 2, 3, 101, 32, 4, 2, 16, 32, 9, 4, 4, 16
+    t, half = b * n, d // 2
+    text, types, cache_results = P.verify_step(b, n, vocab, width, hq, hk, d, hidden, pages, size, cols, positions, layers=2, axes=axes, top=3, dt="f32", cache=cache, products=products, layout=layout,
+                                               rotation=rotation)
+    rng = np.random.default_rng(seed)
+    args = verify_values(rng, text, types, True, b, n, pages, cols, positions, d)
+    for k, (s, dt) in enumerate(types[8:], 8):
+        if len(s) == 2:                              # weights: three numbers of a row, so that roundings stay few
+            x = np.zeros(s)
+            for row in x:
+                row[rng.permutation(s[1])[:3]] = rng.choice([-2, -1, 1, 2], size=3)
+            args[k] = I.Tensor(x, dt)
+        elif dt in EIGHT:                            # what the caches hold already, and its scales
+            x = rng.normal(size=s) * 50
+            args[k] = I.Tensor(np.rint(x.clip(-127, 127)) if dt == "i8" else LF.round_e4m3fn(x.astype(np.float32)), dt)
+        elif len(s) == 3:
+            args[k] = I.Tensor(rng.uniform(0.005, 0.015, size=s), "f32")
+        elif not s:
+            args[k] = I.Tensor(np.float32(rng.uniform(0.05, 0.1)), "f32")
+    mask, lengths = tree(rng, b, n), np.array([5, 0])
+    depth = mask.sum(-1)
+    angle = np.stack([(lengths[:, None] + depth + 2 * a) % positions for a in range(axes)])
+    args[8] = T.rounded(rng.normal(size=(vocab, width)), "f32")
+    for k, v in enumerate((rng.integers(0, vocab, (b, n)), rng.integers(0, vocab, (b, n)), angle, lengths)):
+        args[k] = I.Tensor(v, "i32")
+    args[4] = I.Tensor(mask, "i1")
+    got = [g.a for g in gpu_run(rx, client, text, args)[0]]
+    a = [np.asarray(x.a, dtype=np.float64) if x.dt not in ("i32", "i1") else x.a for x in args]
+    tokens, targets, table, cos, sin, given = a[0].reshape(-1), a[1].reshape(-1), a[5], a[6], a[7], iter(a[8:])
+    position = (lengths[:, None] + np.arange(n)).reshape(-1)
+    page, slot = table[np.arange(t) // n, position // size], position % size
+    axis = np.repeat(np.arange(axes), [half - (axes - 1) * (half // axes)] + [half // axes] * (axes - 1))
+    c, s = (Near(m[angle.reshape(axes, t)[axis].T, np.arange(half)][:, None]) for m in (cos, sin))
+    first = np.arange(half) * (2 if rotation == "pairs" else 1)
+    second = first + (1 if rotation == "pairs" else half)
+
+    def rotated(x):
+        p, q = x[..., first], x[..., second]
+        minus, plus = p * c + q * Near(-s.v), q * c + p * s
+        v, e = np.zeros(x.v.shape), np.zeros(x.v.shape)
+        v[..., first], e[..., first], v[..., second], e[..., second] = minus.v, minus.e, plus.v, plus.e
+        return Near(v, e)
+
+    def attended(q, caches, scales):
+        out_v, out_e = np.zeros((t, hq, d)), np.zeros((t, hq, d))
+        for i in range(t):
+            before = lengths[i // n]
+            at = np.concatenate([np.arange(before), before + np.flatnonzero(mask[i // n, i % n])])
+            if not len(at):
+                continue
+            pg, sl = table[i // n, at // size], at % size
+            for h in range(hq):
+                g = h // (hq // hk)
+                k, v = (rows[pg, sl, g] * Near(sc.v[pg, g, sl][:, None], sc.e[pg, g, sl][:, None]) for rows, sc in zip(caches, scales))
+                x, ax = k.v @ q.v[i, h], np.abs(k.v) + k.e
+                off = (k.e @ np.abs(q.v[i, h]) + ax @ q.e[i, h] + (d + 5) * UF * (ax @ np.abs(q.v[i, h]))) * d ** -0.5
+                w = np.exp((x - x.max()) * d ** -0.5)
+                w /= w.sum()
+                more = np.expm1(2 * off.max()) + (len(at) + 17) * UF + 2.0 ** -23
+                out_v[i, h], out_e[i, h] = w @ v.v, (1 + more) * (w @ v.e) + more * (w @ np.abs(v.v))
+        return Near(out_v, out_e)
+
+    x, late = Near(next(given)[tokens]), None
+    for layer in range(2):
+        w1, wq, wk, wv, wo, w2, gate, up, down = (next(given) for _ in range(9))
+        factors = [Near(next(given)) for _ in range(5)]
+        kc, vc, ks, vs = (next(given) for _ in range(4))
+        x = x if late is None else late + x
+        codes, scale = x.normed(w1).quantized(products)
+        q, k, v = ((codes.product(w) * scale[:, None] * f).reshape(t, -1, d) for w, f in zip((wq, wk, wv), factors))
+        held, held_scales = [], []
+        for r, (old, old_scale, new) in enumerate(((kc, ks, rotated(k)), (vc, vs, v))):
+            number, sc = new.quantized(cache)
+            rows, scales = old if layout == "slots" else old.transpose(0, 2, 1, 3), old_scale
+            now, now_scale = Near(rows.copy(), np.zeros(rows.shape)), Near(scales.copy(), np.zeros(scales.shape))
+            now.e, now_scale.e = np.array(now.e), np.array(now_scale.e)
+            now.v[page, slot], now.e[page, slot], now_scale.v[page, :, slot], now_scale.e[page, :, slot] = number.v, number.e, sc.v, sc.e
+            device = got[cache_results[4 * layer + r]]
+            assert_near(device if layout == "slots" else device.transpose(0, 2, 1, 3), now)
+            assert_near(got[cache_results[4 * layer + 2 + r]], now_scale)
+            held.append(now)
+            held_scales.append(now_scale)
+        x = attended(rotated(q), held, held_scales).reshape(t, hq * d).product(wo) + x
+        codes, scale = x.normed(w2).quantized(products)
+        y, z = (codes.product(w) * scale[:, None] * f for w, f in zip((gate, up), factors[3:]))
+        sig = 1 / (1 + np.exp(-y.v))                 # (its slope is at most 1/4; the exponential and the quotient in f32)
+        late = (y * Near(sig, y.e / 4 + 8 * UF * sig) * z).product(down)
+    logits = (late + x).normed(next(given)).product(next(given))
+    off = logits.e.max(-1) + (vocab / 64 + 108) * UF
+    top = logits.v.max(-1, keepdims=True)
+    lse = np.log(np.exp(logits.v - top).sum(-1)) + top[:, 0]
+    assert off.max() < 0.01                          # (so that a wrong scale or product would show)
+    assert_near(got[1], Near(lse, off + 4 * UF * np.abs(lse)))
+    logp = logits.v - lse[:, None]
+    assert_near(got[0], Near(logp[np.arange(t), targets], 2 * off + 4 * UF * np.abs(logp).max()))
+    assert_near(got[3], Near(-np.sort(-logp, -1)[:, :3], (2 * off + 4 * UF * np.abs(logp).max())[:, None]))
