@@ -147,7 +147,7 @@ OperatorPlan plan_norm_grad(const OperatorSpec& s, bool lean) {
   const bool residual = s.in.size() == 4;
   const int64_t D = s.in[0].dims.back(), rows = s.in[0].numel() / D;
   const Lanes l = lanes_of(D, info(s.in[0].dt).size);
-  const int64_t lines = l.lanes < 256 ? 256 / l.lanes : 1, most = 512;   // (16384 x 4096 bf16: 256 workgroups 113 us, 512 89, 1024 93)
+  const int64_t lines = l.lanes < 256 ? 256 / l.lanes : 1, most = 512;   // (256, 512 and 1024 workgroups: 40960 x 1024 bf16 57, 54 and 57 us, 16384 x 4096 113, 89 and 93, 8192 x 8192 98, 90 and 92, 4096 x 16384 91, 95 and 102)
   const int64_t groups = std::max<int64_t>(1, std::min<int64_t>({(rows + lines - 1) / lines, most, lean ? std::max<int64_t>(1, kLeanBytes / (4 * D)) : most}));
   OperatorPlan p;
   p.header = "rx_lm_norm_kernels.h";
@@ -230,7 +230,9 @@ OperatorPlan plan_write(const OperatorSpec& s) {
   const bool pairs = rotation == "pairs", whole = kc.dim % ne == 0 && vc.dim % ne == 0 && 2 * R2 % ne == 0 && (pairs || R2 % ne == 0);
   int64_t lanes = 1;
   while (lanes * ne < std::max(kc.dim, vc.dim)) lanes *= 2;
-  const int64_t each = T >= 2048 ? 4 : 1;   // heads of a token to a group of lanes: 8191 tokens of 40 heads 41.3 us with two, 38.6 with four, 48.4 with eight; 48 tokens 3.4 with one
+  // heads of a token to a group of lanes: 8191 tokens of 48 heads 41.3 us with two, 38.6 with four, 48.4 with eight; with one and with four 256 tokens 4.8 and 7.4 us,
+  // 1024 9.8 and 10.3, 2048 16.5 and 14.0, 4096 28 and 23; 48 tokens 3.4 with one
+  const int64_t each = T >= 2048 ? 4 : 1;
   std::ostringstream b;
   b << "rx_kv_write<" << elem(in[0].dt) << ", " << stored(in[9].dt) << ", " << HQ << ", " << kc.heads << ", " << kc.dim << ", " << vc.dim << ", " << kc.pages << ", " << kc.slots << ", "
     << in[8].dims[0] << ", " << in[8].dims[1] << ", " << in[3].dims[0] << ", " << R2 << ", " << axes << ", " << ends[0] << ", " << ends[1] << ", " << ends[2] << ", " << (pairs ? "true" : "false") << ", "
@@ -371,10 +373,14 @@ OperatorPlan plan_tree(const OperatorSpec& s, bool lean) {
   if (shared) NT = rows > 64 && registers(2) < 330 ? 2 : 1;
   else NT = rows > 16 && registers(2) < 320 ? 2 : 1;
   const int64_t WR = shared ? 4 : 1, TR = 16 * NT * WR, tiles = (rows + TR - 1) / TR, RT = std::min(rows, TR);
-  const int64_t lds = rings ? ring * stage + 4096 : shared ? 2 * 32 * ((kf * 4 * fe + 16 / size) + (nv * 16 * ve + 16 / size)) * size : 0;
-  // Two wavefronts to a SIMD where the estimate allows it: 64 rows of 128 dimensions to a wavefront pair 610 us with one, 380 with two (16 sequences
-  // of 4001 positions, 64 heads); 32 rows of one sequence of 1000 positions, an estimate of 208, 18.6 and 17.8; four tiles of 16 rows to a wavefront, one to a SIMD, 614.
-  const int waves = registers(NT) <= (wide || shared ? 230 : 210) && lds <= 80000 ? 2 : 1;
+  const int64_t results = 64 * (16 * ve + 4) * 4;   // of four wavefronts' 16 rows
+  const int64_t lds = rings ? std::max(ring * stage, results) + 4096 : shared ? 2 * 32 * ((kf * 4 * fe + 16 / size) + (nv * 16 * ve + 16 / size)) * size + results : 0;
+  // Two wavefronts to a SIMD where the estimate says that they fit.  With one and with two, 16 sequences of 4000 positions, 8 key heads, bf16 unless said otherwise:
+  // an estimate of 208, 8 and 32 rows of 128 dimensions 54 and 57 us, 60 and 63 (one sequence of 1000 positions 18.6 and 17.8); 212 to 224, 8 rows
+  // of 160 and 192, 72 and 67, 84 and 84; 224, 64 rows of 192, 158 and 102; 240, 128 rows of 128, f16 over 8 bits, 157 and 127; 248, 64 rows of 256, 156 and 116; 256,
+  // 32 rows of 80 in f32 115 and 108.  Beyond: 272, 32 rows of 128, f32 over 8 bits, 67 and 71; 280, 8 rows of 256, f16 over 8 bits, 77 and 90; 288, 8 rows
+  // of 160 in f32 140 and 223; 304, 32 rows of 128 in f32 158 and 193.  (Four tiles of 16 rows to a wavefront, one to a SIMD: 614 where two take 380.)
+  const int waves = registers(NT) <= 256 && lds <= 80000 ? 2 : 1;
   const int64_t longest = window ? std::min(M * kc.slots, window + N + 31) : M * kc.slots, units = std::max<int64_t>(1, (longest + 31) / 32);
   const bool once = kc.dim * e % 256 == 0 && vc.dim * e % 256 == 0 && tiles == 1, dies = (by_slot && kc.dim * e % 128 != 0) || tiles > 1;
   const int64_t columns = kc.heads * tiles, room = 256 * waves;
