@@ -496,31 +496,31 @@ RX_DEV __amdgpu_buffer_rsrc_t rx_lm_shared(float* base, const unsigned bytes) { 
 // go to; these are of places that have arrived, and wait for nothing but themselves.
 RX_DEV rx_u32 rx_lm_lds(const void* p) { return (rx_u32)(unsigned long long)(RX_LDS const void*)p; }
 // four places, and the four OFF bytes further
-template <int OFF, int AT>
+template <int OFF>
 RX_DEV void rx_lm_lds_eight(rx_u32x4 (&x)[4], rx_u32x4 (&y)[4], const rx_u32 (&a)[4]) {
   asm volatile(
-      "ds_read_b128 %0, %8 offset:%12\n\tds_read_b128 %1, %9 offset:%12\n\tds_read_b128 %2, %10 offset:%12\n\tds_read_b128 %3, %11 offset:%12\n\t"
-      "ds_read_b128 %4, %8 offset:%13\n\tds_read_b128 %5, %9 offset:%13\n\tds_read_b128 %6, %10 offset:%13\n\tds_read_b128 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+      "ds_read_b128 %4, %8 offset:%12\n\tds_read_b128 %5, %9 offset:%12\n\tds_read_b128 %6, %10 offset:%12\n\tds_read_b128 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
       : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
-      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(AT), "n"(AT + OFF)
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF)
       : "memory");
 }
-template <int OFF, int AT>
+template <int OFF>
 RX_DEV void rx_lm_lds_eight(rx_u32x2 (&x)[4], rx_u32x2 (&y)[4], const rx_u32 (&a)[4]) {
   asm volatile(
-      "ds_read_b64 %0, %8 offset:%12\n\tds_read_b64 %1, %9 offset:%12\n\tds_read_b64 %2, %10 offset:%12\n\tds_read_b64 %3, %11 offset:%12\n\t"
-      "ds_read_b64 %4, %8 offset:%13\n\tds_read_b64 %5, %9 offset:%13\n\tds_read_b64 %6, %10 offset:%13\n\tds_read_b64 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+      "ds_read_b64 %0, %8\n\tds_read_b64 %1, %9\n\tds_read_b64 %2, %10\n\tds_read_b64 %3, %11\n\t"
+      "ds_read_b64 %4, %8 offset:%12\n\tds_read_b64 %5, %9 offset:%12\n\tds_read_b64 %6, %10 offset:%12\n\tds_read_b64 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
       : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
-      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(AT), "n"(AT + OFF)
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF)
       : "memory");
 }
-template <int OFF, int AT>
+template <int OFF>
 RX_DEV void rx_lm_lds_eight(rx_u32 (&x)[4], rx_u32 (&y)[4], const rx_u32 (&a)[4]) {
   asm volatile(
-      "ds_read_b32 %0, %8 offset:%12\n\tds_read_b32 %1, %9 offset:%12\n\tds_read_b32 %2, %10 offset:%12\n\tds_read_b32 %3, %11 offset:%12\n\t"
-      "ds_read_b32 %4, %8 offset:%13\n\tds_read_b32 %5, %9 offset:%13\n\tds_read_b32 %6, %10 offset:%13\n\tds_read_b32 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+      "ds_read_b32 %0, %8\n\tds_read_b32 %1, %9\n\tds_read_b32 %2, %10\n\tds_read_b32 %3, %11\n\t"
+      "ds_read_b32 %4, %8 offset:%12\n\tds_read_b32 %5, %9 offset:%12\n\tds_read_b32 %6, %10 offset:%12\n\tds_read_b32 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
       : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
-      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(AT), "n"(AT + OFF)
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF)
       : "memory");
 }
 // two places, and the two OFF bytes further
@@ -900,7 +900,7 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
 #pragma unroll
           for (int k = 0; k < 4; ++k) a[k] = keys + (((k0 + k < KR ? k0 + k : KR - 1) * 4 + g4) ^ key_turn) * 16;
           if constexpr (KR <= 2) rx_lm_lds_four<256 * PK>(x[0], x[1], y[0], y[1], a[0], a[1]);
-          else rx_lm_lds_eight<256 * PK, 0>(x, y, a);
+          else rx_lm_lds_eight<256 * PK>(x, y, a);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             if (k0 + k >= KR) break;
@@ -941,7 +941,7 @@ RX_DEV void rx_tree_attention(const typename E::S* q, const typename C::S* kc, c
             const int byte = (j * 16 + r) * VE * (int)sizeof(T);
 #pragma unroll
             for (int i = 0; i < 4; ++i) a[i] = values + (g4 * 4 + i) * (PV * 16) + (((byte / 16) & (PV - 1)) ^ turn(g4 * 4 + i, PV)) * 16 + byte % 16;
-            rx_lm_lds_eight<256 * PV, 0>(x, y, a);        // (rows 16 further have the same turn)
+            rx_lm_lds_eight<256 * PV>(x, y, a);        // (rows 16 further have the same turn)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               vf[j][i] = __builtin_bit_cast(CVEC, x[i]);
