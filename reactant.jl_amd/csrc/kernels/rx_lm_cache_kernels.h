@@ -18,8 +18,8 @@ RX_DEV I rx_lm_axis_row(const int a, const I r0, const I r1, const I r2, const I
 }
 // A token's heads, EACH of them after one another, to a group of LANES lanes, NE elements of 16 bytes to a lane: what a head's
 // largest magnitude is found over, and what the cosines and sines of its dimensions are loaded for once.  Every lane loads the
-// pairs' other elements itself.  8191 tokens of 32 and 8 heads of 128 in bf16 into 8 bits, 189 MB, take 38.6 us, 4.9 TB/s: the index
-// arithmetic and the divisions take about half of the vector units' time.  48 tokens take 3.4 us, a launch and four dependent loads.
+// pairs' other elements itself.  8191 tokens of 32 and 8 heads of 128 in bf16 into 8 bits, 189 MB, take 38.6 us, 4.9 TB/s, with inputs in the
+// last-level cache, and 47 us from memory: the index arithmetic and the divisions take about half of the vector units' time.  48 tokens take 3.4 us, a launch and four dependent loads.
 template <typename E, typename C, int HQ, int HK, int DK, int DV, int P, int S, int B, int M, int L, int R2, int A, int S0, int S1, int S2, bool PAIRS, bool BY_SLOT, int T,
           bool WHOLE, int EACH, typename I>
 RX_DEV void rx_kv_write(const typename E::S* q, const typename E::S* k, const typename E::S* v, const float* cos, const float* sin, const I* angle, const I* position,
@@ -230,7 +230,7 @@ RX_DEV void rx_kv_move(const I* lengths, const I* path, const I* pages, U* kc, U
 // One token over 8 sequences of 131072 positions in 8 bits, 64 query heads of 8, 2.2 GB: 379 us, 5.8 TB/s, bound by memory (rows of 128
 // bytes are two half lines to a load; three and four wavefronts to a SIMD 384 and 427 us).  64 drafted tokens of 16 sequences of 4001 positions, 64
 // query heads of 8, 136 GFLOP in f16: 264 us, 517 TFLOP/s, bound by the vector units (65 % of the time; the matrix cores a third): softmax, the weights'
-// second numbers, addresses.  16 tokens of 64 sequences of up to 8192 in 8 bits: 96 us, half of it vector units, half a step's chain.
+// second numbers, addresses.  16 tokens of 64 sequences of up to 8192 in 8 bits: 72 us, half of it vector units, half a step's chain.
 struct rx_lm_tree_span : rx_lm_span { int prefix; };   // positions before the drafted tokens
 template <int S, int B, int M, int N, int W, typename I>
 RX_DEV rx_lm_tree_span rx_lm_tree_span_of(const I len) {

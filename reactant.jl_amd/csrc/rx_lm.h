@@ -28,7 +28,7 @@
 //   rx.token_logprobs_grad(logits, targets, lse, entropy, d_logprob, d_entropy) -> d_logits
 //   rx.rms_norm(x [.., D] [, residual [.., D]], weight [D]) {eps} -> ([h,] y) or ([h,] y in 8 bits, scale [..])
 //       h = x + residual (x itself without one), y = h weight / sqrt(mean(h^2) + eps), of h before it is rounded.  Squares are summed in f32.
-//       1 <= D <= 32768.
+//       1 <= D <= 32768.  (Without residual and 8 bits a reduction says the same, which becomes one launch of the generated code, a faster one.)
 //   rx.rms_norm_grad(h [.., D], weight [D], dy [.., D] [, dh [.., D]]) {eps} -> (dx [.., D], dweight [D] in the type of h, or f32)
 //       gradients by h (which is that by x and by residual) and by weight, for dy and dh arriving at y and h.
 //   rx.kv_write(q [T, Hq, D], k [T, Hk, D], v [T, Hk, Dv], cos [L, R / 2], sin [L, R / 2], angle [A, T], position [T], sequence [T], pages [B, M],
@@ -44,7 +44,7 @@
 //       no two sequences may name one slot.
 //   rx.tree_attention(q [B, N, Hq, D], k_cache, v_cache, pages [B, M], lengths [B] [, mask [N, N] or [B, N, N] i1] [, k_scale, v_scale])
 //               {scale, window, layout} -> out [B, N, Hq, Dv] (or (out, lse [B, N, Hq] f32))
-//       softmax(scale q k') v of N drafted tokens per sequence, which lie at positions lengths[b] .. lengths[b] + N - 1 of the cache.  Token i
+//       softmax(scale q k') v of N <= 1024 drafted tokens per sequence, which lie at positions lengths[b] .. lengths[b] + N - 1 of the cache.  Token i
 //       sees the positions before lengths[b], and drafted token j where mask[.., i, j]; without a mask itself and those before it (N = 1: the
 //       next token).  With a window (0: none, else at least N) a token sees that many positions: the drafted ones that it
 //       sees, and the last of those before.  lengths[b] < 0: the sequence takes no part, and sees nothing.  Positions beyond M S and on pages outside

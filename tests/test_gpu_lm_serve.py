@@ -402,6 +402,15 @@ def test_tree_attention(rx, client, lengths, n, hq, hk, d, dv, size, cols, dt, c
     assert all(np.array_equal(x.a, y.a) for x, y in zip(got, again))            # the same bits every run
 
 
+@pytest.mark.parametrize("dt,cache,layout,window", [("bf16", "bf16", "slots", 0), ("f16", "i8", "heads", 0), ("bf16", "f8E4M3FN", "slots", 1030)])
+def test_the_most_drafted_tokens(rx, client, dt, cache, layout, window):
+    """1024 tokens of a prompt, causal, behind none, a few and many positions; the last sequence's end lies beyond the page table."""
+    rng = np.random.default_rng(18)
+    n, hq, hk, d, size, cols = 1024, 2, 1, 64, 16, 80
+    args, scales = attention_case(rng, [0, 37, 256, 300, -1], n, hq, hk, d, d, size, cols, dt, cache, layout)
+    check_tree(rx, client, args, scales, None, n, hq, hk, d, d, size, cols, dt, cache, layout, window)
+
+
 @pytest.mark.parametrize("n,hq", [(6, 4), (24, 4)])
 @pytest.mark.parametrize("dt,cache", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "f8E4M3FN")])
 def test_special_values_that_a_token_does_not_see(rx, client, n, hq, dt, cache):

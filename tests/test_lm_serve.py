@@ -226,3 +226,9 @@ def test_interpreter_reads_the_calls():
 def test_programs_compile():
     for name in ("write_odd", "move_long", "tree_f32_8", "norm_wide", "verify"):
         assert launches(programs()[name])
+
+
+def test_more_sequences_than_are_counted():
+    with pytest.raises(rx.ReactantInternalError) as e:
+        rx.compile_offline(P.tree_attention(65536, 1, 8, 2, 64, 10, 16, 4))
+    assert "too many sequences or heads" in str(e.value)
