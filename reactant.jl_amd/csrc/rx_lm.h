@@ -54,7 +54,8 @@
 //
 // Numbers of 8 bits (f8E4M3FN, or i8 from -127 to 127) stand for their product with a scale in f32, one for each row of a norm, or for each head's key
 // and value of a position: scale = max(largest magnitude, 2^-100) / 448 (i8: 127), number = value / scale to nearest, ties to even.
-// A row that holds an infinity or NaN has zeros and a scale of NaN.  Scales of caches are [pages, Hk, S] in either layout.
+// A row that holds an infinity or NaN has zeros and a scale of NaN.  Scales of caches are [pages, Hk, S] in either layout.  (An infinite scale of a key, which
+// nothing here writes, makes its score an infinity or NaN.)
 //
 // Caches are [pages, S, Hk, D] (layout "slots") or [pages, Hk, S, D] ("heads").  Floats are f32, bf16 or f16, one type per operator
 // except where noted; integers are i32 or i64.  Sums, statistics and products are carried in f32.

@@ -402,6 +402,17 @@ def test_tree_attention(rx, client, lengths, n, hq, hk, d, dv, size, cols, dt, c
     assert all(np.array_equal(x.a, y.a) for x, y in zip(got, again))            # the same bits every run
 
 
+@pytest.mark.parametrize("n,d,cache,size", [(20, 64, "bf16", 1), (20, 33, "bf16", 1), (20, 64, "f8E4M3FN", 3), (4, 64, "i8", 1)])
+def test_more_positions_than_a_block_of_pages(rx, client, n, d, cache, size):
+    """Positions whose page entries are brought to LDS several times."""
+    rng = np.random.default_rng(n + d)
+    lengths = [2500 * size, 1024 * size, 1010 * size]
+    cols = 2500 + n
+    args, scales = attention_case(rng, lengths, n, 4, 1, d, d, size, cols, "bf16", cache, "slots")
+    args[3].a[0, 1500], args[3].a[2, 100] = -1, args[1].shape[0]
+    check_tree(rx, client, args, scales, tree(rng, 3, n), n, 4, 1, d, d, size, cols, "bf16", cache, "slots", 0)
+
+
 @pytest.mark.parametrize("dt,cache,layout,window", [("bf16", "bf16", "slots", 0), ("f16", "i8", "heads", 0), ("bf16", "f8E4M3FN", "slots", 1030)])
 def test_the_most_drafted_tokens(rx, client, dt, cache, layout, window):
     """1024 tokens of a prompt, causal, behind none, a few and many positions; the last sequence's end lies beyond the page table."""
